@@ -758,6 +758,111 @@ int pe_prefill_attn(const float* q, int64_t q_stride, const float* k_cache, cons
                     int n_head, int n_kv, int head_dim, int64_t capacity, int64_t L, int64_t pos0,
                     float scale, float* out, int64_t out_stride, pe_stream_t stream);
 
+/* ---- a batch of continuations of one prompt -------------------------------------------------
+ * One decode step of `batch` sequences behind a shared prefix: rotary positions with the cache
+ * write, attention, and the rules on the logits. No counterparts in the reference, which decodes
+ * one sequence. Device integers are int32 (dtype 1) or int64 (dtype 2). */
+
+/* Rotary positions of any rows: the first rot_dim elements of every head of token t as rot_dim / 2
+ * pairs -- (j, j + rot_dim / 2), or interleaved (2 j, 2 j + 1) -- turned by the angle positions[t] *
+ * freqs[j] and multiplied by amp; the other elements are copied. freqs (rot_dim / 2) in radians a
+ * position, 64-bit, finite; angles are exact to 2^-52 of themselves at any position (negative ones
+ * turn back). x and y PE_TYPE_F32 or PE_TYPE_F16 (computed in fp32, rounded once), head h of token t
+ * at t * token stride + h * head stride (elements; y's rows must not overlap); y may be x.
+ * pe_rope (kernels.py:50) takes table rows of contiguous positions, the half layout and whole heads. */
+int pe_rope_positions(int type, const void* x, int64_t x_token, int64_t x_head, const void* positions,
+                      int pos_dtype, const double* freqs, int rot_dim, float amp, int interleaved, void* y,
+                      int64_t y_token, int64_t y_head, int64_t tokens, int n_head, int head_dim,
+                      pe_stream_t stream);
+
+/* A decode step's rows of `batch` sequences: qkv (batch, (n_head + 2 n_kv) head_dim) fp32, row stride
+ * qkv_stride; q_out (batch, n_head, head_dim) the rotated q heads; row positions[b] + slot_offset of
+ * sequence b's own cache (batch, n_kv, capacity, head_dim) of cache_type (F32 or F16) the rotated k and
+ * the v heads. A sequence whose row lies outside [0, capacity) writes nothing to the caches. Rotation as
+ * pe_rope_positions, or with freqs NULL by rows positions[b] (clamped to the table) of cos_tab /
+ * sin_tab (tab_rows, rot_dim / 2), times amp. For one token per sequence what pe_rope_kv_write
+ * does for a prompt. */
+int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, int pos_dtype,
+                   const double* freqs, const float* cos_tab, const float* sin_tab, int64_t tab_rows,
+                   int rot_dim, float amp, int interleaved, int n_head, int n_kv, int head_dim, int64_t batch,
+                   float* q_out, int cache_type, void* k_cache, void* v_cache, int64_t capacity,
+                   int64_t slot_offset, pe_stream_t stream);
+
+/* Decode attention of `batch` sequences that share a prefix: for sequence b and head h (kv head
+ * h / (n_head / n_kv)), softmax attention of q[b][h] over the prefix's first prefix_len keys and the
+ * sequence's own first own_len[b] ones. The prefix is read once for the whole batch.
+ *   q, out (batch, n_head, head_dim) fp32; k_prefix, v_prefix (n_kv, prefix_capacity, head_dim) and
+ *   k_own, v_own (batch, n_kv, own_capacity, head_dim) of cache_type (F32 or F16); head_dim 64 or 128;
+ *   prefix_len = (device scalar if prefix_len_dtype) + prefix_len_add, own_len[b] likewise (one device
+ *   integer per sequence), each clamped to its capacity. Nothing behind a length is used: it may hold
+ *   anything. No keys at all, or a negative own_len (a sequence that takes no part): zeros.
+ *   round_fp16 as pe_decode_attn. fp32 products and sums; with fp16 caches the query and the
+ *   probabilities enter the products as two fp16 values each, 22 bits (an infinite key or value that
+ *   a row sees may make it NaN).
+ * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes, any contents, with prefix_keys =
+ * prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in order on one
+ * stream may share it, calls that overlap must not. Two launches. */
+typedef struct pe_shared_prefix_args {
+    const float* q;
+    int cache_type;
+    const void* k_prefix;
+    const void* v_prefix;
+    int64_t prefix_capacity;
+    const void* prefix_len;
+    int prefix_len_dtype;
+    int64_t prefix_len_add;
+    const void* k_own;
+    const void* v_own;
+    int64_t own_capacity;
+    const void* own_len;
+    int own_len_dtype;
+    int64_t own_len_add;
+    int64_t batch;
+    int n_head, n_kv, head_dim;
+    float scale;
+    int round_fp16;
+    float* out;
+    void* workspace;
+    int64_t workspace_bytes;
+} pe_shared_prefix_args;
+int64_t pe_shared_prefix_attn_workspace_bytes(int64_t batch, int n_head, int n_kv, int head_dim,
+                                              int64_t prefix_keys, int64_t own_capacity);
+int pe_shared_prefix_attn(const pe_shared_prefix_args* args, pe_stream_t stream);
+
+/* Rules on the logits of `batch` rows of `vocab` elements (PE_TYPE_F32 or PE_TYPE_F16, computed in
+ * fp32 and rounded once; y may be x), in this order, with c the times a token stands in the first
+ * lengths[b] (NULL: history_len) ids of the row's history:
+ *   z += bias[v]; z = z > 0 ? z / repetition : z * repetition where the token stands in the history or
+ *   the prompt; z -= c * frequency + (c > 0) * presence; z = -inf where bit v % 32 of mask word v / 32
+ *   is 0. Ids outside [0, vocab) are passed over. history, prompt, bias (fp32) and mask (32-bit words)
+ *   may be NULL; their row strides may be 0 (one row for all), x_stride too. repetition_rows,
+ *   frequency_rows, presence_rows: one value per row, or NULL and the plain value for all. */
+typedef struct pe_logit_args {
+    int type;
+    const void* x;
+    int64_t x_stride;
+    void* y;
+    int64_t y_stride;
+    int64_t batch, vocab;
+    const void* history;
+    int history_dtype;
+    int64_t history_stride, history_len;
+    const void* lengths;
+    int lengths_dtype;
+    const void* prompt;
+    int prompt_dtype;
+    int64_t prompt_stride, prompt_len;
+    const float* repetition_rows;
+    const float* frequency_rows;
+    const float* presence_rows;
+    float repetition, frequency, presence;
+    const float* bias;
+    int64_t bias_stride;
+    const void* mask;
+    int64_t mask_stride;
+} pe_logit_args;
+int pe_adjust_logits(const pe_logit_args* args, pe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

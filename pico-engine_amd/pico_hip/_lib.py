@@ -102,6 +102,33 @@ class FfnFixArgs(ctypes.Structure):
     ]
 
 
+class SharedPrefixArgs(ctypes.Structure):
+    """Mirror of pe_shared_prefix_args (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("q", _P), ("cache_type", _I), ("k_prefix", _P), ("v_prefix", _P), ("prefix_capacity", _L),
+        ("prefix_len", _P), ("prefix_len_dtype", _I), ("prefix_len_add", _L),
+        ("k_own", _P), ("v_own", _P), ("own_capacity", _L),
+        ("own_len", _P), ("own_len_dtype", _I), ("own_len_add", _L),
+        ("batch", _L), ("n_head", _I), ("n_kv", _I), ("head_dim", _I), ("scale", _F), ("round_fp16", _I),
+        ("out", _P), ("workspace", _P), ("workspace_bytes", _L),
+    ]
+
+
+class LogitArgs(ctypes.Structure):
+    """Mirror of pe_logit_args (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("type", _I), ("x", _P), ("x_stride", _L), ("y", _P), ("y_stride", _L), ("batch", _L), ("vocab", _L),
+        ("history", _P), ("history_dtype", _I), ("history_stride", _L), ("history_len", _L),
+        ("lengths", _P), ("lengths_dtype", _I),
+        ("prompt", _P), ("prompt_dtype", _I), ("prompt_stride", _L), ("prompt_len", _L),
+        ("repetition_rows", _P), ("frequency_rows", _P), ("presence_rows", _P),
+        ("repetition", _F), ("frequency", _F), ("presence", _F),
+        ("bias", _P), ("bias_stride", _L), ("mask", _P), ("mask_stride", _L),
+    ]
+
+
 _SIGNATURES = {
     "pe_strerror": (ctypes.c_char_p, [_I]),
     "pe_abi_version": (_I, []),
@@ -178,6 +205,11 @@ _SIGNATURES = {
     "pe_ffn_fix": (_I, [ctypes.POINTER(FfnFixArgs), _P]),
     "pe_qkv_fix_rmsnorm_rope": (_I, [ctypes.POINTER(QkvArgs), _P, _I, _L, _P, _P]),
     "pe_qkv_embed_rmsnorm_rope": (_I, [ctypes.POINTER(QkvArgs), _I, _P, _L, _P, _P, _P, _L, _P]),
+    "pe_rope_positions": (_I, [_I, _P, _L, _L, _P, _I, _P, _I, _F, _I, _P, _L, _L, _L, _I, _I, _P]),
+    "pe_rope_append": (_I, [_P, _L, _P, _I, _P, _P, _P, _L, _I, _F, _I, _I, _I, _I, _L, _P, _I, _P, _P, _L, _L, _P]),
+    "pe_shared_prefix_attn_workspace_bytes": (_L, [_L, _I, _I, _I, _L, _L]),
+    "pe_shared_prefix_attn": (_I, [ctypes.POINTER(SharedPrefixArgs), _P]),
+    "pe_adjust_logits": (_I, [ctypes.POINTER(LogitArgs), _P]),
 }
 
 # Every symbol include/pico_hip.h declares (checked by tests/test_abi.py).

@@ -18,14 +18,15 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from dataclasses import dataclass
 
 import os
 
 import torch
 
-from ._lib import (LAYOUT_NATURAL, LAYOUT_X_UT, LAYOUT_Y_UT, AttnOprojArgs, FfnFixArgs, QkvArgs, StepArgs,
-                   StepLayer, check, lib)
+from ._lib import (LAYOUT_NATURAL, LAYOUT_X_UT, LAYOUT_Y_UT, AttnOprojArgs, FfnFixArgs, LogitArgs, QkvArgs,
+                   SharedPrefixArgs, StepArgs, StepLayer, check, lib)
 from .dequant import (BLOCK_SIZE, GGML_F16, GGML_F32, GGML_Q4_K, GGML_Q5_0, GGML_Q6_K, GGML_Q8_0, MATRIX_TYPES,
                       QUANT_TYPES, TYPE_NAMES, nbytes_for)
 
@@ -1560,3 +1561,322 @@ __all__ = ["LAYOUT_NATURAL", "LAYOUT_X_UT", "LAYOUT_Y_UT", "to_ut", "from_ut", "
            "DecodeStep", "decode_step_supported", "decode_step_workspace",
            "gemm_f16", "gemm_f16_silu", "interleave_gate_up_f16", "flash_prefill",
            "BLOCK_SIZE"]
+
+
+# ---- a batch of continuations of one prompt -------------------------------------------------
+
+_INT_CODE = {torch.int32: 1, torch.int64: 2}
+_CACHE_TYPE = {torch.float32: GGML_F32, torch.float16: GGML_F16}
+
+
+def _one_gpu(*ts: torch.Tensor | None) -> torch.device:
+    """The GPU that all the tensors are on."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if dev is None:
+            dev = t.device
+            if dev.type != "cuda":
+                raise ValueError(f"pico_hip kernels need GPU tensors, got a tensor on {dev}")
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    return dev
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Calls an entry point on the tensors' device and its current stream."""
+    if dev.index == torch.cuda.current_device():
+        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if status:
+        check(status, name)
+
+
+def _ints(t: torch.Tensor, n: int, what: str) -> int:
+    """The dtype code of a contiguous vector of n device integers."""
+    code = _INT_CODE.get(t.dtype)
+    if code is None or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 or int64 vector of {n} elements")
+    return code
+
+
+def rope_freqs(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+               original_context: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+               low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+               freq_factors: list[float] | None = None, device="cuda") -> tuple[torch.Tensor, float]:
+    """(freqs, amp) of rope_positions and rope_append: radians a position of the rot_dim / 2 pairs
+    (float64, on the device) and the factor of the rotated values. f_j = base^(-2j/rot_dim), and for
+    contexts of ``factor`` times the trained one (``original_context`` positions):
+
+    * "linear": f / factor;
+    * "ntk": the base times factor^(rot_dim / (rot_dim - 2));
+    * "yarn": f for the pairs that turn more than beta_fast times in the trained context, f / factor
+      below beta_slow turns, a linear blend over the pairs between; amp = 0.1 ln(factor) + 1;
+    * "llama3": f for wavelengths under original_context / high_freq_factor, f / factor over
+      original_context / low_freq_factor, a blend linear in original_context / wavelength between.
+
+    ``freq_factors`` (one per pair, a GGUF's rope_freqs.weight) divide the unscaled f."""
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim} is not a positive even number")
+    if not (base > 0 and factor > 0):
+        raise ValueError("base and factor must be positive")
+    if scaling not in ("none", "linear", "ntk", "yarn", "llama3"):
+        raise ValueError(f"unknown RoPE scaling {scaling!r}")
+    if scaling in ("yarn", "llama3") and original_context <= 0:
+        raise ValueError(f"{scaling} needs the trained context (original_context)")
+    n, amp = rot_dim // 2, 1.0
+    if freq_factors is not None and len(freq_factors) != n:
+        raise ValueError(f"{len(freq_factors)} freq_factors for {n} pairs")
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = [base ** (-2.0 * j / rot_dim) / (1.0 if freq_factors is None else float(freq_factors[j])) for j in range(n)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    elif scaling == "yarn":
+        def pair_of(turns: float) -> float:   # the pair that turns this often in the trained context
+            return rot_dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo, hi = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rot_dim - 1)
+        slow = [min(max((j - lo) / max(hi - lo, 0.001), 0.0), 1.0) for j in range(n)]
+        f = [x * (1 - s) + x / factor * s for x, s in zip(f, slow)]
+        amp = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling == "llama3":
+        if not high_freq_factor > low_freq_factor > 0:
+            raise ValueError("llama3 needs high_freq_factor > low_freq_factor > 0")
+        keep = [min(max((original_context * x / (2 * math.pi) - low_freq_factor) /
+                        (high_freq_factor - low_freq_factor), 0.0), 1.0) for x in f]
+        f = [x * (s + (1 - s) / factor) for x, s in zip(f, keep)]
+    return torch.tensor(f, dtype=torch.float64, device=device), amp
+
+
+def _check_freqs(freqs: torch.Tensor, hd: int) -> int:
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or \
+            not 0 < 2 * freqs.numel() <= hd:
+        raise ValueError(f"freqs must be a contiguous float64 vector of 1 to {hd // 2} elements (rope_freqs)")
+    return 2 * freqs.numel()
+
+
+def rope_positions(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, amp: float = 1.0,
+                   interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE of x (T, n_head, hd), float32 or float16 (rows and heads with any strides), token t at
+    positions[t] (int32 or int64, any order, negative ones turn back): pairs (j, j + r/2) of the first
+    r = 2 len(freqs) elements of a head, or (2j, 2j + 1) if ``interleaved``; the others are copied.
+    freqs and amp from rope_freqs; the angles are made in 64 bits. ``out`` may be x."""
+    dev = _one_gpu(x, positions, freqs, out)
+    code = _CACHE_TYPE.get(x.dtype)
+    if code is None or x.dim() != 3:
+        raise ValueError("x must be a float32 or float16 (T, n_head, hd) tensor")
+    T, n, hd = x.shape
+    rot = _check_freqs(freqs, hd)
+    pos = _ints(positions, T, "positions")
+    if hd > 1 and x.stride(2) != 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty(T, n, hd, device=dev, dtype=x.dtype)
+    elif out.dtype is not x.dtype or out.shape != x.shape or (hd > 1 and out.stride(2) != 1):
+        raise ValueError(f"out must be a {x.dtype} ({T}, {n}, {hd}) tensor whose last dim is contiguous")
+    if T == 0 or n == 0:
+        return out
+    sx, sy = x.stride(), out.stride()
+    _launch(dev, "pe_rope_positions", code, x.data_ptr(), sx[0] if T > 1 else 0, sx[1] if n > 1 else 0,
+            positions.data_ptr(), pos, freqs.data_ptr(), rot, float(amp), int(interleaved), out.data_ptr(),
+            sy[0] if T > 1 else 0, sy[1] if n > 1 else 0, T, n, hd)
+    return out
+
+
+def rope_append(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor | tuple[torch.Tensor, torch.Tensor],
+                n_head: int, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_offset: int = 0, amp: float = 1.0,
+                interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One decode step's fused rows of B sequences: qkv (B, (n_head + 2 n_kv) hd) float32 (rows may be
+    strided) -> the rotated q (B, n_head, hd); the rotated k and v go to row positions[b] + slot_offset
+    of sequence b's own cache (B, n_kv, capacity, hd), float32 or float16 (a row outside the cache is
+    not written: a sequence that takes no part). ``freqs``: rope_freqs' vector, or (cos, sin) tables
+    (rows, hd / 2 at most) read at the positions, as the model's own are."""
+    tab = isinstance(freqs, tuple)
+    cos, sin = freqs if tab else (None, None)
+    dev = _one_gpu(qkv, positions, *((cos, sin) if tab else (freqs,)), k_cache, v_cache, out)
+    code = _CACHE_TYPE.get(k_cache.dtype)
+    if code is None or v_cache.dtype is not k_cache.dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or \
+            not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError("caches must be contiguous float32 or float16 (B, n_kv, capacity, hd) buffers of one shape")
+    B, n_kv, cap, hd = k_cache.shape
+    if qkv.dtype is not torch.float32 or qkv.dim() != 2 or tuple(qkv.shape) != (B, (n_head + 2 * n_kv) * hd):
+        raise ValueError(f"qkv must be a float32 ({B}, {(n_head + 2 * n_kv) * hd}) tensor")
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    pos = _ints(positions, B, "positions")
+    if tab:
+        if not (cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and
+                cos.is_contiguous() and sin.is_contiguous() and cos.shape[0] > 0 and 0 < 2 * cos.shape[1] <= hd):
+            raise ValueError(f"cos and sin must be contiguous float32 tables of 1 to {hd // 2} columns")
+        rot = 2 * cos.shape[1]
+        table = (None, cos.data_ptr(), sin.data_ptr(), cos.shape[0])
+    else:
+        rot = _check_freqs(freqs, hd)
+        table = (freqs.data_ptr(), None, None, 0)
+    if out is None:
+        out = torch.empty(B, n_head, hd, device=dev, dtype=torch.float32)
+    elif out.dtype is not torch.float32 or tuple(out.shape) != (B, n_head, hd) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32 ({B}, {n_head}, {hd}) tensor")
+    if B:
+        _launch(dev, "pe_rope_append", qkv.data_ptr(), qkv.stride(0) if B > 1 else qkv.shape[1], positions.data_ptr(),
+                pos, *table, rot, float(amp), int(interleaved), n_head, n_kv, hd, B, out.data_ptr(), code,
+                k_cache.data_ptr(), v_cache.data_ptr(), cap, int(slot_offset))
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_prefix_bytes(batch: int, n_head: int, n_kv: int, hd: int, keys: int, own: int) -> int:
+    size = lib.pe_shared_prefix_attn_workspace_bytes(batch, n_head, n_kv, hd, keys, own)
+    check(0 if size >= 0 else -size, "pe_shared_prefix_attn_workspace_bytes")
+    return size
+
+
+def shared_prefix_attn_workspace(batch: int, n_head: int, n_kv: int, hd: int, prefix_keys: int, own_capacity: int,
+                                 device) -> torch.Tensor:
+    """A workspace for shared_prefix_attn (any contents; reusable by calls in order on one stream).
+    prefix_keys: the prefix's length, or its capacity where the length is a device tensor."""
+    return torch.empty(_shared_prefix_bytes(batch, n_head, n_kv, hd, prefix_keys, own_capacity), device=device,
+                       dtype=torch.uint8)
+
+
+def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_own: torch.Tensor,
+                       v_own: torch.Tensor, own: torch.Tensor | int, prefix_len: torch.Tensor | int | None = None,
+                       scale: float | None = None, *, own_offset: int = 0, round_fp16: bool = True,
+                       workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Single-token GQA attention of B sequences that share a prefix, whose keys are taken once for
+    all: q (B, n_head, hd) float32, hd 64 or 128; k_prefix / v_prefix (n_kv, P, hd) and each sequence's
+    k_own / v_own (B, n_kv, capacity, hd), all float32 or all float16, contiguous. Sequence b sees the
+    first prefix_len prefix keys (an int, a device integer, or None: all P) and the first
+    own[b] + own_offset of its own (``own`` (B,) device integers, or an int for all). A sequence
+    without keys, or whose own length is negative (one that takes no part), gets zeros. ``round_fp16``
+    as decode_attn. Returns (B, n_head, hd) float32."""
+    dev = _one_gpu(q, k_prefix, v_prefix, k_own, v_own, own if isinstance(own, torch.Tensor) else None,
+                   prefix_len if isinstance(prefix_len, torch.Tensor) else None, workspace, out)
+    if q.dim() != 3:
+        raise ValueError("q must be a (B, n_head, hd) tensor")
+    q = _f32c(q)
+    B, n_head, hd = q.shape
+    n_kv, P = k_prefix.shape[0], k_prefix.shape[1]
+    code = _CACHE_TYPE.get(k_prefix.dtype)
+    cap = k_own.shape[2] if k_own.dim() == 4 else -1
+    if code is None or any(t.dtype is not k_prefix.dtype or not t.is_contiguous()
+                           for t in (k_prefix, v_prefix, k_own, v_own)) or \
+            tuple(k_prefix.shape) != (n_kv, P, hd) or v_prefix.shape != k_prefix.shape or \
+            tuple(k_own.shape) != (B, n_kv, cap, hd) or v_own.shape != k_own.shape:
+        raise ValueError(f"caches must be contiguous float32 or float16 buffers of one type: (n_kv, P, {hd}) for the "
+                         f"prefix, ({B}, n_kv, capacity, {hd}) for the sequences")
+    p_ptr, p_code, p_add = None, 0, P
+    if isinstance(prefix_len, torch.Tensor):
+        prefix_len = prefix_len.reshape(-1)
+        p_ptr, p_code, p_add = prefix_len.data_ptr(), _ints(prefix_len, 1, "prefix_len"), 0
+    elif prefix_len is not None:
+        p_add = int(prefix_len)
+        if not 0 <= p_add <= P:
+            raise ValueError(f"prefix_len {p_add} of a prefix of {P}")
+    o_ptr, o_code, o_add = None, 0, int(own_offset)
+    if isinstance(own, torch.Tensor):
+        o_ptr, o_code = own.data_ptr(), _ints(own, B, "own")
+    else:
+        o_add += int(own)
+    if out is None:
+        out = torch.empty(B, n_head, hd, device=dev, dtype=torch.float32)
+    elif out.dtype is not torch.float32 or tuple(out.shape) != (B, n_head, hd) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32 ({B}, {n_head}, {hd}) tensor")
+    if B == 0:
+        return out
+    need = _shared_prefix_bytes(B, n_head, n_kv, hd, P if p_code else p_add, cap)
+    if workspace is None:
+        workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    a = SharedPrefixArgs(q.data_ptr(), code, k_prefix.data_ptr(), v_prefix.data_ptr(), P, p_ptr, p_code, p_add,
+                         k_own.data_ptr(), v_own.data_ptr(), cap, o_ptr, o_code, o_add, B, n_head, n_kv, hd,
+                         float(hd ** -0.5 if scale is None else scale), int(round_fp16), out.data_ptr(),
+                         workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _launch(dev, "pe_shared_prefix_attn", ctypes.byref(a))
+    return out
+
+
+def _rows(t: torch.Tensor, B: int, n: int, what: str) -> int:
+    """The row stride of a table that is one row for all (n,), (1, n), or a row each (B, n)."""
+    if t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1):
+        return 0
+    if t.dim() == 2 and t.shape[0] in (1, B) and t.shape[1] == n and (n <= 1 or t.stride(1) == 1):
+        return 0 if t.shape[0] == 1 else t.stride(0)
+    raise ValueError(f"{what} must be a vector of {n} elements or ({B}, {n}) rows, its last dim contiguous")
+
+
+def _rule(v: torch.Tensor | float, B: int, what: str) -> tuple[int | None, float]:
+    """A rule's device pointer (one float32 per row) and plain value."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype is not torch.float32 or v.dim() != 1 or v.numel() != B or not v.is_contiguous():
+            raise ValueError(f"{what} must be a number or a contiguous float32 vector of {B} elements")
+        return v.data_ptr(), 0.0
+    v = float(v)
+    if not math.isfinite(v) or (what == "repetition" and v <= 0):
+        raise ValueError(f"{what} {v}")
+    return None, v
+
+
+def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                  prompt: torch.Tensor | None = None, repetition: torch.Tensor | float = 1.0,
+                  frequency: torch.Tensor | float = 0.0, presence: torch.Tensor | float = 0.0,
+                  bias: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rules on logits (B, V) or (V,), float32 or float16, before a token is picked. In this order,
+    with c the times a token stands in a row's history: + bias; divided by ``repetition`` where
+    positive, multiplied where not, for the tokens of history and prompt; - c * frequency - (c > 0) *
+    presence; -inf where the mask bit is 0. history (B, H) int32 or int64, of which the first
+    ``lengths`` (B,) count (None: all); prompt, bias (float32, V) and mask (int32 words, bit v % 32 of
+    word v // 32) one row for all or a row each. Ids outside [0, V) are passed over. The three
+    penalties are numbers or float32 vectors of one value per row. ``out`` may be logits."""
+    one = logits.dim() == 1
+    x = logits.unsqueeze(0) if one else logits
+    if x.dtype not in _CACHE_TYPE or x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError("logits must be float32 or float16 (B, V) rows")
+    B, V = x.shape
+    if V > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    rules = [(v, n) for v, n in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))]
+    dev = _one_gpu(x, history, lengths, prompt, bias, mask, out, *(v for v, _ in rules if isinstance(v, torch.Tensor)))
+    a = LogitArgs()
+    a.type, a.x, a.batch, a.vocab = _CACHE_TYPE[x.dtype], x.data_ptr(), B, V
+    a.x_stride = x.stride(0) if B > 1 else V
+    if history is not None:
+        h = history.unsqueeze(0) if history.dim() == 1 else history
+        if h.dtype not in _INT_CODE or h.dim() != 2 or h.shape[0] != B or (h.shape[1] > 1 and h.stride(1) != 1):
+            raise ValueError(f"history must be int32 or int64 ({B}, H) rows, the last dim contiguous")
+        a.history, a.history_dtype, a.history_len = h.data_ptr(), _INT_CODE[h.dtype], h.shape[1]
+        a.history_stride = h.stride(0) if B > 1 else 0
+    if lengths is not None:
+        a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
+    if prompt is not None:
+        if prompt.dtype not in _INT_CODE:
+            raise ValueError("prompt must hold int32 or int64 ids")
+        a.prompt, a.prompt_dtype, a.prompt_len = prompt.data_ptr(), _INT_CODE[prompt.dtype], prompt.shape[-1]
+        a.prompt_stride = _rows(prompt, B, prompt.shape[-1], "prompt")
+    (a.repetition_rows, a.repetition), (a.frequency_rows, a.frequency), (a.presence_rows, a.presence) = \
+        (_rule(v, B, n) for v, n in rules)
+    if bias is not None:
+        if bias.dtype is not torch.float32:
+            raise ValueError("bias must be float32")
+        a.bias, a.bias_stride = bias.data_ptr(), _rows(bias, B, V, "bias")
+    if mask is not None:
+        if mask.dtype is not torch.int32:
+            raise ValueError("mask must hold int32 words")
+        a.mask, a.mask_stride = mask.data_ptr(), _rows(mask, B, (V + 31) // 32, "mask")
+    if out is None:
+        y = torch.empty(B, V, device=dev, dtype=x.dtype)
+    else:
+        y = out.unsqueeze(0) if out.dim() == 1 else out
+        if y.dtype is not x.dtype or y.shape != x.shape or out.dim() != logits.dim() or (V > 1 and y.stride(1) != 1):
+            raise ValueError(f"out must be {x.dtype} of the logits' shape, its rows contiguous")
+    a.y, a.y_stride = y.data_ptr(), y.stride(0) if B > 1 else V
+    if B:
+        _launch(dev, "pe_adjust_logits", ctypes.byref(a))
+    return out if out is not None else y[0] if one else y
