@@ -11,12 +11,13 @@
 // fp32. Two ways over the keys, by the rows of a kv head:
 //   shared: a workgroup's eight waves take four row tiles of 32 and two halves of every 64-key
 //     block, staged once for all of them in LDS (two buffers, one barrier a block);
-//   solo: a wave takes 32 rows and its own key tiles in its own LDS without barriers, up to eight
-//     waves of an item merged at the end. The own keys, a group's rows each, always go this way.
+//   solo: the eight waves take 32 rows and every eighth key tile each, in their own LDS without
+//     barriers, merged at the end. The own keys go the same way by groups of 16 rows, one to eight
+//     waves an item.
 // Products: fp32 caches that are taken solo run on the fp32 matrix instructions (bound by memory at
 // these row counts). All others run on v_mfma_f32_32x32x16_f16 with the fp32 factors as the sum of
 // two fp16 values, 22 bits (one would cost 2^-12 of each): the query, scaled by a power of two to at
-// most 2^14; the probability times 2^14; and an fp32 cache's keys and values, every 8 keys scaled by a
+// most 2^14; the probability; and an fp32 cache's keys and values, every 8 keys scaled by a
 // power of two of their largest element. Products of two low parts are left out (2^-22). That is 2
 // instructions for 16-bit caches and 3 for fp32 ones in place of 16 fp32 instructions of twice the
 // time each.
@@ -31,7 +32,10 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int kSpWaves = 8;
 constexpr int kSpBlock = 64;       // keys of a shared block
-constexpr float kLift = 14.f;      // log2 of the factor of the probabilities
+// The probabilities are exp2(s - r) for a reference r that starts kUp under a row's maximum and
+// moves when a score comes to lie more than kRoom over it: up to 2^15 they fit fp16, and the rows are
+// rescaled a few times instead of in most tiles.
+constexpr float kUp = 8.f, kRoom = 15.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct SpArgs {
@@ -70,9 +74,10 @@ PE_DEV int64_t sp_length(const void* len, int dtype, int64_t i, int64_t add, int
 PE_DEV uint32_t lds_address(const uint8_t* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
 }
-// 16 bytes per lane from global g into LDS at m0 + 16 lane (one wave instruction: 1 KB)
-PE_DEV void sp_load16(const void* g, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
+// 16 bytes per lane from global g (uniform) + off into LDS at m0 + 16 lane (one wave instruction: 1 KB)
+PE_DEV void sp_load16(const void* g, uint32_t off, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0)
+                 : "memory", "m0");
 }
 template <int N>
 PE_DEV void sp_wait_loads() {
@@ -80,8 +85,48 @@ PE_DEV void sp_wait_loads() {
 }
 PE_DEV void sp_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The largest of a wave's whole numbers.
+template <int CTRL>
+PE_DEV uint32_t dpp_max(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
+    return v > o ? v : o;
+}
+PE_DEV uint32_t wave_max_bits(uint32_t v) {
+    v = dpp_max<0xB1>(v);   // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);   // quad_perm [2,3,0,1]
+    v = dpp_max<0x141>(v);  // row_half_mirror
+    v = dpp_max<0x140>(v);  // row_mirror
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = a[0] > a[1] ? a[0] : a[1];
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(b[0] > b[1] ? b[0] : b[1]);
+}
+
+// Records go past the L2, whose dirty lines the launch's end would have to write back.
+PE_DEV void store_record(float* p, const float4& v) {
+    typedef float f4v __attribute__((ext_vector_type(4)));
+    const f4v x = {v.x, v.y, v.z, v.w};
+    asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1" ::"v"(p), "v"(x) : "memory");
+}
+
 PE_DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 PE_DEV int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
+
+// 8 fp32 values as the sums of two fp16 values, each rounded to nearest: within 2^-23 of the value from
+// 2^-3 on, 2^-25 below. The low part's difference is one instruction that reads the high part's half.
+typedef float f2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+PE_DEV void split2(float a, float b, h2v& hi, h2v& lo) {
+    const f2v x = {a, b};
+    hi = __builtin_convertvector(x, h2v);
+    f2v d;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d.x) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d.y) : "v"(hi), "v"(b));
+    lo = __builtin_convertvector(d, h2v);
+}
+
+// A positive factor of scores: no smaller than fp32's least (a masked score times it stays -inf).
+PE_DEV float sp_positive(float c) { return fminf(fmaxf(c, 1.1754943508222875e-38f), 1.7014118346046923e38f); }
 
 // LDS image of a key tile: row r's 16-byte chunk c at chunk position c ^ swizzle(r), so that the
 // rows that one read takes cover the banks. 16-bit values are read by rows of four (transposing
@@ -91,16 +136,21 @@ PE_DEV int sp_swizzle(int r) {
     return VALUES && SIZE == 2 ? 2 * (r & 3) : r & 7;
 }
 
-// Pieces f0 .. f0 + N - 1 (1 KB each) of the tile of rows row0 .. of base; rows past `last` are
-// the last one again (their scores are masked and their values cleared).
+// Pieces f0 .. f0 + N - 1 (1 KB each) of the tile that starts at base, whose rows behind `last` are that
+// one again (their scores are masked and their values cleared). A piece is contiguous in memory;
+// the lanes take its chunks in the image's order.
 template <typename T, int HD, bool VALUES, int N>
-PE_DEV void sp_stage(const T* base, int64_t row0, int64_t last, uint32_t lds, int lane, int f0) {
-    constexpr int E = 16 / sizeof(T), C = HD / E;
+PE_DEV void sp_stage(const T* base, int64_t last, uint32_t lds, int lane, int f0) {
+    constexpr int E = 16 / sizeof(T), C = HD / E, ROWS = 64 / C;
+    const bool whole = last >= ROWS * (f0 + N) - 1;
 #pragma unroll
     for (int f = 0; f < N; ++f) {
-        const int slot = (f0 + f) * 64 + lane, r = slot / C, c = (slot % C) ^ sp_swizzle<sizeof(T), VALUES>(r);
-        const int64_t row = row0 + r < last ? row0 + r : last;
-        sp_load16(base + row * HD + E * c, __builtin_amdgcn_readfirstlane(lds + (f0 + f) * 1024));
+        const int r = ROWS * (f0 + f) + lane / C, x = lane ^ sp_swizzle<sizeof(T), VALUES>(r);
+        const uint32_t at = __builtin_amdgcn_readfirstlane(lds + (f0 + f) * 1024);
+        if (whole)
+            sp_load16(reinterpret_cast<const uint8_t*>(base) + 1024 * (f0 + f), 16 * x, at);
+        else
+            sp_load16(base, (uint32_t)((r < (int)last ? r : (int)last) * C + x % C) * 16, at);
     }
 }
 
@@ -111,12 +161,24 @@ PE_DEV void sp_clear_rows(uint8_t* vt, int n, int rows, int first, int step) {
         *reinterpret_cast<float4*>(vt + 16 * i) = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
+// A dim's 4 keys from a and 4 from a + STEP, by transposing reads: 16 lanes read 4 keys of 16 dims, 8
+// bytes each, and get one dim's 4 keys each.
+template <int STEP>
+PE_DEV h8v transposed(uint32_t a) {
+    typedef __attribute__((address_space(3))) s4v lds_s4;
+    typedef short s8v __attribute__((ext_vector_type(8)));
+    const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)a);
+    const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(a + STEP));
+    const s8v v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(h8v, v);
+}
+
 // A wave's 32 queries as matrix operands and the products with a tile of 32 keys. One lane: query
 // (or key, or dim) li = lane & 31, half g = lane >> 5. Register r of the scores is key
 // 8 (r / 4) + 4 g + r % 4; they have to be multiplied by `unscale`.
 template <int HD>
 struct RowsF32 {
-    static constexpr float kUp = 0.f, unscale = 1.f;
+    static constexpr float unscale = 1.f;
     float4 q[HD / 8];
     PE_DEV void load(const float* row, float scale, int g) {
 #pragma unroll
@@ -157,7 +219,6 @@ struct RowsF32 {
 
 template <int HD>
 struct RowsF16 {
-    static constexpr float kUp = kLift;
     h8v hi[HD / 16], lo[HD / 16];
     float unscale;
     PE_DEV void load(const float* row, float scale, int g) {
@@ -167,82 +228,93 @@ struct RowsF16 {
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
                 const float4 x = row ? *reinterpret_cast<const float4*>(row + 16 * j + 8 * g + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[8 * j + i] = x.x * scale;
-                v[8 * j + i + 1] = x.y * scale;
-                v[8 * j + i + 2] = x.z * scale;
-                v[8 * j + i + 3] = x.w * scale;
+                v[8 * j + i] = x.x;
+                v[8 * j + i + 1] = x.y;
+                v[8 * j + i + 2] = x.z;
+                v[8 * j + i + 3] = x.w;
             }
 #pragma unroll
         for (int i = 0; i < HD / 2; ++i) top = fmaxf(top, fabsf(v[i]));
         top = swap32_max(top);
-        // 2^(13 - exponent of the largest), within what fp32 holds with its inverse
+        // the row's largest element to 2^13 .. 2^14, within what fp32 holds with its inverse; the scale
+        // of the scores comes after the products
         int e = exponent_of(top);
         e = e < -100 ? -100 : e > 120 ? 120 : e;
-        const float f = exp2_int(13 - e);
-        unscale = exp2_int(e - 13);
+        const float f = copysignf(exp2_int(13 - e), scale);
+        unscale = sp_positive(exp2_int(e - 13) * fabsf(scale));
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = v[8 * j + i] * f;
-                hi[j][i] = (_Float16)x;
-                lo[j][i] = (_Float16)(x - (float)hi[j][i]);
+            for (int i = 0; i < 8; i += 2) {
+                h2v h, l;
+                split2(v[8 * j + i] * f, v[8 * j + i + 1] * f, h, l);
+                hi[j][i] = h.x, hi[j][i + 1] = h.y;
+                lo[j][i] = l.x, lo[j][i + 1] = l.y;
             }
     }
-    // `low`: bytes from a tile to its low parts, 0: it has none
+    // LOW: bytes from a tile to its low parts, 0: it has none. Four operands are in flight: each one's
+    // registers take the fourth next as soon as its products have read them.
     template <int LOW>
     PE_DEV f16v scores(const uint8_t* kt, int li, int g) const {
+        constexpr int J = HD / 16, N = LOW ? 2 * J : J;
+        const uint8_t* at = kt + li * (HD * 2);
+        const int x = (g ^ (li & 7)) * 16;  // chunk 2 j + g: j flips bits above g's
+        const auto operand = [&](int i) { return *reinterpret_cast<const h8v*>(at + (i < J ? 0 : LOW) + (x ^ (32 * (i % J)))); };
+        h8v k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = operand(i);
         f16v s = {};
 #pragma unroll
-        for (int j = 0; j < HD / 16; ++j) {
-            const uint8_t* at = kt + li * (HD * 2) + (((2 * j + g) ^ (li & 7)) * 16);
-            const h8v k = *reinterpret_cast<const h8v*>(at);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, hi[j], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, lo[j], s, 0, 0, 0);
-            if constexpr (LOW) {
-                const h8v l = *reinterpret_cast<const h8v*>(at + LOW);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, hi[j], s, 0, 0, 0);
-            }
+        for (int i = 0; i < N; ++i) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 3], hi[i % J], s, 0, 0, 0);
+            if (i < J) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 3], lo[i % J], s, 0, 0, 0);
+            if (i + 4 < N) k[i & 3] = operand(i + 4);
+            __builtin_amdgcn_sched_barrier(0);
         }
         return s;
     }
-    // a dim's 8 keys of the lane's half, from two transposing reads: 16 lanes read 4 keys of 16 dims,
-    // 8 bytes each, and get one dim's 4 keys each
-    static PE_DEV h8v values(uint32_t a) {
-        typedef __attribute__((address_space(3))) s4v lds_s4;
-        typedef short s8v __attribute__((ext_vector_type(8)));
-        const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)a);
-        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(a + 8 * (HD * 2)));
-        const s8v v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(h8v, v);
+    // operand i of a tile's values: keys 16 (i / D) .., dims 32 (i % D) ..
+    static PE_DEV uint32_t values_at(const uint8_t* vt, int li, int g) {
+        const int i16 = li & 15, key = 4 * g + (i16 >> 2), half = li >> 4;
+        const int c0 = (2 * half + ((i16 >> 1) & 1)) ^ (2 * (key & 3));  // chunk of dims 0 .. 31
+        return lds_address(vt) + key * (HD * 2) + (i16 & 1) * 8 + c0 * 16;
+    }
+    // in the order of use: the dims of the first 16 keys, high and low parts, then of the others
+    template <int LOW>
+    static PE_DEV h8v values_of(uint32_t at, int i) {
+        constexpr int D = HD / 32, P = LOW ? 2 : 1;
+        const int d = i % D, low = i / D % P, b = i / (D * P);
+        return transposed<8 * HD * 2>((at ^ (64 * (d & 1))) + 128 * (d >> 1) + b * 16 * (HD * 2) + low * LOW);
     }
     template <int LOW>
-    static PE_DEV void accumulate(const uint8_t* vt, const f16v& p, f16v* o, int li, int g) {
-        const int i16 = li & 15, key = 4 * g + (i16 >> 2), half = li >> 4;
-        const uint32_t base = lds_address(vt) + key * (HD * 2) + (i16 & 1) * 8;
-        const int c0 = (2 * half + ((i16 >> 1) & 1)) ^ (2 * (key & 3));  // chunk of dims 0 .. 31
+    static PE_DEV void load_values(uint32_t at, h8v* v) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            h8v ph, pl;
+        for (int i = 0; i < 4; ++i) v[i] = values_of<LOW>(at, i);
+    }
+    template <int LOW>
+    static PE_DEV void accumulate(uint32_t at, h8v* v, const f16v& p, f16v* o) {
+        constexpr int D = HD / 32, P = LOW ? 2 : 1, N = 2 * D * P;
+        h8v ph[2], pl[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                ph[i] = (_Float16)p[8 * b + i];
-                pl[i] = (_Float16)(p[8 * b + i] - (float)ph[i]);
-            }
+        for (int i = 0; i < 16; i += 2) {
+            h2v h, l;
+            split2(p[i], p[i + 1], h, l);
+            ph[i >> 3][i & 7] = h.x, ph[i >> 3][(i & 7) + 1] = h.y;
+            pl[i >> 3][i & 7] = l.x, pl[i >> 3][(i & 7) + 1] = l.y;
+        }
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d) {
-                const uint32_t a = base + b * 16 * (HD * 2) + (((4 * (d & 1)) ^ c0) + 8 * (d >> 1)) * 16;
-                const h8v v = values(a);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                if constexpr (LOW) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(a + LOW), ph, o[d], 0, 0, 0);
-            }
+        for (int i = 0; i < N; ++i) {
+            const int d = i % D, low = i / D % P, b = i / (D * P);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 3], ph[b], o[d], 0, 0, 0);
+            if (!low) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 3], pl[b], o[d], 0, 0, 0);
+            if (i + 4 < N) v[i & 3] = values_of<LOW>(at, i + 4);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
 
 // The softmax of a wave's rows so far: o = sum p V, l = sum p (a lane's half) of the probabilities
-// p = exp2(s - r), r the running maximum less `up`.
+// p = exp2(s - r).
 template <int HD>
 struct SpState {
     f16v o[HD / 32];
@@ -258,8 +330,8 @@ struct SpState {
         for (int d = 0; d < HD / 32; ++d) o[d] *= f;
     }
     // scores of a tile, to be multiplied by c[r / 4] (positive) -> its probabilities; keys from n on
-    // are masked
-    PE_DEV void softmax(f16v& s, const float* c, float up, int n, int g) {
+    // are masked; o is multiplied by 2^shift (uniform) besides
+    PE_DEV void softmax(f16v& s, const float* c, int n, int g, int shift = 0) {
         const float NEG_INF = -__builtin_huge_valf();
         if (n < 32) {
 #pragma unroll
@@ -268,20 +340,135 @@ struct SpState {
         }
         float mx = NEG_INF;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) mx = fmaxf(mx, fmaxf(fmaxf(s[i], s[i + 1]), fmaxf(s[i + 2], s[i + 3])) * c[i >> 2]);
+        for (int i = 0; i < 16; i += 4) mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]), s[i + 3]) * c[i >> 2]);
         mx = swap32_max(mx);
-        const float rn = fmaxf(r, mx - up);
-        const float rs = rn == NEG_INF ? 0.f : rn;  // a row none of whose keys came yet
-        const float alpha = __builtin_amdgcn_exp2f(r - rs);
-        if (__any(alpha != 1.f)) {
+        const bool moves = mx > r + kRoom;  // the first finite score does
+        if (__any(moves) || shift) {
+            const float rn = moves ? mx - kUp : r, alpha = moves ? __builtin_amdgcn_exp2f(r - rn) : 1.f;
+            r = rn;
             l *= alpha;
-            scale(alpha);
+            scale(ldexpf(alpha, shift));
         }
-        r = rn;
+        const float rs = r == NEG_INF ? 0.f : r;  // a row none of whose keys came yet
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c[i >> 2], -rs));
             l += s[i];
+        }
+    }
+};
+
+// The own keys of a group: 16 queries and tiles of TK keys, on the 16 x 16 instructions. One lane:
+// query (or key, or dim) qi = lane & 15, quarter h = lane >> 4. Score 4 u + r is key 16 u + 4 h + r.
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+template <typename T, int HD>
+struct OwnRows;
+
+template <int HD>
+struct OwnRows<float, HD> {
+    static constexpr int TK = HD == 64 ? 32 : 16, U = TK / 16;
+    float4 q[HD / 16];
+    static constexpr float unscale = 1.f;
+    PE_DEV void load(const float* row, float scale, int h) {
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) {
+            q[j] = row ? *reinterpret_cast<const float4*>(row + 16 * j + 4 * h) : make_float4(0.f, 0.f, 0.f, 0.f);
+            q[j].x *= scale;
+            q[j].y *= scale;
+            q[j].z *= scale;
+            q[j].w *= scale;
+        }
+    }
+    PE_DEV void scores(const uint8_t* kt, float* out, int qi, int h) const {
+        f4v s[U] = {};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                const float4 k = *reinterpret_cast<const float4*>(kt + (16 * u + qi) * (HD * 4) + (((4 * j + h) ^ (qi & 7)) * 16));
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x, q[j].x, s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.y, q[j].y, s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.z, q[j].z, s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.w, q[j].w, s[u], 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < 4 * U; ++i) out[i] = s[i >> 2][i & 3];
+    }
+    static PE_DEV void accumulate(const uint8_t* vt, const float* p, f4v* o, int qi, int h) {
+#pragma unroll
+        for (int i = 0; i < 4 * U; ++i) {
+            const int row = 16 * (i >> 2) + 4 * h + (i & 3), x = (4 * h + (i & 3)) & 7;
+            const uint8_t* at = vt + row * (HD * 4) + (qi & 3) * 4;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                const int c = ((4 * (d & 1) + (qi >> 2)) ^ x) + 8 * (d >> 1);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float*>(at + 16 * c), p[i], o[d], 0, 0, 0);
+            }
+        }
+    }
+};
+
+template <int HD>
+struct OwnRows<_Float16, HD> {
+    static constexpr int TK = 32, U = 2;
+    h8v hi[HD / 32], lo[HD / 32];
+    float unscale;
+    PE_DEV void load(const float* row, float scale, int h) {
+        float v[HD / 4], top = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 4; i += 4) {
+            const float4 x = row ? *reinterpret_cast<const float4*>(row + 32 * (i / 8) + 8 * h + i % 8) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[i] = x.x;
+            v[i + 1] = x.y;
+            v[i + 2] = x.z;
+            v[i + 3] = x.w;
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(v[i]));
+        top = swap32_max(swap16_max(top));
+        int e = exponent_of(top);
+        e = e < -100 ? -100 : e > 120 ? 120 : e;
+        const float f = copysignf(exp2_int(13 - e), scale);
+        unscale = sp_positive(exp2_int(e - 13) * fabsf(scale));
+#pragma unroll
+        for (int i = 0; i < HD / 4; i += 2) {
+            h2v a, b;
+            split2(v[i] * f, v[i + 1] * f, a, b);
+            hi[i / 8][i % 8] = a.x, hi[i / 8][i % 8 + 1] = a.y;
+            lo[i / 8][i % 8] = b.x, lo[i / 8][i % 8 + 1] = b.y;
+        }
+    }
+    PE_DEV void scores(const uint8_t* kt, float* out, int qi, int h) const {
+        f4v s[U] = {};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                const h8v k = *reinterpret_cast<const h8v*>(kt + (16 * u + qi) * (HD * 2) + (((4 * j + h) ^ (qi & 7)) * 16));
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, hi[j], s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, lo[j], s[u], 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < 4 * U; ++i) out[i] = s[i >> 2][i & 3];
+    }
+    static PE_DEV void accumulate(const uint8_t* vt, const float* p, f4v* o, int qi, int h) {
+        h8v ph, pl;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            h2v a, b;
+            split2(p[i], p[i + 1], a, b);
+            ph[i] = a.x, ph[i + 1] = a.y;
+            pl[i] = b.x, pl[i + 1] = b.y;
+        }
+        const int row = 4 * h + (qi >> 2);  // and 16 on
+        const uint32_t base = lds_address(vt) + row * (HD * 2) + (qi & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+            const int c = ((2 * (d & 3) + ((qi >> 1) & 1)) ^ (2 * (row & 3))) + 8 * (d >> 2);
+            const h8v v = transposed<16 * HD * 2>(base + 16 * c);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[d], 0, 0, 0);
         }
     }
 };
@@ -292,34 +479,39 @@ template <int HD>
 struct SpSplit {
     static constexpr int N = HD / 32, R = 256 / HD, kPlane = kSpBlock * HD * 2;
     float4 k[N], v[N];
-    PE_DEV void load(const float* kb, const float* vb, int64_t row0, int64_t last, int w, int lane) {
+    // the wave's 8 rows of the block that starts at kb and vb, rows behind `last` are that one again
+    PE_DEV void load(const float* kb, const float* vb, int64_t last, int w, int lane) {
+        const bool whole = last >= 8 * w + 7;
 #pragma unroll
         for (int f = 0; f < N; ++f) {
-            int64_t row = row0 + 8 * w + R * f + lane / (HD / 4);
-            row = row < last ? row : last;
-            k[f] = *reinterpret_cast<const float4*>(kb + row * HD + 4 * (lane % (HD / 4)));
-            v[f] = *reinterpret_cast<const float4*>(vb + row * HD + 4 * (lane % (HD / 4)));
+            int at = (8 * w * HD + 256 * f) / 4 + lane;
+            if (!whole) {
+                const int r = 8 * w + R * f + lane / (HD / 4);
+                at = (r < (int)last ? r : (int)last) * (HD / 4) + lane % (HD / 4);
+            }
+            k[f] = reinterpret_cast<const float4*>(kb)[at];
+            v[f] = reinterpret_cast<const float4*>(vb)[at];
         }
     }
     // E, a multiple of 8, with the largest finite element under 2^(15 + E)
     static PE_DEV int exponent(const float4* x) {
         float top = 0.f;
 #pragma unroll
-        for (int f = 0; f < N; ++f)
-            top = fmaxf(fmaxf(fmaxf(top, fabsf(x[f].x)), fmaxf(fabsf(x[f].y), fabsf(x[f].z))), fabsf(x[f].w));
-        top = wave_max<64>(top);
-        if (__float_as_uint(top) >= 0x7F800000u) {  // uniform: the same among the finite ones
+        for (int f = 0; f < N; ++f) {
+            top = fmaxf(fmaxf(top, fabsf(x[f].x)), fabsf(x[f].y));
+            top = fmaxf(fmaxf(top, fabsf(x[f].z)), fabsf(x[f].w));
+        }
+        uint32_t bits = wave_max_bits(__float_as_uint(top));
+        if (bits >= 0x7F800000u) {  // infinities: the largest of the others (x + 0 x is NaN for those)
             top = 0.f;
 #pragma unroll
             for (int f = 0; f < N; ++f) {
-                const float e[4] = {fabsf(x[f].x), fabsf(x[f].y), fabsf(x[f].z), fabsf(x[f].w)};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (__float_as_uint(e[i]) < 0x7F800000u) top = fmaxf(top, e[i]);
+                top = fmaxf(fmaxf(top, fabsf(fmaf(x[f].x, 0.f, x[f].x))), fabsf(fmaf(x[f].y, 0.f, x[f].y)));
+                top = fmaxf(fmaxf(top, fabsf(fmaf(x[f].z, 0.f, x[f].z))), fabsf(fmaf(x[f].w, 0.f, x[f].w)));
             }
-            top = wave_max<64>(top);
+            bits = wave_max_bits(__float_as_uint(top));
         }
-        const int e = exponent_of(top);
+        const int e = (int)(bits >> 23) - 127;
         return ((e < -100 ? -100 : e) - 14 + 7) >> 3 << 3;
     }
     template <bool VALUES>
@@ -327,13 +519,10 @@ struct SpSplit {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = 8 * w + R * i + lane / (HD / 4), c4 = lane % (HD / 4);
-            const float y[4] = {x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f};
-            h4v hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                hi[e] = (_Float16)y[e];
-                lo[e] = (_Float16)(y[e] - (float)hi[e]);
-            }
+            h2v h0, l0, h1, l1;
+            split2(x[i].x * f, x[i].y * f, h0, l0);
+            split2(x[i].z * f, x[i].w * f, h1, l1);
+            const h4v hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
             uint8_t* at = plane + row * (HD * 2) + ((c4 >> 1) ^ sp_swizzle<2, VALUES>(row)) * 16 + (c4 & 1) * 8;
             *reinterpret_cast<h4v*>(at) = hi;
             *reinterpret_cast<h4v*>(at + kPlane) = lo;
@@ -356,6 +545,154 @@ struct SpSplit {
         }
     }
 };
+
+// What a workgroup's waves exchange at the end: the rows of their items ([query][dim]) over the tiles,
+// and per query its reference, sum and output row.
+struct SpShared {
+    uint8_t* lds;
+    float (*ref)[32];
+    float (*sum)[32];
+    int (*row)[32];
+};
+
+// The record of a wave's Q queries (lane = query + Q part; v[i]: dims 256 / Q i + 4 part ..): stored, or
+// merged with those of the item's other waves (sub of split; the waves first, first + step, ..) in LDS.
+template <int HD, int Q>
+PE_DEV void sp_finish(const SpArgs& p, const SpShared& m, float4* v, float r, float l, int my_row, bool works, int live, int chunk,
+                      int item, int sub, int split, int step) {
+    constexpr int W = 256 / Q, N = HD / W, OS = HD + 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qi = lane % Q, at = 4 * (lane / Q);
+    const int chunks = p.p_chunks + p.o_chunks;
+    live = live < Q ? live : Q;
+    if (split == 1) {  // uniform
+        if (works && qi < live) {
+            const int64_t rec = (int64_t)my_row * chunks + chunk;
+#pragma unroll
+            for (int i = 0; i < N; ++i) store_record(p.rec + rec * HD + W * i + at, v[i]);
+            if (at == 0) *reinterpret_cast<float2*>(p.ml + rec * 2) = make_float2(r, l);
+        }
+        return;
+    }
+    if (at == 0) m.ref[w][qi] = r;
+    __syncthreads();  // and the tiles are no longer read
+    const int first = step > 1 ? item : item * split;
+    float most = m.ref[first][qi];
+    for (int s = 1; s < split; ++s) most = fmaxf(most, m.ref[first + step * s][qi]);
+    const float f = __builtin_amdgcn_exp2f(r - (most == -__builtin_huge_valf() ? 0.f : most));
+    float* const po = reinterpret_cast<float*>(m.lds) + (w * Q + qi) * OS + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<float4*>(po + W * i) = make_float4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f);
+    if (at == 0) {
+        m.sum[w][qi] = l * f;
+        m.row[w][qi] = my_row;
+    }
+    __syncthreads();
+    if (!works) return;
+    // every wave of the item takes its share of the rows
+    if (sub == 0 && lane < live) {
+        float sum = m.sum[first][lane];
+        for (int s = 1; s < split; ++s) sum += m.sum[first + step * s][lane];
+        *reinterpret_cast<float2*>(p.ml + ((int64_t)my_row * chunks + chunk) * 2) = make_float2(most, sum);
+    }
+    const float* const p0 = reinterpret_cast<float*>(m.lds) + first * Q * OS;
+#pragma unroll 2
+    for (int it = 64 * sub + lane; it < live * (HD / 4); it += 64 * split) {
+        const int row = it / (HD / 4), c = it % (HD / 4);
+        const float* o = p0 + row * OS + 4 * c;
+        float4 x = *reinterpret_cast<const float4*>(o);
+        for (int s = 1; s < split; ++s) {
+            const float4 y = *reinterpret_cast<const float4*>(o + s * step * Q * OS);
+            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+        store_record(p.rec + ((int64_t)m.row[first][row] * chunks + chunk) * HD + 4 * c, x);
+    }
+}
+
+// The own keys of a group, by the waves of a workgroup: items of split waves each.
+template <typename T, int HD>
+PE_DEV void sp_own(const SpArgs& p, const SpShared& m, int block) {
+    typedef OwnRows<T, HD> Rows;
+    constexpr int TK = Rows::TK, N = 4 * Rows::U, kTile = TK * HD * (int)sizeof(T), kPieces = kTile / 1024;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qi = lane & 15, h = lane >> 4;
+    const int split = p.o_split, item = w / split, sub = w % split;
+    int at = block * (kSpWaves / split) + item;
+    const bool live = at < p.o_items;
+    at = live ? at : 0;
+    const int per = p.batch * p.n_kv * p.o_tiles, chunk = at / per;
+    at -= chunk * per;
+    const int tile = at % p.o_tiles, j = at / p.o_tiles % p.n_kv, b = at / p.o_tiles / p.n_kv;
+    const int64_t len = live ? sp_length(p.o_len, p.o_dtype, b, p.o_add, p.o_cap) : 0, k0 = (int64_t)chunk * p.o_keys;
+    const int keys = len <= k0 ? 0 : len - k0 < p.o_keys ? (int)(len - k0) : p.o_keys;
+    const int64_t first = (((int64_t)b * p.n_kv + j) * p.o_cap + k0) * HD;
+    const T *kb = static_cast<const T*>(p.ko) + first, *vb = static_cast<const T*>(p.vo) + first;
+    const int row0 = 16 * tile, my_row = b * p.n_head + j * p.group + row0 + qi, tiles = (keys + TK - 1) / TK;
+    uint8_t *const kt = m.lds + w * 2 * kTile, *const vt = kt + kTile;
+    const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
+    const auto stage_k = [&](int t) { sp_stage<T, HD, false, kPieces>(kb + (int64_t)t * TK * HD, keys - 1 - t * TK, kt_a, lane, 0); };
+    const auto stage_v = [&](int t) { sp_stage<T, HD, true, kPieces>(vb + (int64_t)t * TK * HD, keys - 1 - t * TK, vt_a, lane, 0); };
+    if (sub < tiles) {
+        stage_k(sub);
+        stage_v(sub);
+    }
+    Rows q;
+    q.load(keys > 0 && row0 + qi < p.group ? p.q + (int64_t)my_row * HD : nullptr, p.scale, h);
+    const float NEG_INF = -__builtin_huge_valf();
+    float r = NEG_INF, l = 0.f;
+    f4v o[HD / 16] = {};
+    for (int t = sub; t < tiles; t += split) {
+        const bool more = t + split < tiles;
+        // K is there, V may be in flight (the first time the queries' loads are behind both)
+        if (t == sub)
+            sp_wait_loads<0>();
+        else
+            sp_wait_loads<kPieces>();
+        float s[N];
+        q.scores(kt, s, qi, h);
+        sp_wait_lds();
+        if (more) stage_k(t + split);
+        const int n = keys - t * TK;
+        if (n < TK) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (16 * (i >> 2) + 4 * h + (i & 3) >= n) s[i] = NEG_INF;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
+        mx = swap32_max(swap16_max(mx)) * q.unscale;
+        const bool moves = mx > r + kRoom;
+        if (__any(moves)) {
+            const float rn = moves ? mx - kUp : r, alpha = moves ? __builtin_amdgcn_exp2f(r - rn) : 1.f;
+            r = rn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+        }
+        const float rs = r == NEG_INF ? 0.f : r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.unscale, -rs));
+            l += s[i];
+        }
+        if (more)
+            sp_wait_loads<kPieces>();  // V is there, the next K may be in flight
+        else
+            sp_wait_loads<0>();
+        if (n < TK) {
+            sp_clear_rows<HD * (int)sizeof(T)>(vt, n, TK, lane, 64);
+            sp_wait_lds();
+        }
+        Rows::accumulate(vt, s, o, qi, h);
+        sp_wait_lds();
+        if (more) stage_v(t + split);
+    }
+    const float down = exp2_int(-(int)kUp);
+    float4 v[HD / 16];
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) v[d] = make_float4(o[d][0] * down, o[d][1] * down, o[d][2] * down, o[d][3] * down);
+    l = swap32_sum(swap16_sum(l)) * down;
+    sp_finish<HD, 16>(p, m, v, r + kUp, l, my_row, keys > 0, p.group - row0, p.p_chunks + chunk, item, sub, split, 1);
+}
 
 // The rows of a solo item: fp32 caches on the fp32 matrix instructions.
 template <typename T, int HD>
@@ -380,126 +717,98 @@ PE_DEV void sp_accumulate(const RowsF32<HD>&, const uint8_t* vt, const f16v& s, 
 }
 template <int HD>
 PE_DEV void sp_accumulate(const RowsF16<HD>&, const uint8_t* vt, const f16v& s, f16v* o, int li, int g) {
-    RowsF16<HD>::template accumulate<0>(vt, s, o, li, g);
+    const uint32_t va = RowsF16<HD>::values_at(vt, li, g);
+    h8v v[4];
+    RowsF16<HD>::template load_values<0>(va, v);
+    RowsF16<HD>::template accumulate<0>(va, v, s, o);
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     constexpr bool kHalf = sizeof(T) == 2;
-    constexpr int kTile = 32 * HD * (int)sizeof(T), kPieces = kTile / 1024, D = HD / 32, OS = HD + 4;
+    constexpr int kTile = 32 * HD * (int)sizeof(T), kPieces = kTile / 1024;
     // solo: a K and a V tile per wave, or one buffer for both in turn where two are over 16 KB
     constexpr bool kOne = kTile > 8192;
     constexpr int kWaveLds = kOne ? kTile : 2 * kTile;
     // shared: two buffers of a block's planes
     constexpr int kPlane = kSpBlock * HD * 2, kPlanes = (kHalf ? 2 : 4) * kPlane, kLow = kHalf ? 0 : kPlane;
-    constexpr int kMerge = kSpWaves * 32 * OS * 4;
+    constexpr int kMerge = kSpWaves * 32 * (HD + 4) * 4;
     constexpr int kSolo = kSpWaves * kWaveLds, kMost = kSolo > 2 * kPlanes ? kSolo : 2 * kPlanes;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kMost > kMerge ? kMost : kMerge];
-    __shared__ float part[kSpWaves][2][32];
-    __shared__ int exps[2][16];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 5, li = lane & 31;
+    __shared__ float ref[kSpWaves][32], sums[kSpWaves][32];
+    __shared__ int exps[2][16], row_of[kSpWaves][32];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, li = lane & 31;
 
-    // The wave's item: which rows, which keys [k0, k1) of which cache.
-    const bool prefix = (int)blockIdx.x < p.p_blocks, shared = prefix && p.shared;
-    const int split = prefix ? (shared ? 2 : kSpWaves) : p.o_split;  // waves that share an item
-    const int item = shared ? w & 3 : w / split, sub = shared ? w >> 2 : w % split;
-    const T *kb = nullptr, *vb = nullptr;
-    int64_t k0 = 0, k1 = 0, row_base;  // output row of r: row_base + r, or by sequence
-    int chunk, row0, rows;
-    if (prefix) {
-        const int kc = p.n_kv * p.p_chunks, tile = blockIdx.x / kc, at = blockIdx.x - tile * kc, j = at % p.n_kv;
-        chunk = at / p.n_kv;
-        const int64_t len = sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
-        k0 = (int64_t)chunk * p.p_keys;
-        k1 = k0 + p.p_keys < len ? k0 + p.p_keys : len;
-        kb = static_cast<const T*>(p.kp) + (int64_t)j * p.p_cap * HD;
-        vb = static_cast<const T*>(p.vp) + (int64_t)j * p.p_cap * HD;
-        row0 = shared ? 128 * tile + 32 * item : 32 * tile;
-        rows = p.batch * p.group;
-        row_base = (int64_t)j * p.group;
-        if (k1 <= k0) return;  // the whole workgroup: a chunk past the length
-    } else {
-        int at = (blockIdx.x - p.p_blocks) * (kSpWaves / split) + item;
-        const bool live = at < p.o_items;
-        at = live ? at : 0;
-        const int per = p.batch * p.n_kv * p.o_tiles;
-        chunk = at / per;
-        at -= chunk * per;
-        const int tile = at % p.o_tiles, j = at / p.o_tiles % p.n_kv, b = at / p.o_tiles / p.n_kv;
-        const int64_t len = live ? sp_length(p.o_len, p.o_dtype, b, p.o_add, p.o_cap) : 0;
-        k0 = (int64_t)chunk * p.o_keys;
-        k1 = k0 + p.o_keys < len ? k0 + p.o_keys : len;
-        kb = static_cast<const T*>(p.ko) + ((int64_t)b * p.n_kv + j) * p.o_cap * HD;
-        vb = static_cast<const T*>(p.vo) + ((int64_t)b * p.n_kv + j) * p.o_cap * HD;
-        row0 = 32 * tile;
-        rows = p.group;
-        row_base = (int64_t)b * p.n_head + j * p.group;
-        chunk += p.p_chunks;
-    }
-    const auto out_row = [&](int64_t base, int r) {
-        if (!prefix) return base + r;
-        const int b = r / p.group;
-        return base + (int64_t)b * p.n_head + (r - b * p.group);
-    };
-    const int keys = k1 > k0 ? (int)(k1 - k0) : 0;
+    const SpShared m{lds, ref, sums, row_of};
+    if ((int)blockIdx.x >= p.p_blocks) return sp_own<T, HD>(p, m, blockIdx.x - p.p_blocks);
+
+    // The wave's rows and the keys [k0, k1).
+    const bool shared = p.shared;
+    const int split = shared ? 2 : kSpWaves;  // waves that share rows
+    const int item = shared ? w & 3 : 0, sub = shared ? w >> 2 : w;
+    const int kc = p.n_kv * p.p_chunks, tile = blockIdx.x / kc, at = blockIdx.x - tile * kc, j = at % p.n_kv, chunk = at / p.n_kv;
+    const int64_t len = sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
+    const int64_t k0 = (int64_t)chunk * p.p_keys, k1 = k0 + p.p_keys < len ? k0 + p.p_keys : len;
+    if (k1 <= k0) return;  // the whole workgroup: a chunk past the length
+    const T* kb = static_cast<const T*>(p.kp) + (int64_t)j * p.p_cap * HD;
+    const T* vb = static_cast<const T*>(p.vp) + (int64_t)j * p.p_cap * HD;
+    const int row0 = shared ? 128 * tile + 32 * item : 32 * tile, rows = p.batch * p.group;
+    const int keys = (int)(k1 - k0);
     const int64_t last = k1 - 1;
-    const int chunks = p.p_chunks + p.o_chunks;
-    const bool works = keys > 0 && row0 < rows;
-    const float* qrow = works && row0 + li < rows ? p.q + out_row(row_base, row0 + li) * HD : nullptr;
+    const bool works = row0 < rows;
+    // the lane's query: row r of the kv head is (sequence r / group, head r % group of the kv head's)
+    const int seq = (row0 + li) / p.group;
+    const int my_row = seq * p.n_head + j * p.group + (row0 + li - seq * p.group);
+    const float* qrow = row0 + li < rows ? p.q + (int64_t)my_row * HD : nullptr;
     SpState<HD> st;
     st.clear();
-    float up = kLift;
     int top = 0;  // exponent of the values that o holds
 
     if (shared) {
         RowsF16<HD> q;
-        q.load(qrow, p.scale, g);
         const int blocks = (keys + kSpBlock - 1) / kSpBlock;
         const auto take = [&](int t) {
             const uint8_t* kt = lds + (t & 1) * kPlanes + 32 * sub * (HD * 2);
-            const int left = keys - kSpBlock * t - 32 * sub, n = left < 32 ? left : 32;
-            if (!works || n <= 0) return;
+            // no branch round waves without rows or keys: o would be copied on every way
+            const int n = keys - kSpBlock * t - 32 * sub;
             f16v s = q.template scores<kLow>(kt, li, g);
             float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
-            float vs[4] = {1.f, 1.f, 1.f, 1.f};
-            bool same = true;
+            int ev[4], shift = 0;
             if constexpr (!kHalf) {
                 const int* e = exps[t & 1] + 4 * sub;
-                int ev[4], t2 = t ? top : -128;
+                int most = t ? top : -128;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // no smaller than fp32's least: a masked score times c stays -inf
-                    c[i] = fminf(fmaxf(ldexpf(c[i], e[i]), 1.1754943508222875e-38f), 1.7014118346046923e38f);
-                    ev[i] = e[8 + i];
-                    t2 = ev[i] > t2 ? ev[i] : t2;
+                    c[i] = sp_positive(ldexpf(c[i], e[i]));
+                    ev[i] = __builtin_amdgcn_readfirstlane(e[8 + i]);
+                    most = ev[i] > most ? ev[i] : most;
                 }
-                t2 = __builtin_amdgcn_readfirstlane(t2);
-                if (t && t2 != top) st.scale(ldexpf(1.f, top - t2));
-                top = t2;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vs[i] = ldexpf(1.f, ev[i] - top);
-                    same = same && ev[i] == top;
-                }
+                shift = t ? top - most : 0;
+                top = most;
             }
-            st.softmax(s, c, kLift, n, g);
+            const uint32_t va = RowsF16<HD>::values_at(kt + (kHalf ? 1 : 2) * kPlane, li, g);
+            h8v v[4];
+            RowsF16<HD>::template load_values<kLow>(va, v);
+            __builtin_amdgcn_sched_barrier(0);
+            st.softmax(s, c, n, g, shift);
             if constexpr (!kHalf) {
-                if (!same) {
+                if (ev[0] != top || ev[1] != top || ev[2] != top || ev[3] != top) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] *= vs[i >> 2];
+                    for (int i = 0; i < 16; ++i) s[i] *= ldexpf(1.f, ev[i >> 2] - top);
                 }
             }
-            RowsF16<HD>::template accumulate<kLow>(kt + (kHalf ? 1 : 2) * kPlane, s, st.o, li, g);
+            RowsF16<HD>::template accumulate<kLow>(va, v, s, st.o);
         };
         if constexpr (kHalf) {
             constexpr int N = kPlane / 1024 / kSpWaves;
             const auto stage = [&](int t) {
                 const uint32_t at = lds_address(lds) + (t & 1) * kPlanes;
-                sp_stage<T, HD, false, N>(kb, k0 + kSpBlock * t, last, at, lane, w * N);
-                sp_stage<T, HD, true, N>(vb, k0 + kSpBlock * t, last, at + kPlane, lane, w * N);
+                const int64_t row = k0 + kSpBlock * t;
+                sp_stage<T, HD, false, N>(kb + row * HD, last - row, at, lane, w * N);
+                sp_stage<T, HD, true, N>(vb + row * HD, last - row, at + kPlane, lane, w * N);
             };
-            sp_wait_loads<0>();
             stage(0);
+            q.load(qrow, p.scale, g);
             for (int t = 0; t < blocks; ++t) {
                 sp_wait_loads<0>();
                 __syncthreads();  // the block is there, and nobody reads the other buffer any more
@@ -513,15 +822,20 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
             }
         } else {
             SpSplit<HD> x;
+            const auto load = [&](int t) {
+                const int64_t row = k0 + kSpBlock * t;
+                x.load(kb + row * HD, vb + row * HD, last - row, w, lane);
+            };
             const auto convert = [&](int t) {
                 const int n = keys - kSpBlock * t;
                 x.convert(lds + (t & 1) * kPlanes, exps[t & 1], n < kSpBlock ? n : kSpBlock, w, lane);
-                if (t + 1 < blocks) x.load(kb, vb, k0 + kSpBlock * (t + 1), last, w, lane);
+                if (t + 1 < blocks) load(t + 1);
             };
-            x.load(kb, vb, k0, last, w, lane);
+            load(0);
+            q.load(qrow, p.scale, g);
             convert(0);
             for (int t = 0; t < blocks; ++t) {
-                __syncthreads();  // the block is there, and nobody reads the other buffer any more
+                __syncthreads();  // block t is there, and nobody reads the other buffer any more
                 // half of the waves split the next block while the others are at their products
                 if (sub == 0 && t + 1 < blocks) convert(t + 1);
                 take(t);
@@ -530,7 +844,6 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
         }
     } else {
         typename SpPick<T, HD>::type q;
-        up = q.kUp;
         q.load(qrow, p.scale, g);
         const int tiles = works ? (keys + 31) / 32 : 0;
         uint8_t* const kt = lds + w * kWaveLds;
@@ -538,22 +851,29 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
         const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
         const float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
         sp_wait_loads<0>();
+        const auto stage_k = [&](int t) {
+            const int64_t row = k0 + 32 * t;
+            sp_stage<T, HD, false, kPieces>(kb + row * HD, last - row, kt_a, lane, 0);
+        };
+        const auto stage_v = [&](int t) {
+            const int64_t row = k0 + 32 * t;
+            sp_stage<T, HD, true, kPieces>(vb + row * HD, last - row, vt_a, lane, 0);
+        };
         if (sub < tiles) {
-            sp_stage<T, HD, false, kPieces>(kb, k0 + 32 * sub, last, kt_a, lane, 0);
-            if (!kOne) sp_stage<T, HD, true, kPieces>(vb, k0 + 32 * sub, last, vt_a, lane, 0);
+            stage_k(sub);
+            if (!kOne) stage_v(sub);
         }
         for (int t = sub; t < tiles; t += split) {
             const bool more = t + split < tiles;
-            const int64_t next = k0 + 32 * (t + split);
             sp_wait_loads<kOne ? 0 : kPieces>();  // K is there, V may be in flight
             f16v s = sp_scores(q, kt, li, g);
             sp_wait_lds();
             if (kOne)
-                sp_stage<T, HD, true, kPieces>(vb, k0 + 32 * t, last, vt_a, lane, 0);
+                stage_v(t);
             else if (more)
-                sp_stage<T, HD, false, kPieces>(kb, next, last, kt_a, lane, 0);
+                stage_k(t + split);
             const int n = keys - 32 * t < 32 ? keys - 32 * t : 32;
-            st.softmax(s, c, q.kUp, n, g);
+            st.softmax(s, c, n, g);
             if (!kOne && more)
                 sp_wait_loads<kPieces>();  // V is there, the next K may be in flight
             else
@@ -566,66 +886,21 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
             sp_wait_lds();
             if (more) {
                 if (kOne)
-                    sp_stage<T, HD, false, kPieces>(kb, next, last, kt_a, lane, 0);
+                    stage_k(t + split);
                 else
-                    sp_stage<T, HD, true, kPieces>(vb, next, last, vt_a, lane, 0);
+                    stage_v(t + split);
             }
         }
     }
 
-    // The records, probabilities and values without their factors. Waves that share an item leave
-    // theirs in LDS ([query][dim]) and merge.
-    const float down = exp2_int(-(int)up), vscale = ldexpf(down, top);
-    const float l = swap32_sum(st.l) * down, r = st.r + up;
-    st.scale(vscale);
-    if (split == 1) {  // uniform
-        if (works && row0 + li < rows) {
-            const int64_t at = out_row(row_base, row0 + li) * chunks + chunk;
+    // the records, probabilities and values without their factors
+    const float down = exp2_int(-(int)kUp);
+    st.scale(ldexpf(down, top));
+    float4 v[HD / 8];
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4*>(p.rec + at * HD + 32 * d + 8 * (i >> 2) + 4 * g) =
-                        make_float4(st.o[d][i], st.o[d][i + 1], st.o[d][i + 2], st.o[d][i + 3]);
-            if (g == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(r, l);
-        }
-        return;
-    }
-    __syncthreads();  // the tiles are no longer read
-    float* const po = reinterpret_cast<float*>(lds) + w * 32 * OS;
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(po + li * OS + 32 * d + 8 * (i >> 2) + 4 * g) =
-                make_float4(st.o[d][i], st.o[d][i + 1], st.o[d][i + 2], st.o[d][i + 3]);
-    if (g == 0) {
-        part[w][0][li] = r;
-        part[w][1][li] = l;
-    }
-    __syncthreads();
-    // the item's waves take its rows; wave `first + step s` holds part s
-    const int first = shared ? item : item * split, step = shared ? 4 : 1;
-    if (!works) return;
-    const int live = rows - row0 < 32 ? rows - row0 : 32;
-    for (int it = 64 * sub + lane; it < live * (HD / 4); it += 64 * split) {
-        const int qi = it / (HD / 4), c = it % (HD / 4);
-        float most = -__builtin_huge_valf();
-        for (int s = 0; s < split; ++s) most = fmaxf(most, part[first + step * s][0][qi]);
-        const float rs = most == -__builtin_huge_valf() ? 0.f : most;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-        for (int s = 0; s < split; ++s) {
-            const int ws = first + step * s;
-            const float f = __builtin_amdgcn_exp2f(part[ws][0][qi] - rs);
-            sum = fmaf(f, part[ws][1][qi], sum);
-            const float4 o = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(lds) + (ws * 32 + qi) * OS + 4 * c);
-            v = make_float4(fmaf(f, o.x, v.x), fmaf(f, o.y, v.y), fmaf(f, o.z, v.z), fmaf(f, o.w, v.w));
-        }
-        const int64_t at = out_row(row_base, row0 + qi) * chunks + chunk;
-        *reinterpret_cast<float4*>(p.rec + at * HD + 4 * c) = v;
-        if (c == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(most, sum);
-    }
+    for (int i = 0; i < HD / 8; ++i)
+        v[i] = make_float4(st.o[i >> 2][4 * (i & 3)], st.o[i >> 2][4 * (i & 3) + 1], st.o[i >> 2][4 * (i & 3) + 2], st.o[i >> 2][4 * (i & 3) + 3]);
+    sp_finish<HD, 32>(p, m, v, st.r + kUp, swap32_sum(st.l) * down, my_row, works, rows - row0, chunk, item, sub, split, shared ? 4 : 1);
 }
 
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
@@ -636,15 +911,15 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     __shared__ float4 rows[4][L];
     __shared__ float sums[4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
-    if (row >= (int64_t)p.batch * p.n_head) return;  // W == 1 only, uniform per wave
-    const int64_t b = row / p.n_head;
+    const int row = __builtin_amdgcn_readfirstlane(W == 1 ? blockIdx.x * 4 + w : blockIdx.x);
+    if (row >= p.batch * p.n_head) return;  // W == 1 only, uniform per wave
+    // lengths are at most 2^30
     const int64_t pl = sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
-    const int64_t ol = sp_length(p.o_len, p.o_dtype, b, p.o_add, p.o_cap);
-    const int np = pl > 0 ? (int)((pl + p.p_keys - 1) / p.p_keys) : 0;
-    const int no = ol > 0 ? (int)((ol + p.o_keys - 1) / p.o_keys) : 0;
+    const int64_t ol = sp_length(p.o_len, p.o_dtype, row / p.n_head, p.o_add, p.o_cap);
+    const int np = pl > 0 ? (int)((uint32_t)(pl + p.p_keys - 1) / (uint32_t)p.p_keys) : 0;
+    const int no = ol > 0 ? (int)((uint32_t)(ol + p.o_keys - 1) / (uint32_t)p.o_keys) : 0;
     const int n = ol < 0 ? 0 : np + no;  // a sequence that takes no part: zeros
-    const int64_t at = row * (p.p_chunks + p.o_chunks);
+    const int64_t at = (int64_t)row * (p.p_chunks + p.o_chunks);
     const auto record = [&](int i) { return at + (i < np ? i : p.p_chunks + i - np); };
     const float NEG_INF = -__builtin_huge_valf();
     float top = NEG_INF;
@@ -696,36 +971,46 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     if (lane >= L) return;
     float4 y = n ? make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum) : v;
     if (p.round_fp16) y = make_float4(round_to_f16(y.x), round_to_f16(y.y), round_to_f16(y.z), round_to_f16(y.w));
-    *reinterpret_cast<float4*>(p.out + row * HD + 4 * lane) = y;
+    *reinterpret_cast<float4*>(p.out + (int64_t)row * HD + 4 * lane) = y;
 }
 
 struct SpPlan {
     int shared, p_chunks, p_keys, p_tiles, o_chunks, o_keys, o_tiles, o_split;
 };
 
-// How the work is cut. Rows of a kv head over 64 go the shared way. The chip holds about 256
-// workgroups of eight waves: the prefix is cut into as many chunks as that takes, the own keys into
-// items of one to eight waves.
-static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int64_t p_keys, int64_t o_cap) {
+// How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup, so the
+// launch is made of about 256 that take equally long: the own keys' items of one to eight waves
+// first, then as many chunks of the prefix as fill the rest in proportion to its share of the work.
+// Times (us, head size 128; measured): a workgroup's start, end and records 10; a shared block of
+// 64 keys 1.8 with 16-bit caches, 3.5 with fp32 ones; a wave's solo tile 1.2 and 7.
+static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, int64_t p_keys, int64_t o_cap) {
     SpPlan s;
     const int64_t group = n_head / n_kv, rows = batch * group;
     s.shared = rows > 64;
     s.p_tiles = (int)(s.shared ? (rows + 127) / 128 : (rows + 31) / 32);
-    s.o_tiles = (int)((group + 31) / 32);
+    s.o_tiles = (int)((group + 15) / 16);
     const auto cut = [](int64_t keys, int64_t want, int64_t step, int& chunks, int& per) {
-        int64_t k = (keys + want - 1) / want;
+        int64_t k = (keys + want - 1) / (want < 1 ? 1 : want);
         k = (k + step - 1) / step * step;
         k = k < step ? step : k;
         per = (int)k;
         chunks = (int)((keys + k - 1) / k);
     };
-    int64_t want = 256 / (n_kv * (int64_t)s.p_tiles);
-    cut(p_keys, want < 1 ? 1 : want, s.shared ? kSpBlock : 32 * kSpWaves, s.p_chunks, s.p_keys);
     const int64_t pairs = batch * n_kv * s.o_tiles, tiles = (o_cap + 31) / 32;
     s.o_split = 1;
-    while (s.o_split < kSpWaves && s.o_split < tiles && pairs * s.o_split < 2048) s.o_split *= 2;
-    want = 2048 / (pairs * s.o_split);
+    while (s.o_split < kSpWaves && s.o_split < tiles && pairs * s.o_split < 1024) s.o_split *= 2;
+    int64_t want = 1024 / (pairs * s.o_split);
     cut(o_cap, want < 1 ? 1 : want, 32 * s.o_split, s.o_chunks, s.o_keys);
+    const double each = hd / 128.0, t_block = (half ? 1.8 : 3.5) * each, t_tile = (half ? 1.2 : 7.0) * each;
+    const int64_t items = pairs * s.o_chunks, o_blocks = (items + kSpWaves / s.o_split - 1) / (kSpWaves / s.o_split);
+    const double own = o_blocks * (10.0 + t_tile * (s.o_keys / (32 * s.o_split)));
+    const int64_t per_chunk = (int64_t)n_kv * s.p_tiles;
+    const int64_t steps = s.shared ? (p_keys + kSpBlock - 1) / kSpBlock : (p_keys + 255) / 256;
+    const double prefix = (double)per_chunk * steps * (s.shared ? t_block : t_tile);
+    // own workgroups that fit beside a chunk's are left room for
+    const double room = o_blocks < 128 ? 256 - o_blocks : 256 * (prefix + 2560) / (prefix + 2560 + own);
+    want = (int64_t)(room / per_chunk);
+    cut(p_keys, want < 1 ? 1 : want, s.shared ? kSpBlock : 32 * kSpWaves, s.p_chunks, s.p_keys);
     return s;
 }
 
@@ -757,7 +1042,11 @@ using namespace pe;
 extern "C" int64_t pe_shared_prefix_attn_workspace_bytes(int64_t batch, int n_head, int n_kv, int head_dim,
                                                          int64_t prefix_keys, int64_t own_capacity) {
     if (!sp_shape_ok(batch, n_head, n_kv, head_dim, prefix_keys, own_capacity)) return -PE_ERR_SHAPE;
-    return sp_bytes(sp_plan(batch, n_head, n_kv, prefix_keys, own_capacity), batch, n_head, head_dim);
+    // of either type of cache
+    const SpPlan a = sp_plan(batch, n_head, n_kv, head_dim, false, prefix_keys, own_capacity);
+    const SpPlan b = sp_plan(batch, n_head, n_kv, head_dim, true, prefix_keys, own_capacity);
+    const int64_t x = sp_bytes(a, batch, n_head, head_dim), y = sp_bytes(b, batch, n_head, head_dim);
+    return x > y ? x : y;
 }
 
 extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t stream) {
@@ -774,7 +1063,8 @@ extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t
         keys = a->prefix_len_add < keys ? a->prefix_len_add : keys;
         if (keys < 0) keys = 0;
     }
-    const SpPlan s = sp_plan(a->batch, a->n_head, a->n_kv, keys, a->own_capacity);
+    const SpPlan s = sp_plan(a->batch, a->n_head, a->n_kv, a->head_dim, a->cache_type == PE_TYPE_F16, keys,
+                             a->own_capacity);
     const int64_t need = sp_bytes(s, a->batch, a->n_head, a->head_dim);
     if (!a->q || !a->out || (keys && (!a->k_prefix || !a->v_prefix)) ||
         (a->own_capacity && (!a->k_own || !a->v_own)) || (a->prefix_len_dtype && !a->prefix_len) ||
