@@ -5,9 +5,11 @@
 //
 // A workgroup takes one segment of one row's vocabulary: it counts the segment's tokens of the
 // history and the prompt in LDS (whole-number additions, so their order does not matter), while its
-// logits are on their way, and stores the segment. One launch, nothing kept between calls; bound by
-// reading and writing the logits once, or by latency for a row or two. The histories are read by
-// every segment of their row: they are short beside the vocabulary and come from L2.
+// logits are on their way, and stores the segment. One launch, nothing kept between calls. Bound by
+// reading and writing the logits once (256 rows of 151643 fp16 from memory: 38 us, 4.1 TB/s), by latency
+// for a row or two (3.6 us), and where the ids are many by looking through them: every segment of a row
+// reads all of them (from L2), a few 32-bit instructions each (24 rows of 152064 with 4000 + 770 ids: 9 us,
+// 5 without; 8 rows with 30000: 14). Compared as 64-bit integers the ids cost twice as much.
 #include "pe_common.h"
 
 namespace pe {
@@ -44,25 +46,55 @@ PE_DEV int64_t id_at(const void* ids, int wide, int64_t i) {
     return wide ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int*>(ids)[i];
 }
 
-// Adds to, or marks, the counters of the ids in [v0, v0 + seg).
-template <bool MARK>
-PE_DEV void count_ids(uint32_t* count, const void* ids, int wide, int64_t at, int64_t n, int64_t v0, int seg) {
-    constexpr int U = 4;  // loads in flight per thread
-    for (int64_t i = threadIdx.x; i < n; i += 256 * U) {
-        int64_t id[U];
+// Adds to, or marks, the counters of the ids in [v0, v0 + seg): two ids a load, four of them in flight.
+// An id under 0 has a high word, or is over every segment.
+template <bool MARK, typename I>
+PE_DEV void count_ids(uint32_t* count, const I* ids, int64_t n, uint32_t v0, uint32_t seg) {
+    constexpr int U = 4;
+    typedef typename Loose<I, 2>::type pair;
+    const auto one = [&](I id) {
+        const uint32_t o = (uint32_t)id - v0;
+        if (o >= seg || (sizeof(I) == 8 && (uint64_t)id >> 32)) return;
+        if constexpr (MARK)
+            atomicOr(&count[o], kInPrompt);
+        else
+            atomicAdd(&count[o], 1u);
+    };
+    int64_t i = 2 * threadIdx.x;
+    for (; i + 512 * (U - 1) + 2 <= n; i += 512 * U) {
+        pair id[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = i + 256 * u < n ? id_at(ids, wide, at + i + 256 * u) : -1;
+        for (int u = 0; u < U; ++u) id[u] = *reinterpret_cast<const pair*>(ids + i + 512 * u);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint64_t o = (uint64_t)(id[u] - v0);
-            if (id[u] >= 0 && o < (uint64_t)seg) {
-                if constexpr (MARK)
-                    atomicOr(&count[o], kInPrompt);
-                else
-                    atomicAdd(&count[o], 1u);
-            }
+            one(id[u].x);
+            one(id[u].y);
         }
     }
+    // under 512 U left: all of a thread's in flight again
+    pair id[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) {
+        const int64_t at = i + 512 * u;
+        id[u] = pair{(I)-1, (I)-1};
+        if (at + 2 <= n)
+            id[u] = *reinterpret_cast<const pair*>(ids + at);
+        else if (at < n)
+            id[u].x = ids[at];
+    }
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) {
+        one(id[u].x);
+        one(id[u].y);
+    }
+    for (i += 512 * (U - 1); i < n; i += 512) one(ids[i]);  // at most one id
+}
+template <bool MARK>
+PE_DEV void count_ids(uint32_t* count, const void* ids, int wide, int64_t at, int64_t n, uint32_t v0, uint32_t seg) {
+    if (wide)
+        count_ids<MARK>(count, static_cast<const int64_t*>(ids) + at, n, v0, seg);
+    else
+        count_ids<MARK>(count, static_cast<const int*>(ids) + at, n, v0, seg);
 }
 
 template <typename T, int STEPS>
@@ -76,7 +108,10 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
     const T* x = static_cast<const T*>(p.x) + b * p.x_row;
     T* y = static_cast<T*>(p.y) + b * p.y_row;
     const bool ids = p.history || p.prompt;
+    // everything the segment needs is on its way before the ids are counted
     vec r[STEPS];
+    float bias[STEPS][V];
+    uint32_t mask[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int64_t v = v0 + (int64_t)(s * 256 + t) * V;
@@ -86,6 +121,23 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) r[s][i] = v + i < p.vocab ? x[v + i] : (T)0.f;
         }
+        if (p.bias) {
+            const float* from = p.bias + b * p.bias_row + v;
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                vec4 w = {0.f, 0.f, 0.f, 0.f};
+                if (v + V <= p.vocab) {
+                    w = *reinterpret_cast<const vec4*>(from + i);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = v + i + k < p.vocab ? from[i + k] : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bias[s][i + k] = w[k];
+            }
+        }
+        // V divides 32: the elements of a vector share a word
+        mask[s] = p.mask && v < p.vocab ? p.mask[b * p.mask_row + (v >> 5)] >> (v & 31) : 0xFFFFFFFFu;
     }
     const float rep = p.rules[0] ? p.rules[0][b] : p.rule[0];
     const float freq = p.rules[1] ? p.rules[1][b] : p.rule[1];
@@ -93,15 +145,16 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
     if (ids) {
         for (int i = t; i < SEG; i += 256) count[i] = 0;
         __syncthreads();
+        if (p.prompt)
+            count_ids<true>(count, p.prompt, p.prompt_wide, b * p.prompt_row, p.prompt_len, (uint32_t)v0, SEG);
         if (p.history) {
             int64_t n = p.history_len;
             if (p.lengths) {
                 const int64_t l = id_at(p.lengths, p.lengths_wide, b);
                 n = l < 0 ? 0 : l < n ? l : n;
             }
-            count_ids<false>(count, p.history, p.ids_wide, b * p.history_row, n, v0, SEG);
+            count_ids<false>(count, p.history, p.ids_wide, b * p.history_row, n, (uint32_t)v0, SEG);
         }
-        if (p.prompt) count_ids<true>(count, p.prompt, p.prompt_wide, b * p.prompt_row, p.prompt_len, v0, SEG);
         __syncthreads();
     }
 #pragma unroll
@@ -114,19 +167,8 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) z[i] = (float)r[s][i];
         if (p.bias) {
-            const float* bias = p.bias + b * p.bias_row + v;
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                if (whole) {
-                    const vec4 w = *reinterpret_cast<const vec4*>(bias + i);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) z[i + k] += w[k];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (v + i + k < p.vocab) z[i + k] += bias[i + k];
-                }
-            }
+            for (int i = 0; i < V; ++i) z[i] += bias[s][i];
         }
         if (ids) {
 #pragma unroll
@@ -140,11 +182,9 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
             }
         }
         if (p.mask) {
-            // V divides 32: the elements of a vector share a word
-            const uint32_t w = p.mask[b * p.mask_row + (v >> 5)] >> (v & 31);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (!(w >> i & 1)) z[i] = -__builtin_huge_valf();
+                if (!(mask[s] >> i & 1)) z[i] = -__builtin_huge_valf();
         }
         if (whole) {
             vec h;
@@ -162,12 +202,15 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
 template <typename T>
 static int launch_logits(const LogitArgs& p, int64_t batch, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    // Long segments read the histories less often, short ones fill the chip: four vectors a thread
-    // from four workgroups a CU on, else one.
+    // Segments of 4096 tokens, or of a vector a thread where those leave fewer than two workgroups per
+    // CU. Longer ones read the ids less often but wait longer for them, shorter ones have too few bytes
+    // on their way (us at 2048 | 4096 | 8192 tokens, 256 rows of 151643 fp16 and 300 ids, from memory:
+    // 43 | 38 | -, from the Infinity Cache: 32 | 32 | 44; 24 rows of 152064 fp32, 4770 ids: 10 | 9 | 12).
+    constexpr int kLong = 16 / V;
     const auto blocks = [&](int steps) { return (p.vocab + 256 * V * steps - 1) / (256 * V * steps); };
-    const bool many = batch * blocks(4) >= 1024;
+    const bool many = batch * blocks(kLong) >= 512;
     // rows per launch: grid.y's limit, and 2^32 threads in a grid
-    int64_t most = (1 << 23) / blocks(many ? 4 : 1);
+    int64_t most = (1 << 23) / blocks(many ? kLong : 1);
     most = most < 1 ? 1 : most > 65535 ? 65535 : most;
     for (int64_t b0 = 0; b0 < batch; b0 += most) {
         LogitArgs a = p;
@@ -182,7 +225,7 @@ static int launch_logits(const LogitArgs& p, int64_t batch, hipStream_t s) {
         if (p.bias) a.bias = p.bias + b0 * p.bias_row;
         if (p.mask) a.mask = p.mask + b0 * p.mask_row;
         if (many)
-            hipLaunchKernelGGL((k_adjust_logits<T, 4>), dim3((unsigned)blocks(4), (unsigned)n), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_adjust_logits<T, kLong>), dim3((unsigned)blocks(kLong), (unsigned)n), dim3(256), 0, s, a);
         else
             hipLaunchKernelGGL((k_adjust_logits<T, 1>), dim3((unsigned)blocks(1), (unsigned)n), dim3(256), 0, s, a);
     }

@@ -21,7 +21,7 @@ def test_rope_positions(lib):
     assert call(tokens=0, x=None) == 0
     for kw in (dict(type=8), dict(pos_dtype=0), dict(pos_dtype=3)):
         assert call(**kw) == 2, kw
-    for kw in (dict(tokens=-1), dict(n_head=0), dict(n_head=65536), dict(hd=0), dict(rot=0), dict(rot=63), dict(rot=66),
+    for kw in (dict(tokens=-1), dict(n_head=0), dict(n_head=4097), dict(hd=0), dict(rot=0), dict(rot=63), dict(rot=66),
                dict(y_token=63), dict(y_head=63), dict(y_token=64, y_head=64), dict(y_token=100), dict(x_token=-1),
                dict(y_token=0), dict(y_head=0)):
         assert call(**kw) == 3, kw
