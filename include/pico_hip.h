@@ -799,9 +799,9 @@ int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, 
  *   round_fp16 as pe_decode_attn. fp32 products and sums; with fp16 caches the query and the
  *   probabilities enter the products as two fp16 values each, 22 bits (an infinite key or value that
  *   a row sees may make it NaN).
- * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes, any contents, with prefix_keys =
- * prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in order on one
- * stream may share it, calls that overlap must not. Two launches. */
+ * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes (0: NULL will do), any contents, with
+ * prefix_keys = prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in
+ * order on one stream may share it, calls that overlap must not. Two launches, one for few keys. */
 typedef struct pe_shared_prefix_args {
     const float* q;
     int cache_type;
@@ -825,8 +825,8 @@ typedef struct pe_shared_prefix_args {
     void* workspace;
     int64_t workspace_bytes;
 } pe_shared_prefix_args;
-int64_t pe_shared_prefix_attn_workspace_bytes(int64_t batch, int n_head, int n_kv, int head_dim,
-                                              int64_t prefix_keys, int64_t own_capacity);
+int64_t pe_shared_prefix_attn_workspace_bytes(int cache_type, int64_t batch, int n_head, int n_kv,
+                                              int head_dim, int64_t prefix_keys, int64_t own_capacity);
 int pe_shared_prefix_attn(const pe_shared_prefix_args* args, pe_stream_t stream);
 
 /* Rules on the logits of `batch` rows of `vocab` elements (PE_TYPE_F32 or PE_TYPE_F16, computed in

@@ -493,7 +493,8 @@ struct SpSplit {
             v[f] = reinterpret_cast<const float4*>(vb)[at];
         }
     }
-    // E, a multiple of 8, with the largest finite element under 2^(15 + E)
+    // E with the largest finite element in [2^(14 + E), 2^(15 + E)): the two parts hold every element to
+    // 2^-23 of itself or 2^-39 of the largest
     static PE_DEV int exponent(const float4* x) {
         float top = 0.f;
 #pragma unroll
@@ -512,7 +513,7 @@ struct SpSplit {
             bits = wave_max_bits(__float_as_uint(top));
         }
         const int e = (int)(bits >> 23) - 127;
-        return ((e < -100 ? -100 : e) - 14 + 7) >> 3 << 3;
+        return (e < -100 ? -100 : e) - 14;
     }
     template <bool VALUES>
     static PE_DEV void store(const float4* x, float f, uint8_t* plane, int w, int lane) {
@@ -555,16 +556,21 @@ struct SpShared {
     int (*row)[32];
 };
 
+PE_DEV float4 sp_rounded(const float4& y, int round_fp16) {
+    return round_fp16 ? make_float4(round_to_f16(y.x), round_to_f16(y.y), round_to_f16(y.z), round_to_f16(y.w)) : y;
+}
+
 // The record of a wave's Q queries (lane = query + Q part; v[i]: dims 256 / Q i + 4 part ..): stored, or
 // merged with those of the item's other waves (sub of split; the waves first, first + step, ..) in LDS.
-template <int HD, int Q>
+// ALL: the waves had all of the queries' keys, so the merge is the output.
+template <int HD, int Q, bool ALL>
 PE_DEV void sp_finish(const SpArgs& p, const SpShared& m, float4* v, float r, float l, int my_row, bool works, int live, int chunk,
                       int item, int sub, int split, int step) {
     constexpr int W = 256 / Q, N = HD / W, OS = HD + 4;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qi = lane % Q, at = 4 * (lane / Q);
     const int chunks = p.p_chunks + p.o_chunks;
     live = live < Q ? live : Q;
-    if (split == 1) {  // uniform
+    if (!ALL && split == 1) {  // uniform
         if (works && qi < live) {
             const int64_t rec = (int64_t)my_row * chunks + chunk;
 #pragma unroll
@@ -587,9 +593,9 @@ PE_DEV void sp_finish(const SpArgs& p, const SpShared& m, float4* v, float r, fl
         m.row[w][qi] = my_row;
     }
     __syncthreads();
-    if (!works) return;
+    if (!ALL && !works) return;
     // every wave of the item takes its share of the rows
-    if (sub == 0 && lane < live) {
+    if (!ALL && sub == 0 && lane < live) {
         float sum = m.sum[first][lane];
         for (int s = 1; s < split; ++s) sum += m.sum[first + step * s][lane];
         *reinterpret_cast<float2*>(p.ml + ((int64_t)my_row * chunks + chunk) * 2) = make_float2(most, sum);
@@ -604,38 +610,65 @@ PE_DEV void sp_finish(const SpArgs& p, const SpShared& m, float4* v, float r, fl
             const float4 y = *reinterpret_cast<const float4*>(o + s * step * Q * OS);
             x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
-        store_record(p.rec + ((int64_t)m.row[first][row] * chunks + chunk) * HD + 4 * c, x);
+        if constexpr (ALL) {
+            float sum = m.sum[first][row];
+            for (int s = 1; s < split; ++s) sum += m.sum[first + step * s][row];
+            // a sequence without keys: zeros
+            x = works ? make_float4(x.x / sum, x.y / sum, x.z / sum, x.w / sum) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(p.out + (int64_t)m.row[first][row] * HD + 4 * c) = sp_rounded(x, p.round_fp16);
+        } else {
+            store_record(p.rec + ((int64_t)m.row[first][row] * chunks + chunk) * HD + 4 * c, x);
+        }
     }
 }
 
-// The own keys of a group, by the waves of a workgroup: items of split waves each.
-template <typename T, int HD>
+// 16 queries of a group on the keys of one sequence, by waves of their own: the own keys' items of split
+// waves each, or, ALL, the prefix's keys and then the own ones by a whole workgroup.
+template <typename T, int HD, bool ALL>
 PE_DEV void sp_own(const SpArgs& p, const SpShared& m, int block) {
     typedef OwnRows<T, HD> Rows;
     constexpr int TK = Rows::TK, N = 4 * Rows::U, kTile = TK * HD * (int)sizeof(T), kPieces = kTile / 1024;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qi = lane & 15, h = lane >> 4;
-    const int split = p.o_split, item = w / split, sub = w % split;
+    const int split = ALL ? kSpWaves : p.o_split, item = ALL ? 0 : w / split, sub = ALL ? w : w % split;
     int at = block * (kSpWaves / split) + item;
     const bool live = at < p.o_items;
     at = live ? at : 0;
-    const int per = p.batch * p.n_kv * p.o_tiles, chunk = at / per;
+    const int per = p.batch * p.n_kv * p.o_tiles, chunk = ALL ? 0 : at / per;
     at -= chunk * per;
     const int tile = at % p.o_tiles, j = at / p.o_tiles % p.n_kv, b = at / p.o_tiles / p.n_kv;
-    const int64_t len = live ? sp_length(p.o_len, p.o_dtype, b, p.o_add, p.o_cap) : 0, k0 = (int64_t)chunk * p.o_keys;
-    const int keys = len <= k0 ? 0 : len - k0 < p.o_keys ? (int)(len - k0) : p.o_keys;
+    const int64_t len = live ? sp_length(p.o_len, p.o_dtype, b, p.o_add, p.o_cap) : 0, k0 = ALL ? 0 : (int64_t)chunk * p.o_keys;
+    const int keys = len <= k0 ? 0 : ALL || len - k0 < p.o_keys ? (int)(len - k0) : p.o_keys;
     const int64_t first = (((int64_t)b * p.n_kv + j) * p.o_cap + k0) * HD;
     const T *kb = static_cast<const T*>(p.ko) + first, *vb = static_cast<const T*>(p.vo) + first;
-    const int row0 = 16 * tile, my_row = b * p.n_head + j * p.group + row0 + qi, tiles = (keys + TK - 1) / TK;
+    // the prefix's keys and tiles in front of them
+    int p_keys = 0, p_tiles = 0;
+    const T *kp = nullptr, *vp = nullptr;
+    if constexpr (ALL) {
+        const int64_t n = len < 0 ? 0 : sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
+        p_keys = n > 0 ? (int)n : 0;
+        p_tiles = (p_keys + TK - 1) / TK;
+        kp = static_cast<const T*>(p.kp) + (int64_t)j * p.p_cap * HD;
+        vp = static_cast<const T*>(p.vp) + (int64_t)j * p.p_cap * HD;
+    }
+    const int row0 = 16 * tile, my_row = b * p.n_head + j * p.group + row0 + qi, tiles = p_tiles + (keys + TK - 1) / TK;
     uint8_t *const kt = m.lds + w * 2 * kTile, *const vt = kt + kTile;
     const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
-    const auto stage_k = [&](int t) { sp_stage<T, HD, false, kPieces>(kb + (int64_t)t * TK * HD, keys - 1 - t * TK, kt_a, lane, 0); };
-    const auto stage_v = [&](int t) { sp_stage<T, HD, true, kPieces>(vb + (int64_t)t * TK * HD, keys - 1 - t * TK, vt_a, lane, 0); };
+    // keys left from tile t on, in its set
+    const auto left = [&](int t) { return t < p_tiles ? p_keys - t * TK : keys - (t - p_tiles) * TK; };
+    const auto stage_k = [&](int t) {
+        const T* from = t < p_tiles ? kp + (int64_t)t * TK * HD : kb + (int64_t)(t - p_tiles) * TK * HD;
+        sp_stage<T, HD, false, kPieces>(from, left(t) - 1, kt_a, lane, 0);
+    };
+    const auto stage_v = [&](int t) {
+        const T* from = t < p_tiles ? vp + (int64_t)t * TK * HD : vb + (int64_t)(t - p_tiles) * TK * HD;
+        sp_stage<T, HD, true, kPieces>(from, left(t) - 1, vt_a, lane, 0);
+    };
     if (sub < tiles) {
         stage_k(sub);
         stage_v(sub);
     }
     Rows q;
-    q.load(keys > 0 && row0 + qi < p.group ? p.q + (int64_t)my_row * HD : nullptr, p.scale, h);
+    q.load(tiles > 0 && row0 + qi < p.group ? p.q + (int64_t)my_row * HD : nullptr, p.scale, h);
     const float NEG_INF = -__builtin_huge_valf();
     float r = NEG_INF, l = 0.f;
     f4v o[HD / 16] = {};
@@ -650,7 +683,7 @@ PE_DEV void sp_own(const SpArgs& p, const SpShared& m, int block) {
         q.scores(kt, s, qi, h);
         sp_wait_lds();
         if (more) stage_k(t + split);
-        const int n = keys - t * TK;
+        const int n = left(t);
         if (n < TK) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -691,7 +724,7 @@ PE_DEV void sp_own(const SpArgs& p, const SpShared& m, int block) {
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) v[d] = make_float4(o[d][0] * down, o[d][1] * down, o[d][2] * down, o[d][3] * down);
     l = swap32_sum(swap16_sum(l)) * down;
-    sp_finish<HD, 16>(p, m, v, r + kUp, l, my_row, keys > 0, p.group - row0, p.p_chunks + chunk, item, sub, split, 1);
+    sp_finish<HD, 16, ALL>(p, m, v, r + kUp, l, my_row, tiles > 0, p.group - row0, p.p_chunks + chunk, item, sub, split, 1);
 }
 
 // The rows of a solo item: fp32 caches on the fp32 matrix instructions.
@@ -740,7 +773,7 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, li = lane & 31;
 
     const SpShared m{lds, ref, sums, row_of};
-    if ((int)blockIdx.x >= p.p_blocks) return sp_own<T, HD>(p, m, blockIdx.x - p.p_blocks);
+    if ((int)blockIdx.x >= p.p_blocks) return sp_own<T, HD, false>(p, m, blockIdx.x - p.p_blocks);
 
     // The wave's rows and the keys [k0, k1).
     const bool shared = p.shared;
@@ -900,7 +933,17 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i)
         v[i] = make_float4(st.o[i >> 2][4 * (i & 3)], st.o[i >> 2][4 * (i & 3) + 1], st.o[i >> 2][4 * (i & 3) + 2], st.o[i >> 2][4 * (i & 3) + 3]);
-    sp_finish<HD, 32>(p, m, v, st.r + kUp, swap32_sum(st.l) * down, my_row, works, rows - row0, chunk, item, sub, split, shared ? 4 : 1);
+    sp_finish<HD, 32, false>(p, m, v, st.r + kUp, swap32_sum(st.l) * down, my_row, works, rows - row0, chunk, item, sub, split, shared ? 4 : 1);
+}
+
+// Few keys: all of them by one workgroup per sequence, kv head and 16 queries of its group, in one launch.
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix_few(SpArgs p) {
+    constexpr int kTiles = kSpWaves * 2 * OwnRows<T, HD>::TK * HD * (int)sizeof(T), kMerge = kSpWaves * 16 * (HD + 4) * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kTiles > kMerge ? kTiles : kMerge];
+    __shared__ float ref[kSpWaves][32], sums[kSpWaves][32];
+    __shared__ int row_of[kSpWaves][32];
+    sp_own<T, HD, true>(p, SpShared{lds, ref, sums, row_of}, blockIdx.x);
 }
 
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
@@ -969,13 +1012,12 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
         }
     }
     if (lane >= L) return;
-    float4 y = n ? make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum) : v;
-    if (p.round_fp16) y = make_float4(round_to_f16(y.x), round_to_f16(y.y), round_to_f16(y.z), round_to_f16(y.w));
-    *reinterpret_cast<float4*>(p.out + (int64_t)row * HD + 4 * lane) = y;
+    const float4 y = n ? make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum) : v;
+    *reinterpret_cast<float4*>(p.out + (int64_t)row * HD + 4 * lane) = sp_rounded(y, p.round_fp16);
 }
 
 struct SpPlan {
-    int shared, p_chunks, p_keys, p_tiles, o_chunks, o_keys, o_tiles, o_split;
+    int few, shared, p_chunks, p_keys, p_tiles, o_chunks, o_keys, o_tiles, o_split;
 };
 
 // How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup, so the
@@ -997,6 +1039,18 @@ static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, in
         chunks = (int)((keys + k - 1) / k);
     };
     const int64_t pairs = batch * n_kv * s.o_tiles, tiles = (o_cap + 31) / 32;
+    // Few keys: the prefix is read again for every sequence (from L2), but there is one launch and
+    // nothing to merge. Measured, few | two launches (us, 4 sequences, own capacity 64, prefix of 256, 512,
+    // 1024; heads 14/2 of 64 and 28/4 of 128): fp32 8.1 | 13.4, 10.5 | 13.3, 15.9 | 14.0 and 11 | 20,
+    // 16 | 21, 27 | 21; fp16 5.5 | 9.8, 6.4 | 9.9, 8.2 | 10.4 and 7.5 | 13, 8.9 | 13.5, 12 | 14; the same
+    // for up to 256 workgroups.
+    s.few = (pairs + 255) / 256 * (p_keys + o_cap) <= (half ? 1280 : 640);
+    if (s.few) {
+        s.p_chunks = s.o_chunks = 0;
+        s.p_keys = s.o_keys = 0;
+        s.o_split = kSpWaves;
+        return s;
+    }
     s.o_split = 1;
     while (s.o_split < kSpWaves && s.o_split < tiles && pairs * s.o_split < 1024) s.o_split *= 2;
     int64_t want = 1024 / (pairs * s.o_split);
@@ -1025,7 +1079,11 @@ static int64_t sp_bytes(const SpPlan& s, int64_t batch, int n_head, int head_dim
 }
 
 template <typename T, int HD>
-static void launch_shared_prefix(const SpArgs& p, int64_t blocks, hipStream_t s) {
+static void launch_shared_prefix(const SpArgs& p, bool few, int64_t blocks, hipStream_t s) {
+    if (few) {
+        hipLaunchKernelGGL((k_shared_prefix_few<T, HD>), dim3((unsigned)p.o_items), dim3(64 * kSpWaves), 0, s, p);
+        return;
+    }
     if (blocks > 0) hipLaunchKernelGGL((k_shared_prefix<T, HD>), dim3((unsigned)blocks), dim3(64 * kSpWaves), 0, s, p);
     const int64_t rows = (int64_t)p.batch * p.n_head;
     // few rows of many records: four waves a row
@@ -1039,14 +1097,12 @@ static void launch_shared_prefix(const SpArgs& p, int64_t blocks, hipStream_t s)
 
 using namespace pe;
 
-extern "C" int64_t pe_shared_prefix_attn_workspace_bytes(int64_t batch, int n_head, int n_kv, int head_dim,
-                                                         int64_t prefix_keys, int64_t own_capacity) {
+extern "C" int64_t pe_shared_prefix_attn_workspace_bytes(int cache_type, int64_t batch, int n_head, int n_kv,
+                                                         int head_dim, int64_t prefix_keys, int64_t own_capacity) {
+    if (cache_type != PE_TYPE_F32 && cache_type != PE_TYPE_F16) return -PE_ERR_TYPE;
     if (!sp_shape_ok(batch, n_head, n_kv, head_dim, prefix_keys, own_capacity)) return -PE_ERR_SHAPE;
-    // of either type of cache
-    const SpPlan a = sp_plan(batch, n_head, n_kv, head_dim, false, prefix_keys, own_capacity);
-    const SpPlan b = sp_plan(batch, n_head, n_kv, head_dim, true, prefix_keys, own_capacity);
-    const int64_t x = sp_bytes(a, batch, n_head, head_dim), y = sp_bytes(b, batch, n_head, head_dim);
-    return x > y ? x : y;
+    const bool half = cache_type == PE_TYPE_F16;
+    return sp_bytes(sp_plan(batch, n_head, n_kv, head_dim, half, prefix_keys, own_capacity), batch, n_head, head_dim);
 }
 
 extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t stream) {
@@ -1077,7 +1133,7 @@ extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t
         return PE_ERR_ALIGN;
     if (a->workspace_bytes < need) return PE_ERR_SPACE;
     const int64_t p_blocks = (int64_t)a->n_kv * s.p_chunks * s.p_tiles;
-    const int64_t items = a->batch * a->n_kv * s.o_tiles * s.o_chunks, per = kSpWaves / s.o_split;
+    const int64_t items = a->batch * a->n_kv * s.o_tiles * (s.few ? 1 : s.o_chunks), per = kSpWaves / s.o_split;
     const int64_t blocks = p_blocks + (items + per - 1) / per;
     if (blocks >= (1 << 23) || items > 0x7FFFFFFF) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
     const int64_t records = a->batch * a->n_head * (int64_t)(s.p_chunks + s.o_chunks);
@@ -1089,10 +1145,10 @@ extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t
              a->round_fp16, a->out};
     hipStream_t st = (hipStream_t)stream;
     if (a->cache_type == PE_TYPE_F16)
-        a->head_dim == 64 ? launch_shared_prefix<_Float16, 64>(p, blocks, st)
-                          : launch_shared_prefix<_Float16, 128>(p, blocks, st);
+        a->head_dim == 64 ? launch_shared_prefix<_Float16, 64>(p, s.few, blocks, st)
+                          : launch_shared_prefix<_Float16, 128>(p, s.few, blocks, st);
     else
-        a->head_dim == 64 ? launch_shared_prefix<float, 64>(p, blocks, st)
-                          : launch_shared_prefix<float, 128>(p, blocks, st);
+        a->head_dim == 64 ? launch_shared_prefix<float, 64>(p, s.few, blocks, st)
+                          : launch_shared_prefix<float, 128>(p, s.few, blocks, st);
     return launch_status();
 }

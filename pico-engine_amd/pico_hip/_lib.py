@@ -207,7 +207,7 @@ _SIGNATURES = {
     "pe_qkv_embed_rmsnorm_rope": (_I, [ctypes.POINTER(QkvArgs), _I, _P, _L, _P, _P, _P, _L, _P]),
     "pe_rope_positions": (_I, [_I, _P, _L, _L, _P, _I, _P, _I, _F, _I, _P, _L, _L, _L, _I, _I, _P]),
     "pe_rope_append": (_I, [_P, _L, _P, _I, _P, _P, _P, _L, _I, _F, _I, _I, _I, _I, _L, _P, _I, _P, _P, _L, _L, _P]),
-    "pe_shared_prefix_attn_workspace_bytes": (_L, [_L, _I, _I, _I, _L, _L]),
+    "pe_shared_prefix_attn_workspace_bytes": (_L, [_I, _L, _I, _I, _I, _L, _L]),
     "pe_shared_prefix_attn": (_I, [ctypes.POINTER(SharedPrefixArgs), _P]),
     "pe_adjust_logits": (_I, [ctypes.POINTER(LogitArgs), _P]),
 }

@@ -1730,18 +1730,19 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor 
 
 
 @functools.lru_cache(maxsize=1024)
-def _shared_prefix_bytes(batch: int, n_head: int, n_kv: int, hd: int, keys: int, own: int) -> int:
-    size = lib.pe_shared_prefix_attn_workspace_bytes(batch, n_head, n_kv, hd, keys, own)
+def _shared_prefix_bytes(cache_type: int, batch: int, n_head: int, n_kv: int, hd: int, keys: int, own: int) -> int:
+    size = lib.pe_shared_prefix_attn_workspace_bytes(cache_type, batch, n_head, n_kv, hd, keys, own)
     check(0 if size >= 0 else -size, "pe_shared_prefix_attn_workspace_bytes")
     return size
 
 
 def shared_prefix_attn_workspace(batch: int, n_head: int, n_kv: int, hd: int, prefix_keys: int, own_capacity: int,
                                  device) -> torch.Tensor:
-    """A workspace for shared_prefix_attn (any contents; reusable by calls in order on one stream).
-    prefix_keys: the prefix's length, or its capacity where the length is a device tensor."""
-    return torch.empty(_shared_prefix_bytes(batch, n_head, n_kv, hd, prefix_keys, own_capacity), device=device,
-                       dtype=torch.uint8)
+    """A workspace for shared_prefix_attn with caches of either type (any contents; reusable by calls in
+    order on one stream). prefix_keys: the prefix's length, or its capacity where the length is a device
+    tensor."""
+    size = max(_shared_prefix_bytes(t, batch, n_head, n_kv, hd, prefix_keys, own_capacity) for t in _CACHE_TYPE.values())
+    return torch.empty(size, device=device, dtype=torch.uint8)
 
 
 def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_own: torch.Tensor,
@@ -1789,15 +1790,16 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
         raise ValueError(f"out must be a contiguous float32 ({B}, {n_head}, {hd}) tensor")
     if B == 0:
         return out
-    need = _shared_prefix_bytes(B, n_head, n_kv, hd, P if p_code else p_add, cap)
+    need = _shared_prefix_bytes(code, B, n_head, n_kv, hd, P if p_code else p_add, cap)
     if workspace is None:
-        workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+        if need:
+            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
     elif not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous")
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     a = SharedPrefixArgs(q.data_ptr(), code, k_prefix.data_ptr(), v_prefix.data_ptr(), P, p_ptr, p_code, p_add,
                          k_own.data_ptr(), v_own.data_ptr(), cap, o_ptr, o_code, o_add, B, n_head, n_kv, hd,
-                         float(hd ** -0.5 if scale is None else scale), int(round_fp16), out.data_ptr(),
-                         workspace.data_ptr(), workspace.numel() * workspace.element_size())
+                         float(hd ** -0.5 if scale is None else scale), int(round_fp16), out.data_ptr(), ws, ws_bytes)
     _launch(dev, "pe_shared_prefix_attn", ctypes.byref(a))
     return out
 

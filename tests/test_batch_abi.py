@@ -49,8 +49,8 @@ def test_rope_append(lib):
 
 def test_shared_prefix_attn(lib):
     from pico_hip._lib import SharedPrefixArgs
-    d = dict(q=F, cache_type=0, k_prefix=F, v_prefix=F, prefix_capacity=300, prefix_len=None, prefix_len_dtype=0,
-             prefix_len_add=300, k_own=F, v_own=F, own_capacity=40, own_len=F, own_len_dtype=2, own_len_add=0, batch=3,
+    d = dict(q=F, cache_type=0, k_prefix=F, v_prefix=F, prefix_capacity=3000, prefix_len=None, prefix_len_dtype=0,
+             prefix_len_add=3000, k_own=F, v_own=F, own_capacity=40, own_len=F, own_len_dtype=2, own_len_add=0, batch=3,
              n_head=14, n_kv=2, head_dim=64, scale=0.125, round_fp16=0, out=F, workspace=F, workspace_bytes=1 << 30)
     def call(**kw):
         v = {**d, **kw}
@@ -60,20 +60,23 @@ def test_shared_prefix_attn(lib):
     for kw in (dict(cache_type=8), dict(prefix_len_dtype=3), dict(own_len_dtype=-1)):
         assert call(**kw) == 2, kw
     for kw in (dict(batch=-1), dict(n_head=15), dict(n_kv=0), dict(head_dim=96), dict(prefix_capacity=-1),
-               dict(own_capacity=-1), dict(prefix_capacity=(1 << 30) + 1), dict(batch=1 << 21)):
+               dict(own_capacity=-1), dict(prefix_capacity=(1 << 30) + 1, prefix_len_add=1 << 40), dict(batch=1 << 21)):
         assert call(**kw) == 3, kw
     for kw in (dict(q=None), dict(out=None), dict(k_prefix=None), dict(v_prefix=None), dict(k_own=None), dict(v_own=None),
                dict(own_len=None), dict(prefix_len_dtype=1), dict(workspace=None)):
         assert call(**kw) == 1, kw
     for name in ("q", "out", "k_prefix", "v_prefix", "k_own", "v_own", "workspace", "own_len"):
         assert call(**{name: ODD}) == 4, name
-    need = lib.pe_shared_prefix_attn_workspace_bytes(3, 14, 2, 64, 300, 40)
+    size = lib.pe_shared_prefix_attn_workspace_bytes
+    need = size(0, 3, 14, 2, 64, 3000, 40)
     assert need > 0 and call(workspace_bytes=need - 1) == 6
     # a shorter prefix needs less; one whose length is on the device, the capacity's
-    less = lib.pe_shared_prefix_attn_workspace_bytes(3, 14, 2, 64, 0, 40)
+    less = size(0, 3, 14, 2, 64, 1000, 40)
     assert less < need and call(prefix_len=F, prefix_len_dtype=2, workspace_bytes=less) == 6
+    assert size(0, 3, 14, 2, 64, 300, 40) == 0      # few keys: one launch
     for args in ((0, 14, 2, 64, 300, 40), (3, 14, 3, 64, 300, 40), (3, 14, 2, 80, 300, 40), (3, 14, 2, 64, -1, 40)):
-        assert lib.pe_shared_prefix_attn_workspace_bytes(*args) == -3, args
+        assert size(0, *args) == -3, args
+    assert size(8, 3, 14, 2, 64, 300, 40) == -2
 
 
 def test_adjust_logits(lib):

@@ -5,7 +5,10 @@ score is a sum of hd products whose roundings (half a step, 2^-24, of partial su
 independent, off by about 2^-24 sqrt(hd) A, four times that at most here; the exponent's reference
 and scale 2 * 2^-24 A; the query's and the probability's 22 bits of fp16 caches 2^-23 each; exp2 and
 the division some 2^-22; the sums over n keys 2 * 2^-24 sqrt(n):
-  |error| <= 2^-24 ((4 sqrt(hd) + 4) A + 2 sqrt(n) + 16) W."""
+  |error| <= 2^-24 ((4 sqrt(hd) + 4) A + 2 sqrt(n) + 16) W.
+fp32 caches behind more than 64 rows add 2^-39 max |v|: a value there is the sum of two fp16 values of v 2^-E,
+whose largest of 8 keys is at least 2^14; the low one's last place is 2^-24 at least (fp16's smallest),
+so an element is off by up to 2^-25 2^E <= 2^-39 max |v| however small it is itself, and sum p = 1."""
 
 import math
 
@@ -42,6 +45,8 @@ def plain(q, kp, vp, ko, vo, P, own, scale=None):
             A = abs(scale) * (x.abs() @ k.abs().T).amax(-1, keepdim=True)
             out[b, h] = p @ v
             tol[b, h] = 2.0 ** -24 * ((4 * math.sqrt(hd) + 4) * A + 2 * math.sqrt(P + n) + 16) * (p @ v.abs())
+            if kp.dtype is torch.float32 and B * (nh // nkv) > 64:
+                tol[b, h] += 2.0 ** -39 * v.abs().max()
     return out, tol
 
 
@@ -60,7 +65,9 @@ def close(got, ref, tol):
     assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - ref).abs() / tol.clamp_min(1e-30)).max()))
 
 
-SHAPES = [(1, 14, 2, 64, 1, 1), (1, 14, 2, 64, 33, 0), (4, 14, 2, 64, 277, 64), (3, 28, 4, 128, 129, 130), (16, 14, 2, 64, 1500, 40),
+# one launch up to 640 (fp32) or 1280 keys (fp16), solo and shared rows beyond
+SHAPES = [(1, 14, 2, 64, 1, 1), (3, 14, 2, 64, 1400, 64), (2, 28, 4, 128, 1281, 300), (1, 28, 4, 128, 3001, 1), (5, 25, 5, 64, 2500, 0),
+          (20, 28, 4, 128, 1500, 70), (80, 16, 16, 64, 130, 129), (129, 14, 2, 64, 1290, 5), (260, 4, 1, 128, 33, 700), (1, 14, 2, 64, 33, 0), (4, 14, 2, 64, 277, 64), (3, 28, 4, 128, 129, 130), (16, 14, 2, 64, 1500, 40),
           (10, 28, 4, 128, 700, 33), (37, 28, 4, 128, 513, 9), (9, 25, 5, 64, 64, 200), (5, 16, 16, 64, 95, 31),
           (70, 12, 1, 64, 260, 3), (2, 64, 1, 128, 300, 300), (130, 4, 4, 64, 31, 5), (2, 8, 2, 128, 4097, 1000), (65, 2, 1, 64, 2000, 128)]
 
@@ -79,15 +86,15 @@ def test_shared_prefix_attn(K, B, nh, nkv, hd, P, cap, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("B", [2, 40])
-def test_lengths_and_what_lies_behind_them(K, B, hd, dtype):
+@pytest.mark.parametrize("B,extra", [(2, 100), (2, 1500), (40, 100), (40, 1500)])
+def test_lengths_and_what_lies_behind_them(K, B, extra, hd, dtype):
     """Prefixes and own lengths of zero, one, around tiles and chunks, on the host and on the device;
     what lies behind a length may be NaN or infinite; negative lengths give zeros."""
     nh, nkv, cap = 4, 2, 300
-    q, kp, vp, ko, vo, _ = make(hd + B, B, nh, nkv, hd, 0, cap, dtype, extra=700)
+    q, kp, vp, ko, vo, _ = make(hd + B, B, nh, nkv, hd, 0, cap, dtype, extra=extra)
     lengths = [0, 1, 31, 32, 33, 127, 128, 129, 255, 256, 300, 1000, -1, -7]
     own = torch.tensor([lengths[i % len(lengths)] for i in range(B)], device=DEV)
-    for P in (0, 1, 32, 127, 128, 300, 513, 700):
+    for P in [n for n in (0, 1, 32, 100, 127, 128, 300, 513, 1500) if n <= extra]:
         for o in (own, own.roll(3), torch.zeros_like(own)):
             k1, v1, k2, v2 = kp.clone(), vp.clone(), ko.clone(), vo.clone()
             k1[:, P:], v1[:, P:] = float("nan"), math.inf
@@ -105,10 +112,11 @@ def test_lengths_and_what_lies_behind_them(K, B, hd, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-def test_seen_infinity_at_the_end_of_a_tile(K, dtype):
+@pytest.mark.parametrize("P", [45, 1645])
+def test_seen_infinity_at_the_end_of_a_tile(K, P, dtype):
     """The last key a row sees is copied behind the length; its infinite value counts once."""
-    q, kp, vp, ko, vo, _ = make(3, 3, 4, 2, 64, 45, 7, dtype)
-    vp[1, 44, 5] = math.inf
+    q, kp, vp, ko, vo, _ = make(3, 3, 4, 2, 64, P, 7, dtype)
+    vp[1, P - 1, 5] = math.inf
     got = K.shared_prefix_attn(q, kp, vp, ko, vo, 3, round_fp16=False)
     assert not bool(torch.isfinite(got[:, 2:, 5]).any()) and bool(torch.isfinite(got[:, :2]).all())
     assert bool(torch.isfinite(got[:, 2:, :5]).all()) and bool(torch.isfinite(got[:, 2:, 6:]).all())
@@ -117,9 +125,9 @@ def test_seen_infinity_at_the_end_of_a_tile(K, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-@pytest.mark.parametrize("B,hd", [(3, 64), (40, 128)])
-def test_nan_keys_reach_the_rows_that_see_them(K, B, hd, dtype):
-    q, kp, vp, ko, vo, own = make(B, B, 4, 2, hd, 400, 40, dtype)
+@pytest.mark.parametrize("B,hd,P", [(3, 64, 400), (3, 64, 1700), (40, 128, 1700)])
+def test_nan_keys_reach_the_rows_that_see_them(K, B, hd, P, dtype):
+    q, kp, vp, ko, vo, own = make(B, B, 4, 2, hd, P, 40, dtype)
     clean = K.shared_prefix_attn(q, kp, vp, ko, vo, own)
     for lo, hi in ((5, 6), (128, 256), (32, 64)):
         bad = kp.clone()
@@ -135,16 +143,47 @@ def test_nan_keys_reach_the_rows_that_see_them(K, B, hd, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("B,P", [(5, 300), (5, 1500), (40, 1500)])
 @pytest.mark.parametrize("mag", [2.0 ** -30, 2.0 ** -12, 1.0, 30.0, 3000.0, 2.0 ** 40])
-def test_magnitudes(K, mag, dtype):
+def test_magnitudes(K, mag, B, P, dtype):
     """Queries of any magnitude (scores from nothing to one key taking all), subnormal fp16 values."""
-    q, kp, vp, ko, vo, own = make(1, 5, 14, 2, 64, 300, 30, dtype)
+    q, kp, vp, ko, vo, own = make(1, B, 14, 2, 64, P, 30, dtype)
     q = q * mag
     vp[:, ::2] *= 2.0 ** -13
     vo[:, :, ::2] *= 2.0 ** -13
     scale = 0.125 if mag < 2.0 ** 30 else 2.0 ** -43
-    ref, tol = plain(q, kp, vp, ko, vo, 300, own, scale)
+    ref, tol = plain(q, kp, vp, ko, vo, P, own, scale)
     got = K.shared_prefix_attn(q, kp, vp, ko, vo, own, scale=scale, round_fp16=False)
+    close(got, ref, tol)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 0.5])
+@pytest.mark.parametrize("B,P", [(2, 100), (2, 1500), (40, 1500)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_scales(K, scale, B, P, dtype):
+    q, kp, vp, ko, vo, own = make(4, B, 14, 2, 64, P, 37, dtype)
+    ref, tol = plain(q, kp, vp, ko, vo, P, own, scale)
+    close(K.shared_prefix_attn(q, kp, vp, ko, vo, own, scale=scale, round_fp16=False), ref, tol)
+
+
+@pytest.mark.parametrize("B", [2, 40])
+def test_fp32_caches_of_any_magnitude(K, B):
+    """Keys and values of fp32 range, groups of keys of very different ones, an infinite value."""
+    q, kp, vp, ko, vo, own = make(6, B, 14, 2, 64, 1500, 20, torch.float32)
+    kp[:, 300:600] *= 1e-6
+    kp[:, 700:708] *= 3.0
+    q[:, 2] *= 1e-20
+    vp[:, 40:60] *= 1e30
+    vp[:, 900:1400] *= 1e-25
+    ref, tol = plain(q, kp, vp, ko, vo, 1500, own)
+    close(K.shared_prefix_attn(q, kp, vp, ko, vo, own, round_fp16=False), ref, tol)
+    kp, vp = kp * 1e18, torch.full_like(vp, 1e-30)
+    ref, tol = plain(q, kp, vp, ko * 1e18, vo * 1e-30, 1500, own, 1e-19)
+    close(K.shared_prefix_attn(q, kp, vp, ko * 1e18, vo * 1e-30, own, scale=1e-19, round_fp16=False), ref, tol)
+    vp[0, 1000, 9] = math.inf
+    got = K.shared_prefix_attn(q, kp, vp, ko * 1e18, vo * 1e-30, own, scale=1e-19, round_fp16=False)
+    assert not bool(torch.isfinite(got[:, :7, 9]).any())
+    got[:, :7, 9], ref[:, :7, 9] = 0, 0
     close(got, ref, tol)
 
 
@@ -238,8 +277,9 @@ def test_refusals(K):
     for args in bad:
         with pytest.raises(ValueError):
             K.shared_prefix_attn(*args)
+    long = torch.zeros(2, 5000, 64, device=DEV)
     with pytest.raises(RuntimeError):    # too small a workspace
-        K.shared_prefix_attn(q, kp, vp, ko, vo, own, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
+        K.shared_prefix_attn(q, long, long, ko, vo, own, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
     with pytest.raises(RuntimeError):    # head sizes of 64 and 128
         K.shared_prefix_attn(*(t[..., :32].contiguous() for t in (q, kp, vp, ko, vo)), own)
     with pytest.raises(RuntimeError):    # whole groups
