@@ -1021,10 +1021,13 @@ struct SpPlan {
 };
 
 // How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup, so the
-// launch is made of about 256 that take equally long: the own keys' items of one to eight waves
-// first, then as many chunks of the prefix as fill the rest in proportion to its share of the work.
-// Times (us, head size 128; measured): a workgroup's start, end and records 10; a shared block of
-// 64 keys 1.8 with 16-bit caches, 3.5 with fp32 ones; a wave's solo tile 1.2 and 7.
+// launch is made of at most about 256 of them that take equally long: the own keys' items of one to
+// eight waves, and as many chunks of the prefix as the rest holds. Of four numbers of own waves the one
+// whose longest workgroup is shortest, by the times measured at head size 128 (us): 10 for a prefix
+// workgroup's start and end, 1.8 (16-bit caches) and 3.5 (fp32) for a shared block of 64 keys, 1.5 and 7 for
+// eight solo tiles; 8 for an own workgroup's, 1.5 and 5.3 for a wave's 32 keys. 33 x 8001 with 515 own keys
+// (28/4 heads, fp32): 62, 40 and 43 us with 256, 512 and 1024 own waves, 57 with the chunks of an empty chip;
+// 16 x 4096 with 2000 (fp16): 37, 26, 22.
 static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, int64_t p_keys, int64_t o_cap) {
     SpPlan s;
     const int64_t group = n_head / n_kv, rows = batch * group;
@@ -1032,7 +1035,8 @@ static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, in
     s.p_tiles = (int)(s.shared ? (rows + 127) / 128 : (rows + 31) / 32);
     s.o_tiles = (int)((group + 15) / 16);
     const auto cut = [](int64_t keys, int64_t want, int64_t step, int& chunks, int& per) {
-        int64_t k = (keys + want - 1) / (want < 1 ? 1 : want);
+        want = want < 1 ? 1 : want;
+        int64_t k = (keys + want - 1) / want;
         k = (k + step - 1) / step * step;
         k = k < step ? step : k;
         per = (int)k;
@@ -1051,20 +1055,28 @@ static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, in
         s.o_split = kSpWaves;
         return s;
     }
-    s.o_split = 1;
-    while (s.o_split < kSpWaves && s.o_split < tiles && pairs * s.o_split < 1024) s.o_split *= 2;
-    int64_t want = 1024 / (pairs * s.o_split);
-    cut(o_cap, want < 1 ? 1 : want, 32 * s.o_split, s.o_chunks, s.o_keys);
-    const double each = hd / 128.0, t_block = (half ? 1.8 : 3.5) * each, t_tile = (half ? 1.2 : 7.0) * each;
-    const int64_t items = pairs * s.o_chunks, o_blocks = (items + kSpWaves / s.o_split - 1) / (kSpWaves / s.o_split);
-    const double own = o_blocks * (10.0 + t_tile * (s.o_keys / (32 * s.o_split)));
-    const int64_t per_chunk = (int64_t)n_kv * s.p_tiles;
-    const int64_t steps = s.shared ? (p_keys + kSpBlock - 1) / kSpBlock : (p_keys + 255) / 256;
-    const double prefix = (double)per_chunk * steps * (s.shared ? t_block : t_tile);
-    // own workgroups that fit beside a chunk's are left room for
-    const double room = o_blocks < 128 ? 256 - o_blocks : 256 * (prefix + 2560) / (prefix + 2560 + own);
-    want = (int64_t)(room / per_chunk);
-    cut(p_keys, want < 1 ? 1 : want, s.shared ? kSpBlock : 32 * kSpWaves, s.p_chunks, s.p_keys);
+    const double each = hd / 128.0, t_step = (s.shared ? (half ? 1.8 : 3.5) : (half ? 1.5 : 7.0)) * each;
+    const double t_own = (half ? 1.5 : 5.3) * each;
+    const int64_t per_chunk = (int64_t)n_kv * s.p_tiles, step = s.shared ? kSpBlock : 32 * kSpWaves;
+    double best = 1e30;
+    for (int64_t waves = 256; waves <= 2048; waves *= 2) {
+        SpPlan c = s;
+        c.o_split = 1;
+        while (c.o_split < kSpWaves && c.o_split < tiles && pairs * c.o_split < waves) c.o_split *= 2;
+        cut(o_cap, waves / (pairs * c.o_split), 32 * c.o_split, c.o_chunks, c.o_keys);
+        const int64_t per = kSpWaves / c.o_split, o_blocks = (pairs * c.o_chunks + per - 1) / per;
+        const int64_t room = o_blocks + per_chunk <= 256 ? 256 - o_blocks : 256;
+        cut(p_keys, room / per_chunk, step, c.p_chunks, c.p_keys);
+        const double own = o_blocks ? 8 + t_own * (c.o_keys / (32 * c.o_split)) : 0;
+        const double prefix = c.p_chunks ? 10 + t_step * (c.p_keys / step) : 0;
+        const double rounds = (o_blocks + 255) / 256 * own;
+        const double time = room < 256 ? (own > prefix ? own : prefix) : rounds + prefix * ((per_chunk * c.p_chunks + 255) / 256);
+        if (time < best) {
+            best = time;
+            s = c;
+        }
+        if (!o_cap) break;
+    }
     return s;
 }
 
