@@ -26,7 +26,7 @@ from . import kernels as K
 from .dequant import GGML_F16, GGML_F32, MATRIX_TYPES
 from .gguf import load as load_gguf, read_tensor_bytes
 from .model import ModelConfig, Transformer
-from .sampler import sample as sample_token
+from .sampler import sample as sample_token, sample_rows
 from .tokenizer import from_gguf as tokenizer_from_gguf
 
 
@@ -249,6 +249,78 @@ class Engine:
             generated.append(nxt)
             logits = self._decode_step(nxt, pos, cache, graph)
         return generated
+
+    def _capture_shared(self, ids, pos, prefix, own, workspace):
+        """decode_shared captured in a graph: (graph, its logits), or (None, None) if capture fails."""
+        try:
+            s = torch.cuda.Stream(self.device)
+            s.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(s):
+                self.model.decode_shared(ids, pos, prefix, own, workspace)
+            torch.cuda.current_stream(self.device).wait_stream(s)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                logits = self.model.decode_shared(ids, pos, prefix, own, workspace)
+            return g, logits
+        except Exception as e:  # noqa: BLE001 -- any capture failure falls back to eager
+            warnings.warn(f"decode step not captured ({e}); each token runs its launches eagerly")
+            return None, None
+
+    @torch.inference_mode()
+    def generate_many(self, ids: list[int], n: int, max_tokens: int = 64, temperature: float = 0.7,
+                      top_k: int = 0, top_p: float = 1.0, *, repetition: float = 1.0, frequency: float = 0.0,
+                      presence: float = 0.0, bias: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                      eos_id: int | None = None, generator: torch.Generator | None = None,
+                      use_graph: bool = True, cache_dtype: torch.dtype = torch.float32) -> list[list[int]]:
+        """``n`` continuations of the prompt ``ids``, up to ``max_tokens`` new ids each. The prompt is
+        prefilled once and its keys are shared by all of them (Transformer.decode_shared); the
+        penalties, ``bias`` and ``mask`` are adjust_logits' rules (repetition counts the prompt too).
+        Tokens are picked on the device; the host looks for the stop token once per ``greedy_chunk``
+        steps, and sequences that met it take no part from then on. ``cache_dtype`` float16 halves the
+        caches."""
+        if not ids or n <= 0 or max_tokens <= 0:
+            return [[] for _ in range(max(n, 0))]
+        P, c = len(ids), self.cfg
+        if P + max_tokens > c.context_len:
+            raise ValueError(f"{P} prompt + {max_tokens} new tokens exceed the model's "
+                             f"context length {c.context_len} (the RoPE table's rows)")
+        if cache_dtype not in (torch.float32, torch.float16):
+            raise ValueError("cache_dtype must be float32 or float16")
+        eos = self.tok.eos_id if eos_id is None else eos_id
+        prompt = torch.tensor(ids, device=self.device)
+        prefix = self._empty_cache(P)
+        logits = self.model.forward(prompt, torch.arange(P, device=self.device), prefix)
+        prefix = [(k.to(cache_dtype), v.to(cache_dtype)) for k, v in prefix]
+        empty = lambda: torch.zeros(n, c.n_kv_head, max_tokens, c.head_dim, device=self.device, dtype=cache_dtype)
+        own = [(empty(), empty()) for _ in range(c.n_layers)]
+        ws = K.shared_prefix_attn_workspace(n, c.n_head, c.n_kv_head, c.head_dim, P, max_tokens, self.device)
+        rules = bias is not None or mask is not None or (repetition, frequency, presence) != (1.0, 0.0, 0.0)
+        log = torch.full((n, max_tokens), -1, dtype=torch.int64, device=self.device)   # -1: no token
+        token = torch.zeros(n, dtype=torch.int64, device=self.device)
+        pos = torch.full((n,), P, dtype=torch.int64, device=self.device)
+        graph, static = self._capture_shared(token, pos, prefix, own, ws) if use_graph and max_tokens > 1 else (None, None)
+        logits = logits.expand(n, -1)
+        for t in range(max_tokens):
+            if t:
+                pos.copy_(torch.where(pos < 0, pos, torch.full_like(pos, P + t - 1)))
+                if graph is not None:
+                    graph.replay()
+                    logits = static
+                else:
+                    logits = self.model.decode_shared(token, pos, prefix, own, ws)
+            if rules:
+                logits = K.adjust_logits(logits, log[:, :t] if t else None, prompt=prompt, repetition=repetition,
+                                         frequency=frequency, presence=presence, bias=bias, mask=mask)
+            token.copy_(sample_rows(logits, temperature, top_k, top_p, generator))
+            log[:, t] = token
+            if eos is not None and (t + 1) % self.greedy_chunk == 0:
+                stopped = (log == eos).any(1)
+                pos.masked_fill_(stopped, -1)
+                if all(stopped.tolist()):
+                    break
+        out = log.tolist()
+        out = [row[:row.index(-1)] if -1 in row else row for row in out]
+        return [row[:row.index(eos)] if eos is not None and eos in row else row for row in out]
 
     @torch.inference_mode()
     def generate(self, prompt: str, max_tokens: int = 64, temperature: float = 0.7,

@@ -422,6 +422,42 @@ class Transformer:
                 x = K.qgemv(act, L.w_down, residual=x, layout=YU)
         return self._lm_head(x, self.output_norm_ut, greedy, XU)
 
+    # ---- several continuations of one prompt -----------------------------------------------
+    @torch.inference_mode()
+    def decode_shared(self, token_ids: torch.Tensor, positions: torch.Tensor,
+                      prefix: list[tuple[torch.Tensor, torch.Tensor]],
+                      own: list[tuple[torch.Tensor, torch.Tensor]],
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """One token of each of B sequences that share a prompt: ``token_ids`` (B,) at ``positions``
+        (B,) int64; per layer the prompt's caches ``prefix`` (n_kv, P, hd), as prefill leaves them,
+        and each sequence's ``own`` (B, n_kv, capacity, hd), all float32 or all float16, where
+        position p's key goes to row p - P. Logits (B, vocab). A sequence at position -1 takes no
+        part (its logits mean nothing). Reads tokens and positions from device memory only, so
+        the step can be captured and replayed."""
+        cfg = self.cfg
+        B, nh, hd = token_ids.shape[0], cfg.n_head, cfg.head_dim
+        qd, kd = nh * hd, cfg.n_kv_head * hd
+        P, capacity = prefix[0][0].shape[1], own[0][0].shape[2]
+        if workspace is None:
+            workspace = K.shared_prefix_attn_workspace(B, nh, cfg.n_kv_head, hd, P, capacity, self.device)
+        x = K.embed_gather(self.embed, token_ids)                       # (B, hidden)
+        qkv = torch.empty(B, qd + 2 * kd, device=self.device, dtype=torch.float32)
+        for L, (kp, vp), (ko, vo) in zip(self.layers, prefix, own):
+            h = K.rmsnorm(x, L.attn_norm, cfg.eps)
+            K.qgemm(h, L.wq, bias=L.bq, out=qkv[:, :qd])
+            K.qgemm(h, L.wk, bias=L.bk, out=qkv[:, qd:qd + kd])
+            K.qgemm(h, L.wv, bias=L.bv, out=qkv[:, qd + kd:])
+            q = K.rope_append(qkv, positions, (self.cos, self.sin), nh, ko, vo, slot_offset=-P)
+            attn = K.shared_prefix_attn(q, kp, vp, ko, vo, positions, own_offset=1 - P, workspace=workspace)
+            x = K.qgemm(attn.view(B, qd), L.wo, residual=x)
+            h = K.rmsnorm(x, L.ffn_norm, cfg.eps)
+            if L.w_gate_up is not None:
+                gu = K.qgemm(h, L.w_gate_up)
+            else:
+                gu = torch.cat([K.qgemm(h, L.w_gate), K.qgemm(h, L.w_up)], dim=1)
+            x = K.qgemm(K.silu_mul(gu, cfg.ffn_dim), L.w_down, residual=x)
+        return K.qgemm(K.rmsnorm(x, self.w["output_norm.weight"], cfg.eps), self.output)
+
     # ---- prefill --------------------------------------------------------------------------
     def _prefill_f16(self, token_ids, positions, cache, greedy=None):
         """The prefill on the matrix cores: GEMMs with fp16 operands and flash attention

@@ -28,3 +28,22 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p
         z[order[cut]] = float("-inf")
     probs = torch.softmax(z, dim=-1)
     return int(torch.multinomial(probs, 1, generator=generator).item())
+
+
+def sample_rows(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                generator: torch.Generator | None = None) -> torch.Tensor:
+    """``sample`` of every row of (B, V) raw ``logits``: (B,) int64 ids on the logits' device, with no
+    read back to the host. A row may hold -inf (tokens that are ruled out)."""
+    if temperature <= 0:
+        return torch.argmax(logits, dim=-1)
+    z = logits.float() / temperature
+    if top_k > 0:
+        kth = torch.topk(z, min(top_k, z.shape[-1]), dim=-1).values[:, -1:]
+        z = z.masked_fill(z < kth, float("-inf"))
+    if top_p < 1.0:
+        order = torch.argsort(z, dim=-1, descending=True)
+        probs = torch.softmax(z.gather(-1, order), dim=-1)
+        cut = torch.cumsum(probs, dim=-1) > top_p
+        cut = torch.cat([torch.zeros_like(cut[:, :1]), cut[:, :-1]], dim=-1)  # keep the token that crosses top_p
+        z = z.masked_fill(torch.zeros_like(cut).scatter(-1, order, cut), float("-inf"))
+    return torch.multinomial(torch.softmax(z, dim=-1), 1, generator=generator).squeeze(-1)
