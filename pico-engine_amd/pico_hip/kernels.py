@@ -1569,28 +1569,28 @@ _INT_CODE = {torch.int32: 1, torch.int64: 2}
 _CACHE_TYPE = {torch.float32: GGML_F32, torch.float16: GGML_F16}
 
 
-def _one_gpu(*ts: torch.Tensor | None) -> torch.device:
-    """The GPU that all the tensors are on."""
+def _one_gpu(*ts: torch.Tensor | None) -> int:
+    """The index of the GPU that all the tensors are on."""
     dev = None
     for t in ts:
-        if t is None:
-            continue
-        if dev is None:
-            dev = t.device
-            if dev.type != "cuda":
-                raise ValueError(f"pico_hip kernels need GPU tensors, got a tensor on {dev}")
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+        if t is not None:
+            i = t.get_device()
+            if i != dev:
+                if i < 0:
+                    raise ValueError(f"pico_hip kernels need GPU tensors, got a tensor on {t.device}")
+                if dev is not None:
+                    raise ValueError(f"tensors on GPU {dev} and GPU {i} in one call")
+                dev = i
     return dev
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """Calls an entry point on the tensors' device and its current stream."""
-    if dev.index == torch.cuda.current_device():
-        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _launch(dev: int, name: str, *args) -> None:
+    """Calls an entry point on GPU ``dev`` and its current stream."""
+    if dev == torch._C._cuda_getDevice():
+        status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+            status = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     if status:
         check(status, name)
 
@@ -1676,7 +1676,7 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor
     if hd > 1 and x.stride(2) != 1:
         x = x.contiguous()
     if out is None:
-        out = torch.empty(T, n, hd, device=dev, dtype=x.dtype)
+        out = x.new_empty((T, n, hd))
     elif out.dtype is not x.dtype or out.shape != x.shape or (hd > 1 and out.stride(2) != 1):
         raise ValueError(f"out must be a {x.dtype} ({T}, {n}, {hd}) tensor whose last dim is contiguous")
     if T == 0 or n == 0:
@@ -1719,7 +1719,7 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor 
         rot = _check_freqs(freqs, hd)
         table = (freqs.data_ptr(), None, None, 0)
     if out is None:
-        out = torch.empty(B, n_head, hd, device=dev, dtype=torch.float32)
+        out = qkv.new_empty((B, n_head, hd))
     elif out.dtype is not torch.float32 or tuple(out.shape) != (B, n_head, hd) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous float32 ({B}, {n_head}, {hd}) tensor")
     if B:
@@ -1756,36 +1756,39 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     own[b] + own_offset of its own (``own`` (B,) device integers, or an int for all). A sequence
     without keys, or whose own length is negative (one that takes no part), gets zeros. ``round_fp16``
     as decode_attn. Returns (B, n_head, hd) float32."""
-    dev = _one_gpu(q, k_prefix, v_prefix, k_own, v_own, own if isinstance(own, torch.Tensor) else None,
-                   prefix_len if isinstance(prefix_len, torch.Tensor) else None, workspace, out)
-    if q.dim() != 3:
-        raise ValueError("q must be a (B, n_head, hd) tensor")
+    own_dev = own if isinstance(own, torch.Tensor) else None
+    p_dev = prefix_len if isinstance(prefix_len, torch.Tensor) else None
+    dev = _one_gpu(q, k_prefix, v_prefix, k_own, v_own, own_dev, p_dev, workspace, out)
+    if q.dim() != 3 or k_prefix.dim() != 3 or k_own.dim() != 4:
+        raise ValueError("q must be (B, n_head, hd), the prefix's caches (n_kv, P, hd), the sequences' "
+                         "(B, n_kv, capacity, hd)")
     q = _f32c(q)
     B, n_head, hd = q.shape
-    n_kv, P = k_prefix.shape[0], k_prefix.shape[1]
-    code = _CACHE_TYPE.get(k_prefix.dtype)
-    cap = k_own.shape[2] if k_own.dim() == 4 else -1
-    if code is None or any(t.dtype is not k_prefix.dtype or not t.is_contiguous()
-                           for t in (k_prefix, v_prefix, k_own, v_own)) or \
-            tuple(k_prefix.shape) != (n_kv, P, hd) or v_prefix.shape != k_prefix.shape or \
-            tuple(k_own.shape) != (B, n_kv, cap, hd) or v_own.shape != k_own.shape:
+    n_kv, P, _ = k_prefix.shape
+    cap, dt = k_own.shape[2], k_prefix.dtype
+    code = _CACHE_TYPE.get(dt)
+    if code is None or not (v_prefix.dtype is dt and k_own.dtype is dt and v_own.dtype is dt and
+                            k_prefix.shape == v_prefix.shape == (n_kv, P, hd) and
+                            k_own.shape == v_own.shape == (B, n_kv, cap, hd) and
+                            k_prefix.is_contiguous() and v_prefix.is_contiguous() and
+                            k_own.is_contiguous() and v_own.is_contiguous()):
         raise ValueError(f"caches must be contiguous float32 or float16 buffers of one type: (n_kv, P, {hd}) for the "
                          f"prefix, ({B}, n_kv, capacity, {hd}) for the sequences")
     p_ptr, p_code, p_add = None, 0, P
-    if isinstance(prefix_len, torch.Tensor):
-        prefix_len = prefix_len.reshape(-1)
-        p_ptr, p_code, p_add = prefix_len.data_ptr(), _ints(prefix_len, 1, "prefix_len"), 0
+    if p_dev is not None:
+        p_dev = p_dev.reshape(-1)
+        p_ptr, p_code, p_add = p_dev.data_ptr(), _ints(p_dev, 1, "prefix_len"), 0
     elif prefix_len is not None:
         p_add = int(prefix_len)
         if not 0 <= p_add <= P:
             raise ValueError(f"prefix_len {p_add} of a prefix of {P}")
     o_ptr, o_code, o_add = None, 0, int(own_offset)
-    if isinstance(own, torch.Tensor):
+    if own_dev is not None:
         o_ptr, o_code = own.data_ptr(), _ints(own, B, "own")
     else:
         o_add += int(own)
     if out is None:
-        out = torch.empty(B, n_head, hd, device=dev, dtype=torch.float32)
+        out = torch.empty_like(q)
     elif out.dtype is not torch.float32 or tuple(out.shape) != (B, n_head, hd) or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous float32 ({B}, {n_head}, {hd}) tensor")
     if B == 0:
@@ -1793,7 +1796,7 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     need = _shared_prefix_bytes(code, B, n_head, n_kv, hd, P if p_code else p_add, cap)
     if workspace is None:
         if need:
-            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+            workspace = q.new_empty(need, dtype=torch.uint8)
     elif not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous")
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
@@ -1844,8 +1847,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     B, V = x.shape
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    rules = [(v, n) for v, n in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))]
-    dev = _one_gpu(x, history, lengths, prompt, bias, mask, out, *(v for v, _ in rules if isinstance(v, torch.Tensor)))
+    dev = _one_gpu(x, history, lengths, prompt, bias, mask, out, *[v for v in (repetition, frequency, presence)
+                                                                   if isinstance(v, torch.Tensor)])
     a = LogitArgs()
     a.type, a.x, a.batch, a.vocab = _CACHE_TYPE[x.dtype], x.data_ptr(), B, V
     a.x_stride = x.stride(0) if B > 1 else V
@@ -1862,8 +1865,9 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
             raise ValueError("prompt must hold int32 or int64 ids")
         a.prompt, a.prompt_dtype, a.prompt_len = prompt.data_ptr(), _INT_CODE[prompt.dtype], prompt.shape[-1]
         a.prompt_stride = _rows(prompt, B, prompt.shape[-1], "prompt")
-    (a.repetition_rows, a.repetition), (a.frequency_rows, a.frequency), (a.presence_rows, a.presence) = \
-        (_rule(v, B, n) for v, n in rules)
+    a.repetition_rows, a.repetition = _rule(repetition, B, "repetition")
+    a.frequency_rows, a.frequency = _rule(frequency, B, "frequency")
+    a.presence_rows, a.presence = _rule(presence, B, "presence")
     if bias is not None:
         if bias.dtype is not torch.float32:
             raise ValueError("bias must be float32")
@@ -1873,7 +1877,7 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
             raise ValueError("mask must hold int32 words")
         a.mask, a.mask_stride = mask.data_ptr(), _rows(mask, B, (V + 31) // 32, "mask")
     if out is None:
-        y = torch.empty(B, V, device=dev, dtype=x.dtype)
+        y = x.new_empty((B, V))
     else:
         y = out.unsqueeze(0) if out.dim() == 1 else out
         if y.dtype is not x.dtype or y.shape != x.shape or out.dim() != logits.dim() or (V > 1 and y.stride(1) != 1):
