@@ -947,12 +947,13 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix_few(SpArgs p
 }
 
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
-// lanes hold a row, the lane groups take every so-many-th record, four loads in flight each.
+// lanes hold a row, the lane groups take every so-many-th record, four loads in flight each, with a
+// running maximum of their own; bound by the latency of lengths and records.
 template <int HD, int W>
 __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     constexpr int L = HD / 4, N = 64 / L * W, U = 4;
     __shared__ float4 rows[4][L];
-    __shared__ float sums[4];
+    __shared__ float refs[4], sums[4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int row = __builtin_amdgcn_readfirstlane(W == 1 ? blockIdx.x * 4 + w : blockIdx.x);
     if (row >= p.batch * p.n_head) return;  // W == 1 only, uniform per wave
@@ -963,53 +964,45 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     const int no = ol > 0 ? (int)((uint32_t)(ol + p.o_keys - 1) / (uint32_t)p.o_keys) : 0;
     const int n = ol < 0 ? 0 : np + no;  // a sequence that takes no part: zeros
     const int64_t at = (int64_t)row * (p.p_chunks + p.o_chunks);
-    const auto record = [&](int i) { return at + (i < np ? i : p.p_chunks + i - np); };
     const float NEG_INF = -__builtin_huge_valf();
-    float top = NEG_INF;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, p.ml[record(i) * 2]);
-    top = wave_max<64>(top);
-    const float rs = top == NEG_INF ? 0.f : top;
+    float top = NEG_INF, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    // takes (x, y): a row over the reference r with the sum l
+    const auto take = [&](float r, float l, const float4& o) {
+        const float most = fmaxf(top, r), rs = most == NEG_INF ? 0.f : most;
+        const float a = __builtin_amdgcn_exp2f(top - rs), f = __builtin_amdgcn_exp2f(r - rs);
+        top = most;
+        sum = fmaf(f, l, a * sum);
+        v = make_float4(fmaf(f, o.x, a * v.x), fmaf(f, o.y, a * v.y), fmaf(f, o.z, a * v.z), fmaf(f, o.w, a * v.w));
+    };
     for (int i0 = (W == 1 ? 0 : w * (64 / L)) + lane / L; i0 < n; i0 += N * U) {
         float2 ml[U];
         float4 o[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + N * u;
-            const int64_t rec = record(i < n ? i : i0);
+            const int i = i0 + N * u < n ? i0 + N * u : i0;
+            const int64_t rec = at + (i < np ? i : p.p_chunks + i - np);
             ml[u] = *reinterpret_cast<const float2*>(p.ml + rec * 2);
             o[u] = *reinterpret_cast<const float4*>(p.rec + rec * HD + 4 * (lane % L));
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + N * u >= n) break;
-            const float f = __builtin_amdgcn_exp2f(ml[u].x - rs);
-            sum = fmaf(f, ml[u].y, sum);
-            v = make_float4(fmaf(f, o[u].x, v.x), fmaf(f, o[u].y, v.y), fmaf(f, o[u].z, v.z), fmaf(f, o[u].w, v.w));
-        }
+        for (int u = 0; u < U; ++u)
+            if (i0 + N * u < n) take(ml[u].x, ml[u].y, o[u]);
     }
 #pragma unroll
     for (int o = 32; o >= L; o >>= 1) {
-        sum += __shfl_xor(sum, o, kWave);
-        v.x += __shfl_xor(v.x, o, kWave);
-        v.y += __shfl_xor(v.y, o, kWave);
-        v.z += __shfl_xor(v.z, o, kWave);
-        v.w += __shfl_xor(v.w, o, kWave);
+        const float r = __shfl_xor(top, o, kWave), l = __shfl_xor(sum, o, kWave);
+        const float4 x = make_float4(__shfl_xor(v.x, o, kWave), __shfl_xor(v.y, o, kWave), __shfl_xor(v.z, o, kWave),
+                                     __shfl_xor(v.w, o, kWave));
+        take(r, l, x);
     }
     if constexpr (W > 1) {
         if (lane < L) rows[w][lane] = v;
-        if (lane == 0) sums[w] = sum;
+        if (lane == 0) refs[w] = top, sums[w] = sum;
         __syncthreads();
         if (w) return;
 #pragma unroll
-        for (int s = 1; s < W; ++s) {
-            if (lane < L) {
-                const float4 o = rows[s][lane];
-                v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
-            }
-            sum += sums[s];
-        }
+        for (int s = 1; s < W; ++s) take(refs[s], sums[s], rows[s][lane % L]);
     }
     if (lane >= L) return;
     const float4 y = n ? make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum) : v;
