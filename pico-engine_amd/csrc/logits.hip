@@ -250,6 +250,7 @@ extern "C" int pe_adjust_logits(const pe_logit_args* a, pe_stream_t stream) {
         return PE_ERR_SHAPE;
     if (a->batch == 0) return PE_OK;
     if (!a->x || !a->y) return PE_ERR_NULL;
+    if (a->x == a->y && a->batch > 1 && a->x_stride != a->y_stride) return PE_ERR_SHAPE;  // in place: the rows stay
     const size_t e = a->type == PE_TYPE_F16 ? 2 : 4;
     const auto wide = [](int dtype) { return dtype == 2; };
     if (!aligned(a->x, e) || !aligned(a->y, e) || !aligned(a->history, wide(a->history_dtype) ? 8 : 4) ||

@@ -278,6 +278,8 @@ extern "C" int pe_rope_positions(int type, const void* x, int64_t x_token, int64
         return PE_ERR_SHAPE;
     if (tokens == 0) return PE_OK;
     if (!x || !positions || !freqs || !y) return PE_ERR_NULL;
+    // in place, every element has to stay where it is
+    if (x == y && ((tokens > 1 && x_token != y_token) || (n_head > 1 && x_head != y_head))) return PE_ERR_SHAPE;
     const size_t e = elem_size(type);
     if (!aligned(x, e) || !aligned(y, e) || !aligned(positions, pos_dtype == 2 ? 8 : 4) || !aligned(freqs, 8))
         return PE_ERR_ALIGN;

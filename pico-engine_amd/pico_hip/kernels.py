@@ -1664,8 +1664,8 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor
                    interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """RoPE of x (T, n_head, hd), float32 or float16 (rows and heads with any strides), token t at
     positions[t] (int32 or int64, any order, negative ones turn back): pairs (j, j + r/2) of the first
-    r = 2 len(freqs) elements of a head, or (2j, 2j + 1) if ``interleaved``; the others are copied.
-    freqs and amp from rope_freqs; the angles are made in 64 bits. ``out`` may be x."""
+    r = 2 len(freqs) elements of a head, or (2j, 2j + 1) if ``interleaved``; the others are copied. Up
+    to 4096 heads. freqs and amp from rope_freqs; the angles are made in 64 bits. ``out`` may be x."""
     dev = _one_gpu(x, positions, freqs, out)
     code = _CACHE_TYPE.get(x.dtype)
     if code is None or x.dim() != 3:
@@ -1839,7 +1839,7 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     presence; -inf where the mask bit is 0. history (B, H) int32 or int64, of which the first
     ``lengths`` (B,) count (None: all); prompt, bias (float32, V) and mask (int32 words, bit v % 32 of
     word v // 32) one row for all or a row each. Ids outside [0, V) are passed over. The three
-    penalties are numbers or float32 vectors of one value per row. ``out`` may be logits."""
+    penalties are numbers or float32 vectors of one value per row. ``out`` may be logits. A row whose tokens are all ruled out is -inf throughout."""
     one = logits.dim() == 1
     x = logits.unsqueeze(0) if one else logits
     if x.dtype not in _CACHE_TYPE or x.dim() != 2 or x.shape[1] == 0:
@@ -1861,8 +1861,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     if lengths is not None:
         a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
     if prompt is not None:
-        if prompt.dtype not in _INT_CODE:
-            raise ValueError("prompt must hold int32 or int64 ids")
+        if prompt.dtype not in _INT_CODE or prompt.dim() == 0:
+            raise ValueError("prompt must be a vector or rows of int32 or int64 ids")
         a.prompt, a.prompt_dtype, a.prompt_len = prompt.data_ptr(), _INT_CODE[prompt.dtype], prompt.shape[-1]
         a.prompt_stride = _rows(prompt, B, prompt.shape[-1], "prompt")
     a.repetition_rows, a.repetition = _rule(repetition, B, "repetition")

@@ -23,7 +23,7 @@ def test_rope_positions(lib):
         assert call(**kw) == 2, kw
     for kw in (dict(tokens=-1), dict(n_head=0), dict(n_head=4097), dict(hd=0), dict(rot=0), dict(rot=63), dict(rot=66),
                dict(y_token=63), dict(y_head=63), dict(y_token=64, y_head=64), dict(y_token=100), dict(x_token=-1),
-               dict(y_token=0), dict(y_head=0)):
+               dict(y_token=0), dict(y_head=0), dict(x_token=192), dict(x_head=0), dict(y_token=64, y_head=256)):
         assert call(**kw) == 3, kw
     for name in ("x", "positions", "freqs", "y"):
         assert call(**{name: None}) == 1, name
@@ -94,7 +94,8 @@ def test_adjust_logits(lib):
     for kw in (dict(type=2), dict(history_dtype=0), dict(lengths_dtype=3), dict(prompt_dtype=0)):
         assert call(**kw) == 2, kw
     for kw in (dict(batch=-1), dict(vocab=0), dict(vocab=1 << 31), dict(y_stride=99), dict(x_stride=-1), dict(history_len=-1),
-               dict(prompt_len=1 << 31), dict(history_stride=-1), dict(bias_stride=-1), dict(mask_stride=-1)):
+               dict(prompt_len=1 << 31), dict(history_stride=-1), dict(bias_stride=-1), dict(mask_stride=-1),
+               dict(x_stride=101), dict(x_stride=0)):
         assert call(**kw) == 3, kw
     for name in ("x", "y"):
         assert call(**{name: None}) == 1, name
