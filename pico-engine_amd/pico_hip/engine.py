@@ -253,14 +253,15 @@ class Engine:
     def _capture_shared(self, ids, pos, prefix, own, workspace):
         """decode_shared captured in a graph: (graph, its logits), or (None, None) if capture fails."""
         try:
-            s = torch.cuda.Stream(self.device)
-            s.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(s):
-                self.model.decode_shared(ids, pos, prefix, own, workspace)
-            torch.cuda.current_stream(self.device).wait_stream(s)
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                logits = self.model.decode_shared(ids, pos, prefix, own, workspace)
+            with torch.cuda.device(self.device):
+                s = torch.cuda.Stream(self.device)
+                s.wait_stream(torch.cuda.current_stream(self.device))
+                with torch.cuda.stream(s):
+                    self.model.decode_shared(ids, pos, prefix, own, workspace)
+                torch.cuda.current_stream(self.device).wait_stream(s)
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    logits = self.model.decode_shared(ids, pos, prefix, own, workspace)
             return g, logits
         except Exception as e:  # noqa: BLE001 -- any capture failure falls back to eager
             warnings.warn(f"decode step not captured ({e}); each token runs its launches eagerly")
@@ -277,7 +278,7 @@ class Engine:
         penalties, ``bias`` and ``mask`` are adjust_logits' rules (repetition counts the prompt too).
         Tokens are picked on the device; the host looks for the stop token once per ``greedy_chunk``
         steps, and sequences that met it take no part from then on. ``cache_dtype`` float16 halves the
-        caches."""
+        caches. For models with heads of 64 or 128; bias and mask must leave every sequence a token."""
         if not ids or n <= 0 or max_tokens <= 0:
             return [[] for _ in range(max(n, 0))]
         P, c = len(ids), self.cfg
@@ -286,6 +287,8 @@ class Engine:
                              f"context length {c.context_len} (the RoPE table's rows)")
         if cache_dtype not in (torch.float32, torch.float16):
             raise ValueError("cache_dtype must be float32 or float16")
+        if c.head_dim not in (64, 128):
+            raise ValueError(f"generate_many needs heads of 64 or 128, the model's have {c.head_dim}")
         eos = self.tok.eos_id if eos_id is None else eos_id
         prompt = torch.tensor(ids, device=self.device)
         prefix = self._empty_cache(P)
@@ -311,10 +314,12 @@ class Engine:
             if rules:
                 logits = K.adjust_logits(logits, log[:, :t] if t else None, prompt=prompt, repetition=repetition,
                                          frequency=frequency, presence=presence, bias=bias, mask=mask)
+                if t == 0 and not bool((logits > float("-inf")).any(-1).all()):
+                    raise ValueError("bias and mask rule out every token of a sequence")
             token.copy_(sample_rows(logits, temperature, top_k, top_p, generator))
             log[:, t] = token
             if eos is not None and (t + 1) % self.greedy_chunk == 0:
-                stopped = (log == eos).any(1)
+                stopped = (log[:, :t + 1] == eos).any(1)
                 pos.masked_fill_(stopped, -1)
                 if all(stopped.tolist()):
                     break

@@ -432,7 +432,7 @@ class Transformer:
         (B,) int64; per layer the prompt's caches ``prefix`` (n_kv, P, hd), as prefill leaves them,
         and each sequence's ``own`` (B, n_kv, capacity, hd), all float32 or all float16, where
         position p's key goes to row p - P. Logits (B, vocab). A sequence at position -1 takes no
-        part (its logits mean nothing). Reads tokens and positions from device memory only, so
+        part (its logits mean nothing). Heads of 64 or 128. Reads tokens and positions from device memory only, so
         the step can be captured and replayed."""
         cfg = self.cfg
         B, nh, hd = token_ids.shape[0], cfg.n_head, cfg.head_dim

@@ -33,7 +33,9 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p
 def sample_rows(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                 generator: torch.Generator | None = None) -> torch.Tensor:
     """``sample`` of every row of (B, V) raw ``logits``: (B,) int64 ids on the logits' device, with no
-    read back to the host. A row may hold -inf (tokens that are ruled out)."""
+    read back to the host. A row may hold -inf (tokens that are ruled out); one that holds nothing else
+    gives id 0. The draw is a race of exponential times, of which token v's ends first with
+    probability p_v (torch.multinomial reads its probabilities back to check them)."""
     if temperature <= 0:
         return torch.argmax(logits, dim=-1)
     z = logits.float() / temperature
@@ -46,4 +48,6 @@ def sample_rows(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, 
         cut = torch.cumsum(probs, dim=-1) > top_p
         cut = torch.cat([torch.zeros_like(cut[:, :1]), cut[:, :-1]], dim=-1)  # keep the token that crosses top_p
         z = z.masked_fill(torch.zeros_like(cut).scatter(-1, order, cut), float("-inf"))
-    return torch.multinomial(torch.softmax(z, dim=-1), 1, generator=generator).squeeze(-1)
+    probs = torch.softmax(z, dim=-1)
+    times = torch.empty_like(probs).exponential_(generator=generator).clamp_(min=torch.finfo(probs.dtype).tiny)
+    return torch.argmax(probs / times, dim=-1)

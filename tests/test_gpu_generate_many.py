@@ -137,6 +137,50 @@ def test_generate_many_stops_and_samples(eng):
         eng.generate_many(ids, 2, 4, cache_dtype=torch.bfloat16)
 
 
+def test_generate_many_refuses_masks_that_leave_nothing(eng):
+    mask = torch.full((2, 32), -1, dtype=torch.int32, device=DEV)
+    mask[1] = 0
+    bias = torch.full((1024,), -math.inf, device=DEV)
+    for rules in (dict(mask=mask), dict(bias=bias)):
+        with pytest.raises(ValueError):
+            eng.generate_many([3, 4, 5], 2, 4, temperature=1.0, eos_id=-2, **rules)
+    mask[1, 3] = 1 << 9             # one token is left
+    got = eng.generate_many([3, 4, 5], 2, 4, temperature=1.0, eos_id=-2, mask=mask)
+    assert got[1] == [3 * 32 + 9] * 4 and len(got[0]) == 4
+
+
+def test_generate_many_stop_token_that_never_comes(eng):
+    """An id that no token has, -1 among them, stops nothing."""
+    n = eng.greedy_chunk + 5
+    want = eng.generate_many([3, 4, 5], 2, n, temperature=0.0, eos_id=-2)
+    assert [len(r) for r in want] == [n, n]
+    assert eng.generate_many([3, 4, 5], 2, n, temperature=0.0, eos_id=-1) == want
+
+
+def test_sample_rows_does_not_wait_for_the_gpu():
+    from pico_hip.sampler import sample_rows
+    z = torch.randn(4, 300, device=DEV)
+    z[3] = -math.inf
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        picks = [sample_rows(z, **kw) for kw in (dict(temperature=0.0), dict(temperature=0.7), dict(temperature=0.7, top_k=5),
+                                                 dict(temperature=0.7, top_p=0.9))]
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    assert all(0 <= v < 300 for p in picks for v in p.tolist()) and all(int(p[3]) == 0 for p in picks)
+
+
+def test_sample_rows_draws_by_the_probabilities():
+    """20000 draws of 5 tokens: every count within 5 standard deviations, sqrt(n p (1 - p)), of n p."""
+    from pico_hip.sampler import sample_rows
+    p, n = torch.tensor([0.5, 0.25, 0.15, 0.1, 0.0]), 20000
+    picks = sample_rows(p.log().to(DEV).expand(n, 5), generator=torch.Generator(DEV).manual_seed(5))
+    counts = torch.bincount(picks.cpu(), minlength=5).double()
+    assert int(counts[4]) == 0 and bool(((counts - n * p).abs() <= 5 * (n * p * (1 - p)).sqrt()).all())
+
+
 def test_sample_rows_matches_sample():
     from pico_hip.sampler import sample, sample_rows
     z = torch.randn(6, 500, device=DEV) * 3
