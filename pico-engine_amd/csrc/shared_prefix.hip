@@ -18,9 +18,20 @@
 // these row counts). All others run on v_mfma_f32_32x32x16_f16 with the fp32 factors as the sum of
 // two fp16 values, 22 bits (one would cost 2^-12 of each): the query, scaled by a power of two to at
 // most 2^14; the probability; and an fp32 cache's keys and values, every 8 keys scaled by a
-// power of two of their largest element. Products of two low parts are left out (2^-22). That is 2
-// instructions for 16-bit caches and 3 for fp32 ones in place of 16 fp32 instructions of twice the
-// time each.
+// power of two of their largest element. Products of two low parts are left out (2^-22). Per 16 elements of
+// a dot product that is 2 instructions for 16-bit caches and 3 for fp32 ones in place of 8 fp32 instructions
+// of twice the time each.
+//
+// Bounds and times (heads 28/4 of 128, then 14/2 of 64; us, the merge after the +):
+//   64 sequences, 32768 fp16 keys, 1000 own: 79 + 6. The matrix cores; a shared block in steady state
+//     keeps them at 1.22 PFLOP/s (a large library product reaches 1.18); the own keys stream at 4.7 to
+//     5.5 TB/s, about 10 us are a workgroup's start and end;
+//   33 sequences, 8001 fp32 keys, 515 own: 32 + 5. The matrix cores at 0.92 PFLOP/s in a shared
+//     block, whose split into fp16 parts and softmax (4000 of 8500 cycles) fill the rest;
+//   3 sequences, 32768 fp16 keys: 9 + 4; 16 sequences, 1500 fp32 keys: 8.6 + 4.1; 4 sequences, 277 fp32
+//     keys: 9.0 in one launch. Latency: lengths, first tiles, a block or two, records.
+// Tried without gain: key rows swizzled over all 64 banks and both exponents of a group reduced at once
+// (the same times), a group's loads from a scalar base (49 registers spilled, 31 -> 49 us).
 #include "pe_common.h"
 
 namespace pe {
@@ -948,7 +959,8 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix_few(SpArgs p
 
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
 // lanes hold a row, the lane groups take every so-many-th record, four loads in flight each, with a
-// running maximum of their own; bound by the latency of lengths and records.
+// running maximum of their own; bound by the latency of lengths and records (14 heads x 16 sequences x
+// 25 records of 64: 4.1 us; 28 x 64 x 15 of 128: 6.0, 14 x 3 x 65 of 64: 4.4).
 template <int HD, int W>
 __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     constexpr int L = HD / 4, N = 64 / L * W, U = 4;
