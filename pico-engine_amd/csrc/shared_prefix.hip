@@ -30,8 +30,8 @@
 //     block, whose split into fp16 parts and softmax (4000 of 8500 cycles) fill the rest;
 //   3 sequences, 32768 fp16 keys: 9 + 4; 16 sequences, 1500 fp32 keys: 8.6 + 4.1; 4 sequences, 277 fp32
 //     keys: 9.0 in one launch. Latency: lengths, first tiles, a block or two, records.
-// Tried without gain: key rows swizzled over all 64 banks and both exponents of a group reduced at once
-// (the same times), a group's loads from a scalar base (49 registers spilled, 31 -> 49 us).
+// Tried without gain: key rows swizzled over all 64 banks; the barrier of a block between softmax and
+// values, so that values and the next scores run back to back (30.3 for 28.9 us, fp16 85 for 75).
 #include "pe_common.h"
 
 namespace pe {
@@ -89,6 +89,10 @@ PE_DEV uint32_t lds_address(const uint8_t* p) {
 PE_DEV void sp_load16(const void* g, uint32_t off, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0)
                  : "memory", "m0");
+}
+// the same from an address per lane
+PE_DEV void sp_load16(const float* g, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
 }
 template <int N>
 PE_DEV void sp_wait_loads() {
@@ -184,6 +188,26 @@ PE_DEV h8v transposed(uint32_t a) {
     return __builtin_bit_cast(h8v, v);
 }
 
+// A wave's share, ROWS, of a workgroup's queries into an LDS image of rows of HD floats, chunk c of row r
+// at c ^ (r & 7): rows [first, first + ROWS) of the kv head, of which `rows` are there (the last one
+// stands in for the others). Read by each lane for itself, 32 rows an instruction, they took 3 of a
+// workgroup's first 6 us.
+template <int HD, int ROWS>
+PE_DEV void sp_stage_queries(const SpArgs& p, int j, int first, int rows, uint32_t lds, int lane) {
+    constexpr int C = HD / 4, R = 64 / C;
+    int r = first + lane / C;
+    int seq = r / p.group, head = r - seq * p.group;
+#pragma unroll
+    for (int f = 0; f < ROWS / R; ++f) {
+        const bool there = r < rows;
+        const int64_t row = there ? (int64_t)seq * p.n_head + j * p.group + head : (int64_t)p.batch * p.n_head - p.n_head + (j + 1) * p.group - 1;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(lds + f * 1024);
+        sp_load16(p.q + row * HD + ((lane % C) ^ (r & 7)) * 4, at);
+        r += R;
+        for (head += R; head >= p.group; head -= p.group) ++seq;
+    }
+}
+
 // A wave's 32 queries as matrix operands and the products with a tile of 32 keys. One lane: query
 // (or key, or dim) li = lane & 31, half g = lane >> 5. Register r of the scores is key
 // 8 (r / 4) + 4 g + r % 4; they have to be multiplied by `unscale`.
@@ -191,10 +215,11 @@ template <int HD>
 struct RowsF32 {
     static constexpr float unscale = 1.f;
     float4 q[HD / 8];
-    PE_DEV void load(const float* row, float scale, int g) {
+    // row r of an image of queries (sp_stage_queries)
+    PE_DEV void load(const uint8_t* image, int r, float scale, int g) {
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) {
-            q[j] = row ? *reinterpret_cast<const float4*>(row + 8 * j + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
+            q[j] = *reinterpret_cast<const float4*>(image + r * (HD * 4) + ((2 * j + g) ^ (r & 7)) * 16);
             q[j].x *= scale;
             q[j].y *= scale;
             q[j].z *= scale;
@@ -232,13 +257,13 @@ template <int HD>
 struct RowsF16 {
     h8v hi[HD / 16], lo[HD / 16];
     float unscale;
-    PE_DEV void load(const float* row, float scale, int g) {
+    PE_DEV void load(const uint8_t* image, int r, float scale, int g) {
         float v[HD / 2], top = 0.f;
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-                const float4 x = row ? *reinterpret_cast<const float4*>(row + 16 * j + 8 * g + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 x = *reinterpret_cast<const float4*>(image + r * (HD * 4) + ((4 * j + 2 * g + i / 4) ^ (r & 7)) * 16);
                 v[8 * j + i] = x.x;
                 v[8 * j + i + 1] = x.y;
                 v[8 * j + i + 2] = x.z;
@@ -264,9 +289,10 @@ struct RowsF16 {
             }
     }
     // LOW: bytes from a tile to its low parts, 0: it has none. Four operands are in flight: each one's
-    // registers take the fourth next as soon as its products have read them.
-    template <int LOW>
-    PE_DEV f16v scores(const uint8_t* kt, int li, int g) const {
+    // registers take the fourth next as soon as its products have read them. beside(i): work for the
+    // vector units while the i-th operand's products run.
+    template <int LOW, typename F>
+    PE_DEV f16v scores(const uint8_t* kt, int li, int g, const F& beside) const {
         constexpr int J = HD / 16, N = LOW ? 2 * J : J;
         const uint8_t* at = kt + li * (HD * 2);
         const int x = (g ^ (li & 7)) * 16;  // chunk 2 j + g: j flips bits above g's
@@ -280,6 +306,7 @@ struct RowsF16 {
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 3], hi[i % J], s, 0, 0, 0);
             if (i < J) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 3], lo[i % J], s, 0, 0, 0);
             if (i + 4 < N) k[i & 3] = operand(i + 4);
+            beside(i);
             __builtin_amdgcn_sched_barrier(0);
         }
         return s;
@@ -302,8 +329,8 @@ struct RowsF16 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = values_of<LOW>(at, i);
     }
-    template <int LOW>
-    static PE_DEV void accumulate(uint32_t at, h8v* v, const f16v& p, f16v* o) {
+    template <int LOW, typename F>
+    static PE_DEV void accumulate(uint32_t at, h8v* v, const f16v& p, f16v* o, const F& beside) {
         constexpr int D = HD / 32, P = LOW ? 2 : 1, N = 2 * D * P;
         h8v ph[2], pl[2];
 #pragma unroll
@@ -319,6 +346,7 @@ struct RowsF16 {
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 3], ph[b], o[d], 0, 0, 0);
             if (!low) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 3], pl[b], o[d], 0, 0, 0);
             if (i + 4 < N) v[i & 3] = values_of<LOW>(at, i + 4);
+            beside(i);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -484,76 +512,87 @@ struct OwnRows<_Float16, HD> {
     }
 };
 
-// An fp32 cache's share of a 64-key block on its way through a wave's registers: 8 keys and their
-// values, split into two fp16 parts each.
-template <int HD>
+// A wave's 8 keys, or their values, of a 64-key block of an fp32 cache on their way through its registers
+// into two fp16 parts each, in kSteps steps that go beside the products with the block before.
+template <int HD, bool VALUES>
 struct SpSplit {
-    static constexpr int N = HD / 32, R = 256 / HD, kPlane = kSpBlock * HD * 2;
-    float4 k[N], v[N];
-    // the wave's 8 rows of the block that starts at kb and vb, rows behind `last` are that one again
-    PE_DEV void load(const float* kb, const float* vb, int64_t last, int w, int lane) {
-        const bool whole = last >= 8 * w + 7;
-#pragma unroll
-        for (int f = 0; f < N; ++f) {
-            int at = (8 * w * HD + 256 * f) / 4 + lane;
-            if (!whole) {
-                const int r = 8 * w + R * f + lane / (HD / 4);
-                at = (r < (int)last ? r : (int)last) * (HD / 4) + lane % (HD / 4);
-            }
-            k[f] = reinterpret_cast<const float4*>(kb)[at];
-            v[f] = reinterpret_cast<const float4*>(vb)[at];
-        }
-    }
-    // E with the largest finite element in [2^(14 + E), 2^(15 + E)): the two parts hold every element to
-    // 2^-23 of itself or 2^-39 of the largest
-    static PE_DEV int exponent(const float4* x) {
-        float top = 0.f;
-#pragma unroll
-        for (int f = 0; f < N; ++f) {
-            top = fmaxf(fmaxf(top, fabsf(x[f].x)), fabsf(x[f].y));
-            top = fmaxf(fmaxf(top, fabsf(x[f].z)), fabsf(x[f].w));
-        }
-        uint32_t bits = wave_max_bits(__float_as_uint(top));
-        if (bits >= 0x7F800000u) {  // infinities: the largest of the others (x + 0 x is NaN for those)
-            top = 0.f;
-#pragma unroll
-            for (int f = 0; f < N; ++f) {
-                top = fmaxf(fmaxf(top, fabsf(fmaf(x[f].x, 0.f, x[f].x))), fabsf(fmaf(x[f].y, 0.f, x[f].y)));
-                top = fmaxf(fmaxf(top, fabsf(fmaf(x[f].z, 0.f, x[f].z))), fabsf(fmaf(x[f].w, 0.f, x[f].w)));
-            }
-            bits = wave_max_bits(__float_as_uint(top));
-        }
-        const int e = (int)(bits >> 23) - 127;
-        return (e < -100 ? -100 : e) - 14;
-    }
-    template <bool VALUES>
-    static PE_DEV void store(const float4* x, float f, uint8_t* plane, int w, int lane) {
+    static constexpr int N = HD / 32, R = 256 / HD, kPlane = kSpBlock * HD * 2, kSteps = HD / 8;
+    float4 x[N];
+    uint32_t top;
+    float f;
+    h2v h0, l0;
+    // the wave's 8 rows of the block at base, which holds n keys; the rows behind them are zeros
+    PE_DEV void load(const float* base, int n, int w, int lane) {
+        typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+        const auto all = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, n * (HD * 4), 0x00020000);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = 8 * w + R * i + lane / (HD / 4), c4 = lane % (HD / 4);
-            h2v h0, l0, h1, l1;
-            split2(x[i].x * f, x[i].y * f, h0, l0);
-            split2(x[i].z * f, x[i].w * f, h1, l1);
-            const h4v hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
-            uint8_t* at = plane + row * (HD * 2) + ((c4 >> 1) ^ sp_swizzle<2, VALUES>(row)) * 16 + (c4 & 1) * 8;
-            *reinterpret_cast<h4v*>(at) = hi;
-            *reinterpret_cast<h4v*>(at + kPlane) = lo;
+            const u4v y = __builtin_amdgcn_raw_buffer_load_b128(all, 8 * w * (HD * 4) + 16 * lane + 1024 * i, 0, 0);
+            x[i] = __builtin_bit_cast(float4, y);
         }
     }
-    // planes: K high, K low, V high, V low; e: exponents of the block's 8 key groups, then of their
-    // values. n: keys of the block, the values behind them are cleared.
-    PE_DEV void convert(uint8_t* planes, int* e, int n, int w, int lane) {
-        if (n < kSpBlock) {
+    // The exponent E with the largest finite element in [2^(14 + E), 2^(15 + E)): the two parts hold every
+    // element to 2^-23 of itself or 2^-39 of the largest. Eight stages.
+    PE_DEV void find(int stage, int* e) {
+        if (stage == 0) {
+            float m = 0.f;
 #pragma unroll
-            for (int f = 0; f < N; ++f)
-                if (8 * w + R * f + lane / (HD / 4) >= n) v[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < N; ++i) {
+                m = fmaxf(fmaxf(m, fabsf(x[i].x)), fabsf(x[i].y));
+                m = fmaxf(fmaxf(m, fabsf(x[i].z)), fabsf(x[i].w));
+            }
+            top = __float_as_uint(m);
         }
-        const int ek = exponent(k), ev = exponent(v);
-        store<false>(k, exp2_int(-ek), planes, w, lane);
-        store<true>(v, exp2_int(-ev), planes + 2 * kPlane, w, lane);
-        if (lane == 0) {
-            e[w] = ek;
-            e[8 + w] = ev;
+        if (stage == 1) top = dpp_max<0xB1>(top);   // quad_perm [1,0,3,2]
+        if (stage == 2) top = dpp_max<0x4E>(top);   // quad_perm [2,3,0,1]
+        if (stage == 3) top = dpp_max<0x141>(top);  // row_half_mirror
+        if (stage == 4) top = dpp_max<0x140>(top);  // row_mirror
+        if (stage == 5) {
+            const auto a = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = a[0] > a[1] ? a[0] : a[1];
+        }
+        if (stage == 6) {
+            const auto a = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = __builtin_amdgcn_readfirstlane(a[0] > a[1] ? a[0] : a[1]);
+        }
+        if (stage == 7) {
+            if (top >= 0x7F800000u) {  // infinities: the largest of the others (x + 0 x is NaN for those)
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    m = fmaxf(fmaxf(m, fabsf(fmaf(x[i].x, 0.f, x[i].x))), fabsf(fmaf(x[i].y, 0.f, x[i].y)));
+                    m = fmaxf(fmaxf(m, fabsf(fmaf(x[i].z, 0.f, x[i].z))), fabsf(fmaf(x[i].w, 0.f, x[i].w)));
+                }
+                top = wave_max_bits(__float_as_uint(m));
+            }
+            int k = (int)(top >> 23) - 127;
+            k = (k < -100 ? -100 : k) - 14;
+            f = exp2_int(-k);
+            if ((threadIdx.x & 63) == 0) *e = k;
+        }
+    }
+    // Where a lane's half chunk of the wave's first rows goes in a plane; those of piece i lie i R rows on, at
+    // the chunk with other bits flipped (sp_swizzle).
+    static PE_DEV uint32_t place(int w, int lane) {
+        const int row = 8 * w + lane / (HD / 4), c4 = lane % (HD / 4);
+        return row * (HD * 2) + ((c4 >> 1) ^ sp_swizzle<2, VALUES>(row)) * 16 + (c4 & 1) * 8;
+    }
+    // step i: planes: LDS address of the high parts, the low ones behind them; e: the group's exponent
+    PE_DEV void step(int i, uint32_t planes, uint32_t place, int* e) {
+        constexpr int H = kSteps / 2;
+        if (i < H) {
+#pragma unroll
+            for (int k = 8 / H * i; k < 8 / H * (i + 1); ++k) find(k, e);
+        } else if (const int n = (i - H) >> 1; (i - H) & 1) {
+            h2v h1, l1;
+            split2(x[n].z * f, x[n].w * f, h1, l1);
+            const h4v hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
+            typedef __attribute__((address_space(3))) h4v lds_h4;
+            const uint32_t at = planes + (place ^ (16 * sp_swizzle<2, VALUES>(R * n))) + R * n * (HD * 2);
+            *(lds_h4*)(uintptr_t)at = hi;
+            *(lds_h4*)(uintptr_t)(at + kPlane) = lo;
+        } else {
+            split2(x[n].x * f, x[n].y * f, h0, l0);
         }
     }
 };
@@ -753,7 +792,7 @@ PE_DEV f16v sp_scores(const RowsF32<HD>& q, const uint8_t* kt, int li, int g) {
 }
 template <int HD>
 PE_DEV f16v sp_scores(const RowsF16<HD>& q, const uint8_t* kt, int li, int g) {
-    return q.template scores<0>(kt, li, g);
+    return q.template scores<0>(kt, li, g, [](int) {});
 }
 template <int HD>
 PE_DEV void sp_accumulate(const RowsF32<HD>&, const uint8_t* vt, const f16v& s, f16v* o, int li, int g) {
@@ -764,7 +803,7 @@ PE_DEV void sp_accumulate(const RowsF16<HD>&, const uint8_t* vt, const f16v& s, 
     const uint32_t va = RowsF16<HD>::values_at(vt, li, g);
     h8v v[4];
     RowsF16<HD>::template load_values<0>(va, v);
-    RowsF16<HD>::template accumulate<0>(va, v, s, o);
+    RowsF16<HD>::template accumulate<0>(va, v, s, o, [](int) {});
 }
 
 template <typename T, int HD>
@@ -777,7 +816,11 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     // shared: two buffers of a block's planes
     constexpr int kPlane = kSpBlock * HD * 2, kPlanes = (kHalf ? 2 : 4) * kPlane, kLow = kHalf ? 0 : kPlane;
     constexpr int kMerge = kSpWaves * 32 * (HD + 4) * 4;
-    constexpr int kSolo = kSpWaves * kWaveLds, kMost = kSolo > 2 * kPlanes ? kSolo : 2 * kPlanes;
+    // the queries' image, read before the loops: shared, fp32: the second buffer, else behind the tiles
+    constexpr int kQueries = kHalf ? 2 * kPlanes : kPlanes, kSolo = kSpWaves * kWaveLds;
+    constexpr int kShared = kHalf ? kQueries + 128 * HD * 4 : 2 * kPlanes, kAlone = kSolo + 32 * HD * 4;
+    constexpr int kMost = kAlone > kShared ? kAlone : kShared;
+    static_assert(kQueries + 128 * HD * 4 <= kMost, "the queries' image");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kMost > kMerge ? kMost : kMerge];
     __shared__ float ref[kSpWaves][32], sums[kSpWaves][32];
     __shared__ int exps[2][16], row_of[kSpWaves][32];
@@ -803,19 +846,21 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     // the lane's query: row r of the kv head is (sequence r / group, head r % group of the kv head's)
     const int seq = (row0 + li) / p.group;
     const int my_row = seq * p.n_head + j * p.group + (row0 + li - seq * p.group);
-    const float* qrow = row0 + li < rows ? p.q + (int64_t)my_row * HD : nullptr;
     SpState<HD> st;
     st.clear();
     int top = 0;  // exponent of the values that o holds
 
     if (shared) {
         RowsF16<HD> q;
+        const uint8_t* const image = lds + kQueries;
+        sp_stage_queries<HD, 16>(p, j, 128 * tile + 16 * w, rows, lds_address(image) + 16 * w * (HD * 4), lane);
         const int blocks = (keys + kSpBlock - 1) / kSpBlock;
-        const auto take = [&](int t) {
+        // the products with block t; kbeside, vbeside: work beside them
+        const auto take = [&](int t, const auto& kbeside, const auto& vbeside) {
             const uint8_t* kt = lds + (t & 1) * kPlanes + 32 * sub * (HD * 2);
             // no branch round waves without rows or keys: o would be copied on every way
             const int n = keys - kSpBlock * t - 32 * sub;
-            f16v s = q.template scores<kLow>(kt, li, g);
+            f16v s = q.template scores<kLow>(kt, li, g, kbeside);
             float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
             int ev[4], shift = 0;
             if constexpr (!kHalf) {
@@ -841,7 +886,7 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
                     for (int i = 0; i < 16; ++i) s[i] *= ldexpf(1.f, ev[i >> 2] - top);
                 }
             }
-            RowsF16<HD>::template accumulate<kLow>(va, v, s, st.o);
+            RowsF16<HD>::template accumulate<kLow>(va, v, s, st.o, vbeside);
         };
         if constexpr (kHalf) {
             constexpr int N = kPlane / 1024 / kSpWaves;
@@ -852,7 +897,9 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
                 sp_stage<T, HD, true, N>(vb + row * HD, last - row, at + kPlane, lane, w * N);
             };
             stage(0);
-            q.load(qrow, p.scale, g);
+            sp_wait_loads<0>();
+            __syncthreads();
+            q.load(image, 32 * item + li, p.scale, g);
             for (int t = 0; t < blocks; ++t) {
                 sp_wait_loads<0>();
                 __syncthreads();  // the block is there, and nobody reads the other buffer any more
@@ -862,39 +909,57 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
                     sp_clear_rows<HD * 2>(lds + (t & 1) * kPlanes + kPlane, n, kSpBlock, threadIdx.x, 64 * kSpWaves);
                     __syncthreads();
                 }
-                take(t);
+                take(t, [](int) {}, [](int) {});
             }
         } else {
-            SpSplit<HD> x;
-            const auto load = [&](int t) {
-                const int64_t row = k0 + kSpBlock * t;
-                x.load(kb + row * HD, vb + row * HD, last - row, w, lane);
+            SpSplit<HD, false> xk;
+            SpSplit<HD, true> xv;
+            const uint32_t k_place = xk.place(w, lane), v_place = xv.place(w, lane) + 2 * kPlane;
+            const auto planes = [&](int t) { return lds_address(lds) + (t & 1) * kPlanes; };
+            const auto left = [&](int t) { return keys - kSpBlock * t < kSpBlock ? keys - kSpBlock * t : kSpBlock; };
+            const auto k_step = [&](int t, int i) { xk.step(i, planes(t), k_place, &exps[t & 1][w]); };
+            const auto v_step = [&](int t, int i) { xv.step(i, planes(t), v_place, &exps[t & 1][8 + w]); };
+            const auto k_load = [&](int t) {
+                if (t < blocks) xk.load(kb + (k0 + kSpBlock * t) * HD, left(t), w, lane);
             };
-            const auto convert = [&](int t) {
-                const int n = keys - kSpBlock * t;
-                x.convert(lds + (t & 1) * kPlanes, exps[t & 1], n < kSpBlock ? n : kSpBlock, w, lane);
-                if (t + 1 < blocks) load(t + 1);
+            const auto v_load = [&](int t) {
+                if (t < blocks) xv.load(vb + (k0 + kSpBlock * t) * HD, left(t), w, lane);
             };
-            load(0);
-            q.load(qrow, p.scale, g);
-            convert(0);
+            k_load(0);
+            v_load(0);
+            sp_wait_loads<0>();
+            __syncthreads();
+            q.load(image, 32 * item + li, p.scale, g);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                k_step(0, i);
+                v_step(0, i);
+            }
+            k_load(1);
+            v_load(1);
             for (int t = 0; t < blocks; ++t) {
                 __syncthreads();  // block t is there, and nobody reads the other buffer any more
-                // half of the waves split the next block while the others are at their products
-                if (sub == 0 && t + 1 < blocks) convert(t + 1);
-                take(t);
-                if (sub == 1 && t + 1 < blocks) convert(t + 1);
+                // beside its products the next block is split (behind the last one, that one again)
+                take(
+                    t,
+                    [&](int i) {
+                        k_step(t + 1, i);
+                        if (i == HD / 8 - 1) k_load(t + 2);
+                    },
+                    [&](int i) {
+                        v_step(t + 1, i);
+                        if (i == HD / 8 - 1) v_load(t + 2);
+                    });
             }
         }
     } else {
         typename SpPick<T, HD>::type q;
-        q.load(qrow, p.scale, g);
+        const uint8_t* const image = lds + kSolo;
+        sp_stage_queries<HD, 4>(p, j, row0 + 4 * w, rows, lds_address(image) + 4 * w * (HD * 4), lane);
         const int tiles = works ? (keys + 31) / 32 : 0;
         uint8_t* const kt = lds + w * kWaveLds;
         uint8_t* const vt = kOne ? kt : kt + kTile;
         const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
-        const float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
-        sp_wait_loads<0>();
         const auto stage_k = [&](int t) {
             const int64_t row = k0 + 32 * t;
             sp_stage<T, HD, false, kPieces>(kb + row * HD, last - row, kt_a, lane, 0);
@@ -907,6 +972,10 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
             stage_k(sub);
             if (!kOne) stage_v(sub);
         }
+        sp_wait_loads<0>();
+        __syncthreads();
+        q.load(image, li, p.scale, g);
+        const float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
         for (int t = sub; t < tiles; t += split) {
             const bool more = t + split < tiles;
             sp_wait_loads<kOne ? 0 : kPieces>();  // K is there, V may be in flight
