@@ -833,7 +833,11 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     const bool shared = p.shared;
     const int split = shared ? 2 : kSpWaves;  // waves that share rows
     const int item = shared ? w & 3 : 0, sub = shared ? w >> 2 : w;
-    const int kc = p.n_kv * p.p_chunks, tile = blockIdx.x / kc, at = blockIdx.x - tile * kc, j = at % p.n_kv, chunk = at / p.n_kv;
+    // The row tiles of a chunk read the same keys: workgroups a multiple of 8 apart, which share an L2.
+    const int kc = p.n_kv * p.p_chunks, even = kc & ~7, b = blockIdx.x;
+    const int unit = b < even * p.p_tiles ? 8 : kc - even, first = b < even * p.p_tiles ? 0 : even;
+    const int turn = (b - first * p.p_tiles) / unit, tile = turn % p.p_tiles;
+    const int at = first + turn / p.p_tiles * unit + (b - first * p.p_tiles) % unit, j = at % p.n_kv, chunk = at / p.n_kv;
     const int64_t len = sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
     const int64_t k0 = (int64_t)chunk * p.p_keys, k1 = k0 + p.p_keys < len ? k0 + p.p_keys : len;
     if (k1 <= k0) return;  // the whole workgroup: a chunk past the length
@@ -1094,22 +1098,23 @@ struct SpPlan {
     int few, shared, p_chunks, p_keys, p_tiles, o_chunks, o_keys, o_tiles, o_split;
 };
 
-// How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup, so the
-// launch is made of at most about 256 of them that take equally long: the own keys' items of one to
-// eight waves, and as many chunks of the prefix as the rest holds. Of four numbers of own waves the one
-// whose longest workgroup is shortest, by the times measured at head size 128 (us): 10 for a prefix
-// workgroup's start and end, 1.8 (16-bit caches) and 3.5 (fp32) for a shared block of 64 keys, 1.5 and 7 for
-// eight solo tiles; 8 for an own workgroup's, 1.5 and 5.3 for a wave's 32 keys. 33 x 8001 with 515 own keys
-// (28/4 heads, fp32): 62, 40 and 43 us with 256, 512 and 1024 own waves, 57 with the chunks of an empty chip;
-// 16 x 4096 with 2000 (fp16): 37, 26, 22.
+// How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup; those of the
+// prefix come first, the own keys' fill the other CUs and follow where one ends. Of a few numbers of waves and
+// chunks for an item's own keys, and of two or three lengths of the prefix's chunks for each, the plan is the one
+// whose longest workgroup, or whose work spread over 256 CUs, and whose records take least, by the times
+// measured at head size 128 (us): 9.5 for a prefix workgroup's start and end, 1.85 (16-bit caches) and 3.1
+// (fp32) for a shared block of 64 keys, 1.5 and 7 for eight solo tiles; 9 and 12 for an own workgroup's, 1.5 and
+// 5.3 for a wave's 32 keys. The own keys' work counts three quarters (their lengths are on the device). Best
+// of 56 cuts | this one (us, caches two thirds full): 33 x 8001 fp32 with 515 own keys (28/4 heads) 36 | 37, 64 x
+// 32768 with 1000 142 | 147 and fp16 80 | 82, 16 x 4096 fp16 with 2000 20 | 20, 24 x 2000 fp32 with 1000 25 | 25,
+// 8 x 30000 fp32 with 4000 56 | 63; with the own waves chosen first and the rest filled with chunks 39, 165, 82, 23, 25, 63.
 static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, int64_t p_keys, int64_t o_cap) {
     SpPlan s;
     const int64_t group = n_head / n_kv, rows = batch * group;
     s.shared = rows > 64;
     s.p_tiles = (int)(s.shared ? (rows + 127) / 128 : (rows + 31) / 32);
     s.o_tiles = (int)((group + 15) / 16);
-    const auto cut = [](int64_t keys, int64_t want, int64_t step, int& chunks, int& per) {
-        want = want < 1 ? 1 : want;
+    const auto cut = [](int64_t keys, int want, int step, int& chunks, int& per) {
         int64_t k = (keys + want - 1) / want;
         k = (k + step - 1) / step * step;
         k = k < step ? step : k;
@@ -1129,28 +1134,50 @@ static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, in
         s.o_split = kSpWaves;
         return s;
     }
-    const double each = hd / 128.0, t_step = (s.shared ? (half ? 1.8 : 3.5) : (half ? 1.5 : 7.0)) * each;
-    const double t_own = (half ? 1.5 : 5.3) * each;
-    const int64_t per_chunk = (int64_t)n_kv * s.p_tiles, step = s.shared ? kSpBlock : 32 * kSpWaves;
+    const double each = hd / 128.0, t_step = (s.shared ? (half ? 1.85 : 3.1) : (half ? 1.5 : 7.0)) * each;
+    const double a_own = half ? 9 : 12, t_own = (half ? 1.5 : 5.3) * each, t_record = (double)batch * n_head * hd * 8 / 5e6;
+    const int per_chunk = n_kv * s.p_tiles, step = s.shared ? kSpBlock : 32 * kSpWaves, steps = (int)((p_keys + step - 1) / step);
     double best = 1e30;
-    for (int64_t waves = 256; waves <= 2048; waves *= 2) {
+    for (int o_split = 1, chunks = 1; o_split <= kSpWaves;) {
         SpPlan c = s;
-        c.o_split = 1;
-        while (c.o_split < kSpWaves && c.o_split < tiles && pairs * c.o_split < waves) c.o_split *= 2;
-        cut(o_cap, waves / (pairs * c.o_split), 32 * c.o_split, c.o_chunks, c.o_keys);
-        const int64_t per = kSpWaves / c.o_split, o_blocks = (pairs * c.o_chunks + per - 1) / per;
-        const int64_t room = o_blocks + per_chunk <= 256 ? 256 - o_blocks : 256;
-        cut(p_keys, room / per_chunk, step, c.p_chunks, c.p_keys);
-        const double own = o_blocks ? 8 + t_own * (c.o_keys / (32 * c.o_split)) : 0;
-        const double prefix = c.p_chunks ? 10 + t_step * (c.p_keys / step) : 0;
-        const double rounds = (o_blocks + 255) / 256 * own;
-        const double time = room < 256 ? (own > prefix ? own : prefix) : rounds + prefix * ((per_chunk * c.p_chunks + 255) / 256);
-        if (time < best) {
-            best = time;
-            s = c;
+        c.o_split = o_split;
+        cut(o_cap, chunks, 32 * o_split, c.o_chunks, c.o_keys);
+        const int per = kSpWaves / o_split, o_tiles = c.o_keys / (32 * o_split);
+        const int o_blocks = (int)((pairs * c.o_chunks + per - 1) / per);
+        const double own = o_blocks ? a_own + t_own * o_tiles : 0, own_work = o_blocks * (a_own + 0.75 * t_own * o_tiles);
+        // steps of a chunk: those of one round, and those where the chunks end with all the work spread evenly
+        const auto consider = [&](double want) {
+            SpPlan n = c;
+            const int k = want < 1 ? 1 : want > steps ? steps : (int)want;
+            n.p_chunks = (steps + k - 1) / k;
+            n.p_keys = (steps + n.p_chunks - 1) / n.p_chunks * step;
+            const int p_blocks = per_chunk * n.p_chunks;
+            const double prefix = 9.5 + t_step * (n.p_keys / step);
+            double time = (p_blocks * prefix + own_work) / 256;
+            if (p_blocks > 256) time += prefix / 2;
+            else if (p_blocks + o_blocks > 256) time += own / 6;
+            time = (time > prefix ? time : prefix);
+            time = (time > own ? time : own) + t_record * (n.p_chunks + n.o_chunks);
+            if (time < best) best = time, s = n;
+        };
+        if (!steps) {
+            const double time = (own > own_work / 256 ? own : own_work / 256) + t_record * c.o_chunks;
+            if (time < best) best = time, s = c;
+        } else {
+            const int room = 256 - o_blocks;
+            if (room >= per_chunk) consider((steps + room / per_chunk - 1) / (room / per_chunk));
+            const double all = (double)per_chunk * steps * t_step, a = 9.5 * per_chunk / 256, k = (all + own_work) / 256 - 9.5;
+            const double even = steps * 2 * a / (sqrt(k * k + 4 * a * steps * t_step) - k);
+            consider(even);
+            consider(even + 1);
         }
-        if (!o_cap) break;
+        if (!o_cap || tiles <= o_split) break;
+        if (o_split < kSpWaves)
+            o_split *= 2;
+        else if (++chunks > 6 || c.o_keys <= 32 * kSpWaves)
+            break;
     }
+    if (!steps) s.p_chunks = 0, s.p_keys = step;
     return s;
 }
 

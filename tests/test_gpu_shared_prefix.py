@@ -69,7 +69,9 @@ def close(got, ref, tol):
 SHAPES = [(1, 14, 2, 64, 1, 1), (3, 14, 2, 64, 1400, 64), (2, 28, 4, 128, 1281, 300), (1, 28, 4, 128, 3001, 1), (5, 25, 5, 64, 2500, 0),
           (20, 28, 4, 128, 1500, 70), (80, 16, 16, 64, 130, 129), (129, 14, 2, 64, 1290, 5), (260, 4, 1, 128, 33, 700), (1, 14, 2, 64, 33, 0), (4, 14, 2, 64, 277, 64), (3, 28, 4, 128, 129, 130), (16, 14, 2, 64, 1500, 40),
           (10, 28, 4, 128, 700, 33), (37, 28, 4, 128, 513, 9), (9, 25, 5, 64, 64, 200), (5, 16, 16, 64, 95, 31),
-          (70, 12, 1, 64, 260, 3), (2, 64, 1, 128, 300, 300), (130, 4, 4, 64, 31, 5), (2, 8, 2, 128, 4097, 1000), (65, 2, 1, 64, 2000, 128)]
+          (70, 12, 1, 64, 260, 3), (2, 64, 1, 128, 300, 300), (130, 4, 4, 64, 31, 5), (2, 8, 2, 128, 4097, 1000), (65, 2, 1, 64, 2000, 128),
+          # several row tiles of a number of chunks that 8 does not divide
+          (20, 15, 5, 64, 3000, 60), (50, 15, 5, 128, 2000, 33), (400, 3, 3, 64, 700, 20), (100, 9, 3, 128, 64, 900)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
