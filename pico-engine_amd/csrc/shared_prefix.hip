@@ -31,8 +31,11 @@
 //     beside them (split, softmax) and the skew of the two waves at the barrier;
 //   3 sequences, 32768 fp16 keys: 9.0 + 4.4; 16 sequences, 1500 fp32 keys: 8.5 + 4.0; 4 sequences, 277 fp32
 //     keys: 8.9 in one launch. Latency: lengths, queries, first tiles, a block or two, records.
-// Tried without gain: key rows swizzled over all 64 banks; the barrier of a block between softmax and
-// values, so that values and the next scores run back to back (30.3 for 28.9 us, fp16 85 for 75).
+// Both run at about 1.8 GHz (busy cycles over time), as long matrix work here does. Tried without gain: key
+// rows swizzled over all 64 banks; the barrier of a block between softmax and values, so that values and
+// the next scores run back to back (30.3 for 28.9 us, fp16 85 for 75); half the waves half a block behind
+// the others, with a barrier every half block (30.5 for 29.5, fp16 83 for 78); low parts by one instruction
+// that rounds to a half register (30.9 for 29.5).
 #include "pe_common.h"
 
 namespace pe {
