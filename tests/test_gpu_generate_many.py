@@ -137,6 +137,17 @@ def test_generate_many_stops_and_samples(eng):
         eng.generate_many(ids, 2, 4, cache_dtype=torch.bfloat16)
 
 
+@pytest.mark.parametrize("n", [2, 9, 70])
+@pytest.mark.parametrize("which", ["eng", "eng128"])
+def test_generate_many_graph_is_eager(which, n, request):
+    """The captured step replayed with the host's work between gives the eager steps' tokens."""
+    eng = request.getfixturevalue(which)
+    kw = dict(temperature=0.8, top_k=20, repetition=1.2, frequency=0.1, eos_id=-2)
+    ids = list(range(7, 60))
+    runs = [eng.generate_many(ids, n, 20, use_graph=g, generator=torch.Generator(DEV).manual_seed(n), **kw) for g in (False, True, True)]
+    assert runs[0] == runs[1] == runs[2] and len({tuple(r) for r in runs[0]}) == n
+
+
 def test_generate_many_refuses_masks_that_leave_nothing(eng):
     mask = torch.full((2, 32), -1, dtype=torch.int32, device=DEV)
     mask[1] = 0
