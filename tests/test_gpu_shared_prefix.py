@@ -268,6 +268,48 @@ def test_long_cache_offsets(K, dtype):
         assert bool(((got[b, :4, 0] - 1).abs() <= 2.0 ** -24 * (2 * math.sqrt(P) + 16)).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_long_cache_offsets_of_many_rows(K, dtype):
+    """The same with row tiles that share the keys; fp32 values have the 2^-39 of their group's largest besides."""
+    hd, nkv, P, B = 128, 5, 1 << 20, 70
+    q = torch.randn(B, nkv, hd, device=DEV) * 4
+    kp = torch.zeros(nkv, P, hd, device=DEV, dtype=dtype)
+    vp = torch.zeros_like(kp)
+    kp[4, P - 40:] = torch.randn(40, hd, device=DEV).to(dtype) * 3
+    vp[4, P - 40:] = torch.randn(40, hd, device=DEV).to(dtype)
+    vp[:, :, 0] = 1.0
+    ko = torch.randn(B, nkv, 3, hd, device=DEV).to(dtype)
+    got = K.shared_prefix_attn(q, kp, vp, ko, ko, 0, round_fp16=False)[:, 4].double()
+    k, v, x = kp[4, P - 40:].double(), vp[4, P - 40:].double(), q[:, 4].double()
+    s = x @ k.T * hd ** -0.5
+    top = s.amax(1, keepdim=True).clamp_min(0)
+    e, rest = torch.exp(s - top), torch.exp(-top) * (P - 40)
+    total = e.sum(1, keepdim=True) + rest
+    A = (x.abs() @ k.abs().T).amax(1, keepdim=True) * hd ** -0.5
+    tol = 2.0 ** -24 * ((4 * math.sqrt(hd) + 4) * A + 2 * math.sqrt(P) + 16) * (e @ v.abs() / total) + 2.0 ** -39 * v.abs().max()
+    assert bool(((got - e @ v / total).abs()[:, 1:] <= tol[:, 1:]).all())
+    assert bool(((got[:, 0] - 1).abs() <= 2.0 ** -24 * (2 * math.sqrt(P) + 16)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_many_sequences(K, dtype):
+    """Thousands of sequences: more workgroups than a round holds, of one chunk each."""
+    B, n, hd, P, cap = 9001, 2, 64, 700, 2
+    q, kp, vp, ko, vo, own = make(8, B, n, n, hd, P, cap, dtype)
+    own[::7] = -1
+    got = K.shared_prefix_attn(q, kp, vp, ko, vo, own, round_fp16=False).double()
+    x, scale = q.double(), hd ** -0.5
+    s = torch.cat([torch.einsum("bhd,hpd->bhp", x, kp.double()), torch.einsum("bhd,bhpd->bhp", x, ko.double())], -1) * scale
+    A = scale * torch.cat([torch.einsum("bhd,hpd->bhp", x.abs(), kp.double().abs()),
+                           torch.einsum("bhd,bhpd->bhp", x.abs(), ko.double().abs())], -1).amax(-1, keepdim=True)
+    s[..., P:].masked_fill_(torch.arange(cap, device=DEV) >= own[:, None, None], -math.inf)
+    p = torch.softmax(s, -1)
+    out = lambda f: torch.einsum("bhp,hpd->bhd", p[..., :P], f(vp.double())) + torch.einsum("bhp,bhpd->bhd", p[..., P:], f(vo.double()))
+    tol = 2.0 ** -24 * ((4 * math.sqrt(hd) + 4) * A + 2 * math.sqrt(P + cap) + 16) * out(torch.abs) + 2.0 ** -39 * 8
+    live = own >= 0
+    assert bool(((got - out(lambda v: v)).abs() <= tol)[live].all()) and bool((got[~live] == 0).all())
+
+
 def test_refusals(K):
     q, kp, vp, ko, vo, own = make(1, 3, 4, 2, 64, 40, 8, torch.float32)
     bad = [(q[0], kp, vp, ko, vo, own), (q, kp.half(), vp, ko, vo, own), (q, kp, vp, ko.half(), vo.half(), own),
