@@ -6,10 +6,11 @@
 // A workgroup takes one segment of one row's vocabulary: it counts the segment's tokens of the
 // history and the prompt in LDS (whole-number additions, so their order does not matter), while its
 // logits are on their way, and stores the segment. One launch, nothing kept between calls. Bound by
-// reading and writing the logits once (256 rows of 151643 fp16 from memory: 38 us, 4.1 TB/s), by latency
-// for a row or two (3.6 us), and where the ids are many by looking through them: every segment of a row
-// reads all of them (from L2), a few 32-bit instructions each (24 rows of 152064 with 4000 + 770 ids: 9 us,
-// 5 without; 8 rows with 30000: 14). Compared as 64-bit integers the ids cost twice as much.
+// reading and writing the logits once (from memory: 256 rows of 151643 fp16 34 us, 4.6 TB/s, of 151936 fp32 57,
+// 5.4), by latency for a row or two (3.5 us), and where the ids are many by looking through them: every segment
+// of a row reads all of them (from L2), a few 32-bit instructions each (24 rows of 152064 with 4000 + 770
+// ids: 9.9 us, 4.8 without; 8 rows with 30000: 11). Compared as 64-bit integers the ids cost twice as much;
+// counters looked at one by one where the vector's were all zero cost 256 rows 4 us more.
 #include "pe_common.h"
 
 namespace pe {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
     constexpr int V = 16 / sizeof(T), SEG = 256 * V * STEPS;
     typedef typename Loose<T, V>::type vec;
     typedef typename Loose<float, 4>::type vec4;
-    __shared__ uint32_t count[SEG];
+    __shared__ __attribute__((aligned(16))) uint32_t count[SEG];
     const int t = threadIdx.x;
     const int64_t b = blockIdx.y, v0 = (int64_t)blockIdx.x * SEG;
     const T* x = static_cast<const T*>(p.x) + b * p.x_row;
@@ -143,7 +144,8 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
     const float freq = p.rules[1] ? p.rules[1][b] : p.rule[1];
     const float pres = p.rules[2] ? p.rules[2][b] : p.rule[2];
     if (ids) {
-        for (int i = t; i < SEG; i += 256) count[i] = 0;
+#pragma unroll
+        for (int i = 0; i < SEG; i += 1024) *reinterpret_cast<uint4*>(count + i + 4 * t) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         if (p.prompt)
             count_ids<true>(count, p.prompt, p.prompt_wide, b * p.prompt_row, p.prompt_len, (uint32_t)v0, SEG);
@@ -171,12 +173,19 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
             for (int i = 0; i < V; ++i) z[i] += bias[s][i];
         }
         if (ids) {
+            uint32_t c[V], any = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const uint32_t c = count[o + i];
-                if (c) {
+            for (int i = 0; i < V; i += 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(count + o + i);
+                c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
+                any |= x.x | x.y | x.z | x.w;
+            }
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (!c[i]) continue;
                     z[i] = z[i] > 0.f ? z[i] / rep : z[i] * rep;
-                    const uint32_t n = c & ~kInPrompt;
+                    const uint32_t n = c[i] & ~kInPrompt;
                     if (n) z[i] = (z[i] - freq * (float)n) - pres;
                 }
             }
@@ -202,11 +211,11 @@ __global__ __launch_bounds__(256) void k_adjust_logits(LogitArgs p) {
 template <typename T>
 static int launch_logits(const LogitArgs& p, int64_t batch, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    // Segments of 4096 tokens, or of a vector a thread where those leave fewer than two workgroups per
-    // CU. Longer ones read the ids less often but wait longer for them, shorter ones have too few bytes
-    // on their way (us at 2048 | 4096 | 8192 tokens, 256 rows of 151643 fp16 and 300 ids, from memory:
-    // 43 | 38 | -, from the Infinity Cache: 32 | 32 | 44; 24 rows of 152064 fp32, 4770 ids: 10 | 9 | 12).
-    constexpr int kLong = 16 / V;
+    // Segments of 8 KB, or of a vector a thread where those leave fewer than two workgroups per CU. Longer
+    // ones read the ids less often but wait longer for them, shorter ones have too few bytes on their way (us
+    // at 4 | 8 | 16 KB, from memory: 256 rows of 151643 fp16 and 300 ids 38 | 34 | 43; at 8 | 16 | 32 KB, 256 rows of 151936
+    // fp32 and 300 ids 57 | 63 | 69, 24 rows of 152064 and 4770 ids 9.9 | 9.3 | 12.5, 8 rows and 30000 ids 11 | 14 | 14).
+    constexpr int kLong = 2;
     const auto blocks = [&](int steps) { return (p.vocab + 256 * V * steps - 1) / (256 * V * steps); };
     const bool many = batch * blocks(kLong) >= 512;
     // rows per launch: grid.y's limit, and 2^32 threads in a grid
