@@ -1036,7 +1036,7 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix_few(SpArgs p
 
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
 // lanes hold a row, the lane groups take every so-many-th record, four loads in flight each, with a
-// running maximum of their own; bound by the latency of lengths and records (14 heads x 16 sequences x
+// running maximum of their own; bound by the latency of a launch and the records (14 heads x 16 sequences x
 // 25 records of 64: 4.3 us; 28 x 64 x 15 of 128: 5.9, 14 x 3 x 65 of 64: 4.6).
 template <int HD, int W>
 __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
@@ -1046,13 +1046,26 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int row = __builtin_amdgcn_readfirstlane(W == 1 ? blockIdx.x * 4 + w : blockIdx.x);
     if (row >= p.batch * p.n_head) return;  // W == 1 only, uniform per wave
+    const int64_t at = (int64_t)row * (p.p_chunks + p.o_chunks);
+    const int total = p.p_chunks + p.o_chunks;
+    int i0 = (W == 1 ? 0 : w * (64 / L)) + lane / L;
+    float2 ml[U];
+    float4 o[U];
+    // the first records come while the lengths do, there or not
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t rec = at + (i0 + N * u < total ? i0 + N * u : 0);
+        ml[u] = *reinterpret_cast<const float2*>(p.ml + rec * 2);
+        o[u] = *reinterpret_cast<const float4*>(p.rec + rec * HD + 4 * (lane % L));
+    }
     // lengths are at most 2^30
     const int64_t pl = sp_length(p.p_len, p.p_dtype, 0, p.p_add, p.p_cap);
     const int64_t ol = sp_length(p.o_len, p.o_dtype, row / p.n_head, p.o_add, p.o_cap);
-    const int np = pl > 0 ? (int)((uint32_t)(pl + p.p_keys - 1) / (uint32_t)p.p_keys) : 0;
+    // a sequence that takes no part has no records: zeros
+    const int np = pl > 0 && ol >= 0 ? (int)((uint32_t)(pl + p.p_keys - 1) / (uint32_t)p.p_keys) : 0;
     const int no = ol > 0 ? (int)((uint32_t)(ol + p.o_keys - 1) / (uint32_t)p.o_keys) : 0;
-    const int n = ol < 0 ? 0 : np + no;  // a sequence that takes no part: zeros
-    const int64_t at = (int64_t)row * (p.p_chunks + p.o_chunks);
+    const int n = np + no;
+    const auto there = [&](int i) { return i < np || (i >= p.p_chunks && i - p.p_chunks < no); };
     const float NEG_INF = -__builtin_huge_valf();
     float top = NEG_INF, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1064,19 +1077,20 @@ __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
         sum = fmaf(f, l, a * sum);
         v = make_float4(fmaf(f, o.x, a * v.x), fmaf(f, o.y, a * v.y), fmaf(f, o.z, a * v.z), fmaf(f, o.w, a * v.w));
     };
-    for (int i0 = (W == 1 ? 0 : w * (64 / L)) + lane / L; i0 < n; i0 += N * U) {
-        float2 ml[U];
-        float4 o[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + N * u < n ? i0 + N * u : i0;
-            const int64_t rec = at + (i < np ? i : p.p_chunks + i - np);
-            ml[u] = *reinterpret_cast<const float2*>(p.ml + rec * 2);
-            o[u] = *reinterpret_cast<const float4*>(p.rec + rec * HD + 4 * (lane % L));
-        }
+    for (int u = 0; u < U; ++u)
+        if (there(i0 + N * u)) take(ml[u].x, ml[u].y, o[u]);
+    for (i0 += N * U; i0 < total; i0 += N * U) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + N * u < n) take(ml[u].x, ml[u].y, o[u]);
+            if (there(i0 + N * u)) {
+                const int64_t rec = at + i0 + N * u;
+                ml[u] = *reinterpret_cast<const float2*>(p.ml + rec * 2);
+                o[u] = *reinterpret_cast<const float4*>(p.rec + rec * HD + 4 * (lane % L));
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (there(i0 + N * u)) take(ml[u].x, ml[u].y, o[u]);
     }
 #pragma unroll
     for (int o = 32; o >= L; o >>= 1) {
