@@ -26,10 +26,10 @@
 //   64 sequences, 32768 fp16 keys, up to 1000 own: 77 + 5.9. The matrix cores; a shared block in steady state
 //     keeps them at 1.22 PFLOP/s (a large library product reaches 1.18); the own keys stream at 4.7 to
 //     5.5 TB/s, about 9 us are a workgroup's start and end;
-//   33 sequences, 8001 fp32 keys, up to 515 own: 31 + 4.6. A shared block takes 6700 cycles, the matrix
+//   33 sequences, 8001 fp32 keys, up to 515 own: 30 + 4.2. A shared block takes 6700 cycles, the matrix
 //     instructions of a SIMD's two waves 3100 of them; the rest is the vector work that does not fit
 //     beside them (split, softmax) and the skew of the two waves at the barrier;
-//   3 sequences, 32768 fp16 keys: 9.1 + 4.6; 16 sequences, 1500 fp32 keys: 8.6 + 4.3; 4 sequences, 277 fp32
+//   3 sequences, 32768 fp16 keys: 9.1 + 4.6; 16 sequences, 1500 fp32 keys: 8.6 + 3.8; 4 sequences, 277 fp32
 //     keys: 9.0 in one launch. Latency: lengths, queries, first tiles, a block or two, records.
 // Both run at about 1.8 GHz (busy cycles over time), as long matrix work here does. Tried without gain: key
 // rows swizzled over all 64 banks; the barrier of a block between softmax and values, so that values and
@@ -1037,7 +1037,7 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix_few(SpArgs p
 // W waves per (sequence, head): the records of the prefix's chunks and then of the own keys'. HD / 4
 // lanes hold a row, the lane groups take every so-many-th record, four loads in flight each, with a
 // running maximum of their own; bound by the latency of a launch and the records (14 heads x 16 sequences x
-// 25 records of 64: 4.3 us; 28 x 64 x 15 of 128: 5.9, 14 x 3 x 65 of 64: 4.6).
+// 25 records of 64: 3.8 us; 28 x 64 x 15 of 128: 5.9, 14 x 3 x 65 of 64: 4.6).
 template <int HD, int W>
 __global__ __launch_bounds__(256) void k_shared_prefix_merge(SpArgs p) {
     constexpr int L = HD / 4, N = 64 / L * W, U = 4;
