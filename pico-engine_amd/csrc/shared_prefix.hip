@@ -121,11 +121,13 @@ PE_DEV uint32_t wave_max_bits(uint32_t v) {
     return __builtin_amdgcn_readfirstlane(b[0] > b[1] ? b[0] : b[1]);
 }
 
-// Records go past the L2, whose dirty lines the launch's end would have to write back.
+// Records go past the L2, whose dirty lines the launch's end would have to write back. A store of 16 bytes reads its
+// data after it has issued, and the compiler does not see this one: the wait keeps the registers from the next
+// instruction.
 PE_DEV void store_record(float* p, const float4& v) {
     typedef float f4v __attribute__((ext_vector_type(4)));
     const f4v x = {v.x, v.y, v.z, v.w};
-    asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1" ::"v"(p), "v"(x) : "memory");
+    asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" ::"v"(p), "v"(x) : "memory");
 }
 
 PE_DEV float exp2_int(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
