@@ -797,9 +797,14 @@ int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, 
  *   prefix_len = (device scalar if prefix_len_dtype) + prefix_len_add, own_len[b] likewise (one device
  *   integer per sequence), each clamped to its capacity. Nothing behind a length is used: it may hold
  *   anything. No keys at all, or a negative own_len (a sequence that takes no part): zeros.
- *   round_fp16 as pe_decode_attn. fp32 products and sums; with fp16 caches the query and the
- *   probabilities enter the products as two fp16 values each, 22 bits (an infinite key or value that
- *   a row sees may make it NaN).
+ *   round_fp16 as pe_decode_attn. Sums and softmax statistics are fp32. Products are fp32 too with fp32
+ *   caches for the own keys, and for the prefix's where a kv head has up to 64 query rows (batch *
+ *   n_head / n_kv). All others take their fp32 factors as the sum of two fp16 values each: the query
+ *   within 2^-22 of an element or 2^-38 of its row's largest, the probabilities within 2^-23 or 2^-33 of the
+ *   row's largest one, and an fp32 prefix's keys and values within 2^-23 of an element or 2^-39 of the
+ *   largest G of 8 keys, its probabilities' 2^-33 being that of the row's largest p G. Keys of an fp32
+ *   prefix that this would cost more than 2^-23 of their four neighbouring dims (2^-27 of a value's), and
+ *   infinite ones, are taken in fp32. With fp16 caches an infinite key or value that a row sees may make it NaN.
  * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes (0: NULL will do), any contents, with
  * prefix_keys = prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in
  * order on one stream may share it, calls that overlap must not. Two launches, one for few keys. */

@@ -18,7 +18,9 @@
 // these row counts). All others run on v_mfma_f32_32x32x16_f16 with the fp32 factors as the sum of
 // two fp16 values, 22 bits (one would cost 2^-12 of each): the query, scaled by a power of two to at
 // most 2^14; the probability; and an fp32 cache's keys and values, every 8 keys scaled by a
-// power of two of their largest element. Products of two low parts are left out (2^-22). Per 16 elements of
+// power of two of their largest element. Products of two low parts are left out (2^-22). A chunk whose keys,
+// values or queries lie too far apart for their two parts (SpSplit::find) is taken again by its workgroup on the fp32
+// instructions (33 x 8001 with such a key: 36 us to 125, with one in every block 149). Per 16 elements of
 // a dot product that is 2 instructions for 16-bit caches and 3 for fp32 ones in place of 8 fp32 instructions
 // of twice the time each.
 //
@@ -52,6 +54,9 @@ constexpr int kSpBlock = 64;       // keys of a shared block
 // rescaled a few times instead of in most tiles.
 constexpr float kUp = 8.f, kRoom = 15.f;
 constexpr float kLog2e = 1.4426950408889634f;
+// Exponents of the values of fp32 caches in the shared way: of a group of zeros, and how far apart those that a
+// wave takes may lie, so that its sums stay within fp32.
+constexpr int kZeros = -114, kFar = 64;
 
 struct SpArgs {
     const float* q;
@@ -109,16 +114,6 @@ template <int CTRL>
 PE_DEV uint32_t dpp_max(uint32_t v) {
     const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
     return v > o ? v : o;
-}
-PE_DEV uint32_t wave_max_bits(uint32_t v) {
-    v = dpp_max<0xB1>(v);   // quad_perm [1,0,3,2]
-    v = dpp_max<0x4E>(v);   // quad_perm [2,3,0,1]
-    v = dpp_max<0x141>(v);  // row_half_mirror
-    v = dpp_max<0x140>(v);  // row_mirror
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = a[0] > a[1] ? a[0] : a[1];
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return __builtin_amdgcn_readfirstlane(b[0] > b[1] ? b[0] : b[1]);
 }
 
 // Records go past the L2, whose dirty lines the launch's end would have to write back. A store of 16 bytes reads its
@@ -263,6 +258,7 @@ template <int HD>
 struct RowsF16 {
     h8v hi[HD / 16], lo[HD / 16];
     float unscale;
+    bool uneven;  // eight neighbouring elements lie 2^-16 under the row's largest, or that one is tiny or huge (SpSplit)
     PE_DEV void load(const uint8_t* image, int r, float scale, int g) {
         float v[HD / 2], top = 0.f;
 #pragma unroll
@@ -275,9 +271,18 @@ struct RowsF16 {
                 v[8 * j + i + 2] = x.z;
                 v[8 * j + i + 3] = x.w;
             }
+        uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < HD / 2; ++i) top = fmaxf(top, fabsf(v[i]));
+        for (int j = 0; j < HD / 16; ++j) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 8 * j; i < 8 * j + 8; ++i) m = fmaxf(m, fabsf(v[i]));
+            top = fmaxf(top, m);
+            const uint32_t b = __float_as_uint(m) - 1;  // zeros are no small values
+            least = b < least ? b : least;
+        }
         top = swap32_max(top);
+        uneven = top > 0.f && (!(top >= 0x1p-99f && top < 0x1p120f) || least < __float_as_uint(top) - (16u << 23));
         // the row's largest element to 2^13 .. 2^14, within what fp32 holds with its inverse; the scale
         // of the scores comes after the products
         int e = exponent_of(top);
@@ -359,7 +364,8 @@ struct RowsF16 {
 };
 
 // The softmax of a wave's rows so far: o = sum p V, l = sum p (a lane's half) of the probabilities
-// p = exp2(s - r).
+// p = exp2(s - r). With weighted values V = 2^w V' the tiles hold V': p = exp2(s + w - r) for the row, without 2^w
+// for the sum.
 template <int HD>
 struct SpState {
     f16v o[HD / 32];
@@ -375,8 +381,11 @@ struct SpState {
         for (int d = 0; d < HD / 32; ++d) o[d] *= f;
     }
     // scores of a tile, to be multiplied by c[r / 4] (positive) -> its probabilities; keys from n on
-    // are masked; o is multiplied by 2^shift (uniform) besides
-    PE_DEV void softmax(f16v& s, const float* c, int n, int g, int shift = 0) {
+    // are masked. WEIGHTED: probabilities times 2^w[r / 4] (uniform, at most 128 apart in all), the exponents of the
+    // keys' values: the largest product sets the reference, so that fp16's bits go to the keys that make the
+    // result and not to those with the largest values.
+    template <bool WEIGHTED>
+    PE_DEV void softmax(f16v& s, const float* c, const int* w, int n, int g) {
         const float NEG_INF = -__builtin_huge_valf();
         if (n < 32) {
 #pragma unroll
@@ -385,20 +394,32 @@ struct SpState {
         }
         float mx = NEG_INF;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]), s[i + 3]) * c[i >> 2]);
+        for (int i = 0; i < 16; i += 4) {
+            const float m = fmaxf(fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]), s[i + 3]);
+            mx = fmaxf(mx, WEIGHTED ? fmaf(m, c[i >> 2], (float)w[i >> 2]) : m * c[i >> 2]);
+        }
         mx = swap32_max(mx);
         const bool moves = mx > r + kRoom;  // the first finite score does
-        if (__any(moves) || shift) {
+        if (__any(moves)) {
             const float rn = moves ? mx - kUp : r, alpha = moves ? __builtin_amdgcn_exp2f(r - rn) : 1.f;
             r = rn;
             l *= alpha;
-            scale(ldexpf(alpha, shift));
+            scale(alpha);
         }
         const float rs = r == NEG_INF ? 0.f : r;  // a row none of whose keys came yet
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c[i >> 2], -rs));
-            l += s[i];
+        for (int i = 0; i < 16; i += 4) {
+            const float from = WEIGHTED ? (float)w[i >> 2] - rs : -rs;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = i; k < i + 4; ++k) {
+                s[k] = __builtin_amdgcn_exp2f(fmaf(s[k], c[i >> 2], from));
+                if constexpr (WEIGHTED)
+                    sum = k > i ? sum + s[k] : s[k];
+                else
+                    l += s[k];
+            }
+            if constexpr (WEIGHTED) l += ldexpf(sum, -w[i >> 2]);
         }
     }
 };
@@ -524,8 +545,9 @@ template <int HD, bool VALUES>
 struct SpSplit {
     static constexpr int N = HD / 32, R = 256 / HD, kPlane = kSpBlock * HD * 2, kSteps = HD / 8;
     float4 x[N];
-    uint32_t top;
+    uint32_t top, least;
     float f;
+    uint64_t uneven = 0;  // not 0: see find
     h2v h0, l0;
     // the wave's 8 rows of the block at base, which holds n keys; the rows behind them are zeros
     PE_DEV void load(const float* base, int n, int w, int lane) {
@@ -537,15 +559,27 @@ struct SpSplit {
             x[i] = __builtin_bit_cast(float4, y);
         }
     }
-    // The exponent E with the largest finite element in [2^(14 + E), 2^(15 + E)): the two parts hold every
-    // element to 2^-23 of itself or 2^-39 of the largest. Eight stages.
+    // The exponent E with the largest element in [2^(14 + E), 2^(15 + E)): the two parts hold every element to
+    // 2^-23 of itself or 2^-39 of the largest. `uneven` says where that is not enough: where four neighbouring
+    // dims of a key lie kUneven under the largest (zeros are exact), so that a value keeps 2^-27 of its neighbours and a
+    // key's element 2^-23, and where the largest is infinite or under 2^-99. Four normal values lie 2^-12 under the
+    // largest of 1024 once in 10^9 blocks. Eight stages.
+    static constexpr uint32_t kUneven = (VALUES ? 12u : 16u) << 23;
+    static PE_DEV float largest(const float4& a) { return fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fabsf(a.z)), fabsf(a.w)); }
+    // the smaller, a zero being no small value: the bits less one
+    static PE_DEV uint32_t smaller(uint32_t least, float a) {
+        const uint32_t b = __float_as_uint(a) - 1;
+        return b < least ? b : least;
+    }
     PE_DEV void find(int stage, int* e) {
         if (stage == 0) {
+            least = 0xFFFFFFFFu;
             float m = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                m = fmaxf(fmaxf(m, fabsf(x[i].x)), fabsf(x[i].y));
-                m = fmaxf(fmaxf(m, fabsf(x[i].z)), fabsf(x[i].w));
+                const float r = largest(x[i]);
+                m = fmaxf(m, r);
+                least = smaller(least, r);
             }
             top = __float_as_uint(m);
         }
@@ -562,19 +596,13 @@ struct SpSplit {
             top = __builtin_amdgcn_readfirstlane(a[0] > a[1] ? a[0] : a[1]);
         }
         if (stage == 7) {
-            if (top >= 0x7F800000u) {  // infinities: the largest of the others (x + 0 x is NaN for those)
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    m = fmaxf(fmaxf(m, fabsf(fmaf(x[i].x, 0.f, x[i].x))), fabsf(fmaf(x[i].y, 0.f, x[i].y)));
-                    m = fmaxf(fmaxf(m, fabsf(fmaf(x[i].z, 0.f, x[i].z))), fabsf(fmaf(x[i].w, 0.f, x[i].w)));
-                }
-                top = wave_max_bits(__float_as_uint(m));
-            }
             int k = (int)(top >> 23) - 127;
             k = (k < -100 ? -100 : k) - 14;
             f = exp2_int(-k);
             if ((threadIdx.x & 63) == 0) *e = k;
+            // zeros alone are even, all that comes with a tiny or infinite largest element is not
+            const bool odd = top - (28u << 23) >= 0x7F800000u - (28u << 23);
+            uneven |= __ballot(least < (!top ? 0 : odd ? 0xFFFFFFFEu : top - kUneven));
         }
     }
     // Where a lane's half chunk of the wave's first rows goes in a plane; those of piece i lie i R rows on, at
@@ -829,16 +857,14 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     static_assert(kQueries + 128 * HD * 4 <= kMost, "the queries' image");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kMost > kMerge ? kMost : kMerge];
     __shared__ float ref[kSpWaves][32], sums[kSpWaves][32];
-    __shared__ int exps[2][16], row_of[kSpWaves][32];
+    __shared__ int exps[2][16], row_of[kSpWaves][32], uneven;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5, li = lane & 31;
 
     const SpShared m{lds, ref, sums, row_of};
     if ((int)blockIdx.x >= p.p_blocks) return sp_own<T, HD, false>(p, m, blockIdx.x - p.p_blocks);
 
-    // The wave's rows and the keys [k0, k1).
+    // The workgroup's rows of a kv head, by tiles of 32, and its keys [k0, k1).
     const bool shared = p.shared;
-    const int split = shared ? 2 : kSpWaves;  // waves that share rows
-    const int item = shared ? w & 3 : 0, sub = shared ? w >> 2 : w;
     // The row tiles of a chunk read the same keys: workgroups a multiple of 8 apart, which share an L2.
     const int kc = p.n_kv * p.p_chunks, even = kc & ~7, b = blockIdx.x;
     const int unit = b < even * p.p_tiles ? 8 : kc - even, first = b < even * p.p_tiles ? 0 : even;
@@ -849,18 +875,85 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
     if (k1 <= k0) return;  // the whole workgroup: a chunk past the length
     const T* kb = static_cast<const T*>(p.kp) + (int64_t)j * p.p_cap * HD;
     const T* vb = static_cast<const T*>(p.vp) + (int64_t)j * p.p_cap * HD;
-    const int row0 = shared ? 128 * tile + 32 * item : 32 * tile, rows = p.batch * p.group;
-    const int keys = (int)(k1 - k0);
+    const int rows = p.batch * p.group, keys = (int)(k1 - k0);
     const int64_t last = k1 - 1;
-    const bool works = row0 < rows;
-    // the lane's query: row r of the kv head is (sequence r / group, head r % group of the kv head's)
-    const int seq = (row0 + li) / p.group;
-    const int my_row = seq * p.n_head + j * p.group + (row0 + li - seq * p.group);
-    SpState<HD> st;
-    st.clear();
-    int top = 0;  // exponent of the values that o holds
+    // the record of a wave's rows from row0 on, by split waves step apart of which it is the sub-th
+    const auto finish = [&](SpState<HD>& st, int base, int row0, int item, int sub, int split, int step) {
+        // row r of the kv head is (sequence r / group, head r % group of the kv head's)
+        const int seq = (row0 + li) / p.group, my_row = seq * p.n_head + j * p.group + (row0 + li - seq * p.group);
+        const float down = exp2_int(-(int)kUp);  // probabilities and values without their factors
+        st.scale(ldexpf(down, base));
+        float4 v[HD / 8];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+            v[i] = make_float4(st.o[i >> 2][4 * (i & 3)], st.o[i >> 2][4 * (i & 3) + 1], st.o[i >> 2][4 * (i & 3) + 2], st.o[i >> 2][4 * (i & 3) + 3]);
+        sp_finish<HD, 32, false>(p, m, v, st.r + kUp, swap32_sum(st.l) * down, my_row, row0 < rows, rows - row0, chunk, item, sub, split, step);
+    };
+
+    // the wave's share of rows [row0, row0 + 32) and all of the chunk's keys, every eighth tile of them
+    const auto solo = [&](int row0, int lane) {
+        const int li = lane & 31, g = lane >> 5;
+        SpState<HD> st;
+        st.clear();
+        typename SpPick<T, HD>::type q;
+        const uint8_t* const image = lds + kSolo;
+        sp_stage_queries<HD, 4>(p, j, row0 + 4 * w, rows, lds_address(image) + 4 * w * (HD * 4), lane);
+        const int tiles = (keys + 31) / 32;
+        uint8_t* const kt = lds + w * kWaveLds;
+        uint8_t* const vt = kOne ? kt : kt + kTile;
+        const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
+        const auto stage_k = [&](int t) {
+            const int64_t row = k0 + 32 * t;
+            sp_stage<T, HD, false, kPieces>(kb + row * HD, last - row, kt_a, lane, 0);
+        };
+        const auto stage_v = [&](int t) {
+            const int64_t row = k0 + 32 * t;
+            sp_stage<T, HD, true, kPieces>(vb + row * HD, last - row, vt_a, lane, 0);
+        };
+        if (w < tiles) {
+            stage_k(w);
+            if (!kOne) stage_v(w);
+        }
+        sp_wait_loads<0>();
+        __syncthreads();
+        q.load(image, li, p.scale, g);
+        const float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
+        for (int t = w; t < tiles; t += kSpWaves) {
+            const bool more = t + kSpWaves < tiles;
+            sp_wait_loads<kOne ? 0 : kPieces>();  // K is there, V may be in flight
+            f16v s = sp_scores(q, kt, li, g);
+            sp_wait_lds();
+            if (kOne)
+                stage_v(t);
+            else if (more)
+                stage_k(t + kSpWaves);
+            const int n = keys - 32 * t < 32 ? keys - 32 * t : 32;
+            st.template softmax<false>(s, c, nullptr, n, g);
+            if (!kOne && more)
+                sp_wait_loads<kPieces>();  // V is there, the next K may be in flight
+            else
+                sp_wait_loads<0>();
+            if (n < 32) {
+                sp_clear_rows<HD * (int)sizeof(T)>(vt, n, 32, lane, 64);
+                sp_wait_lds();
+            }
+            sp_accumulate(q, vt, s, st.o, li, g);
+            sp_wait_lds();
+            if (more) {
+                if (kOne)
+                    stage_k(t + kSpWaves);
+                else
+                    stage_v(t + kSpWaves);
+            }
+        }
+        finish(st, 0, row0, 0, w, kSpWaves, 1);
+    };
 
     if (shared) {
+        const int item = w & 3, sub = w >> 2, row0 = 128 * tile + 32 * item;
+        SpState<HD> st;
+        st.clear();
+        int base = kHalf ? 0 : kZeros, most = kZeros, least = 127;  // exponents of the values: what o holds, and their range
         RowsF16<HD> q;
         const uint8_t* const image = lds + kQueries;
         sp_stage_queries<HD, 16>(p, j, 128 * tile + 16 * w, rows, lds_address(image) + 16 * w * (HD * 4), lane);
@@ -872,30 +965,26 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
             const int n = keys - kSpBlock * t - 32 * sub;
             f16v s = q.template scores<kLow>(kt, li, g, kbeside);
             float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
-            int ev[4], shift = 0;
+            int ev[4];
             if constexpr (!kHalf) {
                 const int* e = exps[t & 1] + 4 * sub;
-                int most = t ? top : -128;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     c[i] = sp_positive(ldexpf(c[i], e[i]));
                     ev[i] = __builtin_amdgcn_readfirstlane(e[8 + i]);
                     most = ev[i] > most ? ev[i] : most;
+                    least = ev[i] > kZeros && ev[i] < least ? ev[i] : least;
                 }
-                shift = t ? top - most : 0;
-                top = most;
+                base = base == kZeros ? most : base;
+                // groups of zeros, which no weight makes larger, count as far under the others
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ev[i] = (ev[i] == kZeros ? most - kFar : ev[i]) - base;
             }
             const uint32_t va = RowsF16<HD>::values_at(kt + (kHalf ? 1 : 2) * kPlane, li, g);
             h8v v[4];
             RowsF16<HD>::template load_values<kLow>(va, v);
             __builtin_amdgcn_sched_barrier(0);
-            st.softmax(s, c, n, g, shift);
-            if constexpr (!kHalf) {
-                if (ev[0] != top || ev[1] != top || ev[2] != top || ev[3] != top) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] *= ldexpf(1.f, ev[i >> 2] - top);
-                }
-            }
+            st.template softmax<!kHalf>(s, c, ev, n, g);
             RowsF16<HD>::template accumulate<kLow>(va, v, s, st.o, vbeside);
         };
         if constexpr (kHalf) {
@@ -937,9 +1026,11 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
             };
             k_load(0);
             v_load(0);
+            if (threadIdx.x == 0) uneven = 0;
             sp_wait_loads<0>();
             __syncthreads();
             q.load(image, 32 * item + li, p.scale, g);
+            if (q.uneven) uneven = 1;
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
                 k_step(0, i);
@@ -961,69 +1052,29 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
                         if (i == HD / 8 - 1) v_load(t + 2);
                     });
             }
+            if (lane == 0 && ((xk.uneven | xv.uneven) || (least <= most && most - least > kFar))) uneven = 1;
         }
-    } else {
-        typename SpPick<T, HD>::type q;
-        const uint8_t* const image = lds + kSolo;
-        sp_stage_queries<HD, 4>(p, j, row0 + 4 * w, rows, lds_address(image) + 4 * w * (HD * 4), lane);
-        const int tiles = works ? (keys + 31) / 32 : 0;
-        uint8_t* const kt = lds + w * kWaveLds;
-        uint8_t* const vt = kOne ? kt : kt + kTile;
-        const uint32_t kt_a = lds_address(kt), vt_a = lds_address(vt);
-        const auto stage_k = [&](int t) {
-            const int64_t row = k0 + 32 * t;
-            sp_stage<T, HD, false, kPieces>(kb + row * HD, last - row, kt_a, lane, 0);
-        };
-        const auto stage_v = [&](int t) {
-            const int64_t row = k0 + 32 * t;
-            sp_stage<T, HD, true, kPieces>(vb + row * HD, last - row, vt_a, lane, 0);
-        };
-        if (sub < tiles) {
-            stage_k(sub);
-            if (!kOne) stage_v(sub);
+        // keys, values or queries too far apart for their two parts: the chunk again on the fp32 instructions, by
+        // 32 rows
+        bool again = false;
+        if constexpr (!kHalf) {
+            __syncthreads();
+            again = __builtin_amdgcn_readfirstlane(uneven);
         }
-        sp_wait_loads<0>();
-        __syncthreads();
-        q.load(image, li, p.scale, g);
-        const float c[4] = {q.unscale, q.unscale, q.unscale, q.unscale};
-        for (int t = sub; t < tiles; t += split) {
-            const bool more = t + split < tiles;
-            sp_wait_loads<kOne ? 0 : kPieces>();  // K is there, V may be in flight
-            f16v s = sp_scores(q, kt, li, g);
-            sp_wait_lds();
-            if (kOne)
-                stage_v(t);
-            else if (more)
-                stage_k(t + split);
-            const int n = keys - 32 * t < 32 ? keys - 32 * t : 32;
-            st.softmax(s, c, n, g);
-            if (!kOne && more)
-                sp_wait_loads<kPieces>();  // V is there, the next K may be in flight
-            else
-                sp_wait_loads<0>();
-            if (n < 32) {
-                sp_clear_rows<HD * (int)sizeof(T)>(vt, n, 32, lane, 64);
-                sp_wait_lds();
-            }
-            sp_accumulate(q, vt, s, st.o, li, g);
-            sp_wait_lds();
-            if (more) {
-                if (kOne)
-                    stage_k(t + split);
-                else
-                    stage_v(t + split);
+        if (__builtin_expect(again, 0)) {
+            for (int row1 = 128 * tile;;) {
+                int l = lane;
+                asm volatile("" : "+v"(l));  // nothing is kept from one tile to the next, for want of registers
+                solo(row1, l);
+                row1 += 32;
+                // ends here, so that the other way's rows need not outlive this
+                if (row1 >= 128 * tile + 128 || row1 >= rows) __builtin_amdgcn_endpgm();
+                __syncthreads();
             }
         }
+        return finish(st, base, row0, item, sub, 2, 4);
     }
-
-    // the records, probabilities and values without their factors
-    const float down = exp2_int(-(int)kUp);
-    st.scale(ldexpf(down, top));
-    float4 v[HD / 8];
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i)
-        v[i] = make_float4(st.o[i >> 2][4 * (i & 3)], st.o[i >> 2][4 * (i & 3) + 1], st.o[i >> 2][4 * (i & 3) + 2], st.o[i >> 2][4 * (i & 3) + 3]);
-    sp_finish<HD, 32, false>(p, m, v, st.r + kUp, swap32_sum(st.l) * down, my_row, works, rows - row0, chunk, item, sub, split, shared ? 4 : 1);
+    solo(32 * tile, lane);
 }
 
 // Few keys: all of them by one workgroup per sequence, kv head and 16 queries of its group, in one launch.
