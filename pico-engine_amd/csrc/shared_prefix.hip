@@ -258,7 +258,7 @@ template <int HD>
 struct RowsF16 {
     h8v hi[HD / 16], lo[HD / 16];
     float unscale;
-    bool uneven;  // eight neighbouring elements lie 2^-16 under the row's largest, or that one is tiny or huge (SpSplit)
+    bool uneven;  // eight neighbouring elements lie 2^-16 under the row's largest, or that one is tiny or infinite (SpSplit)
     PE_DEV void load(const uint8_t* image, int r, float scale, int g) {
         float v[HD / 2], top = 0.f;
 #pragma unroll
@@ -282,11 +282,11 @@ struct RowsF16 {
             least = b < least ? b : least;
         }
         top = swap32_max(top);
-        uneven = top > 0.f && (!(top >= 0x1p-99f && top < 0x1p120f) || least < __float_as_uint(top) - (16u << 23));
-        // the row's largest element to 2^13 .. 2^14, within what fp32 holds with its inverse; the scale
-        // of the scores comes after the products
+        uneven = top > 0.f && (!(top >= 0x1p-99f && top < __builtin_huge_valf()) || least < __float_as_uint(top) - (16u << 23));
+        // the row's largest element to 2^13 .. 2^14, by factors that fp32 holds with their inverses (under
+        // 2^-113 it stays smaller); the scale of the scores comes after the products
         int e = exponent_of(top);
-        e = e < -100 ? -100 : e > 120 ? 120 : e;
+        e = e < -113 ? -113 : e > 127 ? 127 : e;
         const float f = copysignf(exp2_int(13 - e), scale);
         unscale = sp_positive(exp2_int(e - 13) * fabsf(scale));
 #pragma unroll
@@ -494,7 +494,7 @@ struct OwnRows<_Float16, HD> {
         for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(v[i]));
         top = swap32_max(swap16_max(top));
         int e = exponent_of(top);
-        e = e < -100 ? -100 : e > 120 ? 120 : e;
+        e = e < -113 ? -113 : e > 127 ? 127 : e;
         const float f = copysignf(exp2_int(13 - e), scale);
         unscale = sp_positive(exp2_int(e - 13) * fabsf(scale));
 #pragma unroll

@@ -11,7 +11,8 @@ Tolerance, per row and dim, with p the probabilities, A_k = scale * sum |q_i k_i
   parts end at 2^-39 G, and only groups in which every four neighbouring dims of a key hold 2^-12 G (or
   zeros) are taken that way, so 2^-27 sum p c, c the largest of an element's four neighbours; a
   probability's end at 2^-25 where the largest p G of a row stands for 2^8 2^14 at least, so
-  2^-32 max(p G) sum |v| / G, over keys with G <= 2^12 c alone.
+  2^-32 max(p G) sum |v| / G, over keys with G <= 2^12 c alone;
+* with fp16 caches a probability ends at 2^-33 of the row's largest one: 2^-33 max(p) sum |v|.
 Nothing in it grows with a value that has no weight."""
 
 import math
@@ -48,7 +49,9 @@ def plain(q, kp, vp, ko, vo, own, scale):
             W = p @ v.abs()
             t = 2.0 ** -24 * (4 * math.sqrt(hd) + 8) * ((p * A) @ v.abs() + (p * A).sum(-1, keepdim=True) * o.abs())
             t += 2.0 ** -24 * (2 * math.sqrt(P + n) + 20) * W
-            if B * group > 64:
+            if kp.dtype is torch.float16:
+                t += 2.0 ** -33 * p.amax(-1, keepdim=True) * v.abs().sum(0)
+            elif B * group > 64:
                 w = torch.nn.functional.pad(vp[j].double().abs(), (0, 0, 0, -P % 8)).view(-1, 8, hd)
                 G = w.amax((1, 2))[:, None].expand(-1, 8).reshape(-1)[:P]
                 c = vp[j].double().abs().view(P, hd // 4, 4).amax(-1, keepdim=True).expand(-1, -1, 4).reshape(P, hd)
@@ -208,3 +211,14 @@ def test_rows_do_not_depend_on_the_batch(K):
     many = check(K, q, kp, vp, ko, vo, own)
     _, tol = plain(q[:5], kp, vp, ko[:5], vo[:5], own[:5], 0.125)
     assert bool(((few - many[:5]).double().abs() <= 2 * tol + 2.0 ** -27).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("P", [300, 1500])
+@pytest.mark.parametrize("B,hd", SHAPES)
+def test_largest_queries(K, B, hd, P, dtype):
+    """Queries near the end of fp32's range, which the scale brings back."""
+    q, kp, vp, ko, vo, own = make(10, B, hd, P, 20)
+    kp, vp, ko, vo = (t.to(dtype) for t in (kp, vp, ko, vo))
+    for e in (110, 119, 120, 121, 124):
+        check(K, q * 2.0 ** e, kp, vp, ko, vo, own, scale=2.0 ** (-3 - e))
