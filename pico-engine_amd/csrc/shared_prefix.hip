@@ -258,6 +258,7 @@ template <int HD>
 struct RowsF16 {
     h8v hi[HD / 16], lo[HD / 16];
     float unscale;
+    int down;     // unscale is 2^down times the scale's magnitude
     bool uneven;  // eight neighbouring elements lie 2^-16 under the row's largest, or that one is tiny or infinite (SpSplit)
     PE_DEV void load(const uint8_t* image, int r, float scale, int g) {
         float v[HD / 2], top = 0.f;
@@ -288,7 +289,8 @@ struct RowsF16 {
         int e = exponent_of(top);
         e = e < -113 ? -113 : e > 127 ? 127 : e;
         const float f = copysignf(exp2_int(13 - e), scale);
-        unscale = sp_positive(exp2_int(e - 13) * fabsf(scale));
+        down = e - 13;
+        unscale = sp_positive(exp2_int(down) * fabsf(scale));
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
 #pragma unroll
@@ -970,7 +972,7 @@ __global__ __launch_bounds__(64 * kSpWaves, 2) void k_shared_prefix(SpArgs p) {
                 const int* e = exps[t & 1] + 4 * sub;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    c[i] = sp_positive(ldexpf(c[i], e[i]));
+                    c[i] = sp_positive(ldexpf(fabsf(p.scale), q.down + e[i]));  // together: one of them may leave fp32's range
                     ev[i] = __builtin_amdgcn_readfirstlane(e[8 + i]);
                     most = ev[i] > most ? ev[i] : most;
                     least = ev[i] > kZeros && ev[i] < least ? ev[i] : least;

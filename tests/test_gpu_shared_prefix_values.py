@@ -222,3 +222,12 @@ def test_largest_queries(K, B, hd, P, dtype):
     kp, vp, ko, vo = (t.to(dtype) for t in (kp, vp, ko, vo))
     for e in (110, 119, 120, 121, 124):
         check(K, q * 2.0 ** e, kp, vp, ko, vo, own, scale=2.0 ** (-3 - e))
+
+
+@pytest.mark.parametrize("P", [300, 1500])
+@pytest.mark.parametrize("B,hd", SHAPES)
+def test_small_queries_with_huge_keys(K, B, hd, P):
+    """Factors of the scores that leave fp32's range one by one and not together."""
+    q, kp, vp, ko, vo, own = make(11, B, hd, P, 20)
+    for qe, ke, se in ((-90, 118, -31), (-60, 100, -43), (-95, 60, 32)):
+        check(K, q * 2.0 ** qe, kp * 2.0 ** ke, vp, ko * 2.0 ** ke, vo, own, scale=2.0 ** se)
