@@ -797,7 +797,7 @@ int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, 
  *   prefix_len = (device scalar if prefix_len_dtype) + prefix_len_add, own_len[b] likewise (one device
  *   integer per sequence), each clamped to its capacity. Nothing behind a length is used: it may hold
  *   anything. No keys at all, or a negative own_len (a sequence that takes no part): zeros.
- *   round_fp16 as pe_decode_attn. Sums and softmax statistics are fp32. Products are fp32 too with fp32
+ *   scale: finite, of any sign. round_fp16 as pe_decode_attn. Sums and softmax statistics are fp32. Products are fp32 too with fp32
  *   caches for the own keys, and for the prefix's where a kv head has up to 64 query rows (batch *
  *   n_head / n_kv). All others take their fp32 factors as the sum of two fp16 values each: the query
  *   within 2^-22 of an element or 2^-38 of its row's largest, the probabilities within 2^-23 or 2^-33 of the

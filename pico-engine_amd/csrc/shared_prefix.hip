@@ -40,6 +40,8 @@
 // that rounds to a half register (30.9 for 29.5).
 #include "pe_common.h"
 
+#include <cmath>
+
 namespace pe {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -1297,7 +1299,8 @@ extern "C" int pe_shared_prefix_attn(const pe_shared_prefix_args* a, pe_stream_t
     if (a->prefix_len_dtype < 0 || a->prefix_len_dtype > 2 || a->own_len_dtype < 0 || a->own_len_dtype > 2)
         return PE_ERR_TYPE;
     if (a->batch == 0) return PE_OK;
-    if (!sp_shape_ok(a->batch, a->n_head, a->n_kv, a->head_dim, a->prefix_capacity, a->own_capacity))
+    if (!sp_shape_ok(a->batch, a->n_head, a->n_kv, a->head_dim, a->prefix_capacity, a->own_capacity) ||
+        !std::isfinite(a->scale))
         return PE_ERR_SHAPE;
     // the prefix's keys that the launch is cut for: its length where the host knows it
     int64_t keys = a->prefix_capacity;

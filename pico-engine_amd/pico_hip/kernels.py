@@ -1787,6 +1787,9 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
         o_ptr, o_code = own.data_ptr(), _ints(own, B, "own")
     else:
         o_add += int(own)
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale {scale}")
     if out is None:
         out = torch.empty_like(q)
     elif out.dtype is not torch.float32 or tuple(out.shape) != (B, n_head, hd) or not out.is_contiguous():
@@ -1802,7 +1805,7 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     a = SharedPrefixArgs(q.data_ptr(), code, k_prefix.data_ptr(), v_prefix.data_ptr(), P, p_ptr, p_code, p_add,
                          k_own.data_ptr(), v_own.data_ptr(), cap, o_ptr, o_code, o_add, B, n_head, n_kv, hd,
-                         float(hd ** -0.5 if scale is None else scale), int(round_fp16), out.data_ptr(), ws, ws_bytes)
+                         scale, int(round_fp16), out.data_ptr(), ws, ws_bytes)
     _launch(dev, "pe_shared_prefix_attn", ctypes.byref(a))
     return out
 

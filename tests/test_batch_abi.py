@@ -101,3 +101,14 @@ def test_adjust_logits(lib):
         assert call(**{name: None}) == 1, name
     for name in ("x", "y", "history", "lengths", "prompt", "repetition_rows", "frequency_rows", "presence_rows", "bias", "mask"):
         assert call(**{name: ODD}) == 4, name
+
+
+def test_shared_prefix_attn_scale(lib):
+    """A scale that is no number, or infinite, is refused."""
+    from pico_hip._lib import SharedPrefixArgs
+    d = dict(q=F, cache_type=1, k_prefix=F, v_prefix=F, prefix_capacity=3000, prefix_len_add=3000, k_own=F, v_own=F,
+             own_capacity=40, own_len=F, own_len_dtype=2, batch=3, n_head=14, n_kv=2, head_dim=64, out=ODD, workspace=F,
+             workspace_bytes=1 << 30)
+    call = lambda x: lib.pe_shared_prefix_attn(ctypes.byref(SharedPrefixArgs(scale=x, **d)), None)
+    assert [call(x) for x in (0.125, -2.0, 0.0, 3e38)] == [4] * 4      # as far as the misaligned output
+    assert [call(x) for x in (float("nan"), float("inf"), float("-inf"))] == [3] * 3

@@ -231,3 +231,10 @@ def test_small_queries_with_huge_keys(K, B, hd, P):
     q, kp, vp, ko, vo, own = make(11, B, hd, P, 20)
     for qe, ke, se in ((-90, 118, -31), (-60, 100, -43), (-95, 60, 32)):
         check(K, q * 2.0 ** qe, kp * 2.0 ** ke, vp, ko * 2.0 ** ke, vo, own, scale=2.0 ** se)
+
+
+def test_scales_that_are_no_numbers(K):
+    q, kp, vp, ko, vo, own = make(12, 5, 64, 1500, 20)
+    for x in (math.nan, math.inf, -math.inf):
+        with pytest.raises(ValueError):
+            K.shared_prefix_attn(q, kp, vp, ko, vo, own, scale=x)
