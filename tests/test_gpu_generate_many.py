@@ -120,6 +120,18 @@ def test_generate_many_plain_greedy_is_generate(eng):
         assert got[0] == got[1] and got[0][:min(sure, 24)] == want[:sure] or dtype is torch.float16
 
 
+@pytest.mark.parametrize("dtype,bound", [(torch.float32, 1e-3), (torch.float16, 3e-3)])
+def test_generate_many_plain_greedy_with_either_cache(eng, dtype, bound):
+    """Without rules the tokens are the host loop's up to the first pick that both sides' bound on the logits leaves
+    open, twice that of test_decode_shared_matches_single_sequences."""
+    for ids in ([5, 77, 901, 3, 12, 640], list(range(300, 340))):
+        want, margins = host_loop(eng, ids, 24, dict(repetition=1.0, frequency=0.0, presence=0.0), torch.zeros(1024), [])
+        sure = next((i for i, m in enumerate(margins) if m < 2 * bound), 24)
+        got = eng.generate_many(ids, 3, 24, temperature=0.0, eos_id=-2, cache_dtype=dtype)
+        assert got[0] == got[1] == got[2] and len(got[0]) == 24
+        assert sure >= 3 and got[0][:sure] == want[:sure], (sure, got[0], want)
+
+
 def test_generate_many_stops_and_samples(eng):
     """A stop token ends its sequence only; sampled continuations differ and repeat with the generator."""
     ids = list(range(20, 40))
