@@ -1560,7 +1560,8 @@ __all__ = ["LAYOUT_NATURAL", "LAYOUT_X_UT", "LAYOUT_Y_UT", "to_ut", "from_ut", "
            "fix_acc_block", "fix_stride", "qkv_fix_rmsnorm_rope", "FFN_REPLICAS",
            "DecodeStep", "decode_step_supported", "decode_step_workspace",
            "gemm_f16", "gemm_f16_silu", "interleave_gate_up_f16", "flash_prefill",
-           "BLOCK_SIZE"]
+           "rope_freqs", "rope_positions", "rope_append", "shared_prefix_attn", "shared_prefix_attn_workspace",
+           "adjust_logits", "BLOCK_SIZE"]
 
 
 # ---- a batch of continuations of one prompt -------------------------------------------------

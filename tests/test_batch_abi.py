@@ -112,3 +112,10 @@ def test_shared_prefix_attn_scale(lib):
     call = lambda x: lib.pe_shared_prefix_attn(ctypes.byref(SharedPrefixArgs(scale=x, **d)), None)
     assert [call(x) for x in (0.125, -2.0, 0.0, 3e38)] == [4] * 4      # as far as the misaligned output
     assert [call(x) for x in (float("nan"), float("inf"), float("-inf"))] == [3] * 3
+
+
+def test_public_names():
+    """The batch operators are among the names that the module offers."""
+    from pico_hip import kernels
+    names = {"rope_freqs", "rope_positions", "rope_append", "shared_prefix_attn", "shared_prefix_attn_workspace", "adjust_logits"}
+    assert names <= set(kernels.__all__) and all(hasattr(kernels, n) for n in kernels.__all__)
