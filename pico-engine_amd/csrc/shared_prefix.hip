@@ -399,7 +399,7 @@ struct SpState {
         float mx = NEG_INF;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const float m = fmaxf(fmaxf(fmaxf(s[i], s[i + 1]), s[i + 2]), s[i + 3]);
+            const float m = fmaxf(fmaxf(fmaxf(fmaxf(NEG_INF, s[i]), s[i + 1]), s[i + 2]), s[i + 3]);
             mx = fmaxf(mx, WEIGHTED ? fmaf(m, c[i >> 2], (float)w[i >> 2]) : m * c[i >> 2]);
         }
         mx = swap32_max(mx);
@@ -569,7 +569,8 @@ struct SpSplit {
     // key's element 2^-23, and where the largest is infinite or under 2^-99. Four normal values lie 2^-12 under the
     // largest of 1024 once in 10^9 blocks. Eight stages.
     static constexpr uint32_t kUneven = (VALUES ? 12u : 16u) << 23;
-    static PE_DEV float largest(const float4& a) { return fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fabsf(a.z)), fabsf(a.w)); }
+    // from 0 on, two instructions: maxima of two unknown values quieten both first
+    static PE_DEV float largest(const float4& a) { return fmaxf(fmaxf(fmaxf(fmaxf(0.f, fabsf(a.x)), fabsf(a.y)), fabsf(a.z)), fabsf(a.w)); }
     // the smaller, a zero being no small value: the bits less one
     static PE_DEV uint32_t smaller(uint32_t least, float a) {
         const uint32_t b = __float_as_uint(a) - 1;
