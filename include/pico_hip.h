@@ -803,7 +803,7 @@ int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, 
  *   within 2^-22 of an element or 2^-38 of its row's largest, the probabilities within 2^-23 or 2^-33 of the
  *   row's largest one, and an fp32 prefix's keys and values within 2^-23 of an element or 2^-39 of the
  *   largest G of 8 keys, its probabilities' 2^-33 being that of the row's largest p G. Keys of an fp32
- *   prefix that this would cost more than 2^-23 of their four neighbouring dims (2^-27 of a value's), and
+ *   prefix that this would cost more than 2^-23 of their four neighbouring dims (2^-25 of a value's), and
  *   infinite ones, are taken in fp32. With fp16 caches an infinite key or value that a row sees may make it NaN.
  * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes (0: NULL will do), any contents, with
  * prefix_keys = prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in

@@ -565,10 +565,11 @@ struct SpSplit {
     }
     // The exponent E with the largest element in [2^(14 + E), 2^(15 + E)): the two parts hold every element to
     // 2^-23 of itself or 2^-39 of the largest. `uneven` says where that is not enough: where four neighbouring
-    // dims of a key lie kUneven under the largest (zeros are exact), so that a value keeps 2^-27 of its neighbours and a
-    // key's element 2^-23, and where the largest is infinite or under 2^-99. Four normal values lie 2^-12 under the
-    // largest of 1024 once in 10^9 blocks. Eight stages.
-    static constexpr uint32_t kUneven = (VALUES ? 12u : 16u) << 23;
+    // dims of a key lie kUneven under the largest (zeros are exact), so that a value keeps 2^-25 of its neighbours and a
+    // key's element 2^-23, and where the largest is infinite or under 2^-99. Four normal values lie 2^-14 under the
+    // largest of 1024 once in 10^11 blocks, and a key whose values are all 2^8 smaller than the others' stays even. Eight
+    // stages.
+    static constexpr uint32_t kUneven = (VALUES ? 14u : 16u) << 23;
     // from 0 on, two instructions: maxima of two unknown values quieten both first
     static PE_DEV float largest(const float4& a) { return fmaxf(fmaxf(fmaxf(fmaxf(0.f, fabsf(a.x)), fabsf(a.y)), fabsf(a.z)), fabsf(a.w)); }
     // the smaller, a zero being no small value: the bits less one

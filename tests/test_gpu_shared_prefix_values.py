@@ -8,10 +8,10 @@ Tolerance, per row and dim, with p the probabilities, A_k = scale * sum |q_i k_i
   2^-24 (4 sqrt(hd) + 8) sum p_k A_k (|v_k| + |o|);
 * exp2, the division, 22 bits of probability and value, sums over n keys: 2^-24 (2 sqrt(n) + 20) W, W = sum p |v|;
 * behind more than 64 rows, by groups of 8 keys from the prefix's start with G the largest magnitude of a group: a value's two
-  parts end at 2^-39 G, and only groups in which every four neighbouring dims of a key hold 2^-12 G (or
-  zeros) are taken that way, so 2^-27 sum p c, c the largest of an element's four neighbours; a
+  parts end at 2^-39 G, and only groups in which every four neighbouring dims of a key hold 2^-14 G (or
+  zeros) are taken that way, so 2^-25 sum p c, c the largest of an element's four neighbours; a
   probability's end at 2^-25 where the largest p G of a row stands for 2^8 2^14 at least, so
-  2^-32 max(p G) sum |v| / G, over keys with G <= 2^12 c alone;
+  2^-32 max(p G) sum |v| / G, over keys with G <= 2^14 c alone;
 * with fp16 caches a probability ends at 2^-33 of the row's largest one: 2^-33 max(p) sum |v|.
 Nothing in it grows with a value that has no weight."""
 
@@ -55,9 +55,9 @@ def plain(q, kp, vp, ko, vo, own, scale):
                 w = torch.nn.functional.pad(vp[j].double().abs(), (0, 0, 0, -P % 8)).view(-1, 8, hd)
                 G = w.amax((1, 2))[:, None].expand(-1, 8).reshape(-1)[:P]
                 c = vp[j].double().abs().view(P, hd // 4, 4).amax(-1, keepdim=True).expand(-1, -1, 4).reshape(P, hd)
-                t += 2.0 ** -27 * p[:, :P] @ c
+                t += 2.0 ** -25 * p[:, :P] @ c
                 least = torch.where(c > 0, c, torch.full_like(c, math.inf)).amin(1)
-                most = torch.minimum(G, 2.0 ** 12 * least.nan_to_num(posinf=0.0))
+                most = torch.minimum(G, 2.0 ** 14 * least.nan_to_num(posinf=0.0))
                 t += 2.0 ** -32 * (p[:, :P] * most).amax(-1, keepdim=True) * (vp[j].double().abs() / G.clamp_min(1e-300)[:, None]).sum(0)
             out[b, h], tol[b, h] = o, t
     return out, tol
