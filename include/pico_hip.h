@@ -769,7 +769,7 @@ int pe_prefill_attn(const float* q, int64_t q_stride, const float* k_cache, cons
  * position, 64-bit, finite; angles are exact to 2^-52 of themselves at any position (negative ones
  * turn back). x and y PE_TYPE_F32 or PE_TYPE_F16 (computed in fp32, rounded once), head h of token t
  * at t * token stride + h * head stride (elements; y's rows must not overlap); y may be x, with x's
- * strides. n_head up to 4096, head_dim up to 65536.
+ * strides; otherwise they share no memory. n_head up to 4096, head_dim up to 65536.
  * pe_rope (kernels.py:50) takes table rows of contiguous positions, the half layout and whole heads. */
 int pe_rope_positions(int type, const void* x, int64_t x_token, int64_t x_head, const void* positions,
                       int pos_dtype, const double* freqs, int rot_dim, float amp, int interleaved, void* y,
@@ -806,7 +806,8 @@ int pe_rope_append(const float* qkv, int64_t qkv_stride, const void* positions, 
  *   prefix that this would cost more than 2^-23 of their four neighbouring dims (2^-25 of a value's), and
  *   infinite ones, are taken in fp32. With fp16 caches an infinite key or value that a row sees may make it NaN.
  * workspace: pe_shared_prefix_attn_workspace_bytes(...) bytes (0: NULL will do), any contents, with
- * prefix_keys = prefix_len_add where the host knows the length (dtype 0), else the capacity. Calls in
+ * prefix_keys = prefix_len_add where the host knows the length (dtype 0), else the capacity. Another
+ * length's size may be larger, a shorter one's too (how the keys are cut follows the length). Calls in
  * order on one stream may share it, calls that overlap must not. Two launches, one for few keys. */
 typedef struct pe_shared_prefix_args {
     const float* q;
@@ -836,7 +837,7 @@ int64_t pe_shared_prefix_attn_workspace_bytes(int cache_type, int64_t batch, int
 int pe_shared_prefix_attn(const pe_shared_prefix_args* args, pe_stream_t stream);
 
 /* Rules on the logits of `batch` rows of `vocab` elements (PE_TYPE_F32 or PE_TYPE_F16, computed in
- * fp32 and rounded once; y may be x, with x's stride), in this order, with c the times a token stands in the first
+ * fp32 and rounded once; y may be x, with x's stride, and else shares no memory with it), in this order, with c the times a token stands in the first
  * lengths[b] (NULL: history_len) ids of the row's history:
  *   z += bias[v]; z = z > 0 ? z / repetition : z * repetition where the token stands in the history or
  *   the prompt; z -= c * frequency + (c > 0) * presence; z = -inf where bit v % 32 of mask word v / 32

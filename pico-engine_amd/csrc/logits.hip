@@ -6,7 +6,7 @@
 // A workgroup takes one segment of one row's vocabulary: it counts the segment's tokens of the
 // history and the prompt in LDS (whole-number additions, so their order does not matter), while its
 // logits are on their way, and stores the segment. One launch, nothing kept between calls. Bound by
-// reading and writing the logits once (from memory: 256 rows of 151643 fp16 34 us, 4.6 TB/s, of 151936 fp32 57,
+// reading and writing the logits once (from memory: 256 rows of 151643 fp16 31.4 us, 5.0 TB/s, of 151936 fp32 57,
 // 5.4), by latency for a row or two (3.5 us), and where the ids are many by looking through them: every segment
 // of a row reads all of them (from L2), a few 32-bit instructions each (24 rows of 152064 with 4000 + 770
 // ids: 9.9 us, 4.8 without; 8 rows with 30000: 11). Compared as 64-bit integers the ids cost twice as much;

@@ -20,18 +20,18 @@
 // most 2^14; the probability; and an fp32 cache's keys and values, every 8 keys scaled by a
 // power of two of their largest element. Products of two low parts are left out (2^-22). A chunk whose keys,
 // values or queries lie too far apart for their two parts (SpSplit::find) is taken again by its workgroup on the fp32
-// instructions (33 x 8001 with such a key: 36 us to 125, with one in every block 149). Per 16 elements of
+// instructions (33 x 8001 with such a key: 36 us to 124, with one in every block 149). Per 16 elements of
 // a dot product that is 2 instructions for 16-bit caches and 3 for fp32 ones in place of 8 fp32 instructions
 // of twice the time each.
 //
 // Bounds and times (heads 28/4 of 128, then 14/2 of 64; us, the merge after the +):
-//   64 sequences, 32768 fp16 keys, up to 1000 own: 77 + 5.9. The matrix cores; a shared block in steady state
+//   64 sequences, 32768 fp16 keys, up to 1000 own: 77 + 5.6. The matrix cores; a shared block in steady state
 //     keeps them at 1.22 PFLOP/s (a large library product reaches 1.18); the own keys stream at 4.7 to
 //     5.5 TB/s, about 9 us are a workgroup's start and end;
-//   33 sequences, 8001 fp32 keys, up to 515 own: 30 + 4.2. A shared block takes 6700 cycles, the matrix
+//   33 sequences, 8001 fp32 keys, up to 515 own: 31 + 4.4. A shared block takes 6800 cycles, the matrix
 //     instructions of a SIMD's two waves 3100 of them; the rest is the vector work that does not fit
 //     beside them (split, softmax) and the skew of the two waves at the barrier;
-//   3 sequences, 32768 fp16 keys: 9.1 + 4.6; 16 sequences, 1500 fp32 keys: 8.6 + 3.8; 4 sequences, 277 fp32
+//   3 sequences, 32768 fp16 keys: 8.6 + 4.2; 16 sequences, 1500 fp32 keys: 8.6 + 3.8; 4 sequences, 277 fp32
 //     keys: 9.0 in one launch. Latency: lengths, queries, first tiles, a block or two, records.
 // Both run at about 1.8 GHz (busy cycles over time), as long matrix work here does. Tried without gain: key
 // rows swizzled over all 64 banks; the barrier of a block between softmax and values, so that values and
@@ -1175,16 +1175,24 @@ struct SpPlan {
     int few, shared, p_chunks, p_keys, p_tiles, o_chunks, o_keys, o_tiles, o_split;
 };
 
-// How the work is cut. Rows of a kv head over 64 go the shared way. A CU holds one workgroup; those of the
+// How the work is cut. Rows of a kv head over 64 go the shared way: up to there an fp32 prefix keeps fp32 products. Solo | shared
+// (us, 2000 and 30000 keys at head size 64, then at 128):
+//   fp16, 64 rows  9.7 | 10.3, 13 | 17, 12.6 | 14.2, 22 | 33    fp32, 33 rows  13.0 | 11.6, 21 | 21, 19 | 17, 56 | 48
+//         96 rows  9.7 | 10.3, 15 | 17, 12.9 | 15.2, 27 | 29          64 rows  13.4 | 11.8, 21 | 22, 19 | 17, 60 | 49
+//        128 rows  9.7 | 10.4, 16 | 18, 13.3 | 15.8, 31 | 30          96 rows  13.1 | 12.0, 32 | 22, 20 | 18, 77 | 51
+// so by time alone the line would lie near 128 rows for fp16 and 33 for fp32. A CU holds one workgroup (by its LDS; 16-bit
+// caches at head size 64 by its registers); those of the
 // prefix come first, the own keys' fill the other CUs and follow where one ends. Of a few numbers of waves and
 // chunks for an item's own keys, and of two or three lengths of the prefix's chunks for each, the plan is the one
 // whose longest workgroup, or whose work spread over 256 CUs, and whose records take least, by the times
 // measured at head size 128 (us): 9.5 for a prefix workgroup's start and end, 1.85 (16-bit caches) and 3.1
 // (fp32) for a shared block of 64 keys, 1.5 and 7 for eight solo tiles; 9 and 12 for an own workgroup's, 1.5 and
-// 5.3 for a wave's 32 keys. The own keys' work counts three quarters (their lengths are on the device). Best
+// 5.3 for a wave's 32 keys (at 64 the steps count half). The own keys' work counts three quarters (their lengths are on the device). Best
 // of 56 cuts | this one (us, caches two thirds full): 33 x 8001 fp32 with 515 own keys (28/4 heads) 36 | 37, 64 x
 // 32768 with 1000 142 | 147 and fp16 80 | 82, 16 x 4096 fp16 with 2000 20 | 20, 24 x 2000 fp32 with 1000 25 | 25,
 // 8 x 30000 fp32 with 4000 56 | 63; with the own waves chosen first and the rest filled with chunks 39, 165, 82, 23, 25, 63.
+// An item's own keys are cut into six chunks at most, so a few sequences with tens of thousands of them leave most
+// CUs idle: one of 30000 fp32 own keys at head size 64 takes 65 us, 6 at the copy rate.
 static SpPlan sp_plan(int64_t batch, int n_head, int n_kv, int hd, bool half, int64_t p_keys, int64_t o_cap) {
     SpPlan s;
     const int64_t group = n_head / n_kv, rows = batch * group;

@@ -1666,7 +1666,8 @@ def rope_positions(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor
     """RoPE of x (T, n_head, hd), float32 or float16 (rows and heads with any strides), token t at
     positions[t] (int32 or int64, any order, negative ones turn back): pairs (j, j + r/2) of the first
     r = 2 len(freqs) elements of a head, or (2j, 2j + 1) if ``interleaved``; the others are copied. Up
-    to 4096 heads. freqs and amp from rope_freqs; the angles are made in 64 bits. ``out`` may be x."""
+    to 4096 heads. freqs and amp from rope_freqs; the angles are made in 64 bits. ``out`` may be x, and shares no
+    memory with it otherwise."""
     dev = _one_gpu(x, positions, freqs, out)
     code = _CACHE_TYPE.get(x.dtype)
     if code is None or x.dim() != 3:
@@ -1741,7 +1742,7 @@ def shared_prefix_attn_workspace(batch: int, n_head: int, n_kv: int, hd: int, pr
                                  device) -> torch.Tensor:
     """A workspace for shared_prefix_attn with caches of either type (any contents; reusable by calls in
     order on one stream). prefix_keys: the prefix's length, or its capacity where the length is a device
-    tensor."""
+    tensor; a shorter prefix may need more than a longer one, and a workspace that is too small is refused."""
     size = max(_shared_prefix_bytes(t, batch, n_head, n_kv, hd, prefix_keys, own_capacity) for t in _CACHE_TYPE.values())
     return torch.empty(size, device=device, dtype=torch.uint8)
 
@@ -1756,7 +1757,8 @@ def shared_prefix_attn(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     first prefix_len prefix keys (an int, a device integer, or None: all P) and the first
     own[b] + own_offset of its own (``own`` (B,) device integers, or an int for all). A sequence
     without keys, or whose own length is negative (one that takes no part), gets zeros. ``round_fp16``
-    as decode_attn. Returns (B, n_head, hd) float32."""
+    as decode_attn. Factors that are not taken in fp32 keep 22 bits; which ones those are, and what becomes of
+    values far apart, stands at pe_shared_prefix_attn (include/pico_hip.h). Returns (B, n_head, hd) float32."""
     own_dev = own if isinstance(own, torch.Tensor) else None
     p_dev = prefix_len if isinstance(prefix_len, torch.Tensor) else None
     dev = _one_gpu(q, k_prefix, v_prefix, k_own, v_own, own_dev, p_dev, workspace, out)
@@ -1843,7 +1845,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     presence; -inf where the mask bit is 0. history (B, H) int32 or int64, of which the first
     ``lengths`` (B,) count (None: all); prompt, bias (float32, V) and mask (int32 words, bit v % 32 of
     word v // 32) one row for all or a row each. Ids outside [0, V) are passed over. The three
-    penalties are numbers or float32 vectors of one value per row. ``out`` may be logits. A row whose tokens are all ruled out is -inf throughout."""
+    penalties are numbers or float32 vectors of one value per row. ``out`` may be logits, and shares no memory with
+    them otherwise. A row whose tokens are all ruled out is -inf throughout."""
     one = logits.dim() == 1
     x = logits.unsqueeze(0) if one else logits
     if x.dtype not in _CACHE_TYPE or x.dim() != 2 or x.shape[1] == 0:
