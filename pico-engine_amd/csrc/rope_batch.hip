@@ -286,7 +286,8 @@ extern "C" int pe_rope_positions(int type, const void* x, int64_t x_token, int64
         return PE_ERR_ALIGN;
     RopeArgs p{x, x_token, x_head, y, y_token, y_head, positions, pos_dtype == 2, freqs, rot_dim / 2, head_dim, amp,
                n_head, 1, 0, tokens};
-    // 16 bytes at a time where every piece of a row is whole and aligned
+    // 16 bytes at a time where every piece of a row is whole and aligned, else single elements (65536 x 4 heads of 80:
+    // 20 rotated 39 to 41 us in fp32, 4.2 TB/s, 28 to 29 in fp16, 2.9; all 80 rotated 16.5 to 17 in fp16, 5.0)
     const int v = (int)(16 / e);
     const int64_t strides = x_token | x_head | y_token | y_head;
     const bool vec = (interleaved ? rot_dim % (2 * v) == 0 : rot_dim / 2 % v == 0) && head_dim % v == 0 &&

@@ -238,3 +238,34 @@ def test_scales_that_are_no_numbers(K):
     for x in (math.nan, math.inf, -math.inf):
         with pytest.raises(ValueError):
             K.shared_prefix_attn(q, kp, vp, ko, vo, own, scale=x)
+
+
+def test_uneven_values_in_a_graph(K):
+    """A captured call meets even and uneven keys and values in turn, and a prefix of any length; every replay is the
+    eager call's result."""
+    q, kp, vp, ko, vo, own = make(13, 37, 128, 1536, 20)
+    plen = torch.tensor([1536], device=DEV)
+    out = torch.empty_like(q)
+    K.shared_prefix_attn(q, kp, vp, ko, vo, own, plen, round_fp16=False, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.shared_prefix_attn(q, kp, vp, ko, vo, own, plen, round_fp16=False, out=out)
+    clean = kp.clone(), vp.clone()
+    for n, factor in ((1536, 1.0), (1536, 1e9), (1000, 1e9), (1536, 1.0), (801, 1e9), (7, 1.0), (1536, math.inf), (1536, 1.0)):
+        kp.copy_(clean[0])
+        vp.copy_(clean[1])
+        plen.fill_(n)
+        kp[:, 800, 0] = -60.0 * 128 ** 0.5
+        if math.isinf(factor):
+            kp[:, 800, 0] = -math.inf
+        else:
+            vp[:, 800] *= factor
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, K.shared_prefix_attn(q, kp, vp, ko, vo, own, plen, round_fp16=False))
+        assert torch.equal(got, K.shared_prefix_attn(q, kp, vp, ko, vo, own, plen, round_fp16=False))
+        if not math.isinf(factor):
+            ref, tol = plain(q, kp[:, :n], vp[:, :n], ko, vo, own, 128 ** -0.5)
+            assert bool(((got.double() - ref).abs() <= tol).all())
+        else:
+            assert bool(torch.isfinite(got).all())
