@@ -96,9 +96,14 @@ PE_DEV int64_t sp_length(const void* len, int dtype, int64_t i, int64_t add, int
 PE_DEV uint32_t lds_address(const uint8_t* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
 }
-// 16 bytes per lane from global g (uniform) + off into LDS at m0 + 16 lane (one wave instruction: 1 KB)
+// 16 bytes per lane from global g (uniform) + off into LDS at m0 + 16 lane (one wave instruction: 1 KB). The
+// address goes through a scalar copy: read back from a spill, which is a vector instruction's work, it would have to
+// be five wait states old, and the compiler does not see the load.
 PE_DEV void sp_load16(const void* g, uint32_t off, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0)
+    const void* at;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(at)
+                 : "v"(off), "s"(g), "s"(m0)
                  : "memory", "m0");
 }
 // the same from an address per lane
