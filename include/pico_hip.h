@@ -870,6 +870,134 @@ typedef struct pe_logit_args {
 } pe_logit_args;
 int pe_adjust_logits(const pe_logit_args* args, pe_stream_t stream);
 
+/* ---- a paged cache held in 4 bits -------------------------------------------------------------
+ * Norms of query and key heads with their rotary positions; keys and values of several sequences in pages that a
+ * table hands out, rounded to 4 bits as they are appended; attention over them; the values read back. No
+ * counterparts in the reference. Device integers are int32 (dtype 1) or int64 (dtype 2), a table's int32. */
+
+/* y = turn(x * w / sqrt(mean(x^2) + eps), positions[t]) of the q and the k heads of every token, the rotation as in
+ * pe_rope_positions. type PE_TYPE_F32 or PE_TYPE_F16 (computed in fp32, rounded once). Head h of token t at t * token
+ * stride + h * head stride (elements; rows of an output must not overlap). Weights fp32, head h's at h * weight
+ * head stride (0: one for all), NULL: no norm. An output may be its input, with the same strides; otherwise outputs share no
+ * memory with inputs or each other. n_head or n_kv may be 0 (that side's pointers are not looked at), each up to 4096; head_dim up to 512. */
+typedef struct pe_qk_norm_args {
+    int type;
+    const void* q;
+    int64_t q_token, q_head;
+    void* q_out;
+    int64_t q_out_token, q_out_head;
+    const float* q_weight;
+    int64_t q_weight_head;
+    const void* k;
+    int64_t k_token, k_head;
+    void* k_out;
+    int64_t k_out_token, k_out_head;
+    const float* k_weight;
+    int64_t k_weight_head;
+    const void* positions;
+    int pos_dtype;
+    const double* freqs;
+    int rot_dim;
+    float amp;
+    int interleaved;
+    float eps;
+    int64_t tokens;
+    int n_head, n_kv, head_dim;
+} pe_qk_norm_args;
+int pe_qk_norm_rope(const pe_qk_norm_args* args, pe_stream_t stream);
+
+/* A pool of pages of page_tokens tokens (a multiple of 16), page i at pages + i * page_stride bytes (a multiple of 16),
+ * 16-byte aligned, and the table of a batch: slot s of sequence b lies on page table[b * table_stride + s /
+ * page_tokens], place s % page_tokens. A page number outside [0, n_pages) stands for no page: what would be
+ * written there is dropped, its keys are seen by nobody, its values read as zeros. Sequences may share pages
+ * that are only read.
+ * A page is, for every kv head, page_tokens / 16 tiles of 16 tokens, 17 * head_dim bytes each:
+ *   8 head_dim bytes   key codes [16 tokens][head_dim / 2], the even element in a byte's low half
+ *   8 head_dim bytes   value codes [4 token groups][16 runs of head_dim / 16 elements][4 tokens][head_dim / 32]
+ *   head_dim / 2 bytes key scales [16 tokens][head_dim / 32]
+ *   head_dim / 2 bytes value scales [4 token groups][head_dim / 32][4 tokens]
+ * 32 neighbouring elements share the scale 2^e, its byte e + 127. A code is a sign (8) and one of the magnitudes 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6. e is the least in [-100, 125] that leaves the largest magnitude at 7 * 2^e or less; the nearest
+ * code is taken, halfway the even one, 6 beyond 6. Byte 255: an element was infinite or no number, all 32 are NaN. */
+typedef struct pe_kv4_pool {
+    void* pages;
+    int64_t n_pages, page_stride, page_tokens;
+    const int* table;
+    int64_t table_stride, table_cols;
+} pe_kv4_pool;
+
+/* Appends `tokens` new rows to the sequences of a batch: sequence b's are the rows starts[b] .. starts[b + 1] - 1
+ * (starts NULL: row b alone, tokens == batch), and row i of them goes to slot lengths[b] + i. k (and q, unless it is NULL) is
+ * normed by k_weight / q_weight (fp32, head_dim elements, NULL: not) and rotated by the slot's number (freqs NULL: not) as in
+ * pe_qk_norm_rope; v is taken as it is. q_out gets the q rows of q's type. Keys are computed in 64 bits, so that what is
+ * stored depends on no rounding before its own. A slot behind the table, or of a sequence of negative length (one that takes
+ * no part), is not written; its q row is. Rows before starts[0] or from starts[batch] on are left out, their q_out rows
+ * as they were. Two rows of a call must not go to one slot. tokens below 2^23, and below 2^24 over (n_head + 15) / 16 + (2 n_kv + 15) / 16;
+ * strides as in pe_qk_norm_rope (q_out may be q). */
+typedef struct pe_kv4_append_args {
+    int type; /* of q, k, v: PE_TYPE_F32 or PE_TYPE_F16 */
+    const void* q;
+    int64_t q_token, q_head;
+    void* q_out;
+    int64_t q_out_token, q_out_head;
+    const void* k;
+    int64_t k_token, k_head;
+    const void* v;
+    int64_t v_token, v_head;
+    pe_kv4_pool pool;
+    const void* lengths;
+    int lengths_dtype;
+    const void* starts;
+    int starts_dtype;
+    const double* freqs;
+    int rot_dim;
+    float amp;
+    int interleaved;
+    const float* q_weight;
+    const float* k_weight;
+    float eps;
+    int64_t tokens, batch;
+    int n_head, n_kv, head_dim; /* head_dim 64 or 128 */
+} pe_kv4_append_args;
+int pe_kv4_append(const pe_kv4_append_args* args, pe_stream_t stream);
+
+/* The values that the first `rows` slots of every sequence stand for: k, v (batch, n_kv, rows, head_dim) of `type` (PE_TYPE_F32:
+ * exact; PE_TYPE_F16: rounded), 16-byte aligned; zeros from slot lengths[b] on. */
+int pe_kv4_read(int type, const pe_kv4_pool* pool, const void* lengths, int lengths_dtype, int64_t batch, int n_kv,
+                int head_dim, int64_t rows, void* k, void* v, pe_stream_t stream);
+
+/* Attention of new rows over their sequences' pages: row i of sequence b (rows as in pe_kv4_append) sees the first
+ * lengths[b] + first + i slots, so with first 1 and the lengths before the rows were appended, all keys up to its own.
+ * Head h takes kv head h / (n_head / n_kv); q and out of `type` (PE_TYPE_F32 or PE_TYPE_F16), head h of row t at t * token stride + h * head
+ * stride; out's rows must not overlap and share no memory with q. Numbers of keys are clamped to the table's; a row that sees none, or whose
+ * sequence has a negative length, gets zeros. What lies in slots that a row does not see may be anything. scale: finite.
+ * The cache's values are taken exactly, fp32 queries and their probabilities in 24 bits, fp16 queries exactly and their
+ * probabilities in 16 bits; sums and softmax statistics are fp32. Queries of 2^127 and more, infinite ones and NaN make their row NaN.
+ * workspace: pe_kv4_attn_workspace_bytes(...) bytes (0: NULL will do), any contents; capacity = table_cols * page_tokens, ragged: starts
+ * is given. Calls in order on one stream, and graphs replayed in order, may share it, calls that overlap must not. One
+ * launch, or two where keys are cut. tokens up to 2^22. */
+typedef struct pe_kv4_attn_args {
+    int type;
+    const void* q;
+    int64_t q_token, q_head;
+    void* out;
+    int64_t out_token, out_head;
+    pe_kv4_pool pool;
+    const void* lengths;
+    int lengths_dtype;
+    int64_t first;
+    const void* starts;
+    int starts_dtype;
+    int64_t tokens, batch;
+    int n_head, n_kv, head_dim;
+    float scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} pe_kv4_attn_args;
+int64_t pe_kv4_attn_workspace_bytes(int64_t tokens, int64_t batch, int ragged, int n_head, int n_kv, int head_dim,
+                                    int64_t capacity);
+int pe_kv4_attn(const pe_kv4_attn_args* args, pe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -129,6 +129,50 @@ class LogitArgs(ctypes.Structure):
     ]
 
 
+class QkNormArgs(ctypes.Structure):
+    """Mirror of pe_qk_norm_args (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("type", _I), ("q", _P), ("q_token", _L), ("q_head", _L), ("q_out", _P), ("q_out_token", _L), ("q_out_head", _L),
+        ("q_weight", _P), ("q_weight_head", _L), ("k", _P), ("k_token", _L), ("k_head", _L), ("k_out", _P),
+        ("k_out_token", _L), ("k_out_head", _L), ("k_weight", _P), ("k_weight_head", _L), ("positions", _P),
+        ("pos_dtype", _I), ("freqs", _P), ("rot_dim", _I), ("amp", _F), ("interleaved", _I), ("eps", _F), ("tokens", _L),
+        ("n_head", _I), ("n_kv", _I), ("head_dim", _I),
+    ]
+
+
+class Kv4Pool(ctypes.Structure):
+    """Mirror of pe_kv4_pool (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("pages", _P), ("n_pages", _L), ("page_stride", _L), ("page_tokens", _L), ("table", _P), ("table_stride", _L),
+        ("table_cols", _L),
+    ]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    """Mirror of pe_kv4_append_args (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("type", _I), ("q", _P), ("q_token", _L), ("q_head", _L), ("q_out", _P), ("q_out_token", _L), ("q_out_head", _L),
+        ("k", _P), ("k_token", _L), ("k_head", _L), ("v", _P), ("v_token", _L), ("v_head", _L), ("pool", Kv4Pool),
+        ("lengths", _P), ("lengths_dtype", _I), ("starts", _P), ("starts_dtype", _I), ("freqs", _P), ("rot_dim", _I),
+        ("amp", _F), ("interleaved", _I), ("q_weight", _P), ("k_weight", _P), ("eps", _F), ("tokens", _L), ("batch", _L),
+        ("n_head", _I), ("n_kv", _I), ("head_dim", _I),
+    ]
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    """Mirror of pe_kv4_attn_args (include/pico_hip.h)."""
+
+    _fields_ = [
+        ("type", _I), ("q", _P), ("q_token", _L), ("q_head", _L), ("out", _P), ("out_token", _L), ("out_head", _L),
+        ("pool", Kv4Pool), ("lengths", _P), ("lengths_dtype", _I), ("first", _L), ("starts", _P), ("starts_dtype", _I),
+        ("tokens", _L), ("batch", _L), ("n_head", _I), ("n_kv", _I), ("head_dim", _I), ("scale", _F), ("workspace", _P),
+        ("workspace_bytes", _L),
+    ]
+
+
 _SIGNATURES = {
     "pe_strerror": (ctypes.c_char_p, [_I]),
     "pe_abi_version": (_I, []),
@@ -210,6 +254,11 @@ _SIGNATURES = {
     "pe_shared_prefix_attn_workspace_bytes": (_L, [_I, _L, _I, _I, _I, _L, _L]),
     "pe_shared_prefix_attn": (_I, [ctypes.POINTER(SharedPrefixArgs), _P]),
     "pe_adjust_logits": (_I, [ctypes.POINTER(LogitArgs), _P]),
+    "pe_qk_norm_rope": (_I, [ctypes.POINTER(QkNormArgs), _P]),
+    "pe_kv4_append": (_I, [ctypes.POINTER(Kv4AppendArgs), _P]),
+    "pe_kv4_read": (_I, [_I, ctypes.POINTER(Kv4Pool), _P, _I, _L, _I, _I, _L, _P, _P, _P]),
+    "pe_kv4_attn_workspace_bytes": (_L, [_L, _L, _I, _I, _I, _I, _L]),
+    "pe_kv4_attn": (_I, [ctypes.POINTER(Kv4AttnArgs), _P]),
 }
 
 # Every symbol include/pico_hip.h declares (checked by tests/test_abi.py).

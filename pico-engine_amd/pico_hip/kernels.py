@@ -25,8 +25,8 @@ import os
 
 import torch
 
-from ._lib import (LAYOUT_NATURAL, LAYOUT_X_UT, LAYOUT_Y_UT, AttnOprojArgs, FfnFixArgs, LogitArgs, QkvArgs,
-                   SharedPrefixArgs, StepArgs, StepLayer, check, lib)
+from ._lib import (LAYOUT_NATURAL, LAYOUT_X_UT, LAYOUT_Y_UT, AttnOprojArgs, FfnFixArgs, Kv4AppendArgs, Kv4AttnArgs,
+                   Kv4Pool, LogitArgs, QkNormArgs, QkvArgs, SharedPrefixArgs, StepArgs, StepLayer, check, lib)
 from .dequant import (BLOCK_SIZE, GGML_F16, GGML_F32, GGML_Q4_K, GGML_Q5_0, GGML_Q6_K, GGML_Q8_0, MATRIX_TYPES,
                       QUANT_TYPES, TYPE_NAMES, nbytes_for)
 
@@ -1561,7 +1561,8 @@ __all__ = ["LAYOUT_NATURAL", "LAYOUT_X_UT", "LAYOUT_Y_UT", "to_ut", "from_ut", "
            "DecodeStep", "decode_step_supported", "decode_step_workspace",
            "gemm_f16", "gemm_f16_silu", "interleave_gate_up_f16", "flash_prefill",
            "rope_freqs", "rope_positions", "rope_append", "shared_prefix_attn", "shared_prefix_attn_workspace",
-           "adjust_logits", "BLOCK_SIZE"]
+           "adjust_logits", "qk_norm_rope", "kv4_pages", "kv4_append", "kv4_read", "kv4_attn", "kv4_attn_workspace",
+           "BLOCK_SIZE"]
 
 
 # ---- a batch of continuations of one prompt -------------------------------------------------
@@ -1893,3 +1894,218 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
     if B:
         _launch(dev, "pe_adjust_logits", ctypes.byref(a))
     return out if out is not None else y[0] if one else y
+
+
+# ---- a paged cache held in 4 bits -------------------------------------------------------------
+
+def _heads(t: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -> tuple[int, int]:
+    """(token, head) strides of rows of heads (T, n, hd) whose last dim is contiguous; 0 where there is one of them."""
+    if t.dtype is not dtype or tuple(t.shape) != shape or (shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{what} must be a {dtype} {shape} tensor whose last dim is contiguous")
+    return t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+
+
+def _weight(w: torch.Tensor | None, n: int, hd: int, what: str) -> tuple[int | None, int]:
+    """The pointer and head stride of a norm's weight: (hd,) for all heads or (n, hd)."""
+    if w is None:
+        return None, 0
+    if w.dtype is not torch.float32 or tuple(w.shape) not in ((hd,), (n, hd)) or not w.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous float32 ({hd},) or ({n}, {hd}) tensor")
+    return w.data_ptr(), 0 if w.dim() == 1 else hd
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 positions: torch.Tensor, freqs: torch.Tensor, eps: float = 1e-6, amp: float = 1.0, interleaved: bool = False,
+                 out: tuple[torch.Tensor, torch.Tensor | None] | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMSNorm of every query and key head and its RoPE in one launch: q (T, n_head, hd) and k (T, n_kv, hd), float32 or
+    float16 of one type (rows and heads with any strides, hd up to 512), x * weight / sqrt(mean(x^2) + eps) turned by
+    positions[t] as in rope_positions. Weights float32, (hd,) or one row a head, None: not normed; k None: q alone. ``out``:
+    the two outputs, which may be q and k, and share no memory with them otherwise. Returns (q, k)."""
+    dev = _one_gpu(q, k, q_weight, k_weight, positions, freqs, *(out or ()))
+    code = _CACHE_TYPE.get(q.dtype)
+    if code is None or q.dim() != 3 or (k is not None and (k.dim() != 3 or k.dtype is not q.dtype or
+                                                           (k.shape[0], k.shape[2]) != (q.shape[0], q.shape[2]))):
+        raise ValueError("q and k must be float32 or float16 (T, n_head, hd) and (T, n_kv, hd) tensors of one type")
+    T, n, hd = q.shape
+    rot = _check_freqs(freqs, hd)
+    pos = _ints(positions, T, "positions")
+    if out is None:
+        out = (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
+    elif (out[1] is None) != (k is None):
+        raise ValueError("out must hold an output for q and one for k, or None where k is")
+    a = QkNormArgs()
+    a.type, a.positions, a.pos_dtype, a.freqs, a.rot_dim = code, positions.data_ptr(), pos, freqs.data_ptr(), rot
+    a.amp, a.interleaved, a.eps, a.tokens, a.n_head, a.head_dim = float(amp), int(interleaved), float(eps), T, n, hd
+    if hd > 1 and q.stride(2) != 1:
+        q = q.contiguous()
+    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, (T, n, hd), q.dtype, "q")
+    a.q_out, (a.q_out_token, a.q_out_head) = out[0].data_ptr(), _heads(out[0], (T, n, hd), q.dtype, "out's q")
+    a.q_weight, a.q_weight_head = _weight(q_weight, n, hd, "q_weight")
+    if k is not None:
+        m = k.shape[1]
+        if hd > 1 and k.stride(2) != 1:
+            k = k.contiguous()
+        a.n_kv, a.k, (a.k_token, a.k_head) = m, k.data_ptr(), _heads(k, (T, m, hd), q.dtype, "k")
+        a.k_out, (a.k_out_token, a.k_out_head) = out[1].data_ptr(), _heads(out[1], (T, m, hd), q.dtype, "out's k")
+        a.k_weight, a.k_weight_head = _weight(k_weight, m, hd, "k_weight")
+    if T and (n or a.n_kv):
+        _launch(dev, "pe_qk_norm_rope", ctypes.byref(a))
+    return out
+
+
+def kv4_pages(n_pages: int, n_kv: int, hd: int, page_tokens: int, device) -> torch.Tensor:
+    """A zeroed pool of pages of a paged 4-bit cache (kv4_append, kv4_attn, kv4_read): uint8 (n_pages, n_kv, page_tokens
+    / 16, 17 hd), page_tokens a multiple of 16, hd 64 or 128; 17 bytes for 32 elements. The form of a page stands at
+    pe_kv4_pool (include/pico_hip.h)."""
+    if page_tokens <= 0 or page_tokens % 16 or hd not in (64, 128):
+        raise ValueError(f"pages of {page_tokens} tokens of heads of {hd}: tokens must be a multiple of 16, hd 64 or 128")
+    return torch.zeros(n_pages, n_kv, page_tokens // 16, 17 * hd, device=device, dtype=torch.uint8)
+
+
+def _kv4_pool(pages: torch.Tensor, table: torch.Tensor, batch: int) -> tuple[Kv4Pool, int, int]:
+    """The C view of a pool and its table, with n_kv and hd."""
+    if pages.dtype is not torch.uint8 or pages.dim() != 4 or pages.shape[3] not in (17 * 64, 17 * 128) or \
+            pages.shape[0] == 0 or not pages[0].is_contiguous():
+        raise ValueError("pages must be a uint8 (n_pages, n_kv, page_tokens / 16, 17 hd) pool (kv4_pages), each page contiguous")
+    n, n_kv, tiles, tile = pages.shape
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != batch or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"table must hold int32 page numbers, ({batch}, pages of a sequence), its rows contiguous")
+    return Kv4Pool(pages.data_ptr(), n, pages.stride(0) if n > 1 else n_kv * tiles * tile, 16 * tiles, table.data_ptr(),
+                   table.stride(0) if batch > 1 else table.shape[1], table.shape[1]), n_kv, tile // 17
+
+
+def _kv4_rows(starts: torch.Tensor | None, tokens: int, batch: int) -> tuple[int | None, int]:
+    """Where the sequences' new rows begin: pointer and dtype code."""
+    if starts is None:
+        if tokens != batch:
+            raise ValueError(f"{tokens} rows for {batch} sequences: starts must say where each one's rows begin")
+        return None, 0
+    return starts.data_ptr(), _ints(starts, batch + 1, "starts")
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+               starts: torch.Tensor | None = None, q: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+               amp: float = 1.0, interleaved: bool = False, q_norm: torch.Tensor | None = None,
+               k_norm: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """New rows of B sequences into a paged 4-bit cache (kv4_pages): k, v (T, n_kv, hd) float32 or float16, any row and head
+    strides. Sequence b's rows are starts[b] .. starts[b + 1] - 1 (starts (B + 1,); None: one each, T == B); its row i goes to slot
+    lengths[b] + i, on page table[b, slot // page_tokens] (table (B, pages) int32). On the way k is normed by k_norm
+    (float32 (hd,), None: not) and rotated by its slot's number (freqs and amp from rope_freqs, None: not), in 64 bits;
+    ``q`` (T, n_head, hd) likewise by q_norm, and returned in its own type (None without q). ``lengths`` is not
+    changed. Rows that find no page (slots behind the table, page numbers outside the pool, a negative length: a sequence
+    that takes no part) are not stored; rows of no sequence are left out, their output as it was. Two rows must not go
+    to one slot. ``out`` may be q, and shares no memory with the inputs otherwise."""
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    dev = _one_gpu(k, v, pages, table, lengths, starts, q, freqs, q_norm, k_norm, out)
+    pool, n_kv, hd = _kv4_pool(pages, table, B)
+    code = _CACHE_TYPE.get(k.dtype)
+    if code is None or k.dim() != 3:
+        raise ValueError(f"k must be a float32 or float16 (T, {n_kv}, {hd}) tensor")
+    T = k.shape[0]
+    a = Kv4AppendArgs()
+    a.type, a.pool, a.tokens, a.batch, a.n_kv, a.head_dim, a.eps = code, pool, T, B, n_kv, hd, float(eps)
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.dim() == 3 and v.stride(2) != 1:
+        v = v.contiguous()
+    a.k, (a.k_token, a.k_head) = k.data_ptr(), _heads(k, (T, n_kv, hd), k.dtype, "k")
+    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, (T, n_kv, hd), k.dtype, "v")
+    a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
+    a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
+    if freqs is not None:
+        a.freqs, a.rot_dim, a.amp, a.interleaved = freqs.data_ptr(), _check_freqs(freqs, hd), float(amp), int(interleaved)
+    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None and (w.dtype is not torch.float32 or tuple(w.shape) != (hd,) or not w.is_contiguous()):
+            raise ValueError(f"{what} must be a contiguous float32 ({hd},) tensor")
+    a.k_weight = None if k_norm is None else k_norm.data_ptr()
+    if q is not None:
+        if q.dim() != 3 or q.shape[1] == 0:
+            raise ValueError(f"q must be a {k.dtype} ({T}, n_head, {hd}) tensor")
+        n = q.shape[1]
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        if out is None:
+            out = q.new_empty((T, n, hd))
+        a.n_head, a.q, (a.q_token, a.q_head) = n, q.data_ptr(), _heads(q, (T, n, hd), k.dtype, "q")
+        a.q_out, (a.q_out_token, a.q_out_head) = out.data_ptr(), _heads(out, (T, n, hd), k.dtype, "out")
+        a.q_weight = None if q_norm is None else q_norm.data_ptr()
+    elif out is not None or q_norm is not None:
+        raise ValueError("out and q_norm go with q")
+    if T and B:
+        _launch(dev, "pe_kv4_append", ctypes.byref(a))
+    return out
+
+
+def kv4_read(pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, rows: int,
+             dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that a paged 4-bit cache holds: (B, n_kv, rows, hd) each, float32 (exact) or float16 (rounded), slot s of
+    sequence b in row s, zeros from lengths[b] on and where there is no page."""
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    dev = _one_gpu(pages, table, lengths)
+    pool, n_kv, hd = _kv4_pool(pages, table, B)
+    if dtype not in _CACHE_TYPE or rows < 0:
+        raise ValueError(f"{rows} rows of {dtype}: dtype must be float32 or float16")
+    code = _ints(lengths, B, "lengths")
+    k, v = (torch.empty(B, n_kv, rows, hd, device=pages.device, dtype=dtype) for _ in range(2))
+    if B and rows:
+        _launch(dev, "pe_kv4_read", _CACHE_TYPE[dtype], ctypes.byref(pool), lengths.data_ptr(), code, B, n_kv, hd, int(rows),
+                k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_bytes(tokens: int, batch: int, ragged: bool, n_head: int, n_kv: int, hd: int, capacity: int) -> int:
+    size = lib.pe_kv4_attn_workspace_bytes(tokens, batch, int(ragged), n_head, n_kv, hd, capacity)
+    check(0 if size >= 0 else -size, "pe_kv4_attn_workspace_bytes")
+    return size
+
+
+def kv4_attn_workspace(tokens: int, batch: int, n_head: int, n_kv: int, hd: int, capacity: int, device,
+                       ragged: bool = False) -> torch.Tensor:
+    """A workspace for kv4_attn (any contents; reusable by calls in order on one stream): ``tokens`` rows of ``batch``
+    sequences, tables of ``capacity`` slots (pages of a sequence times page_tokens); ragged: with ``starts``."""
+    return torch.empty(_kv4_bytes(tokens, batch, bool(ragged), n_head, n_kv, hd, capacity), device=device, dtype=torch.uint8)
+
+
+def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+             starts: torch.Tensor | None = None, first: int = 1, scale: float | None = None,
+             workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of new rows of B sequences over their pages of a 4-bit cache (kv4_pages): q (T, n_head, hd) float32 or
+    float16, any row and head strides. Sequence b's rows are starts[b] .. starts[b + 1] - 1 (None: one each, T == B); its row
+    i sees the first lengths[b] + first + i slots: with the lengths from before kv4_append's rows, all keys up to its own.
+    A row that sees none, or of a sequence of negative length (one that takes no part), gets zeros; rows of no sequence are left as they
+    were. Keys and values are taken exactly as stored, float32 queries in 24 bits. Returns (T, n_head, hd) of q's type;
+    ``out`` shares no memory with q."""
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    dev = _one_gpu(q, pages, table, lengths, starts, workspace, out)
+    pool, n_kv, hd = _kv4_pool(pages, table, B)
+    code = _CACHE_TYPE.get(q.dtype)
+    if code is None or q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % n_kv or q.shape[2] != hd:
+        raise ValueError(f"q must be a float32 or float16 (T, n_head, {hd}) tensor, n_head a multiple of {n_kv}")
+    T, n, _ = q.shape
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    a = Kv4AttnArgs()
+    a.type, a.pool, a.tokens, a.batch, a.n_head, a.n_kv, a.head_dim, a.first = code, pool, T, B, n, n_kv, hd, int(first)
+    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, (T, n, hd), q.dtype, "q")
+    a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
+    a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
+    a.scale = hd ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(a.scale):
+        raise ValueError(f"scale {scale}")
+    if out is None:
+        out = q.new_empty((T, n, hd))
+    a.out, (a.out_token, a.out_head) = out.data_ptr(), _heads(out, (T, n, hd), q.dtype, "out")
+    if T == 0 or B == 0:
+        return out
+    need = _kv4_bytes(T, B, starts is not None, n, n_kv, hd, pool.table_cols * pool.page_tokens)
+    if workspace is None:
+        if need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(dev, "pe_kv4_attn", ctypes.byref(a))
+    return out
