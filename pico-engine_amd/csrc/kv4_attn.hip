@@ -17,8 +17,13 @@
 
 namespace pe {
 
-constexpr int kKv4Step = 64;    // keys a wave takes at a time
-constexpr int kKv4Waves = 4;    // of a workgroup
+// Tiles of 16 keys that a wave takes at a time: two, with which the state of 16 rows leaves room for three waves a SIMD
+// (64 x 16384 keys of 8 heads of 128, fp16: 150 us with four, 140 with two); four for 32 rows of heads of 128, whose
+// state leaves room for two waves a SIMD or one either way (2 x 1021 rows of 28 heads on 8000 keys: 385 us with two, 372 with four).
+template <int HD, int RT>
+constexpr int kKv4Tiles = HD == 128 && RT == 2 ? 4 : 2;
+constexpr int kKv4Waves = 4;   // of a workgroup
+constexpr int kKv4Span = 64;   // chunks are whole multiples of it
 constexpr float kKv4Log2e = 1.4426950408889634f;
 
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
@@ -45,9 +50,13 @@ struct Kv4AttnArgs {
     int starts_wide;
     int64_t tokens;
     int batch, n_head, n_kv, group;
-    float scale;  // times log2 e
+    float scale, sign;  // the scale's magnitude times log2 e, its sign (0: the queries are zeros, the magnitude 1)
+    int64_t capacity;   // slots of a sequence
+    int vec;            // q's rows are whole pieces of 16 bytes
     int items, blocks;  // workgroups a kv head, row blocks at most
-    int min_chunk;
+    int min_chunk;         // least keys of a chunk
+    float weight;
+    int rec_rows;          // rows of a record
     int4* plan;         // of every sequence: first item, chunks, row blocks
     float* record;      // [kv head][item][row][HD]
     float* stat;        // [kv head][item][row] (maximum, sum)
@@ -55,9 +64,9 @@ struct Kv4AttnArgs {
 
 // Work of a sequence.
 struct Kv4Seq {
-    int64_t lo;      // first row
-    int rows;        // rows times the heads of a group
-    int64_t keys;    // keys that its first row sees (0: it takes no part)
+    int64_t lo;   // first row
+    int rows;     // rows times the heads of a group
+    int64_t keys; // keys that its first row sees (far below 0: it takes no part)
 };
 
 PE_DEV Kv4Seq kv4_seq(const Kv4AttnArgs& p, int b) {
@@ -69,13 +78,18 @@ PE_DEV Kv4Seq kv4_seq(const Kv4AttnArgs& p, int b) {
 
 // Keys that row i (of a token) sees.
 PE_DEV int kv4_keys(const Kv4AttnArgs& p, int64_t first_keys, int i) {
-    const int64_t cap = (int64_t)p.table_cols * p.tiles * kKv4Tile, k = first_keys + i;
-    return (int)(k < 0 ? 0 : k > cap ? cap : k);
+    const int64_t k = first_keys + i;
+    return (int)(k < 0 ? 0 : k > p.capacity ? p.capacity : k);
 }
 
-PE_DEV int64_t wave_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, kWave);
+// Sum over the lanes up to and including each (six steps of DPP: rows of 16, then the rows below).
+PE_DEV int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);  // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);  // row_bcast 31 into rows 2 and 3
     return v;
 }
 
@@ -83,40 +97,53 @@ struct Kv4Item {
     int b, block, chunk, chunks, blocks, base, span;  // span: keys of a chunk
 };
 
-// Which work the item is: a (sequence, row block, chunk of keys). All sequences' keys times row blocks are cut by
-// one length, the least (in steps) that makes no more items than the launch has. Every wave finds it for itself.
+// Which work the item is: a (sequence, row block, chunk of keys). Every wave finds it for itself, from all lengths.
+// A chunk's length S weighs what workgroups cost beside their keys against the time that the last one takes
+// alone, cost(all keys) + S a + (all keys / S) F / (256 c) with a of a key, F of a workgroup, c of them on a CU
+// at once: the least is at S = sqrt(all keys F / (256 c a)), p.weight the factor behind the root.
 template <int RB>
 PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
     const int lane = threadIdx.x & 63;
+    const auto look = [&](int b, int& nb, int& keys) {  // row blocks, keys of the last row
+        nb = keys = 0;
+        if (b >= p.batch) return;
+        const Kv4Seq s = kv4_seq(p, b);
+        nb = (s.rows + RB - 1) / RB;
+        if (nb) keys = kv4_keys(p, s.keys, s.rows / p.group - 1);
+    };
+    const auto chunks_of = [](int keys, int span) { return keys > span ? (int)((uint32_t)(keys + span - 1) / (uint32_t)span) : 1; };
+    int nb0, keys0;
+    look(lane, nb0, keys0);
     int span = 1 << 30;
     if (p.items > p.blocks) {
-        int64_t cost = 0;
-        for (int b = lane; b < p.batch; b += 64) {
-            const Kv4Seq s = kv4_seq(p, b);
-            const int nb = (s.rows + RB - 1) / RB;
-            if (nb) cost += (int64_t)nb * kv4_keys(p, s.keys, s.rows / p.group - 1);
+        int64_t cost = (int64_t)nb0 * keys0;
+        for (int b = lane + 64; b < p.batch; b += 64) {
+            int nb, keys;
+            look(b, nb, keys);
+            cost += (int64_t)nb * keys;
         }
-        cost = wave_sum64(cost);
-        const int64_t room = p.items - p.blocks, even = ((cost + room - 1) / room + kKv4Step - 1) / kKv4Step * kKv4Step;
-        span = (int)(even < p.min_chunk ? p.min_chunk : even > (1 << 30) ? 1 << 30 : even);
+        const float all = wave_sum<64>((float)cost);
+        span = ((int)fmaxf(sqrtf(all * p.weight), (float)p.min_chunk) + kKv4Span - 1) / kKv4Span * kKv4Span;
+        int count = nb0 * chunks_of(keys0, span);
+        for (int b = lane + 64; b < p.batch; b += 64) {
+            int nb, keys;
+            look(b, nb, keys);
+            count += nb * chunks_of(keys, span);
+        }
+        // more than the launch has (or than an int holds): keys times blocks shared out evenly, in 32-bit floats, and a 4096th
+        // more, which is beyond what their rounding takes off
+        if (wave_sum<64>((float)count) > (float)p.items * (1.f - 1.f / 4096)) {
+            const float safe = all / (float)(p.items - p.blocks) * (1.f + 1.f / 4096) + kKv4Span;
+            span = safe < (float)(1 << 30) ? (int)safe / kKv4Span * kKv4Span : 1 << 30;
+            span = span < p.min_chunk ? p.min_chunk : span;
+        }
     }
     int base = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        int nb = 0, chunks = 1;
-        if (b0 + lane < p.batch) {
-            const Kv4Seq s = kv4_seq(p, b0 + lane);
-            nb = (s.rows + RB - 1) / RB;
-            if (nb) {
-                const int keys = kv4_keys(p, s.keys, s.rows / p.group - 1);
-                chunks = keys > span ? (keys + span - 1) / span : 1;
-            }
-        }
-        int upto = nb * chunks;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, kWave);
-            if (lane >= o) upto += v;
-        }
+        int nb = nb0, keys = keys0;
+        if (b0) look(b0 + lane, nb, keys);
+        const int chunks = chunks_of(keys, span);
+        const int upto = wave_scan(nb * chunks);
         const uint64_t beyond = __ballot(base + upto > item);
         if (beyond) {
             const int at = __builtin_ctzll(beyond);
@@ -126,7 +153,7 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             w.base = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
             w.span = span;
             // blocks of the same keys one after the other
-            w.chunk = (item - w.base) / w.blocks;
+            w.chunk = w.blocks == 1 ? item - w.base : (item - w.base) / w.blocks;
             w.block = item - w.base - w.chunk * w.blocks;
             return true;
         }
@@ -147,7 +174,8 @@ PE_DEV void split_pair(float a, float b, uint32_t* w) {
     }
 }
 
-// The two codes of byte SEL of w as a pair of bf16 (low half: the low four bits), times scale.
+// The two codes of byte sel of w as a pair of bf16 (low half: the low four bits), times scale, of which the exponent's
+// bits alone count; all of them set makes NaN.
 PE_DEV uint32_t two_codes(uint32_t w, float scale, int sel) {
     bf2v z;
     if (sel == 0)
@@ -161,64 +189,93 @@ PE_DEV uint32_t two_codes(uint32_t w, float scale, int sel) {
     return __builtin_bit_cast(uint32_t, z);
 }
 
-// A lane's part of 64 keys: codes, scale bytes, and the number of each 16 keys' first one (scalar).
-template <int HD>
-struct Kv4Raw {
-    static constexpr int N = HD / 32;  // words of codes per 16 keys
-    uint32_t k[4][N], v[4][N], ks[4], vs[4];
-    int key[4];
-};
-
-// Where a wave's next 64 keys lie.
+// Which keys a wave takes next, and where they lie: all scalar.
+template <int TS>
 struct Kv4Walk {
-    int col, tile;   // page of the table, tile in it, of the next step's first 16 keys
-    int key, end;    // the first key, the item's last
-    int step_cols, step_tiles;
+    const uint8_t* at[TS];  // the 16 keys' tiles
+    int key[TS];    // numbers of their first keys
+    int id[TS];     // pages of the step behind
+    int col, tile;         // page of the table, tile in it, of that step's first 16 keys
+    int next, end;         // its first key, the item's last
+    int cols, tiles;       // from step to step
 };
 
 constexpr int kNoKeys = 0x7FFFFF00;  // number of the first key of 16 that are not there
 
-template <int HD>
-PE_DEV void kv4_load(const Kv4AttnArgs& p, const int* table, const uint8_t* head, Kv4Walk& w, int lane, Kv4Raw<HD>& r) {
-    constexpr int N = HD / 32;
-    const int n = lane & 15, g = lane >> 4;
+// The table's pages of the next step: read a step ahead of the loads that go there.
+template <int TS>
+PE_DEV void kv4_pages(const Kv4AttnArgs& p, const int* table, Kv4Walk<TS>& w) {
+    typedef const __attribute__((address_space(4))) int* scalar_ints;
+    const scalar_ints ids = (scalar_ints)(uintptr_t)table;
     int col = w.col, tile = w.tile;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        int page = -1;
-        if (w.key + 16 * i < w.end) page = table[col];
-        page = __builtin_amdgcn_readfirstlane(page);
-        const bool there = page >= 0 && page < p.n_pages;
-        r.key[i] = there ? w.key + 16 * i : kNoKeys;
-        // keys that are not there are loaded from the pool's first page, and masked
-        const uint8_t* z = head + (there ? page * p.page_stride + (int64_t)tile * (17 * HD) : 0);
-        const uint8_t* kc = z + n * (HD / 2) + g * (HD / 8);
-        const uint8_t* vc = z + 8 * HD + g * (2 * HD) + n * (HD / 8);
-        if constexpr (N == 4) {
-            const u4v a = *reinterpret_cast<const u4v*>(kc), b = *reinterpret_cast<const u4v*>(vc);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r.k[i][j] = a[j], r.v[i][j] = b[j];
-        } else {
-            const u2v a = *reinterpret_cast<const u2v*>(kc), b = *reinterpret_cast<const u2v*>(vc);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) r.k[i][j] = a[j], r.v[i][j] = b[j];
-        }
-        r.ks[i] = z[16 * HD + n * (HD / 32) + g * (HD / 32) / 4];
-        r.vs[i] = *reinterpret_cast<const uint32_t*>(z + 16 * HD + HD / 2 + (g * (HD / 32) + n * (HD / 16) / 32) * 4);
+    for (int i = 0; i < TS; ++i) {
+        w.id[i] = -1;
+        if (w.next + 16 * i < w.end) w.id[i] = ids[col];
         if (++tile == p.tiles) tile = 0, ++col;
     }
-    w.key += (w.step_cols * p.tiles + w.step_tiles) * kKv4Tile;
-    w.col += w.step_cols;
-    w.tile += w.step_tiles;
+}
+
+template <int HD, int TS>
+PE_DEV void kv4_advance(const Kv4AttnArgs& p, const int* table, const uint8_t* head, Kv4Walk<TS>& w) {
+    int tile = w.tile;
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        const bool there = (uint32_t)w.id[i] < (uint32_t)p.n_pages;
+        w.key[i] = there ? w.next + 16 * i : kNoKeys;
+        // keys that are not there are loaded from the pool's first page, and masked
+        w.at[i] = head + (there ? w.id[i] * p.page_stride + (int64_t)tile * (17 * HD) : 0);
+        if (++tile == p.tiles) tile = 0;
+    }
+    w.next += (w.cols * p.tiles + w.tiles) * kKv4Tile;
+    w.col += w.cols;
+    w.tile += w.tiles;
     if (w.tile >= p.tiles) w.tile -= p.tiles, ++w.col;
+    kv4_pages<TS>(p, table, w);
+}
+
+// A lane's part of a step's keys: codes and scale bytes.
+template <int HD, int TS>
+struct Kv4Raw {
+    static constexpr int N = HD / 32;  // words of codes per 16 keys
+    uint32_t c[TS][N], s[TS];
+};
+template <int N>
+PE_DEV void kv4_words(const uint8_t* at, uint32_t* w) {
+    if constexpr (N == 4) {
+        const u4v a = *reinterpret_cast<const u4v*>(at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = a[j];
+    } else {
+        const u2v a = *reinterpret_cast<const u2v*>(at);
+        w[0] = a[0], w[1] = a[1];
+    }
+}
+template <int HD, int TS>
+PE_DEV void kv4_load_keys(const Kv4Walk<TS>& w, int lane, Kv4Raw<HD, TS>& r) {
+    const uint32_t n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        kv4_words<HD / 32>(w.at[i] + (n * (HD / 2) + g * (HD / 8)), r.c[i]);
+        r.s[i] = w.at[i][16 * HD + (n * (HD / 32) + g * (HD / 32) / 4)];
+    }
+}
+template <int HD, int TS>
+PE_DEV void kv4_load_values(const Kv4Walk<TS>& w, int lane, Kv4Raw<HD, TS>& r) {
+    const uint32_t n = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        kv4_words<HD / 32>(w.at[i] + 8 * HD + (g * (2 * HD) + n * (HD / 8)), r.c[i]);
+        r.s[i] = *reinterpret_cast<const uint32_t*>(w.at[i] + 16 * HD + HD / 2 + (g * (HD / 32) + n * (HD / 16) / 32) * 4);
+    }
 }
 
 // The state of RT x 16 query rows.
 template <int HD, int RT, int NP>
 struct Kv4State {
-    uint32_t q[RT][NP][HD / 32][4];  // parts of the queries, in the operand's order
+    const u4v* q;                    // LDS: parts of the queries [RT][NP][HD / 32][64 lanes], the lane's operands
     f4v o[RT][HD / 16];              // O^T: channel (4 g + i) HD/16 + j of row lane % 16 in o[j][i]
-    float m[RT], l[RT];              // maximum (of the row), sum (of the lane's keys), base 2
+    float m[RT], l[RT];              // what exponents are taken from (of the row), sum (of the lane's keys), base 2
     int lim[RT];                     // keys that the lane's row sees
 };
 
@@ -227,111 +284,111 @@ PE_DEV bf8v operand(const uint32_t* w) {
     return __builtin_bit_cast(bf8v, z);
 }
 
-template <int HD, int RT, int NP>
-PE_DEV void kv4_step(const Kv4AttnArgs& p, Kv4Raw<HD>& r, Kv4State<HD, RT, NP>& st, int least, int most, int lane) {
-    constexpr int N = HD / 32, E = HD / 16;
-    const int g = lane >> 4;
-    // scores: [rows][16 keys][4 keys of the lane]
-    float s[RT][4][4];
+// Scores of a step's keys: s[row][16 keys][4 keys of the lane]. A scale byte of 255 converts every code to NaN.
+template <int HD, int RT, int NP, int TS>
+PE_DEV void kv4_scores(const Kv4Raw<HD, TS>& r, const Kv4State<HD, RT, NP>& st, f4v (&s)[RT][TS]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float scale = __uint_as_float(r.ks[i] << 23);
-        f4v acc[RT] = {};
+    for (int i = 0; i < TS; ++i) {
+        const float scale = __uint_as_float(r.s[i] << 23);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
+        for (int t = 0; t < RT; ++t) s[t][i] = f4v{};
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
             uint32_t w[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = two_codes(r.k[i][j], scale, c);
+            for (int c = 0; c < 4; ++c) w[c] = two_codes(r.c[i][j], scale, c);
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
                 for (int n = 0; n < NP; ++n)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w), operand(st.q[t][n][j]), acc[t], 0, 0, 0);
+                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w), __builtin_bit_cast(bf8v, st.q[((t * NP + n) * (HD / 32) + j) * 64]), s[t][i], 0, 0, 0);
         }
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) s[t][i][c] = acc[t][c] * p.scale;
     }
-    // keys that some row does not see, or that are not there
-    const bool masked = r.key[0] + 16 > least || r.key[1] + 16 > least || r.key[2] + 16 > least || r.key[3] + 16 > least;
-    uint32_t bad[2] = {0, 0};  // 16 keys: the lane's value scales (bit c: key c) that are no number
-    if (masked) {
+}
+
+// Scores of keys that a row does not see become -inf. Values that no row sees may hold anything, and one that is no number
+// must not reach rows that do not see it: their codes become 0 and their scale 1, and bad tells of those that some row
+// sees (bit 4 (i % 2) + c of bad[i / 2]: key c of the lane's in the 16 keys i).
+template <int HD, int RT, int NP, int TS>
+PE_DEV void kv4_mask(const int* keys, int most, int g, Kv4Raw<HD, TS>& v, const Kv4State<HD, RT, NP>& st, f4v (&s)[RT][TS], uint32_t* bad) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // a key scale that is no number: the byte's 2^128 made infinities of the codes, and NaN of zeros only
-            uint64_t nan = __ballot(r.ks[i] == 255);
-            nan |= nan >> 32;
-            const uint32_t rows = (uint32_t)(nan | nan >> 16) >> (4 * g);
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int key = keys[i] + 4 * g + c;
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                if (key >= st.lim[t]) s[t][i][c] = -INFINITY;
+            const bool none = key >= most, nan = (v.s[i] >> (8 * c) & 255) == 255;
+            if (!none && nan) bad[i >> 1] |= 1u << ((i & 1) * 4 + c);
+            if (none || nan) {
+                v.s[i] = (v.s[i] & ~(255u << (8 * c))) | 127u << (8 * c);
+                if constexpr (HD == 128)
+                    v.c[i][c] = 0;
+                else
+                    v.c[i][c >> 1] &= c & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+            }
+        }
+}
+
+// NaN into the channels of the runs whose values are no numbers, of the rows that see them: counted by a product of both.
+template <int HD, int RT, int NP, int TS>
+PE_DEV void kv4_no_numbers(const int* keys, int g, const uint32_t* bad, Kv4State<HD, RT, NP>& st) {
+#pragma unroll
+    for (int h = 0; h < TS / 2; ++h) {
+        if (!__ballot(bad[h] != 0)) continue;
+        uint32_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            w[c] = (bad[h] >> (2 * c) & 1 ? 0x3F80u : 0u) | (bad[h] >> (2 * c + 1) & 1 ? 0x3F800000u : 0u);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            uint32_t sees[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int key = r.key[i] + 4 * g + c;
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    if (rows >> c & 1) s[t][i][c] = __uint_as_float(0x7FC00000u);
-                    if (key >= st.lim[t]) s[t][i][c] = -INFINITY;
-                }
-                const bool none = key >= most;
-                const uint32_t byte = r.vs[i] >> (8 * c) & 255;
-                if (!none && byte == 255) bad[i >> 1] |= 1u << ((i & 1) * 4 + c);
-                // what no row sees may hold anything, and a value that is no number must not reach rows that do not
-                // see it: zero codes, and scale 1
-                if (none || byte == 255) {
-                    r.vs[i] = (r.vs[i] & ~(255u << (8 * c))) | 127u << (8 * c);
-                    if constexpr (HD == 128)
-                        r.v[i][c] = 0;
-                    else
-                        r.v[i][c >> 1] &= c & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                }
+                const int key = keys[2 * h + (c >> 1)] + 4 * g + 2 * (c & 1);
+                sees[c] = (key < st.lim[t] ? 0x3F80u : 0u) | (key + 1 < st.lim[t] ? 0x3F800000u : 0u);
             }
-        }
-    } else {
+            f4v count = {};
+            count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w), operand(sees), count, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint64_t nan = __ballot(r.ks[i] == 255);
-            if (nan) {
-                nan |= nan >> 32;
-                const uint32_t rows = (uint32_t)(nan | nan >> 16) >> (4 * g);
+            for (int i = 0; i < 4; ++i)
+                if (count[i] > 0.f)
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (rows >> c & 1) s[t][i][c] = __uint_as_float(0x7FC00000u);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if ((r.vs[i] >> (8 * c) & 255) == 255) {
-                    bad[i >> 1] |= 1u << ((i & 1) * 4 + c);
-                    r.vs[i] = (r.vs[i] & ~(255u << (8 * c))) | 127u << (8 * c);
-                    if constexpr (HD == 128)
-                        r.v[i][c] = 0;
-                    else
-                        r.v[i][c >> 1] &= c & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                }
+                    for (int j = 0; j < HD / 16; ++j) st.o[t][j][i] = __uint_as_float(0x7FC00000u);
         }
     }
-    // running maximum and sum
-    uint32_t pr[RT][2][NP][4];
+}
+
+// How far above the number that exponents are taken from a score may lie before the state is rescaled (base 2):
+// probabilities up to 2^6 cost no accuracy, and after a sequence's first keys hardly a step rescales.
+constexpr float kKv4Slack = 6.f;
+
+template <int HD, int RT, int NP, int TS>
+PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT, NP>& st, const f4v (&s)[RT][TS], uint32_t (&pr)[RT][TS / 2][NP][4]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < TS; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) top = fmaxf(top, s[t][i][c]);
-        top = swap32_max(swap16_max(top));
-        const float m = fmaxf(st.m[t], top), base = m == -INFINITY ? 0.f : m;
-        const float shrink = __builtin_amdgcn_exp2f(st.m[t] - base);
-        st.m[t] = m;
-        st.l[t] *= shrink;
+        top *= scale;
+        if (__ballot(top > st.m[t] + kKv4Slack)) {
+            const float m = fmaxf(st.m[t], swap32_max(swap16_max(top)));
+            const float shrink = __builtin_amdgcn_exp2f(st.m[t] - (m == -INFINITY ? 0.f : m));
+            st.m[t] = m;
+            st.l[t] *= shrink;
 #pragma unroll
-        for (int j = 0; j < E; ++j) st.o[t][j] *= shrink;
+            for (int j = 0; j < HD / 16; ++j) st.o[t][j] *= shrink;
+        }
+        const float base = st.m[t] == -INFINITY ? 0.f : -st.m[t];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < TS; ++i) {
             float e[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                e[c] = __builtin_amdgcn_exp2f(s[t][i][c] - base);
+                e[c] = __builtin_amdgcn_exp2f(fmaf(s[t][i][c], scale, base));
                 st.l[t] += e[c];
             }
 #pragma unroll
@@ -343,20 +400,27 @@ PE_DEV void kv4_step(const Kv4AttnArgs& p, Kv4Raw<HD>& r, Kv4State<HD, RT, NP>& 
             }
         }
     }
-    // values: 32 keys at a time, two channels of a run at a time
+}
+
+// O^T += V^T P^T, 32 keys at a time, two channels of a run at a time: a conversion gives two channels of one key, a
+// permutation two keys of one channel.
+template <int HD, int RT, int NP, int TS>
+PE_DEV void kv4_values(const Kv4Raw<HD, TS>& r, Kv4State<HD, RT, NP>& st, const uint32_t (&pr)[RT][TS / 2][NP][4]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float scale[8];
+    for (int h = 0; h < TS / 2; ++h) {
+        float scale[8];  // the conversion looks at the exponent's bits alone
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            scale[c] = __uint_as_float((r.vs[2 * h + (c >> 2)] >> (8 * (c & 3)) & 255u) << 23);
+        for (int c = 0; c < 8; ++c) {
+            const uint32_t w = r.s[2 * h + (c >> 2)];
+            scale[c] = __uint_as_float((c & 3) < 3 ? w << (23 - 8 * (c & 3)) : w >> 1);
+        }
 #pragma unroll
-        for (int j = 0; j < E; j += 2) {
+        for (int j = 0; j < HD / 16; j += 2) {
             uint32_t two[8], lo[4], hi[4];
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 const int i = 2 * h + (c >> 2), k = c & 3;
-                two[c] = HD == 128 ? two_codes(r.v[i][k], scale[c], j >> 1) : two_codes(r.v[i][k >> 1], scale[c], (k & 1) * 2 + (j >> 1));
+                two[c] = HD == 128 ? two_codes(r.c[i][k], scale[c], j >> 1) : two_codes(r.c[i][k >> 1], scale[c], (k & 1) * 2 + (j >> 1));
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -372,29 +436,6 @@ PE_DEV void kv4_step(const Kv4AttnArgs& p, Kv4Raw<HD>& r, Kv4State<HD, RT, NP>& 
                         __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi), operand(pr[t][h][n]), st.o[t][j + 1], 0, 0, 0);
                 }
         }
-        // values that are no number: how many of them a row sees, in every run (all its channels share the scale)
-        if (__ballot(bad[h] != 0)) {
-            uint32_t w[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                w[c] = (bad[h] >> (2 * c) & 1 ? 0x3F80u : 0u) | (bad[h] >> (2 * c + 1) & 1 ? 0x3F800000u : 0u);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                uint32_t sees[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int key = r.key[2 * h + (c >> 1)] + 4 * g + 2 * (c & 1);
-                    sees[c] = (key < st.lim[t] ? 0x3F80u : 0u) | (key + 1 < st.lim[t] ? 0x3F800000u : 0u);
-                }
-                f4v count = {};
-                count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w), operand(sees), count, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (count[i] > 0.f)
-#pragma unroll
-                        for (int j = 0; j < E; ++j) st.o[t][j][i] = __uint_as_float(0x7FC00000u);
-            }
-        }
     }
 }
 
@@ -404,8 +445,8 @@ constexpr int kKv4Parts = sizeof(T) == 2 ? 2 : 3;
 // SPLIT: the workgroup's rows are RT x 16, its waves take steps in turn and are merged in LDS. Otherwise every wave has
 // RT x 16 rows of its own and takes all the item's keys.
 template <typename T, int HD, int RT, bool SPLIT>
-__global__ __launch_bounds__(64 * kKv4Waves) void k_kv4_attn(Kv4AttnArgs p) {
-    constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16 * RT, RB = SPLIT ? R : R * kKv4Waves;
+__global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv4AttnArgs p) {
+    constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16 * RT, RB = SPLIT ? R : R * kKv4Waves, TS = kKv4Tiles<HD, RT>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int item = blockIdx.x, kvh = blockIdx.y;
     Kv4Item w;
@@ -416,53 +457,112 @@ __global__ __launch_bounds__(64 * kKv4Waves) void k_kv4_attn(Kv4AttnArgs p) {
 
     // the wave's rows: r0 + 16 t + n
     const int r0 = w.block * RB + (SPLIT ? 0 : wave * R), last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
+    const bool rows = r0 < seq.rows;
+    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0, most = rows ? kv4_keys(p, seq.keys, last / p.group) : 0;
+    const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
+    Kv4Walk<TS> walk;
+    walk.end = (int)(stop < most ? stop : most);
+    walk.next = (int)begin + (SPLIT ? wave * TS * kKv4Tile : 0);
     Kv4State<HD, RT, NP> st;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const int row = r0 + 16 * t + n, i = row / p.group;
-        const bool there = row < seq.rows;
-        st.lim[t] = there ? kv4_keys(p, seq.keys, i) : 0;
         st.m[t] = -INFINITY;
         st.l[t] = 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j) st.o[t][j] = f4v{};
-        const T* q = static_cast<const T*>(p.q) + (seq.lo + i) * p.q_token + (int64_t)(kvh * p.group + row - i * p.group) * p.q_head +
-                     g * (HD / 4);
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t z[NP];
-                split_pair<NP>(there ? (float)q[8 * j + 2 * c] : 0.f, there ? (float)q[8 * j + 2 * c + 1] : 0.f, z);
-#pragma unroll
-                for (int k = 0; k < NP; ++k) st.q[t][k][j][c] = z[k];
-            }
     }
-    const bool rows = r0 < seq.rows;
-    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0, most = rows ? kv4_keys(p, seq.keys, last / p.group) : 0;
-    const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
-    Kv4Walk walk;
-    walk.end = (int)(stop < most ? stop : most);
-    walk.key = (int)begin + (SPLIT ? wave * kKv4Step : 0);
-    const int stride = SPLIT ? 4 * kKv4Waves : 4;  // tiles from step to step
-    walk.step_cols = stride / p.tiles;
-    walk.step_tiles = stride - walk.step_cols * p.tiles;
-    walk.col = walk.key / kKv4Tile / p.tiles;
-    walk.tile = walk.key / kKv4Tile - walk.col * p.tiles;
-    const int* table = p.table + w.b * p.table_row;
-    const uint8_t* head = p.pages + (int64_t)kvh * p.tiles * (17 * HD);
-    while (walk.key < walk.end) {
-        Kv4Raw<HD> raw;
-        kv4_load<HD>(p, table, head, walk, lane, raw);
-        kv4_step<HD, RT, NP>(p, raw, st, least, most, lane);
+    // The queries' parts go to LDS: SPLIT, a wave for every 16 rows that all waves share, else every wave its own.
+    // 32 (16) elements of a row in a lane; rows that are not there take the last one's, as zeros.
+    constexpr int QW = RT * NP * (HD / 32) * 64;
+    constexpr int PART = SPLIT ? kKv4Waves * R * (HD + 4 + 2) * 4 : 0, QUERIES = (SPLIT ? QW : QW * kKv4Waves) * 16;
+    __shared__ __attribute__((aligned(16))) char lds[PART > QUERIES ? PART : QUERIES];
+    st.q = reinterpret_cast<const u4v*>(lds) + (SPLIT ? 0 : wave * QW) + lane;
+    if (rows) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            int row = r0 + 16 * t + n;
+            const bool there = row < seq.rows;
+            row = there ? row : last;
+            const int i = row / p.group;
+            st.lim[t] = there ? kv4_keys(p, seq.keys, i) : 0;
+            if (SPLIT && wave != t) continue;
+            const T* x = static_cast<const T*>(p.q) + (seq.lo + i) * p.q_token +
+                         (int64_t)(kvh * p.group + row - i * p.group) * p.q_head + g * (HD / 4);
+            float q[HD / 4];
+            if (p.vec) {
+                typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+                for (int j = 0; j < HD / 4; j += 16 / (int)sizeof(T)) {
+                    const piece z = *reinterpret_cast<const piece*>(x + j);
+#pragma unroll
+                    for (int c = 0; c < 16 / (int)sizeof(T); ++c) q[j + c] = (float)z[c];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < HD / 4; ++j) q[j] = (float)x[j];
+            }
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                uint32_t z[4][NP];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float a = q[8 * j + 2 * c] * p.sign, b = q[8 * j + 2 * c + 1] * p.sign;
+                    split_pair<NP>(there ? a : 0.f, there ? b : 0.f, z[c]);
+                }
+#pragma unroll
+                for (int k = 0; k < NP; ++k)
+                    const_cast<u4v*>(st.q)[((t * NP + k) * (HD / 32) + j) * 64] = u4v{z[0][k], z[1][k], z[2][k], z[3][k]};
+            }
+        }
+    }
+    if constexpr (SPLIT) __syncthreads();
+    if (walk.next < walk.end) {
+        const int stride = SPLIT ? TS * kKv4Waves : TS;  // tiles from step to step
+        walk.cols = stride / p.tiles;
+        walk.tiles = stride - walk.cols * p.tiles;
+        walk.col = walk.next / kKv4Tile / p.tiles;
+        walk.tile = walk.next / kKv4Tile - walk.col * p.tiles;
+        const int* table = p.table + w.b * p.table_row;
+        const uint8_t* head = p.pages + (int64_t)kvh * p.tiles * (17 * HD);
+        kv4_pages<TS>(p, table, walk);
+        Kv4Raw<HD, TS> keys, values;
+        kv4_advance<HD, TS>(p, table, head, walk);
+        kv4_load_keys<HD, TS>(walk, lane, keys);
+        kv4_load_values<HD, TS>(walk, lane, values);
+        // the next step's keys are under way during softmax and values, its values during the next scores
+        for (;;) {
+            asm volatile("" ::: "memory");  // the queries stay in LDS: registers for more waves are worth more
+            int at[TS];
+            bool masked = false;
+#pragma unroll
+            for (int i = 0; i < TS; ++i) {
+                at[i] = walk.key[i];
+                masked |= at[i] + kKv4Tile > least;
+            }
+            const bool more = walk.next < walk.end;
+            f4v s[RT][TS];
+            kv4_scores<HD, RT, NP, TS>(keys, st, s);
+            if (more) {
+                kv4_advance<HD, TS>(p, table, head, walk);
+                kv4_load_keys<HD, TS>(walk, lane, keys);
+            }
+            uint32_t bad[TS / 2] = {}, pr[RT][TS / 2][NP][4];
+            if (masked) kv4_mask<HD, RT, NP, TS>(at, most, g, values, st, s, bad);
+            kv4_softmax<HD, RT, NP, TS>(p.scale, st, s, pr);
+            kv4_values<HD, RT, NP, TS>(values, st, pr);
+            if (masked) kv4_no_numbers<HD, RT, NP, TS>(at, g, bad, st);
+            if (!more) break;
+            kv4_load_values<HD, TS>(walk, lane, values);
+        }
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) st.l[t] = swap32_sum(swap16_sum(st.l[t]));
 
-    const int64_t rec = ((int64_t)kvh * p.items + item) * RB;
+    const int64_t rec = ((int64_t)kvh * p.items + item) * p.rec_rows;
     if constexpr (SPLIT) {
-        __shared__ float part[kKv4Waves][R][HD + 4];
-        __shared__ float pm[kKv4Waves][R], pl[kKv4Waves][R];
+        float(*part)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(lds);
+        float(*pm)[R] = reinterpret_cast<float(*)[R]>(lds + kKv4Waves * R * (HD + 4) * 4), (*pl)[R] = pm + kKv4Waves;
+        __syncthreads();  // the queries have been read
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const int row = 16 * t + n;
@@ -526,36 +626,72 @@ __global__ __launch_bounds__(64 * kKv4Waves) void k_kv4_attn(Kv4AttnArgs p) {
     }
 }
 
-// The chunks of a row: one wave per row of q, a lane HD / 64 channels.
-template <typename T, int HD, int RB>
+// The chunks of a row of q, joined by WAVES waves: HD / 4 lanes take a chunk's record, so a wave has 256 / HD of them
+// in flight beside each other, with the row's maximum known before the first.
+template <typename T, int HD, int RB, int WAVES>
 __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
-    constexpr int C = HD / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = x / p.n_head;
+    constexpr int L = HD / 4, SIDE = WAVES * 64 / L;
+    __shared__ float4 part[4][64];
+    __shared__ float parts[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w = wave % WAVES;
+    const int64_t x = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES, t = x / p.n_head;
     const int h = (int)(x - t * p.n_head);
-    if (t >= p.tokens) return;
-    const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
-    if (b < 0) return;
-    const Kv4Seq seq = kv4_seq(p, (int)b);
-    const int kvh = h / p.group, r = (int)(t - seq.lo) * p.group + h - kvh * p.group;
-    const int4 plan = p.plan[b];
-    // (a plan that no workgroup wrote, of starts that are out of order, holds anything)
-    if (plan.y <= 1 || plan.z <= 0 || plan.x < 0 || r < 0 || r / RB >= plan.z || (int64_t)plan.x + (int64_t)plan.y * plan.z > p.items) return;
-    float m = -INFINITY, l = 0.f, o[C] = {};
-    for (int c = 0; c < plan.y; ++c) {
-        const int64_t rec = ((int64_t)kvh * p.items + plan.x + c * plan.z + r / RB) * RB + r % RB;
-        const float mc = p.stat[2 * rec], lc = p.stat[2 * rec + 1];
-        const float top = fmaxf(m, mc), base = top == -INFINITY ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f(m - base), e = __builtin_amdgcn_exp2f(mc - base);
-        l = l * f + lc * e;
-#pragma unroll
-        for (int j = 0; j < C; ++j) o[j] = o[j] * f + p.record[rec * HD + lane * C + j] * e;
-        m = top;
+    int chunks = 0, r = 0;
+    int64_t first = 0, step = 0;
+    if (t < p.tokens) {
+        const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
+        if (b >= 0) {
+            const int4 plan = p.plan[b];
+            int64_t lo, hi;
+            rows_of(p.starts, p.starts_wide, b, p.tokens, lo, hi);
+            const int kvh = h / p.group;
+            r = (int)(t - lo) * p.group + h - kvh * p.group;
+            // (a plan that no workgroup wrote, of starts that are out of order, holds anything)
+            if (plan.y > 1 && plan.z > 0 && plan.x >= 0 && r >= 0 && r / RB < plan.z && (int64_t)plan.x + (int64_t)plan.y * plan.z <= p.items) {
+                chunks = plan.y;
+                first = ((int64_t)kvh * p.items + plan.x + r / RB) * p.rec_rows + r % RB;
+                step = (int64_t)plan.z * p.rec_rows;
+            }
+        }
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    T* y = static_cast<T*>(p.out) + t * p.out_token + (int64_t)h * p.out_head + lane * C;
+    float m = -INFINITY;
+    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, p.stat[2 * (first + c * step)]);
+    m = wave_max<64>(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[4] = {};
+    const int ch = lane % L * 4;
+#pragma unroll 4
+    for (int c = w * (64 / L) + lane / L; c < chunks; c += SIDE) {
+        const int64_t rec = first + c * step;
+        const float f = __builtin_amdgcn_exp2f(p.stat[2 * rec] - base);
+        const float4 v = *reinterpret_cast<const float4*>(p.record + rec * HD + ch);
+        l = fmaf(p.stat[2 * rec + 1], f, l);
+        o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+    }
+    const auto join = [&](float v) {
+        if constexpr (L == 16) v = swap16_sum(v);
+        return swap32_sum(v);
+    };
+    l = join(l);
 #pragma unroll
-    for (int j = 0; j < C; ++j) y[j] = (T)(o[j] * f);
+    for (int j = 0; j < 4; ++j) o[j] = join(o[j]);
+    if constexpr (WAVES > 1) {
+        part[wave][lane] = make_float4(o[0], o[1], o[2], o[3]);
+        parts[wave][lane] = l;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) {
+            const float4 v = part[wave + k][lane];
+            o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
+            l += parts[wave + k][lane];
+        }
+    }
+    if (chunks == 0 || lane >= L) return;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    T* y = static_cast<T*>(p.out) + t * p.out_token + (int64_t)h * p.out_head + ch;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (T)(o[j] * f);
 }
 
 // How a call is cut: rows of a workgroup and workgroups of a kv head, from what the host knows (the lengths are on the device).
@@ -563,22 +699,25 @@ struct Kv4Plan {
     int rt, split;   // 16-row tiles of a wave; the waves share the rows and split the keys
     int rb;          // rows of a workgroup
     int64_t blocks, items;
-    int min_chunk;
+    int min_chunk, rec_rows;
+    float weight;  // of all keys in the square of a chunk's length
 };
 
-static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, int n_kv, int64_t capacity) {
+static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, int n_kv, int hd, int64_t capacity) {
     Kv4Plan s;
     const int group = n_head / n_kv;
     const int64_t rows = ragged ? (tokens + batch - 1) / batch * group : group;  // of a sequence, on average
-    s.rt = rows <= 16 ? 1 : 2;
     s.split = rows <= 32;
+    s.rt = s.split ? 1 : 2;
     s.rb = 16 * s.rt * (s.split ? 1 : kKv4Waves);
     s.blocks = ragged ? tokens * group / s.rb + batch : batch * ((group + s.rb - 1) / s.rb);
-    s.min_chunk = kKv4Step * (s.split ? kKv4Waves : 4);
-    // as many workgroups more as fill the chip, three on each CU, and let uneven sequences be cut evenly
-    const int64_t want = (768 + n_kv - 1) / n_kv, chunks = (capacity + s.min_chunk - 1) / s.min_chunk;
-    int64_t extra = s.blocks < want ? want - s.blocks : 0;
-    if (extra < want / 4) extra = want / 4;
+    s.min_chunk = 64 * (s.split ? kKv4Waves : 4);
+    s.rec_rows = ragged || group > s.rb ? s.rb : group;
+    s.weight = 0.75f * (float)n_kv;
+    // the most workgroups that a chunk's length makes of any lengths, within reason
+    const int64_t chunks = (capacity + s.min_chunk - 1) / s.min_chunk;
+    int64_t extra = (int64_t)sqrt((double)s.blocks * (double)capacity / s.weight) + 1;
+    if (extra > 8192 / n_kv + 1) extra = 8192 / n_kv + 1;
     if (chunks <= 1)
         extra = 0;
     else if (extra > s.blocks * (chunks - 1))
@@ -594,21 +733,28 @@ static bool kv4_shape_ok(int64_t tokens, int64_t batch, bool ragged, int n_head,
 }
 
 static int64_t kv4_bytes(const Kv4Plan& s, int64_t batch, int n_kv, int hd) {
-    return s.items > s.blocks ? (batch * 16 + s.items * n_kv * s.rb * (int64_t)(hd + 2) * 4 + 15) / 16 * 16 : 0;
+    return s.items > s.blocks ? (batch * 16 + s.items * n_kv * s.rec_rows * (int64_t)(hd + 2) * 4 + 15) / 16 * 16 : 0;
+}
+
+template <typename T, int HD, int RB>
+static void launch_merge(const Kv4AttnArgs& p, hipStream_t st) {
+    const int64_t rows = p.tokens * p.n_head;
+    if (!p.plan) return;
+    if (rows < 2048)  // few rows: four waves each
+        hipLaunchKernelGGL((k_kv4_merge<T, HD, RB, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((k_kv4_merge<T, HD, RB, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
 }
 
 template <typename T, int HD>
 static void launch_kv4(const Kv4AttnArgs& p, const Kv4Plan& s, hipStream_t st) {
-    const dim3 g((unsigned)s.items, (unsigned)p.n_kv), m((unsigned)((p.tokens * p.n_head + 3) / 4));
+    const dim3 g((unsigned)s.items, (unsigned)p.n_kv);
     if (!s.split) {
         hipLaunchKernelGGL((k_kv4_attn<T, HD, 2, false>), g, dim3(64 * kKv4Waves), 0, st, p);
-        if (p.plan) hipLaunchKernelGGL((k_kv4_merge<T, HD, 32 * kKv4Waves>), m, dim3(256), 0, st, p);
-    } else if (s.rt == 2) {
-        hipLaunchKernelGGL((k_kv4_attn<T, HD, 2, true>), g, dim3(64 * kKv4Waves), 0, st, p);
-        if (p.plan) hipLaunchKernelGGL((k_kv4_merge<T, HD, 32>), m, dim3(256), 0, st, p);
+        launch_merge<T, HD, 32 * kKv4Waves>(p, st);
     } else {
         hipLaunchKernelGGL((k_kv4_attn<T, HD, 1, true>), g, dim3(64 * kKv4Waves), 0, st, p);
-        if (p.plan) hipLaunchKernelGGL((k_kv4_merge<T, HD, 16>), m, dim3(256), 0, st, p);
+        launch_merge<T, HD, 16>(p, st);
     }
 }
 
@@ -619,7 +765,7 @@ using namespace pe;
 extern "C" int64_t pe_kv4_attn_workspace_bytes(int64_t tokens, int64_t batch, int ragged, int n_head, int n_kv, int head_dim,
                                                int64_t capacity) {
     if (!kv4_shape_ok(tokens, batch, ragged, n_head, n_kv, head_dim, capacity)) return -PE_ERR_SHAPE;
-    return kv4_bytes(kv4_plan(tokens, batch, ragged, n_head, n_kv, capacity), batch, n_kv, head_dim);
+    return kv4_bytes(kv4_plan(tokens, batch, ragged, n_head, n_kv, head_dim, capacity), batch, n_kv, head_dim);
 }
 
 extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
@@ -631,13 +777,13 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
     if (const int st = kv4_pool_ok(&a->pool, a->n_kv, a->head_dim)) return st;
     const int64_t T = a->tokens, capacity = a->pool.table_cols * a->pool.page_tokens;
     const bool ragged = a->starts != nullptr;
-    if (!kv4_shape_ok(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity) || !std::isfinite(a->scale) ||
+    if (!kv4_shape_ok(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity) || !std::isfinite(a->scale * kKv4Log2e) ||
         a->first < -(1LL << 40) || a->first > (1LL << 40) || a->q_token < 0 || a->q_head < 0 || a->out_token < 0 || a->out_head < 0 ||
         (a->n_head > 1 && a->out_head < a->head_dim) || (T > 1 && a->out_token < a->head_dim) ||
         (T > 1 && a->n_head > 1 && a->out_token < a->out_head * (a->n_head - 1) + a->head_dim &&
          a->out_head < a->out_token * (T - 1) + a->head_dim))
         return PE_ERR_SHAPE;
-    const Kv4Plan s = kv4_plan(T, a->batch, ragged, a->n_head, a->n_kv, capacity);
+    const Kv4Plan s = kv4_plan(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity);
     const int64_t need = kv4_bytes(s, a->batch, a->n_kv, a->head_dim);
     if (!a->q || !a->out || !a->lengths || (need && !a->workspace)) return PE_ERR_NULL;
     const size_t e = a->type == PE_TYPE_F16 ? 2 : 4;
@@ -646,14 +792,17 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
         return PE_ERR_ALIGN;
     if (a->workspace_bytes < need) return PE_ERR_SPACE;
     if (s.items * a->n_kv >= (1 << 24) || T * a->n_head >= (1LL << 26)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    const int piece = (int)(16 / e);
+    const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
+    const float sign = a->scale > 0 ? 1.f : a->scale < 0 ? -1.f : 0.f, scale = sign == 0.f ? 1.f : std::fabs(a->scale) * kKv4Log2e;
     int4* plan = need ? static_cast<int4*>(a->workspace) : nullptr;
     float* record = need ? reinterpret_cast<float*>(plan + a->batch) : nullptr;
     Kv4AttnArgs p{a->q, a->q_token, a->q_head, a->out, a->out_token, a->out_head, static_cast<const uint8_t*>(a->pool.pages),
                   a->pool.page_stride, (int)a->pool.n_pages, (int)(a->pool.page_tokens / kKv4Tile), a->pool.table,
                   a->pool.table_stride, (int)a->pool.table_cols, a->lengths, a->lengths_dtype == 2, a->first, a->starts,
-                  a->starts_dtype == 2, T, (int)a->batch, a->n_head, a->n_kv, a->n_head / a->n_kv, a->scale * kKv4Log2e,
-                  (int)s.items, (int)s.blocks, s.min_chunk, plan, record,
-                  need ? record + s.items * a->n_kv * s.rb * a->head_dim : nullptr};
+                  a->starts_dtype == 2, T, (int)a->batch, a->n_head, a->n_kv, a->n_head / a->n_kv, scale, sign, capacity, vec,
+                  (int)s.items, (int)s.blocks, s.min_chunk, s.weight, s.rec_rows, plan, record,
+                  need ? record + s.items * a->n_kv * s.rec_rows * a->head_dim : nullptr};
     hipStream_t st = (hipStream_t)stream;
     if (a->type == PE_TYPE_F16)
         a->head_dim == 64 ? launch_kv4<_Float16, 64>(p, s, st) : launch_kv4<_Float16, 128>(p, s, st);
