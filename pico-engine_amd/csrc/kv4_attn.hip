@@ -50,7 +50,8 @@ struct Kv4AttnArgs {
     int starts_wide;
     int64_t tokens;
     int batch, n_head, n_kv, group;
-    float scale, sign;  // the scale's magnitude times log2 e, its sign (0: the queries are zeros, the magnitude 1)
+    float scale;        // of scores, above 0
+    double q_scale;     // of queries: their product is the scale times log2 e
     int64_t capacity;   // slots of a sequence
     int vec;            // q's rows are whole pieces of 16 bytes
     int items, blocks;  // workgroups a kv head, row blocks at most
@@ -58,8 +59,8 @@ struct Kv4AttnArgs {
     float weight;
     int rec_rows;          // rows of a record
     int4* plan;         // of every sequence: first item, chunks, row blocks
-    float* record;      // [kv head][item][row][HD]
-    float* stat;        // [kv head][item][row] (maximum, sum)
+    float* record;      // [kv head][items][row][HD], a row block's chunks one after the other
+    float* stat;        // [kv head][items][row] (maximum, sum)
 };
 
 // Work of a sequence.
@@ -152,9 +153,20 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             w.chunks = __builtin_amdgcn_readlane(chunks, at);
             w.base = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
             w.span = span;
-            // blocks of the same keys one after the other
-            w.chunk = w.blocks == 1 ? item - w.base : (item - w.base) / w.blocks;
-            w.block = item - w.base - w.chunk * w.blocks;
+            const int local = item - w.base;
+            if (w.blocks == 1) {
+                w.chunk = local, w.block = 0;
+            } else if (RB == 16) {
+                // Few blocks: eight chunks side by side, the blocks of each eight items apart. Workgroups go to the eight
+                // XCDs in turn, so blocks that read the same keys find them in one L2 (two blocks on 65536 keys: 43 -> 41.5 us).
+                const int eight = local / (8 * w.blocks), rest = local - eight * 8 * w.blocks;
+                const int side = w.chunks - 8 * eight < 8 ? w.chunks - 8 * eight : 8;
+                w.block = rest / side;
+                w.chunk = 8 * eight + rest - w.block * side;
+            } else {  // many blocks: those of the same keys one after the other (2 x 1021 rows: 379 us, as above 390)
+                w.chunk = local / w.blocks;
+                w.block = local - w.chunk * w.blocks;
+            }
             return true;
         }
         base += __builtin_amdgcn_readlane(upto, 63);
@@ -506,7 +518,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv
                 uint32_t z[4][NP];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const float a = q[8 * j + 2 * c] * p.sign, b = q[8 * j + 2 * c + 1] * p.sign;
+                    const float a = (float)(q[8 * j + 2 * c] * p.q_scale), b = (float)(q[8 * j + 2 * c + 1] * p.q_scale);
                     split_pair<NP>(there ? a : 0.f, there ? b : 0.f, z[c]);
                 }
 #pragma unroll
@@ -558,7 +570,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv
 #pragma unroll
     for (int t = 0; t < RT; ++t) st.l[t] = swap32_sum(swap16_sum(st.l[t]));
 
-    const int64_t rec = ((int64_t)kvh * p.items + item) * p.rec_rows;
+    const int64_t rec = ((int64_t)kvh * p.items + w.base + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;
     if constexpr (SPLIT) {
         float(*part)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(lds);
         float(*pm)[R] = reinterpret_cast<float(*)[R]>(lds + kKv4Waves * R * (HD + 4) * 4), (*pl)[R] = pm + kKv4Waves;
@@ -637,7 +649,7 @@ __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
     const int64_t x = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES, t = x / p.n_head;
     const int h = (int)(x - t * p.n_head);
     int chunks = 0, r = 0;
-    int64_t first = 0, step = 0;
+    int64_t first = 0;
     if (t < p.tokens) {
         const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
         if (b >= 0) {
@@ -649,20 +661,19 @@ __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
             // (a plan that no workgroup wrote, of starts that are out of order, holds anything)
             if (plan.y > 1 && plan.z > 0 && plan.x >= 0 && r >= 0 && r / RB < plan.z && (int64_t)plan.x + (int64_t)plan.y * plan.z <= p.items) {
                 chunks = plan.y;
-                first = ((int64_t)kvh * p.items + plan.x + r / RB) * p.rec_rows + r % RB;
-                step = (int64_t)plan.z * p.rec_rows;
+                first = ((int64_t)kvh * p.items + plan.x + (int64_t)(r / RB) * plan.y) * p.rec_rows + r % RB;
             }
         }
     }
     float m = -INFINITY;
-    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, p.stat[2 * (first + c * step)]);
+    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, p.stat[2 * (first + (int64_t)c * p.rec_rows)]);
     m = wave_max<64>(m);
     const float base = m == -INFINITY ? 0.f : m;
     float l = 0.f, o[4] = {};
     const int ch = lane % L * 4;
 #pragma unroll 4
     for (int c = w * (64 / L) + lane / L; c < chunks; c += SIDE) {
-        const int64_t rec = first + c * step;
+        const int64_t rec = first + (int64_t)c * p.rec_rows;
         const float f = __builtin_amdgcn_exp2f(p.stat[2 * rec] - base);
         const float4 v = *reinterpret_cast<const float4*>(p.record + rec * HD + ch);
         l = fmaf(p.stat[2 * rec + 1], f, l);
@@ -748,7 +759,7 @@ static void launch_merge(const Kv4AttnArgs& p, hipStream_t st) {
 
 template <typename T, int HD>
 static void launch_kv4(const Kv4AttnArgs& p, const Kv4Plan& s, hipStream_t st) {
-    const dim3 g((unsigned)s.items, (unsigned)p.n_kv);
+    const dim3 g((unsigned)(s.items + 7) / 8 * 8, (unsigned)p.n_kv);
     if (!s.split) {
         hipLaunchKernelGGL((k_kv4_attn<T, HD, 2, false>), g, dim3(64 * kKv4Waves), 0, st, p);
         launch_merge<T, HD, 32 * kKv4Waves>(p, st);
@@ -791,16 +802,20 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
         (ragged && !aligned(a->starts, a->starts_dtype == 2 ? 8 : 4)) || !aligned(a->workspace, 16))
         return PE_ERR_ALIGN;
     if (a->workspace_bytes < need) return PE_ERR_SPACE;
-    if (s.items * a->n_kv >= (1 << 24) || T * a->n_head >= (1LL << 26)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    if ((s.items + 7) * a->n_kv >= (1 << 24) || T * a->n_head >= (1LL << 26)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
     const int piece = (int)(16 / e);
     const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
-    const float sign = a->scale > 0 ? 1.f : a->scale < 0 ? -1.f : 0.f, scale = sign == 0.f ? 1.f : std::fabs(a->scale) * kKv4Log2e;
+    // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores;
+    // fp16 ones only turned by its sign, so that their parts stay exact
+    const bool half = a->type == PE_TYPE_F16;
+    const float scale = half && a->scale != 0 ? std::fabs(a->scale) * kKv4Log2e : 1.f;
+    const double q_scale = half ? (a->scale > 0) - (a->scale < 0) : (double)a->scale * 1.4426950408889634;
     int4* plan = need ? static_cast<int4*>(a->workspace) : nullptr;
     float* record = need ? reinterpret_cast<float*>(plan + a->batch) : nullptr;
     Kv4AttnArgs p{a->q, a->q_token, a->q_head, a->out, a->out_token, a->out_head, static_cast<const uint8_t*>(a->pool.pages),
                   a->pool.page_stride, (int)a->pool.n_pages, (int)(a->pool.page_tokens / kKv4Tile), a->pool.table,
                   a->pool.table_stride, (int)a->pool.table_cols, a->lengths, a->lengths_dtype == 2, a->first, a->starts,
-                  a->starts_dtype == 2, T, (int)a->batch, a->n_head, a->n_kv, a->n_head / a->n_kv, scale, sign, capacity, vec,
+                  a->starts_dtype == 2, T, (int)a->batch, a->n_head, a->n_kv, a->n_head / a->n_kv, scale, q_scale, capacity, vec,
                   (int)s.items, (int)s.blocks, s.min_chunk, s.weight, s.rec_rows, plan, record,
                   need ? record + s.items * a->n_kv * s.rec_rows * a->head_dim : nullptr};
     hipStream_t st = (hipStream_t)stream;

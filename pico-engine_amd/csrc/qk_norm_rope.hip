@@ -40,6 +40,17 @@ PE_DEV float lanes_sum(float v) {
     return v;
 }
 
+// V weights, 16 bytes at a time where the rows go so (the caller sees to the alignment then).
+template <int V>
+PE_DEV void load_weights(const float* w, float* v) {
+    if constexpr (V == 1) {
+        v[0] = w[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) load_vec<float, 4>(w + i, v + i);
+    }
+}
+
 // A group of W lanes holds a head, a lane NI pieces of V pairs or of 2 V elements that stay.
 template <typename T, int V, bool IL, int W, int NI>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(QkNormArgs p) {
@@ -68,43 +79,62 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(QkNormArgs p) {
         }
     }
     const float inv_hd = 1.0f / (float)p.hd;
-    for (int h = h0; h < p.heads; h += p.groups) {
-        const bool isq = h < p.n_head;
-        const NormSide& s = isq ? p.q : p.k;
-        const int hh = isq ? h : h - p.n_head;
-        const T* x = static_cast<const T*>(s.x) + t * s.x_token + hh * s.x_head;
-        T* y = static_cast<T*>(s.y) + t * s.y_token + hh * s.y_head;
-        float a[NI][V], b[NI][V], sum = 0.f;
+    const auto side = [&](int h) -> const NormSide& { return h < p.n_head ? p.q : p.k; };
+    const auto load = [&](int h, float (&a)[NI][V], float (&b)[NI][V]) {
+        const NormSide& s = side(h);
+        const T* x = static_cast<const T*>(s.x) + t * s.x_token + (h < p.n_head ? h : h - p.n_head) * s.x_head;
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
 #pragma unroll
             for (int i = 0; i < V; ++i) a[n][i] = b[n][i] = 0.f;
             if (one[n]) load_vec<T, V>(x + at[n], a[n]);
             if (two[n]) load_vec<T, V>(x + at[n] + far[n], b[n]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) sum = fmaf(a[n][i], a[n][i], fmaf(b[n][i], b[n][i], sum));
         }
+    };
+    float a[NI][V], b[NI][V], wa[NI][V], wb[NI][V];
+    const float* held = nullptr;  // the weights in wa, wb
+    load(h0, a, b);
+    for (int h = h0; h < p.heads; h += p.groups) {
+        // the next head is under way while this one is summed up and turned
+        float na[NI][V], nb[NI][V];
+        if (h + p.groups < p.heads) load(h + p.groups, na, nb);
+        const NormSide& s = side(h);
+        const int hh = h < p.n_head ? h : h - p.n_head;
         if (s.w) {
-            const float r = 1.0f / sqrtf(lanes_sum<W>(sum) * inv_hd + p.eps);
             const float* w = s.w + hh * s.w_head;
+            if (w != held) {
+                held = w;
 #pragma unroll
-            for (int n = 0; n < NI; ++n) {
-                if (one[n]) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) a[n][i] = a[n][i] * r * w[at[n] + i];
-                }
-                if (two[n]) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) b[n][i] = b[n][i] * r * w[at[n] + far[n] + i];
+                for (int n = 0; n < NI; ++n) {
+                    if (one[n]) load_weights<V>(w + at[n], wa[n]);
+                    if (two[n]) load_weights<V>(w + at[n] + far[n], wb[n]);
                 }
             }
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum = fmaf(a[n][i], a[n][i], fmaf(b[n][i], b[n][i], sum));
+            const float r = 1.0f / sqrtf(lanes_sum<W>(sum) * inv_hd + p.eps);
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    a[n][i] = a[n][i] * r * (one[n] ? wa[n][i] : 0.f);
+                    b[n][i] = b[n][i] * r * (two[n] ? wb[n][i] : 0.f);
+                }
         }
+        T* y = static_cast<T*>(s.y) + t * s.y_token + hh * s.y_head;
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
             if (turns[n]) rotate<V, IL>(a[n], b[n], sc[n]);
             if (one[n]) store_vec<T, V>(y + at[n], a[n]);
             if (two[n]) store_vec<T, V>(y + at[n] + far[n], b[n]);
         }
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) a[n][i] = na[n][i], b[n][i] = nb[n][i];
     }
 }
 
@@ -175,7 +205,7 @@ extern "C" int pe_qk_norm_rope(const pe_qk_norm_args* a, pe_stream_t stream) {
     for (const NormSide* s : {&q, &k})
         if (s == &q ? a->n_head : a->n_kv)
             vec = vec && (s->x_token | s->x_head | s->y_token | s->y_head) % v == 0 && aligned(s->x, 16) &&
-                  aligned(s->y, 16);
+                  aligned(s->y, 16) && aligned(s->w, 16) && s->w_head % 4 == 0;
     hipStream_t s = (hipStream_t)stream;
     if (a->type == PE_TYPE_F16)
         return a->interleaved ? launch_qk_norm<_Float16, true>(p, vec, s) : launch_qk_norm<_Float16, false>(p, vec, s);
