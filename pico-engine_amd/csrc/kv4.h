@@ -38,16 +38,18 @@ PE_DEV void rows_of(const void* starts, int wide, int64_t b, int64_t tokens, int
     hi = hi < lo ? lo : hi > tokens ? tokens : hi;
 }
 
-// The sequence that row t belongs to, or -1: the last b with starts[b] <= t, if t lies before starts[b + 1].
+// The sequence that row t belongs to, or -1: the last b with starts[b] <= t, if t lies before starts[b + 1]. All lanes of a
+// wave look for the same row, 64 places at a time.
 PE_DEV int64_t sequence_of(const void* starts, int wide, int64_t batch, int64_t t) {
     if (!starts) return t < batch ? t : -1;
-    int64_t lo = 0, hi = batch + 1;  // the first of starts that is beyond t
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (int_at(starts, wide, mid) <= t)
-            lo = mid + 1;
-        else
-            hi = mid;
+    int64_t lo = 0, n = batch + 1;  // the first of starts that is beyond t lies in [lo, lo + n]
+    while (n > 0) {
+        const int64_t step = (n + 63) >> 6, at = (int64_t)(threadIdx.x & 63) * step;
+        const int below = __popcll(__ballot(at < n && int_at(starts, wide, lo + (at < n ? at : 0)) <= t));
+        if (below == 0) break;
+        lo += (below - 1) * step + 1;
+        n -= (below - 1) * step + 1;
+        if (n > step - 1) n = step - 1;
     }
     return lo >= 1 && lo <= batch ? lo - 1 : -1;
 }

@@ -2,6 +2,8 @@
 //   kv4_append  new rows of several sequences: q and k normed and rotated, k and v rounded to 4 bits and written to
 //               the slots behind what their sequence holds
 //   kv4_read    the values a cache stands for
+#include <type_traits>
+
 #include "kv4.h"
 #include "rope_common.h"
 
@@ -84,36 +86,45 @@ PE_DEV void store_run(T* p, const float* v) {
     for (int i = 0; i < E; i += N) store_vec<T, N>(p + i, v + i);
 }
 
-// Codes of the E elements of a lane, the scale shared with the 32 / E lanes of its block.
+// A 64-bit number in 32 bits, cut off, its last bit set if anything was: comparisons with short numbers, and rounding to
+// far fewer bits, come out as they would in 64. Beyond 2^128 the largest number, below 2^-126 zero; infinities and NaN stay so.
+PE_DEV uint32_t cut_short(double y) {
+    const uint64_t w = (uint64_t)__double_as_longlong(y);
+    const uint32_t hi = (uint32_t)(w >> 32), lo = (uint32_t)w, m = hi & 0x7FFFFFFFu;
+    uint32_t f = ((m - 0x38000000u) << 3 | lo >> 29) | (lo << 3 ? 1u : 0u);
+    f = m >= 0x47F00000u ? (m >= 0x7FF00000u ? 0x7FC00000u : 0x7F7FFFFFu) : m < 0x38100000u ? 0u : f;
+    return f | (hi & 0x80000000u);
+}
+
+// Codes of the E elements of a lane (bits of floats), the scale shared with the 32 / E lanes of its block.
 template <int E>
-PE_DEV uint32_t encode(const double* y, uint32_t& scale) {
-    uint64_t top = 0;  // the bits of magnitudes order as they do, infinities and NaN above all
+PE_DEV uint32_t encode(const uint32_t* y, uint32_t& scale) {
+    uint32_t top = 0;  // the bits of magnitudes order as they do, infinities and NaN above all
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const uint64_t m = (uint64_t)__double_as_longlong(y[i]) & 0x7FFFFFFFFFFFFFFFull;
-        top = m > top ? m : top;
-    }
-#pragma unroll
-    for (int o = 16 / E; o > 0; o >>= 1) {
-        const uint64_t m = (uint64_t)__shfl_xor((unsigned long long)top, o, kWave);
-        top = m > top ? m : top;
-    }
-    if (top >= 0x7FF0000000000000ull) {
+    for (int i = 0; i < E; ++i) top = max(top, y[i] & 0x7FFFFFFFu);
+    const auto other = [](uint32_t v, auto ctrl) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xF, 0xF, false); };
+    top = max(top, other(top, std::integral_constant<int, 0xB1>{}));                        // quad_perm [1,0,3,2]
+    top = max(top, other(top, std::integral_constant<int, 0x4E>{}));                        // quad_perm [2,3,0,1]
+    if constexpr (E == 4) top = max(top, other(top, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    if (top >= 0x7F800000u) {
         scale = 255;
         return 0;
     }
-    int e = (int)(top >> 52) - 1023 - 2 + ((top & 0xFFFFFFFFFFFFFull) > 0xC000000000000ull);
-    e = e < kKv4MinExp ? kKv4MinExp : e > kKv4MaxExp ? kKv4MaxExp : e;
-    scale = e + 127;
-    const double f = __longlong_as_double((long long)(1023 - e) << 52);  // 2^-e
+    // the mantissa beyond 1.75: 7 times a quarter of the power of two
+    int e = (int)(top >> 23) - 2 + ((top & 0x7FFFFFu) > 0x600000u);
+    e = e < kKv4MinExp + 127 ? kKv4MinExp + 127 : e > kKv4MaxExp + 127 ? kKv4MaxExp + 127 : e;
+    scale = e;
+    // to the nearest code, halfway to the even one, 6 beyond 6: what the conversion does
+    const float f = __uint_as_float((uint32_t)e << 23);
     uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const double z = y[i] * f, a = fabs(z);
-        // halfway values go to the even code
-        const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
-        codes |= (c | (z < 0 ? 8u : 0u)) << (4 * i);
+#define PE_TWO(i) codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, __uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]), f, i)
+    PE_TWO(0);
+    PE_TWO(1);
+    if constexpr (E == 8) {
+        PE_TWO(2);
+        PE_TWO(3);
     }
+#undef PE_TWO
     return codes;
 }
 
@@ -201,6 +212,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
                      hh * (isq ? p.q_head : isv ? p.v_head : p.k_head);
         load_pairs<T, E, VEC>(x, at, rot, p.half, own, other);
     }
+    const double freq = p.freqs && (int)threadIdx.x < p.half ? p.freqs[threadIdx.x] * 0.63661977236758134 : 0;
     const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
     if (b < 0) return;
     int64_t len = int_at(p.lengths, p.len_wide, b);
@@ -210,7 +222,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
         SinCos* turn32 = reinterpret_cast<SinCos*>(turn);
         if (p.freqs) {
             if ((int)threadIdx.x < p.half)
-                turn32[threadIdx.x] = sincos_quarters((double)slot, p.freqs[threadIdx.x] * 0.63661977236758134, 1.f);
+                turn32[threadIdx.x] = sincos_quarters((double)slot, freq, 1.f);
             __syncthreads();
         }
         float y[E];
@@ -227,18 +239,21 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     }
     if (p.freqs) {
         if ((int)threadIdx.x < p.half)
-            turn[threadIdx.x] = sincos_quarters64((double)slot, p.freqs[threadIdx.x] * 0.63661977236758134);
+            turn[threadIdx.x] = sincos_quarters64((double)slot, freq);
         __syncthreads();
     }
-    double y[E];
+    uint32_t bits[E];
     if (isv) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = own[i];
+        for (int i = 0; i < E; ++i) bits[i] = __float_as_uint(own[i]);
     } else {
+        double y[E];
         turn_run<HD, double>(p, own, other, at, p.k_weight, turn, y);
+#pragma unroll
+        for (int i = 0; i < E; ++i) bits[i] = cut_short(y[i]);
     }
     uint32_t scale;
-    const uint32_t codes = encode<E>(y, scale);
+    const uint32_t codes = encode<E>(bits, scale);
     // a negative length takes no part; a slot behind the table's end or on a page that there is not is not written
     const int page_tokens = p.tiles * kKv4Tile;
     if (!active || len < 0 || slot >= (int64_t)p.table_cols * page_tokens) return;
@@ -269,7 +284,7 @@ struct Kv4ReadArgs {
     int len_wide;
     int n_kv;
     int64_t rows;
-    int row_tiles;
+    int row_blocks;  // workgroups of a sequence and kv head
     void* k;
     void* v;
 };
@@ -286,40 +301,85 @@ PE_DEV void decode(uint32_t codes, uint32_t scale, float* y) {
     }
 }
 
-// A workgroup takes a tile of a sequence and kv head, 16 lanes a token.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_kv4_read(Kv4ReadArgs p) {
-    constexpr int E = HD / 16;
-    const int lane = threadIdx.x % 16, tok = threadIdx.x / 16;
-    const uint32_t pair = blockIdx.x / (uint32_t)p.row_tiles;
-    const int rt = (int)(blockIdx.x - pair * (uint32_t)p.row_tiles);
-    const int64_t b = pair / (uint32_t)p.n_kv;
-    const int h = (int)(pair - (uint32_t)b * (uint32_t)p.n_kv);
-    const int64_t row = (int64_t)rt * kKv4Tile + tok;
-    if (row >= p.rows) return;
-    float k[E] = {}, v[E] = {};
-    const int col = rt / p.tiles;
-    if (row < int_at(p.lengths, p.len_wide, b) && col < p.table_cols) {
-        const int page = p.table[b * p.table_row + col];
-        if (page >= 0 && page < p.n_pages) {
-            const uint8_t* z = p.pages + page * p.page_stride + ((int64_t)h * p.tiles + rt % p.tiles) * (17 * HD);
-            const uint8_t* kc = z + tok * (HD / 2) + lane * (E / 2);
-            const uint8_t* vc = z + 8 * HD + tok / 4 * (2 * HD) + lane * (2 * E) + tok % 4 * (E / 2);
-            const int block = lane * E / 32;
-            const uint32_t ks = z[16 * HD + tok * (HD / 32) + block];
-            const uint32_t vs = z[16 * HD + HD / 2 + (tok / 4 * (HD / 32) + block) * 4 + tok % 4];
-            if constexpr (E == 8) {
-                decode<E>(*reinterpret_cast<const uint32_t*>(kc), ks, k);
-                decode<E>(*reinterpret_cast<const uint32_t*>(vc), vs, v);
-            } else {
-                decode<E>(*reinterpret_cast<const uint16_t*>(kc), ks, k);
-                decode<E>(*reinterpret_cast<const uint16_t*>(vc), vs, v);
-            }
+// A run to memory, past the caches where STREAM.
+template <typename T, int E, bool STREAM>
+PE_DEV void write_run(T* p, const float* v) {
+    if constexpr (!STREAM) {
+        store_run<T, E>(p, v);
+    } else {
+        constexpr int N = E * sizeof(T) > 16 ? 16 / sizeof(T) : E;
+#pragma unroll
+        for (int i = 0; i < E; i += N) {
+            typename Vec<T, N>::type x;
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = (T)v[i + j];
+            __builtin_nontemporal_store(x, reinterpret_cast<typename Vec<T, N>::type*>(p + i));
         }
     }
-    const int64_t at = ((int64_t)pair * p.rows + row) * HD + lane * E;
-    store_run<T, E>(static_cast<T*>(p.k) + at, k);
-    store_run<T, E>(static_cast<T*>(p.v) + at, v);
+}
+
+// A workgroup takes NT tiles of a sequence and kv head, 16 lanes a token; the tiles' pages, then their codes, are under
+// way together.
+template <typename T, int HD, int NT, bool STREAM>
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4ReadArgs p) {
+    constexpr int E = HD / 16;
+    typedef typename std::conditional<E == 8, uint32_t, uint16_t>::type run;
+    const int lane = threadIdx.x % 16, tok = threadIdx.x / 16;
+    const uint32_t pair = blockIdx.x / (uint32_t)p.row_blocks;
+    const int rt = (int)(blockIdx.x - pair * (uint32_t)p.row_blocks) * NT;
+    const int64_t b = pair / (uint32_t)p.n_kv;
+    const int h = (int)(pair - (uint32_t)b * (uint32_t)p.n_kv);
+    const int64_t len = int_at(p.lengths, p.len_wide, b);
+    int page[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int col = (rt + i) / p.tiles;
+        page[i] = col < p.table_cols ? p.table[b * p.table_row + col] : -1;
+    }
+    uint32_t kc[NT], vc[NT], ks[NT], vs[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        kc[i] = vc[i] = ks[i] = vs[i] = 0;
+        if ((int64_t)(rt + i) * kKv4Tile + tok < len && (uint32_t)page[i] < (uint32_t)p.n_pages) {
+            const uint8_t* z = p.pages + page[i] * p.page_stride + ((int64_t)h * p.tiles + (rt + i) % p.tiles) * (17 * HD);
+            const int block = lane * E / 32;
+            kc[i] = *reinterpret_cast<const run*>(z + tok * (HD / 2) + lane * (E / 2));
+            vc[i] = *reinterpret_cast<const run*>(z + 8 * HD + tok / 4 * (2 * HD) + lane * (2 * E) + tok % 4 * (E / 2));
+            ks[i] = z[16 * HD + tok * (HD / 32) + block];
+            vs[i] = z[16 * HD + HD / 2 + (tok / 4 * (HD / 32) + block) * 4 + tok % 4];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t row = (int64_t)(rt + i) * kKv4Tile + tok;
+        if (row >= p.rows) return;
+        const int64_t at = ((int64_t)pair * p.rows + row) * HD + lane * E;
+        float y[E];
+        decode<E>(kc[i], ks[i], y);
+        write_run<T, E, STREAM>(static_cast<T*>(p.k) + at, y);
+        decode<E>(vc[i], vs[i], y);
+        write_run<T, E, STREAM>(static_cast<T*>(p.v) + at, y);
+    }
+}
+
+template <typename T, int HD>
+static int launch_read(Kv4ReadArgs p, int64_t pairs, hipStream_t s) {
+    const int64_t tiles = (p.rows + kKv4Tile - 1) / kKv4Tile;
+    // Two tiles a workgroup where that leaves 20 of one tile and more to each CU (3 x 3833 rows of 8 heads of 128, fp16, 13.4 us
+    // against 16; 48 x 397 of 4, fp32, 16.5 against 15.5; four tiles are slower at both). Outputs that the last-level
+    // cache would not hold go past it (5 x 20000 of 4, fp16, 205 MB, 50 -> 42 us; 78 MB 16 -> 23).
+    const int nt = tiles * pairs >= 20 * 256 ? 2 : 1;
+    const bool stream = 2 * pairs * p.rows * HD * (int64_t)sizeof(T) > (128 << 20);
+    p.row_blocks = (int)((tiles + nt - 1) / nt);
+    if (p.row_blocks * pairs >= (1 << 24)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    const dim3 g((unsigned)(p.row_blocks * pairs));
+    if (stream)
+        hipLaunchKernelGGL((k_kv4_read<T, HD, 2, true>), g, dim3(256), 0, s, p);
+    else if (nt == 2)
+        hipLaunchKernelGGL((k_kv4_read<T, HD, 2, false>), g, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((k_kv4_read<T, HD, 1, false>), g, dim3(256), 0, s, p);
+    return launch_status();
 }
 
 template <typename T>
@@ -393,22 +453,15 @@ extern "C" int pe_kv4_read(int type, const pe_kv4_pool* pool, const void* length
     if (batch < 0 || batch > (1 << 20) || rows < 0 || rows > (1LL << 30)) return PE_ERR_SHAPE;
     if (const int st = kv4_pool_ok(pool, n_kv, head_dim)) return st;
     if (batch == 0 || rows == 0) return PE_OK;
-    const int64_t row_tiles = (rows + kKv4Tile - 1) / kKv4Tile;
-    if (row_tiles * n_kv * batch >= (1 << 24)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    if ((rows + 2 * kKv4Tile - 1) / (2 * kKv4Tile) * n_kv * batch >= (1 << 24)) return PE_ERR_SHAPE;
     if (!lengths || !k || !v) return PE_ERR_NULL;
     if (!aligned(k, 16) || !aligned(v, 16) || !int_aligned(lengths, lengths_dtype)) return PE_ERR_ALIGN;
     Kv4ReadArgs p{static_cast<const uint8_t*>(pool->pages), pool->page_stride, pool->n_pages,
                   (int)(pool->page_tokens / kKv4Tile), pool->table, pool->table_stride, (int)pool->table_cols, lengths,
-                  lengths_dtype == 2, n_kv, rows, (int)row_tiles, k, v};
-    const dim3 g((unsigned)(row_tiles * n_kv * batch));
+                  lengths_dtype == 2, n_kv, rows, 0, k, v};
     hipStream_t s = (hipStream_t)stream;
-    if (type == PE_TYPE_F16 && head_dim == 64)
-        hipLaunchKernelGGL((k_kv4_read<_Float16, 64>), g, dim3(256), 0, s, p);
-    else if (type == PE_TYPE_F16)
-        hipLaunchKernelGGL((k_kv4_read<_Float16, 128>), g, dim3(256), 0, s, p);
-    else if (head_dim == 64)
-        hipLaunchKernelGGL((k_kv4_read<float, 64>), g, dim3(256), 0, s, p);
-    else
-        hipLaunchKernelGGL((k_kv4_read<float, 128>), g, dim3(256), 0, s, p);
-    return launch_status();
+    const int64_t pairs = batch * n_kv;
+    if (type == PE_TYPE_F16)
+        return head_dim == 64 ? launch_read<_Float16, 64>(p, pairs, s) : launch_read<_Float16, 128>(p, pairs, s);
+    return head_dim == 64 ? launch_read<float, 64>(p, pairs, s) : launch_read<float, 128>(p, pairs, s);
 }
