@@ -300,21 +300,25 @@ PE_DEV bf8v operand(const uint32_t* w) {
 template <int HD, int RT, int NP, int TS>
 PE_DEV void kv4_scores(const Kv4Raw<HD, TS>& r, const Kv4State<HD, RT, NP>& st, f4v (&s)[RT][TS]) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-        const float scale = __uint_as_float(r.s[i] << 23);
+    for (int i = 0; i < TS; ++i)
 #pragma unroll
         for (int t = 0; t < RT; ++t) s[t][i] = f4v{};
+    // products of different scores one after the other: one that adds to the last one's would wait for it
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-            uint32_t w[4];
+    for (int j = 0; j < HD / 32; ++j) {
+        uint32_t w[TS][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = two_codes(r.c[i][j], scale, c);
+        for (int i = 0; i < TS; ++i)
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+            for (int c = 0; c < 4; ++c) w[i][c] = two_codes(r.c[i][j], __uint_as_float(r.s[i] << 23), c);
 #pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w), __builtin_bit_cast(bf8v, st.q[((t * NP + n) * (HD / 32) + j) * 64]), s[t][i], 0, 0, 0);
-        }
+        for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const bf8v q = __builtin_bit_cast(bf8v, st.q[((t * NP + n) * (HD / 32) + j) * 64]);
+#pragma unroll
+                for (int i = 0; i < TS; ++i) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w[i]), q, s[t][i], 0, 0, 0);
+            }
     }
 }
 
@@ -440,9 +444,9 @@ PE_DEV void kv4_values(const Kv4Raw<HD, TS>& r, Kv4State<HD, RT, NP>& st, const 
                 hi[c] = __builtin_amdgcn_perm(two[2 * c + 1], two[2 * c], 0x07060302u);
             }
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+            for (int n = 0; n < NP; ++n)
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
+                for (int t = 0; t < RT; ++t) {
                     st.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo), operand(pr[t][h][n]), st.o[t][j], 0, 0, 0);
                     st.o[t][j + 1] =
                         __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi), operand(pr[t][h][n]), st.o[t][j + 1], 0, 0, 0);
@@ -536,8 +540,8 @@ __global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv
         walk.tile = walk.next / kKv4Tile - walk.col * p.tiles;
         const int* table = p.table + w.b * p.table_row;
         const uint8_t* head = p.pages + (int64_t)kvh * p.tiles * (17 * HD);
-        kv4_pages<TS>(p, table, walk);
         Kv4Raw<HD, TS> keys, values;
+        kv4_pages<TS>(p, table, walk);
         kv4_advance<HD, TS>(p, table, head, walk);
         kv4_load_keys<HD, TS>(walk, lane, keys);
         kv4_load_values<HD, TS>(walk, lane, values);
@@ -729,7 +733,9 @@ static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, 
     const int64_t chunks = (capacity + s.min_chunk - 1) / s.min_chunk;
     int64_t extra = (int64_t)sqrt((double)s.blocks * (double)capacity / s.weight) + 1;
     if (extra > 8192 / n_kv + 1) extra = 8192 / n_kv + 1;
-    if (chunks <= 1)
+    // up to four chunks (of heads of 64; three of 128) one workgroup takes them all: the second launch costs as much (14 heads, 500
+    // keys: 7.6 us in one launch, 9.9 in two; 1000 keys 10.6 and 10.3, of 28 heads of 128 13.2 and 11.6)
+    if (chunks <= (!s.split ? 1 : hd == 64 ? 4 : 3))
         extra = 0;
     else if (extra > s.blocks * (chunks - 1))
         extra = s.blocks * (chunks - 1);

@@ -1898,11 +1898,12 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
 
 # ---- a paged cache held in 4 bits -------------------------------------------------------------
 
-def _heads(t: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -> tuple[int, int]:
+def _heads(t: torch.Tensor, T: int, n: int, hd: int, dtype: torch.dtype, what: str) -> tuple[int, int]:
     """(token, head) strides of rows of heads (T, n, hd) whose last dim is contiguous; 0 where there is one of them."""
-    if t.dtype is not dtype or tuple(t.shape) != shape or (shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"{what} must be a {dtype} {shape} tensor whose last dim is contiguous")
-    return t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+    s = t.stride()
+    if t.dtype is not dtype or t.shape != (T, n, hd) or (s[2] != 1 and hd > 1):
+        raise ValueError(f"{what} must be a {dtype} ({T}, {n}, {hd}) tensor whose last dim is contiguous")
+    return s[0] if T > 1 else 0, s[1] if n > 1 else 0
 
 
 def _weight(w: torch.Tensor | None, n: int, hd: int, what: str) -> tuple[int | None, int]:
@@ -1938,15 +1939,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     a.amp, a.interleaved, a.eps, a.tokens, a.n_head, a.head_dim = float(amp), int(interleaved), float(eps), T, n, hd
     if hd > 1 and q.stride(2) != 1:
         q = q.contiguous()
-    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, (T, n, hd), q.dtype, "q")
-    a.q_out, (a.q_out_token, a.q_out_head) = out[0].data_ptr(), _heads(out[0], (T, n, hd), q.dtype, "out's q")
+    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, T, n, hd, q.dtype, "q")
+    a.q_out, (a.q_out_token, a.q_out_head) = out[0].data_ptr(), _heads(out[0], T, n, hd, q.dtype, "out's q")
     a.q_weight, a.q_weight_head = _weight(q_weight, n, hd, "q_weight")
     if k is not None:
         m = k.shape[1]
         if hd > 1 and k.stride(2) != 1:
             k = k.contiguous()
-        a.n_kv, a.k, (a.k_token, a.k_head) = m, k.data_ptr(), _heads(k, (T, m, hd), q.dtype, "k")
-        a.k_out, (a.k_out_token, a.k_out_head) = out[1].data_ptr(), _heads(out[1], (T, m, hd), q.dtype, "out's k")
+        a.n_kv, a.k, (a.k_token, a.k_head) = m, k.data_ptr(), _heads(k, T, m, hd, q.dtype, "k")
+        a.k_out, (a.k_out_token, a.k_out_head) = out[1].data_ptr(), _heads(out[1], T, m, hd, q.dtype, "out's k")
         a.k_weight, a.k_weight_head = _weight(k_weight, m, hd, "k_weight")
     if T and (n or a.n_kv):
         _launch(dev, "pe_qk_norm_rope", ctypes.byref(a))
@@ -1964,15 +1965,16 @@ def kv4_pages(n_pages: int, n_kv: int, hd: int, page_tokens: int, device) -> tor
 
 def _kv4_pool(pages: torch.Tensor, table: torch.Tensor, batch: int) -> tuple[Kv4Pool, int, int]:
     """The C view of a pool and its table, with n_kv and hd."""
-    if pages.dtype is not torch.uint8 or pages.dim() != 4 or pages.shape[3] not in (17 * 64, 17 * 128) or \
-            pages.shape[0] == 0 or not pages[0].is_contiguous():
+    shape, s, ts = pages.shape, pages.stride(), table.stride()
+    if pages.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in (17 * 64, 17 * 128) or shape[0] == 0 or \
+            s[1:] != (shape[2] * shape[3], shape[3], 1):
         raise ValueError("pages must be a uint8 (n_pages, n_kv, page_tokens / 16, 17 hd) pool (kv4_pages), each page contiguous")
-    n, n_kv, tiles, tile = pages.shape
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != batch or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
+    n, n_kv, tiles, tile = shape
+    cols = table.shape[-1] if len(ts) else 0
+    if table.dtype is not torch.int32 or table.shape != (batch, cols) or (cols > 1 and ts[1] != 1):
         raise ValueError(f"table must hold int32 page numbers, ({batch}, pages of a sequence), its rows contiguous")
-    return Kv4Pool(pages.data_ptr(), n, pages.stride(0) if n > 1 else n_kv * tiles * tile, 16 * tiles, table.data_ptr(),
-                   table.stride(0) if batch > 1 else table.shape[1], table.shape[1]), n_kv, tile // 17
+    return Kv4Pool(pages.data_ptr(), n, s[0] if n > 1 else n_kv * tiles * tile, 16 * tiles, table.data_ptr(),
+                   ts[0] if batch > 1 else cols, cols), n_kv, tile // 17
 
 
 def _kv4_rows(starts: torch.Tensor | None, tokens: int, batch: int) -> tuple[int | None, int]:
@@ -2009,8 +2011,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: tor
         k = k.contiguous()
     if v.dim() == 3 and v.stride(2) != 1:
         v = v.contiguous()
-    a.k, (a.k_token, a.k_head) = k.data_ptr(), _heads(k, (T, n_kv, hd), k.dtype, "k")
-    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, (T, n_kv, hd), k.dtype, "v")
+    a.k, (a.k_token, a.k_head) = k.data_ptr(), _heads(k, T, n_kv, hd, k.dtype, "k")
+    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, T, n_kv, hd, k.dtype, "v")
     a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
     a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
     if freqs is not None:
@@ -2027,8 +2029,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: tor
             q = q.contiguous()
         if out is None:
             out = q.new_empty((T, n, hd))
-        a.n_head, a.q, (a.q_token, a.q_head) = n, q.data_ptr(), _heads(q, (T, n, hd), k.dtype, "q")
-        a.q_out, (a.q_out_token, a.q_out_head) = out.data_ptr(), _heads(out, (T, n, hd), k.dtype, "out")
+        a.n_head, a.q, (a.q_token, a.q_head) = n, q.data_ptr(), _heads(q, T, n, hd, k.dtype, "q")
+        a.q_out, (a.q_out_token, a.q_out_head) = out.data_ptr(), _heads(out, T, n, hd, k.dtype, "out")
         a.q_weight = None if q_norm is None else q_norm.data_ptr()
     elif out is not None or q_norm is not None:
         raise ValueError("out and q_norm go with q")
@@ -2047,7 +2049,7 @@ def kv4_read(pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, ro
     if dtype not in _CACHE_TYPE or rows < 0:
         raise ValueError(f"{rows} rows of {dtype}: dtype must be float32 or float16")
     code = _ints(lengths, B, "lengths")
-    k, v = (torch.empty(B, n_kv, rows, hd, device=pages.device, dtype=dtype) for _ in range(2))
+    k, v = pages.new_empty((B, n_kv, rows, hd), dtype=dtype), pages.new_empty((B, n_kv, rows, hd), dtype=dtype)
     if B and rows:
         _launch(dev, "pe_kv4_read", _CACHE_TYPE[dtype], ctypes.byref(pool), lengths.data_ptr(), code, B, n_kv, hd, int(rows),
                 k.data_ptr(), v.data_ptr())
@@ -2088,7 +2090,7 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
         q = q.contiguous()
     a = Kv4AttnArgs()
     a.type, a.pool, a.tokens, a.batch, a.n_head, a.n_kv, a.head_dim, a.first = code, pool, T, B, n, n_kv, hd, int(first)
-    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, (T, n, hd), q.dtype, "q")
+    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, T, n, hd, q.dtype, "q")
     a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
     a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
     a.scale = hd ** -0.5 if scale is None else float(scale)
@@ -2096,7 +2098,7 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
         raise ValueError(f"scale {scale}")
     if out is None:
         out = q.new_empty((T, n, hd))
-    a.out, (a.out_token, a.out_head) = out.data_ptr(), _heads(out, (T, n, hd), q.dtype, "out")
+    a.out, (a.out_token, a.out_head) = out.data_ptr(), _heads(out, T, n, hd, q.dtype, "out")
     if T == 0 or B == 0:
         return out
     need = _kv4_bytes(T, B, starts is not None, n, n_kv, hd, pool.table_cols * pool.page_tokens)
