@@ -17,11 +17,6 @@
 
 namespace pe {
 
-// Tiles of 16 keys that a wave takes at a time: two, with which the state of 16 rows leaves room for three waves a SIMD
-// (64 x 16384 keys of 8 heads of 128, fp16: 150 us with four, 140 with two); four for 32 rows of heads of 128, whose
-// state leaves room for two waves a SIMD or one either way (2 x 1021 rows of 28 heads on 8000 keys: 385 us with two, 372 with four).
-template <int HD, int RT>
-constexpr int kKv4Tiles = HD == 128 && RT == 2 ? 4 : 2;
 constexpr int kKv4Waves = 4;   // of a workgroup
 constexpr int kKv4Span = 64;   // chunks are whole multiples of it
 constexpr float kKv4Log2e = 1.4426950408889634f;
@@ -283,9 +278,8 @@ PE_DEV void kv4_load_values(const Kv4Walk<TS>& w, int lane, Kv4Raw<HD, TS>& r) {
 }
 
 // The state of RT x 16 query rows.
-template <int HD, int RT, int NP>
+template <int HD, int RT>
 struct Kv4State {
-    const u4v* q;                    // LDS: parts of the queries [RT][NP][HD / 32][64 lanes], the lane's operands
     f4v o[RT][HD / 16];              // O^T: channel (4 g + i) HD/16 + j of row lane % 16 in o[j][i]
     float m[RT], l[RT];              // what exponents are taken from (of the row), sum (of the lane's keys), base 2
     int lim[RT];                     // keys that the lane's row sees
@@ -296,13 +290,12 @@ PE_DEV bf8v operand(const uint32_t* w) {
     return __builtin_bit_cast(bf8v, z);
 }
 
-// Scores of a step's keys: s[row][16 keys][4 keys of the lane]. A scale byte of 255 converts every code to NaN.
-template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_scores(const Kv4Raw<HD, TS>& r, const Kv4State<HD, RT, NP>& st, f4v (&s)[RT][TS]) {
+// Scores of a step's keys for 16 rows: s[16 keys][4 keys of the lane]. q: the lane's operands in LDS, parts of the queries
+// [NP][HD / 32][64 lanes]. A scale byte of 255 converts every code to NaN.
+template <int HD, int NP, int TS>
+PE_DEV void kv4_scores(const Kv4Raw<HD, TS>& r, const u4v* q, f4v (&s)[TS]) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) s[t][i] = f4v{};
+    for (int i = 0; i < TS; ++i) s[i] = f4v{};
     // products of different scores one after the other: one that adds to the last one's would wait for it
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) {
@@ -312,21 +305,40 @@ PE_DEV void kv4_scores(const Kv4Raw<HD, TS>& r, const Kv4State<HD, RT, NP>& st, 
 #pragma unroll
             for (int c = 0; c < 4; ++c) w[i][c] = two_codes(r.c[i][j], __uint_as_float(r.s[i] << 23), c);
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
+        for (int n = 0; n < NP; ++n) {
+            const bf8v z = __builtin_bit_cast(bf8v, q[(n * (HD / 32) + j) * 64]);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const bf8v q = __builtin_bit_cast(bf8v, st.q[((t * NP + n) * (HD / 32) + j) * 64]);
-#pragma unroll
-                for (int i = 0; i < TS; ++i) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w[i]), q, s[t][i], 0, 0, 0);
-            }
+            for (int i = 0; i < TS; ++i) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w[i]), z, s[i], 0, 0, 0);
+        }
     }
 }
 
-// Scores of keys that a row does not see become -inf. Values that no row sees may hold anything, and one that is no number
-// must not reach rows that do not see it: their codes become 0 and their scale 1, and bad tells of those that some row
-// sees (bit 4 (i % 2) + c of bad[i / 2]: key c of the lane's in the 16 keys i).
-template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_mask(const int* keys, int most, int g, Kv4Raw<HD, TS>& v, const Kv4State<HD, RT, NP>& st, f4v (&s)[RT][TS], uint32_t* bad) {
+// Values that no row sees (from key `most` on) may hold anything, and one that is no number must not reach rows that do not
+// see it: their codes become 0 and their scale 1. bad tells of the latter that some row sees (bit 4 (i % 2) + c of bad[i /
+// 2]: key c of the lane's in the 16 keys i).
+template <int HD, int TS>
+PE_DEV void kv4_mask_value(int key, int i, int c, int most, Kv4Raw<HD, TS>& v, uint32_t* bad) {
+    const bool none = key >= most, nan = (v.s[i] >> (8 * c) & 255) == 255;
+    if (!none && nan) bad[i >> 1] |= 1u << ((i & 1) * 4 + c);
+    if (none || nan) {
+        v.s[i] = (v.s[i] & ~(255u << (8 * c))) | 127u << (8 * c);
+        if constexpr (HD == 128)
+            v.c[i][c] = 0;
+        else
+            v.c[i][c >> 1] &= c & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+    }
+}
+template <int HD, int TS>
+PE_DEV void kv4_mask_values(const int* keys, int most, int g, Kv4Raw<HD, TS>& v, uint32_t* bad) {
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kv4_mask_value<HD, TS>(keys[i] + 4 * g + c, i, c, most, v, bad);
+}
+// Scores of keys that a row does not see become -inf; the values too are masked, if the wave holds them.
+template <int HD, int RT, int TS>
+PE_DEV void kv4_mask_scores(const int* keys, int g, const Kv4State<HD, RT>& st, f4v (&s)[RT][TS], int most = 0,
+                            Kv4Raw<HD, TS>* v = nullptr, uint32_t* bad = nullptr) {
 #pragma unroll
     for (int i = 0; i < TS; ++i)
 #pragma unroll
@@ -335,21 +347,13 @@ PE_DEV void kv4_mask(const int* keys, int most, int g, Kv4Raw<HD, TS>& v, const 
 #pragma unroll
             for (int t = 0; t < RT; ++t)
                 if (key >= st.lim[t]) s[t][i][c] = -INFINITY;
-            const bool none = key >= most, nan = (v.s[i] >> (8 * c) & 255) == 255;
-            if (!none && nan) bad[i >> 1] |= 1u << ((i & 1) * 4 + c);
-            if (none || nan) {
-                v.s[i] = (v.s[i] & ~(255u << (8 * c))) | 127u << (8 * c);
-                if constexpr (HD == 128)
-                    v.c[i][c] = 0;
-                else
-                    v.c[i][c >> 1] &= c & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-            }
+            if (v) kv4_mask_value<HD, TS>(key, i, c, most, *v, bad);
         }
 }
 
 // NaN into the channels of the runs whose values are no numbers, of the rows that see them: counted by a product of both.
-template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_no_numbers(const int* keys, int g, const uint32_t* bad, Kv4State<HD, RT, NP>& st) {
+template <int HD, int RT, int TS>
+PE_DEV void kv4_no_numbers(const int* keys, int g, const uint32_t* bad, Kv4State<HD, RT>& st) {
 #pragma unroll
     for (int h = 0; h < TS / 2; ++h) {
         if (!__ballot(bad[h] != 0)) continue;
@@ -381,7 +385,7 @@ PE_DEV void kv4_no_numbers(const int* keys, int g, const uint32_t* bad, Kv4State
 constexpr float kKv4Slack = 6.f;
 
 template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT, NP>& st, const f4v (&s)[RT][TS], uint32_t (&pr)[RT][TS / 2][NP][4]) {
+PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT>& st, const f4v (&s)[RT][TS], uint32_t (&pr)[RT][TS / 2][NP][4]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = -INFINITY;
@@ -418,39 +422,49 @@ PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT, NP>& st, const f4v (&s)[RT
     }
 }
 
-// O^T += V^T P^T, 32 keys at a time, two channels of a run at a time: a conversion gives two channels of one key, a
-// permutation two keys of one channel.
-template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_values(const Kv4Raw<HD, TS>& r, Kv4State<HD, RT, NP>& st, const uint32_t (&pr)[RT][TS / 2][NP][4]) {
+// The scales of the lane's 8 keys of tiles i and i + 1; the conversion looks at the exponent's bits alone.
+template <int HD, int TS>
+PE_DEV void kv4_value_scales(const Kv4Raw<HD, TS>& r, int i, float (&scale)[8]) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const uint32_t w = r.s[i + (c >> 2)];
+        scale[c] = __uint_as_float((c & 3) < 3 ? w << (23 - 8 * (c & 3)) : w >> 1);
+    }
+}
+
+// The operands of channels j and j + 1 of the lane's run (j even), for the 32 keys of tiles i and i + 1: a conversion
+// gives two channels of one key, a permutation two keys of one channel.
+template <int HD, int TS>
+PE_DEV void kv4_value_operands(const Kv4Raw<HD, TS>& r, int i, int j, const float* scale, uint32_t (&lo)[4], uint32_t (&hi)[4]) {
+    uint32_t two[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const int k = c & 3, at = i + (c >> 2);
+        two[c] = HD == 128 ? two_codes(r.c[at][k], scale[c], j >> 1) : two_codes(r.c[at][k >> 1], scale[c], (k & 1) * 2 + (j >> 1));
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        lo[c] = __builtin_amdgcn_perm(two[2 * c + 1], two[2 * c], 0x05040100u);
+        hi[c] = __builtin_amdgcn_perm(two[2 * c + 1], two[2 * c], 0x07060302u);
+    }
+}
+
+// O^T += V^T P^T, 32 keys at a time, two channels of a run at a time.
+template <int HD, int NP, int TS>
+PE_DEV void kv4_values(const Kv4Raw<HD, TS>& r, Kv4State<HD, 1>& st, const uint32_t (&pr)[1][TS / 2][NP][4]) {
 #pragma unroll
     for (int h = 0; h < TS / 2; ++h) {
-        float scale[8];  // the conversion looks at the exponent's bits alone
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const uint32_t w = r.s[2 * h + (c >> 2)];
-            scale[c] = __uint_as_float((c & 3) < 3 ? w << (23 - 8 * (c & 3)) : w >> 1);
-        }
+        float scale[8];
+        kv4_value_scales<HD, TS>(r, 2 * h, scale);
 #pragma unroll
         for (int j = 0; j < HD / 16; j += 2) {
-            uint32_t two[8], lo[4], hi[4];
+            uint32_t lo[4], hi[4];
+            kv4_value_operands<HD, TS>(r, 2 * h, j, scale, lo, hi);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const int i = 2 * h + (c >> 2), k = c & 3;
-                two[c] = HD == 128 ? two_codes(r.c[i][k], scale[c], j >> 1) : two_codes(r.c[i][k >> 1], scale[c], (k & 1) * 2 + (j >> 1));
+            for (int n = 0; n < NP; ++n) {
+                st.o[0][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo), operand(pr[0][h][n]), st.o[0][j], 0, 0, 0);
+                st.o[0][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi), operand(pr[0][h][n]), st.o[0][j + 1], 0, 0, 0);
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                lo[c] = __builtin_amdgcn_perm(two[2 * c + 1], two[2 * c], 0x05040100u);
-                hi[c] = __builtin_amdgcn_perm(two[2 * c + 1], two[2 * c], 0x07060302u);
-            }
-#pragma unroll
-            for (int n = 0; n < NP; ++n)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    st.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo), operand(pr[t][h][n]), st.o[t][j], 0, 0, 0);
-                    st.o[t][j + 1] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi), operand(pr[t][h][n]), st.o[t][j + 1], 0, 0, 0);
-                }
         }
     }
 }
@@ -458,86 +472,90 @@ PE_DEV void kv4_values(const Kv4Raw<HD, TS>& r, Kv4State<HD, RT, NP>& st, const 
 template <typename T>
 constexpr int kKv4Parts = sizeof(T) == 2 ? 2 : 3;
 
-// SPLIT: the workgroup's rows are RT x 16, its waves take steps in turn and are merged in LDS. Otherwise every wave has
-// RT x 16 rows of its own and takes all the item's keys.
-template <typename T, int HD, int RT, bool SPLIT>
-__global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv4AttnArgs p) {
-    constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16 * RT, RB = SPLIT ? R : R * kKv4Waves, TS = kKv4Tiles<HD, RT>;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int item = blockIdx.x, kvh = blockIdx.y;
-    Kv4Item w;
-    if (!kv4_find<RB>(p, item, w)) return;
-    const Kv4Seq seq = kv4_seq(p, w.b);
+// A lane's HD / 4 elements of query row `row` (of the sequence's rows times heads) as operands: to(j, z) gets the NP
+// parts z[four words][NP] of the j-th 32 channels; zeros where the row is not there.
+template <typename T, int HD, int NP, typename F>
+PE_DEV void kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row, int last, int g, const F& to) {
+    const bool there = row < seq.rows;
+    row = there ? row : last;
+    const int i = row / p.group;
+    const T* x = static_cast<const T*>(p.q) + (seq.lo + i) * p.q_token + (int64_t)(kvh * p.group + row - i * p.group) * p.q_head +
+                 g * (HD / 4);
+    float q[HD / 4];
+    if (p.vec) {
+        typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+        for (int j = 0; j < HD / 4; j += 16 / (int)sizeof(T)) {
+            const piece z = *reinterpret_cast<const piece*>(x + j);
+#pragma unroll
+            for (int c = 0; c < 16 / (int)sizeof(T); ++c) q[j + c] = (float)z[c];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < HD / 4; ++j) q[j] = (float)x[j];
+    }
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        uint32_t z[4][NP];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float a = (float)(q[8 * j + 2 * c] * p.q_scale), b = (float)(q[8 * j + 2 * c + 1] * p.q_scale);
+            split_pair<NP>(there ? a : 0.f, there ? b : 0.f, z[c]);
+        }
+        to(j, z);
+    }
+}
+
+template <int TS>
+PE_DEV void kv4_begin(const Kv4AttnArgs& p, Kv4Walk<TS>& w, int first, int end, int stride) {
+    w.next = first;
+    w.end = end;
+    w.cols = stride / p.tiles;
+    w.tiles = stride - w.cols * p.tiles;
+    w.col = first / kKv4Tile / p.tiles;
+    w.tile = first / kKv4Tile - w.col * p.tiles;
+}
+
+PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
     if (w.chunk == 0 && w.block == 0 && kvh == 0 && threadIdx.x == 0 && p.plan)
         p.plan[w.b] = make_int4(w.base, w.chunks, w.blocks, 0);
+}
 
-    // the wave's rows: r0 + 16 t + n
-    const int r0 = w.block * RB + (SPLIT ? 0 : wave * R), last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
-    const bool rows = r0 < seq.rows;
-    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0, most = rows ? kv4_keys(p, seq.keys, last / p.group) : 0;
+// Few rows (one new token, a few drafted ones): 16 rows a workgroup, its waves take steps of 32 keys in turn, each with a
+// state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x 16384 keys of 8 heads of
+// 128, fp16: 135 us, 4.3 TB/s), else the start's chain of loads (lengths, queries, table, keys), about 4 us of a
+// workgroup's time. Three and four waves a SIMD are what keeps enough keys under way: with the queries in
+// registers and steps of 64 keys, two waves, 145 us; with a second step in registers 150.
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
+    constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16, TS = 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.y;
+    Kv4Item w;
+    if (!kv4_find<R>(p, blockIdx.x, w)) return;
+    const Kv4Seq seq = kv4_seq(p, w.b);
+    kv4_tell(p, w, kvh);
+    const int r0 = w.block * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
+    const int least = kv4_keys(p, seq.keys, r0 / p.group), most = kv4_keys(p, seq.keys, last / p.group);
     const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
+    constexpr int QUERIES = NP * (HD / 32) * 64, PART = kKv4Waves * R * (HD + 4 + 2) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[PART > QUERIES * 16 ? PART : QUERIES * 16];
+    u4v* queries = reinterpret_cast<u4v*>(lds) + lane;
+    if (wave == 0)
+        kv4_query<T, HD, NP>(p, seq, kvh, r0 + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
+#pragma unroll
+            for (int k = 0; k < NP; ++k) queries[(k * (HD / 32) + j) * 64] = u4v{z[0][k], z[1][k], z[2][k], z[3][k]};
+        });
+    Kv4State<HD, 1> st;
+    st.lim[0] = r0 + n < seq.rows ? kv4_keys(p, seq.keys, (r0 + n) / p.group) : 0;
+    st.m[0] = -INFINITY;
+    st.l[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) st.o[0][j] = f4v{};
+    __syncthreads();
     Kv4Walk<TS> walk;
-    walk.end = (int)(stop < most ? stop : most);
-    walk.next = (int)begin + (SPLIT ? wave * TS * kKv4Tile : 0);
-    Kv4State<HD, RT, NP> st;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        st.m[t] = -INFINITY;
-        st.l[t] = 0.f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) st.o[t][j] = f4v{};
-    }
-    // The queries' parts go to LDS: SPLIT, a wave for every 16 rows that all waves share, else every wave its own.
-    // 32 (16) elements of a row in a lane; rows that are not there take the last one's, as zeros.
-    constexpr int QW = RT * NP * (HD / 32) * 64;
-    constexpr int PART = SPLIT ? kKv4Waves * R * (HD + 4 + 2) * 4 : 0, QUERIES = (SPLIT ? QW : QW * kKv4Waves) * 16;
-    __shared__ __attribute__((aligned(16))) char lds[PART > QUERIES ? PART : QUERIES];
-    st.q = reinterpret_cast<const u4v*>(lds) + (SPLIT ? 0 : wave * QW) + lane;
-    if (rows) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            int row = r0 + 16 * t + n;
-            const bool there = row < seq.rows;
-            row = there ? row : last;
-            const int i = row / p.group;
-            st.lim[t] = there ? kv4_keys(p, seq.keys, i) : 0;
-            if (SPLIT && wave != t) continue;
-            const T* x = static_cast<const T*>(p.q) + (seq.lo + i) * p.q_token +
-                         (int64_t)(kvh * p.group + row - i * p.group) * p.q_head + g * (HD / 4);
-            float q[HD / 4];
-            if (p.vec) {
-                typedef T piece __attribute__((ext_vector_type(16 / sizeof(T))));
-#pragma unroll
-                for (int j = 0; j < HD / 4; j += 16 / (int)sizeof(T)) {
-                    const piece z = *reinterpret_cast<const piece*>(x + j);
-#pragma unroll
-                    for (int c = 0; c < 16 / (int)sizeof(T); ++c) q[j + c] = (float)z[c];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < HD / 4; ++j) q[j] = (float)x[j];
-            }
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) {
-                uint32_t z[4][NP];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float a = (float)(q[8 * j + 2 * c] * p.q_scale), b = (float)(q[8 * j + 2 * c + 1] * p.q_scale);
-                    split_pair<NP>(there ? a : 0.f, there ? b : 0.f, z[c]);
-                }
-#pragma unroll
-                for (int k = 0; k < NP; ++k)
-                    const_cast<u4v*>(st.q)[((t * NP + k) * (HD / 32) + j) * 64] = u4v{z[0][k], z[1][k], z[2][k], z[3][k]};
-            }
-        }
-    }
-    if constexpr (SPLIT) __syncthreads();
+    kv4_begin(p, walk, (int)begin + wave * TS * kKv4Tile, (int)(stop < most ? stop : most), TS * kKv4Waves);
     if (walk.next < walk.end) {
-        const int stride = SPLIT ? TS * kKv4Waves : TS;  // tiles from step to step
-        walk.cols = stride / p.tiles;
-        walk.tiles = stride - walk.cols * p.tiles;
-        walk.col = walk.next / kKv4Tile / p.tiles;
-        walk.tile = walk.next / kKv4Tile - walk.col * p.tiles;
         const int* table = p.table + w.b * p.table_row;
         const uint8_t* head = p.pages + (int64_t)kvh * p.tiles * (17 * HD);
         Kv4Raw<HD, TS> keys, values;
@@ -556,88 +574,238 @@ __global__ __launch_bounds__(64 * kKv4Waves, RT == 1 ? 3 : 2) void k_kv4_attn(Kv
                 masked |= at[i] + kKv4Tile > least;
             }
             const bool more = walk.next < walk.end;
-            f4v s[RT][TS];
-            kv4_scores<HD, RT, NP, TS>(keys, st, s);
+            f4v s[1][TS];
+            kv4_scores<HD, NP, TS>(keys, queries, s[0]);
             if (more) {
                 kv4_advance<HD, TS>(p, table, head, walk);
                 kv4_load_keys<HD, TS>(walk, lane, keys);
             }
-            uint32_t bad[TS / 2] = {}, pr[RT][TS / 2][NP][4];
-            if (masked) kv4_mask<HD, RT, NP, TS>(at, most, g, values, st, s, bad);
-            kv4_softmax<HD, RT, NP, TS>(p.scale, st, s, pr);
-            kv4_values<HD, RT, NP, TS>(values, st, pr);
-            if (masked) kv4_no_numbers<HD, RT, NP, TS>(at, g, bad, st);
+            uint32_t bad[TS / 2] = {}, pr[1][TS / 2][NP][4];
+            if (masked) kv4_mask_scores<HD, 1, TS>(at, g, st, s, most, &values, bad);
+            kv4_softmax<HD, 1, NP, TS>(p.scale, st, s, pr);
+            kv4_values<HD, NP, TS>(values, st, pr);
+            if (masked) kv4_no_numbers<HD, 1, TS>(at, g, bad, st);
             if (!more) break;
             kv4_load_values<HD, TS>(walk, lane, values);
         }
     }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) st.l[t] = swap32_sum(swap16_sum(st.l[t]));
+    st.l[0] = swap32_sum(swap16_sum(st.l[0]));
 
     const int64_t rec = ((int64_t)kvh * p.items + w.base + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;
-    if constexpr (SPLIT) {
-        float(*part)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(lds);
-        float(*pm)[R] = reinterpret_cast<float(*)[R]>(lds + kKv4Waves * R * (HD + 4) * 4), (*pl)[R] = pm + kKv4Waves;
-        __syncthreads();  // the queries have been read
+    float(*part)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(lds);
+    float(*pm)[R] = reinterpret_cast<float(*)[R]>(lds + kKv4Waves * R * (HD + 4) * 4), (*pl)[R] = pm + kKv4Waves;
+    __syncthreads();  // the queries have been read
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int row = 16 * t + n;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < E; ++j) part[wave][n][(4 * g + i) * E + j] = st.o[0][j][i];
+    if (g == 0) pm[wave][n] = st.m[0], pl[wave][n] = st.l[0];
+    __syncthreads();
+    const int row = threadIdx.x / 16, c = threadIdx.x % 16 * E, r = r0 + row;
+    if (r >= seq.rows) return;
+    float m = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < E; ++j) part[wave][row][(4 * g + i) * E + j] = st.o[t][j][i];
-            if (g == 0) pm[wave][row] = st.m[t], pl[wave][row] = st.l[t];
-        }
-        __syncthreads();
-        for (int x = threadIdx.x; x < R * 16; x += 64 * kKv4Waves) {
-            const int row = x / 16, c = x % 16 * E, r = r0 + row;
-            if (r >= seq.rows) break;
-            float m = -INFINITY;
+    for (int k = 0; k < kKv4Waves; ++k) m = fmaxf(m, pm[k][row]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[E] = {};
 #pragma unroll
-            for (int k = 0; k < kKv4Waves; ++k) m = fmaxf(m, pm[k][row]);
-            const float base = m == -INFINITY ? 0.f : m;
-            float l = 0.f, o[E] = {};
+    for (int k = 0; k < kKv4Waves; ++k) {
+        const float f = __builtin_amdgcn_exp2f(pm[k][row] - base);
+        l = fmaf(pl[k][row], f, l);
 #pragma unroll
-            for (int k = 0; k < kKv4Waves; ++k) {
-                const float f = __builtin_amdgcn_exp2f(pm[k][row] - base);
-                l = fmaf(pl[k][row], f, l);
+        for (int j = 0; j < E; ++j) o[j] = fmaf(part[k][row][c + j], f, o[j]);
+    }
+    if (w.chunks == 1) {
+        const int i = r / p.group;
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        T* y = static_cast<T*>(p.out) + (seq.lo + i) * p.out_token + (int64_t)(kvh * p.group + r - i * p.group) * p.out_head + c;
 #pragma unroll
-                for (int j = 0; j < E; ++j) o[j] = fmaf(part[k][row][c + j], f, o[j]);
-            }
-            if (w.chunks == 1) {
-                const int i = r / p.group;
-                const float f = l == 0.f ? 0.f : 1.f / l;
-                T* y = static_cast<T*>(p.out) + (seq.lo + i) * p.out_token + (int64_t)(kvh * p.group + r - i * p.group) * p.out_head + c;
-#pragma unroll
-                for (int j = 0; j < E; ++j) y[j] = (T)(o[j] * f);
-            } else {
-                float* y = p.record + (rec + row) * HD + c;
-#pragma unroll
-                for (int j = 0; j < E; ++j) y[j] = o[j];
-                if (c == 0) p.stat[2 * (rec + row)] = m, p.stat[2 * (rec + row) + 1] = l;
-            }
-        }
+        for (int j = 0; j < E; ++j) y[j] = (T)(o[j] * f);
     } else {
+        float* y = p.record + (rec + row) * HD + c;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int row = wave * R + 16 * t + n, r = r0 + 16 * t + n;
-            if (r >= seq.rows) continue;
-            const int i = r / p.group;
-            const float f = st.l[t] == 0.f ? 0.f : 1.f / st.l[t];
-            if (w.chunks == 1) {
-                T* y = static_cast<T*>(p.out) + (seq.lo + i) * p.out_token + (int64_t)(kvh * p.group + r - i * p.group) * p.out_head;
+        for (int j = 0; j < E; ++j) y[j] = o[j];
+        if (c == 0) p.stat[2 * (rec + row)] = m, p.stat[2 * (rec + row) + 1] = l;
+    }
+}
+
+// Many rows (pieces of prompts): 32 rows a wave, 128 a workgroup, all on the same keys. The waves convert a step's codes
+// for one another, into LDS in the order of the products' operands, two steps deep; the queries are in registers.
+template <typename T, int HD>
+constexpr int kKv4RowTiles = sizeof(T) == 4 && HD == 128 ? 2 : 4;  // 16 keys a step; fp32's queries take half the registers
+
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs p) {
+    constexpr int NP = kKv4Parts<T>, E = HD / 16, RT = 2, R = 16 * RT, RB = R * kKv4Waves, TS = kKv4RowTiles<T, HD>, N = HD / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.y;
+    Kv4Item w;
+    if (!kv4_find<RB>(p, blockIdx.x, w)) return;
+    const Kv4Seq seq = kv4_seq(p, w.b);
+    kv4_tell(p, w, kvh);
+    // the workgroup's rows, and the wave's (it has none: it converts alone)
+    const int b0 = w.block * RB, b1 = (b0 + RB < seq.rows ? b0 + RB : seq.rows) - 1;
+    const int least_all = kv4_keys(p, seq.keys, b0 / p.group), most_all = kv4_keys(p, seq.keys, b1 / p.group);
+    const int r0 = b0 + wave * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
+    const bool rows = r0 < seq.rows;
+    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0, most = rows ? kv4_keys(p, seq.keys, last / p.group) : 0;
+    const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
+    const int end = (int)(stop < most_all ? stop : most_all);
+
+    // Operands: keys [tile][32 channels][64 lanes], values [32 keys][channel of a run][64 lanes]. A wave converts a
+    // quarter of each: KF of the keys' (of one tile), VF pairs of the values' (of 32 keys).
+    constexpr int KF = TS * N / kKv4Waves, VF = TS / 2 * (E / 2) / kKv4Waves, PER = kKv4Waves / (TS / 2);
+    __shared__ u4v k_ops[2][TS * N][64], v_ops[2][TS / 2 * E][64];
+    __shared__ uint32_t no_number[2][TS / 2][64];
+    __shared__ int first_key[2][TS];
+    const int k_tile = wave * KF / N, k_part = wave * KF % N, v_half = wave / PER, v_pair = wave % PER * VF;
+
+    Kv4State<HD, RT> st;
+    uint32_t q[RT][NP][N][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+    for (int t = 0; t < RT; ++t) {
+        if (rows)
+            kv4_query<T, HD, NP>(p, seq, kvh, r0 + 16 * t + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
 #pragma unroll
-                    for (int j = 0; j < E; ++j) y[(4 * g + k) * E + j] = (T)(st.o[t][j][k] * f);
-            } else {
-                float* y = p.record + (rec + row) * HD;
+                for (int k = 0; k < NP; ++k)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                    for (int c = 0; c < 4; ++c) q[t][k][j][c] = z[c][k];
+            });
+        const int row = r0 + 16 * t + n;
+        st.lim[t] = row < seq.rows ? kv4_keys(p, seq.keys, row / p.group) : 0;
+        st.m[t] = -INFINITY;
+        st.l[t] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < E; ++j) y[(4 * g + k) * E + j] = st.o[t][j][k];
-                if (g == 0) p.stat[2 * (rec + row)] = st.m[t], p.stat[2 * (rec + row) + 1] = st.l[t];
+        for (int j = 0; j < E; ++j) st.o[t][j] = f4v{};
+    }
+    if (begin < end) {
+        const int* table = p.table + w.b * p.table_row;
+        const uint8_t* head = p.pages + (int64_t)kvh * p.tiles * (17 * HD);
+        Kv4Walk<1> kw;
+        Kv4Walk<2> vw;
+        kv4_begin(p, kw, (int)begin + k_tile * kKv4Tile, end, TS);
+        kv4_begin(p, vw, (int)begin + v_half * 2 * kKv4Tile, end, TS);
+        kv4_pages<1>(p, table, kw);
+        kv4_pages<2>(p, table, vw);
+        Kv4Raw<HD, 1> keys;
+        Kv4Raw<HD, 2> values;
+        const auto load = [&] {
+            kv4_advance<HD, 1>(p, table, head, kw);
+            kv4_advance<HD, 2>(p, table, head, vw);
+            kv4_load_keys<HD, 1>(kw, lane, keys);
+            kv4_load_values<HD, 2>(vw, lane, values);
+        };
+        // a wave's pairs of channels are the lowest bytes of its words once they are shifted
+        const auto mask = [&](int to) {
+            uint32_t bad[1] = {0};
+            if (vw.key[0] + kKv4Tile > least_all || vw.key[1] + kKv4Tile > least_all) kv4_mask_values<HD, 2>(vw.key, most_all, g, values, bad);
+            no_number[to][v_half][lane] = bad[0];  // (several waves hold the same)
+            first_key[to][k_tile] = kw.key[0];
+        };
+        const auto convert = [&](int to) {
+            const float scale = __uint_as_float(keys.s[0] << 23);
+#pragma unroll
+            for (int f = 0; f < KF; ++f) {
+                const uint32_t c = KF == N || k_part == 0 ? keys.c[0][f] : keys.c[0][f + N - KF];
+                k_ops[to][k_tile * N + k_part + f][lane] = u4v{two_codes(c, scale, 0), two_codes(c, scale, 1), two_codes(c, scale, 2), two_codes(c, scale, 3)};
             }
+            float scales[8];
+            kv4_value_scales<HD, 2>(values, 0, scales);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) values.c[i][j] >>= 8 * v_pair;
+#pragma unroll
+            for (int f = 0; f < VF; ++f) {
+                uint32_t lo[4], hi[4];
+                kv4_value_operands<HD, 2>(values, 0, 2 * f, scales, lo, hi);
+                v_ops[to][v_half * E + 2 * (v_pair + f)][lane] = u4v{lo[0], lo[1], lo[2], lo[3]};
+                v_ops[to][v_half * E + 2 * (v_pair + f) + 1][lane] = u4v{hi[0], hi[1], hi[2], hi[3]};
+            }
+        };
+        load();
+        mask(0);
+        convert(0);
+        load();  // (past the end: keys that are not there, from the pool's first page)
+        __syncthreads();
+        int at = 0;
+        for (int key = (int)begin; key < end; key += TS * kKv4Tile, at ^= 1) {
+            int keys_at[TS];
+            bool masked = false, masked_all = false;  // for the wave's rows, for the workgroup's (and in its conversions)
+#pragma unroll
+            for (int i = 0; i < TS; ++i) {
+                keys_at[i] = __builtin_amdgcn_readfirstlane(first_key[at][i]);
+                masked |= keys_at[i] + kKv4Tile > least;
+                masked_all |= keys_at[i] + kKv4Tile > least_all;
+            }
+            f4v s[RT][TS];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < TS; ++i) s[t][i] = f4v{};
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                bf8v k[TS];
+#pragma unroll
+                for (int i = 0; i < TS; ++i) k[i] = __builtin_bit_cast(bf8v, k_ops[at][i * N + j][lane]);
+#pragma unroll
+                for (int c = 0; c < NP; ++c)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+#pragma unroll
+                        for (int i = 0; i < TS; ++i) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i], operand(q[t][c][j]), s[t][i], 0, 0, 0);
+            }
+            if (masked) kv4_mask_scores<HD, RT, TS>(keys_at, g, st, s);
+            mask(at ^ 1);
+            uint32_t pr[RT][TS / 2][NP][4];
+            kv4_softmax<HD, RT, NP, TS>(p.scale, st, s, pr);
+            // the next step's conversions beside this one's second product
+            convert(at ^ 1);
+#pragma unroll
+            for (int h = 0; h < TS / 2; ++h)
+#pragma unroll
+                for (int j = 0; j < E; j += 2) {
+                    const bf8v v0 = __builtin_bit_cast(bf8v, v_ops[at][h * E + j][lane]), v1 = __builtin_bit_cast(bf8v, v_ops[at][h * E + j + 1][lane]);
+#pragma unroll
+                    for (int c = 0; c < NP; ++c)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) {
+                            st.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, operand(pr[t][h][c]), st.o[t][j], 0, 0, 0);
+                            st.o[t][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, operand(pr[t][h][c]), st.o[t][j + 1], 0, 0, 0);
+                        }
+                }
+            if (masked_all) {
+                uint32_t bad[TS / 2];
+#pragma unroll
+                for (int h = 0; h < TS / 2; ++h) bad[h] = no_number[at][h][lane];
+                kv4_no_numbers<HD, RT, TS>(keys_at, g, bad, st);
+            }
+            load();
+            __syncthreads();  // the next step's operands are there, this one's have been read
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) st.l[t] = swap32_sum(swap16_sum(st.l[t]));
+    const int64_t rec = ((int64_t)kvh * p.items + w.base + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int row = wave * R + 16 * t + n, r = r0 + 16 * t + n;
+        if (r >= seq.rows) continue;
+        const int i = r / p.group;
+        const float f = st.l[t] == 0.f ? 0.f : 1.f / st.l[t];
+        if (w.chunks == 1) {
+            T* y = static_cast<T*>(p.out) + (seq.lo + i) * p.out_token + (int64_t)(kvh * p.group + r - i * p.group) * p.out_head;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < E; ++j) y[(4 * g + k) * E + j] = (T)(st.o[t][j][k] * f);
+        } else {
+            float* y = p.record + (rec + row) * HD;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < E; ++j) y[(4 * g + k) * E + j] = st.o[t][j][k];
+            if (g == 0) p.stat[2 * (rec + row)] = st.m[t], p.stat[2 * (rec + row) + 1] = st.l[t];
         }
     }
 }
@@ -767,10 +935,10 @@ template <typename T, int HD>
 static void launch_kv4(const Kv4AttnArgs& p, const Kv4Plan& s, hipStream_t st) {
     const dim3 g((unsigned)(s.items + 7) / 8 * 8, (unsigned)p.n_kv);
     if (!s.split) {
-        hipLaunchKernelGGL((k_kv4_attn<T, HD, 2, false>), g, dim3(64 * kKv4Waves), 0, st, p);
+        hipLaunchKernelGGL((k_kv4_attn_rows<T, HD>), g, dim3(64 * kKv4Waves), 0, st, p);
         launch_merge<T, HD, 32 * kKv4Waves>(p, st);
     } else {
-        hipLaunchKernelGGL((k_kv4_attn<T, HD, 1, true>), g, dim3(64 * kKv4Waves), 0, st, p);
+        hipLaunchKernelGGL((k_kv4_attn<T, HD>), g, dim3(64 * kKv4Waves), 0, st, p);
         launch_merge<T, HD, 16>(p, st);
     }
 }
