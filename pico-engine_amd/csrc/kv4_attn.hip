@@ -120,15 +120,15 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
         }
         const float all = wave_sum<64>((float)cost);
         span = ((int)fmaxf(sqrtf(all * p.weight), (float)p.min_chunk) + kKv4Span - 1) / kKv4Span * kKv4Span;
-        int count = nb0 * chunks_of(keys0, span);
+        float count = (float)nb0 * (float)chunks_of(keys0, span);
         for (int b = lane + 64; b < p.batch; b += 64) {
             int nb, keys;
             look(b, nb, keys);
-            count += nb * chunks_of(keys, span);
+            count += (float)nb * (float)chunks_of(keys, span);
         }
-        // more than the launch has (or than an int holds): keys times blocks shared out evenly, in 32-bit floats, and a 4096th
-        // more, which is beyond what their rounding takes off
-        if (wave_sum<64>((float)count) > (float)p.items * (1.f - 1.f / 4096)) {
+        // more than the launch has: keys times blocks shared out evenly, in 32-bit floats, and a 4096th more, which is beyond
+        // what their rounding takes off
+        if (wave_sum<64>(count) > (float)p.items * (1.f - 1.f / 4096)) {
             const float safe = all / (float)(p.items - p.blocks) * (1.f + 1.f / 4096) + kKv4Span;
             span = safe < (float)(1 << 30) ? (int)safe / kKv4Span * kKv4Span : 1 << 30;
             span = span < p.min_chunk ? p.min_chunk : span;
@@ -521,7 +521,7 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
         p.plan[w.b] = make_int4(w.base, w.chunks, w.blocks, 0);
 }
 
-// Few rows (one new token, a few drafted ones): 16 rows a workgroup, its waves take steps of 32 keys in turn, each with a
+// Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32 keys in turn, each with a
 // state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x 16384 keys of 8 heads of
 // 128, fp16: 135 us, 4.3 TB/s), else the start's chain of loads (lengths, queries, table, keys), about 4 us of a
 // workgroup's time. Three and four waves a SIMD are what keeps enough keys under way: with the queries in
@@ -890,7 +890,9 @@ static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, 
     Kv4Plan s;
     const int group = n_head / n_kv;
     const int64_t rows = ragged ? (tokens + batch - 1) / batch * group : group;  // of a sequence, on average
-    s.split = rows <= 32;
+    // Up to 512 rows in blocks of 16 (one sequence with 16000 keys, heads of 128, fp16, of 64 fp32; us in blocks of 16 | of
+    // 128: 160 rows 47 | 70, 280 24 | 33; 320 73 | 85, 560 36 | 42; 600 122 | 115, 1050 55 | 64; 2400 384 | 318, 4200 158 | 145).
+    s.split = rows <= 512;
     s.rt = s.split ? 1 : 2;
     s.rb = 16 * s.rt * (s.split ? 1 : kKv4Waves);
     s.blocks = ragged ? tokens * group / s.rb + batch : batch * ((group + s.rb - 1) / s.rb);
