@@ -128,6 +128,12 @@ PE_DEV uint32_t encode(const uint32_t* y, uint32_t& scale) {
     return codes;
 }
 
+// A value that all lanes hold, in scalar registers: what follows from it is then computed once a wave.
+PE_DEV int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // A lane's run of E elements from channel `at` on (own), and of what each is turned with (other).
 template <typename T, int E, bool VEC>
 PE_DEV void load_pairs(const T* x, int at, int rot, int half, float* own, float* other) {
@@ -200,7 +206,11 @@ template <typename T, int HD, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     constexpr int E = HD / 16;
     __shared__ SinCos64 turn[HD / 2];
-    const int64_t t = blockIdx.x;
+    // Workgroups go to the eight XCDs in turn: of each 128, sixteen neighbours go to one, whose L2 then gathers the pieces
+    // of a tile's lines.
+    int t = blockIdx.x;
+    if ((t | 127) < (int)p.tokens) t = (t & ~127) + (t & 7) * 16 + (t >> 3 & 15);
+    if (t >= (int)p.tokens) return;
     const int lane = threadIdx.x % 16, at = lane * E, group = threadIdx.x / 16;
     const bool isq = (int)blockIdx.y < p.q_parts;
     const int h = (isq ? blockIdx.y : blockIdx.y - p.q_parts) * 16 + group;
@@ -215,9 +225,9 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     const double freq = p.freqs && (int)threadIdx.x < p.half ? p.freqs[threadIdx.x] * 0.63661977236758134 : 0;
     const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
     if (b < 0) return;
-    int64_t len = int_at(p.lengths, p.len_wide, b);
+    int64_t len = uniform(int_at(p.lengths, p.len_wide, b));
     len = len > (1LL << 40) ? 1LL << 40 : len;
-    const int64_t slot = len + (p.starts ? t - int_at(p.starts, p.starts_wide, b) : 0);
+    const int64_t slot = len + (p.starts ? t - uniform(int_at(p.starts, p.starts_wide, b)) : 0);
     if (isq) {
         SinCos* turn32 = reinterpret_cast<SinCos*>(turn);
         if (p.freqs) {
@@ -256,10 +266,10 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     const uint32_t codes = encode<E>(bits, scale);
     // a negative length takes no part; a slot behind the table's end or on a page that there is not is not written
     const int page_tokens = p.tiles * kKv4Tile;
-    if (!active || len < 0 || slot >= (int64_t)p.table_cols * page_tokens) return;
+    if (len < 0 || slot >= (int64_t)p.table_cols * page_tokens) return;
     const int col = (int)slot / page_tokens, off = (int)slot - col * page_tokens, tok = off % kKv4Tile;
-    const int page = p.table[b * p.table_row + col];
-    if (page < 0 || page >= p.n_pages) return;
+    const int page = __builtin_amdgcn_readfirstlane(p.table[b * p.table_row + col]);
+    if (!active || page < 0 || page >= p.n_pages) return;
     uint8_t* z = p.pages + page * p.page_stride + ((int64_t)hh * p.tiles + off / kKv4Tile) * (17 * HD);
     uint8_t* c = isv ? z + 8 * HD + tok / 4 * (2 * HD) + lane * (2 * E) + tok % 4 * (E / 2)
                      : z + tok * (HD / 2) + lane * (E / 2);
@@ -384,7 +394,7 @@ static int launch_read(Kv4ReadArgs p, int64_t pairs, hipStream_t s) {
 
 template <typename T>
 static int launch_append(const Kv4AppendArgs& p, int hd, bool vec, hipStream_t s) {
-    const dim3 g((unsigned)p.tokens, (unsigned)(p.q_parts + (2 * p.n_kv + 15) / 16));
+    const dim3 g((unsigned)(p.tokens + 7) / 8 * 8, (unsigned)(p.q_parts + (2 * p.n_kv + 15) / 16));
     if (hd == 64 && vec)
         hipLaunchKernelGGL((k_kv4_append<T, 64, true>), g, dim3(256), 0, s, p);
     else if (hd == 64)
