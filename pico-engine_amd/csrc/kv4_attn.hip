@@ -50,9 +50,9 @@ struct Kv4AttnArgs {
     int64_t capacity;   // slots of a sequence
     int vec;            // q's rows are whole pieces of 16 bytes
     int items, blocks;  // workgroups a kv head, row blocks at most
-    int min_chunk;         // least keys of a chunk
-    float weight;
-    int rec_rows;          // rows of a record
+    int min_chunk;      // least keys of a chunk
+    float weight;       // of all keys in the square of a chunk's length
+    int rec_rows;       // rows of a record
     int4* plan;         // of every sequence: first item, chunks, row blocks
     float* record;      // [kv head][items][row][HD], a row block's chunks one after the other
     float* stat;        // [kv head][items][row] (maximum, sum)
@@ -95,8 +95,10 @@ struct Kv4Item {
 
 // Which work the item is: a (sequence, row block, chunk of keys). Every wave finds it for itself, from all lengths.
 // A chunk's length S weighs what workgroups cost beside their keys against the time that the last one takes
-// alone, cost(all keys) + S a + (all keys / S) F / (256 c) with a of a key, F of a workgroup, c of them on a CU
-// at once: the least is at S = sqrt(all keys F / (256 c a)), p.weight the factor behind the root.
+// alone: all keys' time + S a + (all keys / S) F / (256 c), with a of a key, F of a workgroup, c of them on a CU
+// at once, is least at S = sqrt(all keys F / (256 c a)). Keys of all kv heads times row blocks, and 0.75 for the rest: with 0.25,
+// 0.75 and 2.5 one new row on 33 x 4001 keys (28 heads of 128, fp32) takes 24.9, 21.2 and 22.9 us, on 64 x 16384 (32
+// heads, fp16) 152, 143 and 142, 2 x 1021 rows on 8000 keys 421, 385 and 396.
 template <int RB>
 PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
     const int lane = threadIdx.x & 63;
@@ -200,11 +202,11 @@ PE_DEV uint32_t two_codes(uint32_t w, float scale, int sel) {
 template <int TS>
 struct Kv4Walk {
     const uint8_t* at[TS];  // the 16 keys' tiles
-    int key[TS];    // numbers of their first keys
-    int id[TS];     // pages of the step behind
-    int col, tile;         // page of the table, tile in it, of that step's first 16 keys
-    int next, end;         // its first key, the item's last
-    int cols, tiles;       // from step to step
+    int key[TS];            // numbers of their first keys
+    int id[TS];             // pages of the step behind
+    int col, tile;          // page of the table, tile in it, of that step's first 16 keys
+    int next, end;          // its first key, the item's last
+    int cols, tiles;        // from step to step
 };
 
 constexpr int kNoKeys = 0x7FFFFF00;  // number of the first key of 16 that are not there
@@ -280,9 +282,9 @@ PE_DEV void kv4_load_values(const Kv4Walk<TS>& w, int lane, Kv4Raw<HD, TS>& r) {
 // The state of RT x 16 query rows.
 template <int HD, int RT>
 struct Kv4State {
-    f4v o[RT][HD / 16];              // O^T: channel (4 g + i) HD/16 + j of row lane % 16 in o[j][i]
-    float m[RT], l[RT];              // what exponents are taken from (of the row), sum (of the lane's keys), base 2
-    int lim[RT];                     // keys that the lane's row sees
+    f4v o[RT][HD / 16];  // O^T: channel (4 g + i) HD/16 + j of row lane % 16 in o[j][i]
+    float m[RT], l[RT];  // what exponents are taken from (of the row), sum (of the lane's keys), base 2
+    int lim[RT];         // keys that the lane's row sees
 };
 
 PE_DEV bf8v operand(const uint32_t* w) {
@@ -524,8 +526,9 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
 // Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32 keys in turn, each with a
 // state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x 16384 keys of 8 heads of
 // 128, fp16: 135 us, 4.3 TB/s), else the start's chain of loads (lengths, queries, table, keys), about 4 us of a
-// workgroup's time. Three and four waves a SIMD are what keeps enough keys under way: with the queries in
-// registers and steps of 64 keys, two waves, 145 us; with a second step in registers 150.
+// workgroup's time (28 heads of 128 on 33 x 4001 keys, fp32: 21 us with the join, 7.4 at the copy rate). Three and four
+// waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of 64 keys, two waves, 145 us;
+// with a second step in registers 150.
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16, TS = 2;
@@ -630,7 +633,10 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
 }
 
 // Many rows (pieces of prompts): 32 rows a wave, 128 a workgroup, all on the same keys. The waves convert a step's codes
-// for one another, into LDS in the order of the products' operands, two steps deep; the queries are in registers.
+// for one another, into LDS in the order of the products' operands, two steps deep; the queries are in registers. Bound by
+// the matrix cores and the vector instructions, which add up with two waves a SIMD (2 x 1021 rows of 28 heads of 128
+// on 8000 keys, fp16: 45 % and 54 % of the cycles, 330 us, the join of the chunks 34; the two parts of each factor alone are 273
+// at the rate of a large product). With every wave converting for itself 367 and, fp32, 588 us; so 360 and 490.
 template <typename T, int HD>
 constexpr int kKv4RowTiles = sizeof(T) == 4 && HD == 128 ? 2 : 4;  // 16 keys a step; fp32's queries take half the registers
 
@@ -661,7 +667,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
     const int k_tile = wave * KF / N, k_part = wave * KF % N, v_half = wave / PER, v_pair = wave % PER * VF;
 
     Kv4State<HD, RT> st;
-    uint32_t q[RT][NP][N][4];
+    uint32_t q[RT][NP][N][4] = {};
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         if (rows)

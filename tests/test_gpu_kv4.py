@@ -464,3 +464,91 @@ def test_two_streams(K):
     torch.cuda.synchronize()
     for i, x in enumerate(got):
         assert torch.equal(x, want[i % 2]), i
+
+
+def test_moved_pages_in_a_graph(K):
+    """A captured call reads the table anew: pages handed out again between replays, eager work of the same kind beside it."""
+    B, nh, n_kv, hd, page = 3, 28, 4, 128, 32
+    pages, table = tables(K, B, n_kv, hd, page, 2000, 7, spare=40)
+    lengths = torch.tensor([1999, 700, 31], device=DEV)
+    q = rand(1, B, nh, hd) * 0.5
+    g = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        K.kv4_attn(q, pages, table, lengths)
+        with torch.cuda.graph(g, stream=s):
+            out = K.kv4_attn(q, pages, table, lengths)
+            k, v = K.kv4_read(pages, table, lengths, 100)
+    torch.cuda.current_stream().wait_stream(s)
+    for i in range(4):
+        perm = torch.randperm(pages.shape[0], generator=torch.Generator().manual_seed(i))[:table.numel()]
+        table.copy_(perm.view(table.shape).int())
+        lengths.copy_(torch.tensor([[5, 1999, 300], [1999, 1, 0], [800, -1, 1200], [64, 63, 65]][i]))
+        want, rows = K.kv4_attn(q, pages, table, lengths), K.kv4_read(pages, table, lengths, 100)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(k, rows[0]) and torch.equal(v, rows[1]), i
+        close(want, pages, table, lengths, q)
+
+
+@pytest.mark.parametrize("sizes", [None, [1, 0, 3] * 100, [90] * 70])
+def test_many_sequences(K, sizes):
+    """More sequences than a wave looks at together, one row each, ragged, and in the kernel of many rows."""
+    B, nh, n_kv, hd, page = 300 if sizes is None else len(sizes), 8, 1, 64, 16
+    pages, table = tables(K, B, n_kv, hd, page, 600, 7, spare=0)
+    lengths = torch.randint(0, 500, (B,), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    starts = None if sizes is None else torch.tensor([sum(sizes[:b]) for b in range(B + 1)], device=DEV)
+    q = (rand(2, B if sizes is None else sum(sizes), nh, hd) * 0.5).half()
+    got = K.kv4_attn(q, pages, table, lengths, starts=starts)
+    some = list(range(0, B, 37)) + [B - 1]                    # (the oracle goes row by row)
+    for b in some:
+        lo, hi = (b, b + 1) if starts is None else starts[b:b + 2].tolist()
+        if hi > lo:
+            close(got[lo:hi], pages, table[b:b + 1], lengths[b:b + 1], q[lo:hi], starts=torch.tensor([0, hi - lo], device=DEV))
+    k, v = rand(3, q.shape[0], n_kv, hd), rand(4, q.shape[0], n_kv, hd)
+    before = pages.clone()
+    K.kv4_append(k, v, pages, table, lengths, starts=starts)
+    for b in some:
+        lo, hi = (b, b + 1) if starts is None else starts[b:b + 2].tolist()
+        want = appended(before, table[b:b + 1], lengths[b:b + 1], torch.tensor([0, hi - lo], device=DEV), k[lo:hi], v[lo:hi], None, 1.0, False, None, 0)
+        for p in table[b].tolist():
+            assert torch.equal(pages[p].cpu(), want[p])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_one_kv_head_for_many(K, dtype):
+    """More query heads on a kv head than the kernel of few rows takes."""
+    pages, table = tables(K, 2, 1, 64, 32, 700, 7)
+    lengths = torch.tensor([650, 3], device=DEV)
+    q = (rand(2, 2, 530, 64) * 0.5).to(dtype)
+    close(K.kv4_attn(q, pages, table, lengths), pages, table, lengths, q)
+
+
+@pytest.mark.parametrize("nh,n_kv,hd", [(14, 2, 64), (28, 4, 128)])
+def test_as_the_plain_caches(K, nh, n_kv, hd):
+    """The operators one after the other against those of plain caches on the values that are read back: norms, rotation
+    and attention of a piece of a prompt, then of a token behind it. Both attentions keep 2^-17 of a score's magnitude
+    (up to 2^6 here) and of the probabilities: 2^-10 of sum p |v|, which is under 4."""
+    page, L, old = 32, 60, 200
+    pages = K.kv4_pages(12, n_kv, hd, page, DEV)
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(1)).view(1, 12).int().to(DEV)
+    freqs, _ = K.rope_freqs(hd)
+    w = 1 + rand(5, hd) * 0.1
+    lengths, at = torch.tensor([0], device=DEV), 0
+    for rows in (old, L, 1):
+        x = rand(rows, rows, (nh + 2 * n_kv), hd)
+        starts = torch.tensor([0, rows], device=DEV)
+        q = K.kv4_append(x[:, nh:nh + n_kv], x[:, nh + n_kv:], pages, table, lengths, starts=starts, q=x[:, :nh], freqs=freqs, q_norm=w, k_norm=w)
+        got = K.kv4_attn(q, pages, table, lengths, starts=starts)
+        q2, k2 = K.qk_norm_rope(x[:, :nh], x[:, nh:nh + n_kv], w, w, torch.arange(at, at + rows, device=DEV), freqs)
+        assert torch.allclose(q, q2, rtol=2.0 ** -18, atol=2.0 ** -18)
+        k, v = K.kv4_read(pages, table, lengths + rows, at + rows)
+        want = K.prefill_attn(q, k[0].contiguous(), v[0].contiguous(), pos0=at)
+        assert float((got.view(rows, -1) - want).abs().max()) < 4 * 2.0 ** -10
+        # a code is off by one scale at most, at 5 (kept as 4) of a block whose largest is 5 at least; by a half at most below
+        # 4, of a block whose largest is beyond 3.5; by one beyond 6, at 7: a fifth of the largest, 2^-18 for k2's own rounding
+        top = k2.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True).expand(-1, -1, -1, 32).flatten(-2)
+        assert bool(((k[0, :, at:].transpose(0, 1) - k2).abs() <= top * (0.2 + 2.0 ** -18)).all())
+        lengths += rows
+        at += rows
