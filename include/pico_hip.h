@@ -932,7 +932,7 @@ typedef struct pe_kv4_pool {
  * pe_qk_norm_rope; v is taken as it is. q_out gets the q rows of q's type. Keys are computed in 64 bits, so that what is
  * stored depends on no rounding before its own. A slot behind the table, or of a sequence of negative length (one that takes
  * no part), is not written; its q row is. Rows before starts[0] or from starts[batch] on are left out, their q_out rows
- * as they were. Two rows of a call must not go to one slot. tokens below 2^23, and below 2^24 over (n_head + 15) / 16 + (2 n_kv + 15) / 16;
+ * as they were. starts must not fall; where they do, some of the rows may be left out or be wrong, and nothing else is touched. Two rows of a call must not go to one slot. tokens below 2^23, and below 2^24 over (n_head + 15) / 16 + (2 n_kv + 15) / 16;
  * strides as in pe_qk_norm_rope (q_out may be q). */
 typedef struct pe_kv4_append_args {
     int type; /* of q, k, v: PE_TYPE_F32 or PE_TYPE_F16 */

@@ -150,6 +150,8 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             w.chunks = __builtin_amdgcn_readlane(chunks, at);
             w.base = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
             w.span = span;
+            // starts that are out of order can ask for more items than there are room for
+            if (w.base < 0 || w.base + (int64_t)w.blocks * w.chunks > p.items) return false;
             const int local = item - w.base;
             if (w.blocks == 1) {
                 w.chunk = local, w.block = 0;

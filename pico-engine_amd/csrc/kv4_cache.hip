@@ -227,7 +227,10 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     if (b < 0) return;
     int64_t len = uniform(int_at(p.lengths, p.len_wide, b));
     len = len > (1LL << 40) ? 1LL << 40 : len;
-    const int64_t slot = len + (p.starts ? t - uniform(int_at(p.starts, p.starts_wide, b)) : 0);
+    int64_t lo = p.starts ? uniform(int_at(p.starts, p.starts_wide, b)) : t;
+    lo = lo < 0 ? 0 : lo;
+    if (t < lo) return;  // starts that are out of order
+    const int64_t slot = len + (t - lo);
     if (isq) {
         SinCos* turn32 = reinterpret_cast<SinCos*>(turn);
         if (p.freqs) {

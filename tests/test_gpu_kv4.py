@@ -373,6 +373,29 @@ def test_attn_far_pages(K):
         assert torch.equal(a, b)
 
 
+def test_starts_out_of_order(K):
+    """They name rows twice or before their sequence begins: only pages of the table and rows of the output are written."""
+    nh, n_kv, hd, page, T = 4, 1, 64, 16, 64
+    for edges in ([0, 64, 0, 64, 0], [40, 0, 8, 64, 64], [64, 32, 0, 16, 8], [-(1 << 40), 1 << 40, -5, 70, 3]):
+        B = len(edges) - 1
+        pages, table = tables(K, B, n_kv, hd, page, 4096, 7, spare=64)
+        starts, lengths = torch.tensor(edges, device=DEV), torch.tensor([4000, 0, 3990, 30], device=DEV)
+        spare = torch.tensor(sorted(set(range(len(pages))) - set(table.flatten().tolist())), device=DEV)
+        before = pages[spare].clone()
+        k, q = rand(1, T, n_kv, hd), rand(2, T, nh, hd)
+        wide = torch.full((T + 2, nh, hd), 7.0, device=DEV)
+        K.kv4_append(k, k, pages, table, lengths, starts=starts, q=q, out=wide[1:-1])
+        assert torch.equal(pages[spare], before) and bool((wide[0] == 7).all() and (wide[-1] == 7).all())
+        R.fill(pages, 3)
+        for heads in (4, 48):  # in blocks of 16 rows and of 128
+            q = rand(2, T, heads, hd)
+            need = K.kv4_attn_workspace(T, B, heads, n_kv, hd, 4096, DEV, ragged=True).numel()
+            room = torch.full((need + 4096,), 77, device=DEV, dtype=torch.uint8)
+            wide = torch.full((T + 2, heads, hd), 7.0, device=DEV)
+            K.kv4_attn(q, pages, table, lengths, starts=starts, workspace=room[:need], out=wide[1:-1])
+            assert need and bool((room[need:] == 77).all() and (wide[0] == 7).all() and (wide[-1] == 7).all())
+
+
 def test_empty(K):
     pages, table = tables(K, 2, 2, 64, 16, 16, 1)
     none = torch.empty(0, device=DEV, dtype=torch.int64)
