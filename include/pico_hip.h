@@ -975,7 +975,7 @@ int pe_kv4_read(int type, const pe_kv4_pool* pool, const void* lengths, int leng
  * probabilities in 16 bits; sums and softmax statistics are fp32. Queries of 2^127 and more, infinite ones and NaN make their row NaN.
  * workspace: pe_kv4_attn_workspace_bytes(...) bytes (0: NULL will do), any contents; capacity = table_cols * page_tokens, ragged: starts
  * is given. Calls in order on one stream, and graphs replayed in order, may share it, calls that overlap must not. One
- * launch, or two where keys are cut. tokens up to 2^22, tokens times n_head below 2^26. */
+ * launch, or two where keys are cut. tokens up to 2^22, tokens times n_head up to 2^26 - 4. */
 typedef struct pe_kv4_attn_args {
     int type;
     const void* q;

@@ -986,7 +986,7 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
         (ragged && !aligned(a->starts, a->starts_dtype == 2 ? 8 : 4)) || !aligned(a->workspace, 16))
         return PE_ERR_ALIGN;
     if (a->workspace_bytes < need) return PE_ERR_SPACE;
-    if ((s.items + 7) * a->n_kv >= (1 << 24) || T * a->n_head >= (1LL << 26)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    if ((s.items + 7) * a->n_kv >= (1 << 24) || T * a->n_head > (1LL << 26) - 4) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
     const int piece = (int)(16 / e);
     const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
     // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores;

@@ -121,6 +121,16 @@ def test_attn(lib):
         assert size(*args) == -3, args
 
 
+def test_attn_most_rows(lib):
+    """2^26 - 1 rows of heads: the join's grid of four rows a workgroup would be 2^32 threads."""
+    from pico_hip._lib import Kv4AttnArgs
+    d = dict(type=1, q=F, q_token=2731 * 64, q_head=64, out=F, out_token=2731 * 64, out_head=64, lengths=F, lengths_dtype=2, first=1,
+             starts=F, starts_dtype=1, tokens=24573, batch=3, n_head=2731, n_kv=1, head_dim=64, scale=0.125, workspace=F,
+             workspace_bytes=1 << 50, pool=pool(table_cols=300))
+    assert 24573 * 2731 == (1 << 26) - 1
+    assert call_of(lib.pe_kv4_attn, Kv4AttnArgs, d)() == 3
+
+
 def test_public_names():
     from pico_hip import kernels
     names = {"qk_norm_rope", "kv4_pages", "kv4_append", "kv4_read", "kv4_attn", "kv4_attn_workspace"}
