@@ -1898,21 +1898,28 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor | None = None, len
 
 # ---- a paged cache held in 4 bits -------------------------------------------------------------
 
-def _heads(t: torch.Tensor, T: int, n: int, hd: int, dtype: torch.dtype, what: str) -> tuple[int, int]:
-    """(token, head) strides of rows of heads (T, n, hd) whose last dim is contiguous; 0 where there is one of them."""
+def _heads(t: torch.Tensor, T: int, n: int, hd: int, dtype: torch.dtype, what: str, copy: bool = False) -> tuple[torch.Tensor, int, int]:
+    """Rows of heads (T, n, hd) whose last dim is contiguous, with their token and head strides (0 where there is one of them);
+    ``copy``: an input, copied if its last dim is not."""
+    if t.dtype is not dtype or t.shape != (T, n, hd):
+        raise ValueError(f"{what} must be a {dtype} ({T}, {n}, {hd}) tensor, not {t.dtype} {tuple(t.shape)}")
     s = t.stride()
-    if t.dtype is not dtype or t.shape != (T, n, hd) or (s[2] != 1 and hd > 1):
-        raise ValueError(f"{what} must be a {dtype} ({T}, {n}, {hd}) tensor whose last dim is contiguous")
-    return s[0] if T > 1 else 0, s[1] if n > 1 else 0
+    if s[2] != 1 and hd > 1:
+        if not copy:
+            raise ValueError(f"{what}'s last dim must be contiguous")
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[0] if T > 1 else 0, s[1] if n > 1 else 0
 
 
-def _weight(w: torch.Tensor | None, n: int, hd: int, what: str) -> tuple[int | None, int]:
-    """The pointer and head stride of a norm's weight: (hd,) for all heads or (n, hd)."""
+def _weight(w: torch.Tensor | None, hd: int, what: str, n: int | None = None) -> tuple[int | None, int]:
+    """The pointer and head stride of a norm's weight: (hd,) for all heads or, given n, (n, hd)."""
     if w is None:
         return None, 0
-    if w.dtype is not torch.float32 or tuple(w.shape) not in ((hd,), (n, hd)) or not w.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous float32 ({hd},) or ({n}, {hd}) tensor")
-    return w.data_ptr(), 0 if w.dim() == 1 else hd
+    shape = w.shape
+    if w.dtype is not torch.float32 or (shape != (hd,) and shape != (n, hd)) or not w.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous float32 ({hd},) {'' if n is None else f'or ({n}, {hd}) '}tensor")
+    return w.data_ptr(), 0 if len(shape) == 1 else hd
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -1930,26 +1937,26 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     T, n, hd = q.shape
     rot = _check_freqs(freqs, hd)
     pos = _ints(positions, T, "positions")
+    m = 0 if k is None else k.shape[1]
     if out is None:
-        out = (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
+        out = q.new_empty(T, n, hd), None if k is None else q.new_empty(T, m, hd)
     elif (out[1] is None) != (k is None):
         raise ValueError("out must hold an output for q and one for k, or None where k is")
+    yq, yk = out
     a = QkNormArgs()
     a.type, a.positions, a.pos_dtype, a.freqs, a.rot_dim = code, positions.data_ptr(), pos, freqs.data_ptr(), rot
     a.amp, a.interleaved, a.eps, a.tokens, a.n_head, a.head_dim = float(amp), int(interleaved), float(eps), T, n, hd
-    if hd > 1 and q.stride(2) != 1:
-        q = q.contiguous()
-    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, T, n, hd, q.dtype, "q")
-    a.q_out, (a.q_out_token, a.q_out_head) = out[0].data_ptr(), _heads(out[0], T, n, hd, q.dtype, "out's q")
-    a.q_weight, a.q_weight_head = _weight(q_weight, n, hd, "q_weight")
+    dtype = q.dtype
+    q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
+    _, a.q_out_token, a.q_out_head = _heads(yq, T, n, hd, dtype, "out's q")
+    a.q, a.q_out = q.data_ptr(), yq.data_ptr()
+    a.q_weight, a.q_weight_head = _weight(q_weight, hd, "q_weight", n)
     if k is not None:
-        m = k.shape[1]
-        if hd > 1 and k.stride(2) != 1:
-            k = k.contiguous()
-        a.n_kv, a.k, (a.k_token, a.k_head) = m, k.data_ptr(), _heads(k, T, m, hd, q.dtype, "k")
-        a.k_out, (a.k_out_token, a.k_out_head) = out[1].data_ptr(), _heads(out[1], T, m, hd, q.dtype, "out's k")
-        a.k_weight, a.k_weight_head = _weight(k_weight, m, hd, "k_weight")
-    if T and (n or a.n_kv):
+        k, a.k_token, a.k_head = _heads(k, T, m, hd, dtype, "k", copy=True)
+        _, a.k_out_token, a.k_out_head = _heads(yk, T, m, hd, dtype, "out's k")
+        a.n_kv, a.k, a.k_out = m, k.data_ptr(), yk.data_ptr()
+        a.k_weight, a.k_weight_head = _weight(k_weight, hd, "k_weight", m)
+    if T and (n or m):
         _launch(dev, "pe_qk_norm_rope", ctypes.byref(a))
     return out
 
@@ -2007,31 +2014,25 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: tor
     T = k.shape[0]
     a = Kv4AppendArgs()
     a.type, a.pool, a.tokens, a.batch, a.n_kv, a.head_dim, a.eps = code, pool, T, B, n_kv, hd, float(eps)
-    if k.stride(2) != 1:
-        k = k.contiguous()
-    if v.dim() == 3 and v.stride(2) != 1:
-        v = v.contiguous()
-    a.k, (a.k_token, a.k_head) = k.data_ptr(), _heads(k, T, n_kv, hd, k.dtype, "k")
-    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, T, n_kv, hd, k.dtype, "v")
+    dtype = k.dtype
+    k, a.k_token, a.k_head = _heads(k, T, n_kv, hd, dtype, "k", copy=True)
+    v, a.v_token, a.v_head = _heads(v, T, n_kv, hd, dtype, "v", copy=True)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
     a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
     a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
     if freqs is not None:
         a.freqs, a.rot_dim, a.amp, a.interleaved = freqs.data_ptr(), _check_freqs(freqs, hd), float(amp), int(interleaved)
-    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None and (w.dtype is not torch.float32 or tuple(w.shape) != (hd,) or not w.is_contiguous()):
-            raise ValueError(f"{what} must be a contiguous float32 ({hd},) tensor")
-    a.k_weight = None if k_norm is None else k_norm.data_ptr()
+    a.k_weight, _ = _weight(k_norm, hd, "k_norm")
     if q is not None:
         if q.dim() != 3 or q.shape[1] == 0:
-            raise ValueError(f"q must be a {k.dtype} ({T}, n_head, {hd}) tensor")
+            raise ValueError(f"q must be a {dtype} ({T}, n_head, {hd}) tensor")
         n = q.shape[1]
-        if q.stride(2) != 1:
-            q = q.contiguous()
         if out is None:
-            out = q.new_empty((T, n, hd))
-        a.n_head, a.q, (a.q_token, a.q_head) = n, q.data_ptr(), _heads(q, T, n, hd, k.dtype, "q")
-        a.q_out, (a.q_out_token, a.q_out_head) = out.data_ptr(), _heads(out, T, n, hd, k.dtype, "out")
-        a.q_weight = None if q_norm is None else q_norm.data_ptr()
+            out = q.new_empty(T, n, hd)
+        q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
+        _, a.q_out_token, a.q_out_head = _heads(out, T, n, hd, dtype, "out")
+        a.n_head, a.q, a.q_out = n, q.data_ptr(), out.data_ptr()
+        a.q_weight, _ = _weight(q_norm, hd, "q_norm")
     elif out is not None or q_norm is not None:
         raise ValueError("out and q_norm go with q")
     if T and B:
@@ -2086,19 +2087,20 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
     if code is None or q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % n_kv or q.shape[2] != hd:
         raise ValueError(f"q must be a float32 or float16 (T, n_head, {hd}) tensor, n_head a multiple of {n_kv}")
     T, n, _ = q.shape
-    if q.stride(2) != 1:
-        q = q.contiguous()
+    dtype = q.dtype
     a = Kv4AttnArgs()
     a.type, a.pool, a.tokens, a.batch, a.n_head, a.n_kv, a.head_dim, a.first = code, pool, T, B, n, n_kv, hd, int(first)
-    a.q, (a.q_token, a.q_head) = q.data_ptr(), _heads(q, T, n, hd, q.dtype, "q")
+    q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
+    a.q = q.data_ptr()
     a.lengths, a.lengths_dtype = lengths.data_ptr(), _ints(lengths, B, "lengths")
     a.starts, a.starts_dtype = _kv4_rows(starts, T, B)
     a.scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(a.scale):
         raise ValueError(f"scale {scale}")
     if out is None:
-        out = q.new_empty((T, n, hd))
-    a.out, (a.out_token, a.out_head) = out.data_ptr(), _heads(out, T, n, hd, q.dtype, "out")
+        out = q.new_empty(T, n, hd)
+    _, a.out_token, a.out_head = _heads(out, T, n, hd, dtype, "out")
+    a.out = out.data_ptr()
     if T == 0 or B == 0:
         return out
     need = _kv4_bytes(T, B, starts is not None, n, n_kv, hd, pool.table_cols * pool.page_tokens)
