@@ -532,12 +532,12 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
         p.plan[w.b] = make_int4(w.base, w.chunks, w.blocks, 0);
 }
 
-// Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32 keys in turn, each with a
-// state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x 16384 keys of 8 heads of
-// 128, fp16: 135 us, 4.3 TB/s), else the start's chain of loads (lengths, queries, table, keys), about 4 us of a
-// workgroup's time (28 heads of 128 on 33 x 4001 keys, fp32: 21 us with the join, 7.4 at the copy rate). Three and four
-// waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of 64 keys, two waves, 145 us;
-// with a second step in registers 150.
+// Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32
+// keys in turn, each with a state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x
+// 16384 keys of 8 heads of 128, fp16: 136 to 143 us with the join, 4.1 to 4.3 TB/s), else the start's chain of loads (lengths,
+// queries, table, keys), about 4 us of a workgroup's time (28 heads of 128 on 33 x 4001 keys, fp32: 22 us with the join, 7.4 at
+// the copy rate). Three and four waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of
+// 64 keys, two waves, 145 us where this is 135; with a second step in registers 150.
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16, TS = 2;

@@ -51,7 +51,8 @@ PE_DEV void load_weights(const float* w, float* v) {
     }
 }
 
-// A group of W lanes holds a head, a lane NI pieces of V pairs or of 2 V elements that stay.
+// A group of W lanes holds a head, a lane NI pieces of V pairs or of 2 V elements that stay. Bound by memory: 8191 x 40 heads
+// of 128, fp16, 168 MB, 38 us, 4.4 TB/s (45.8 us without the next head under way); one token 3.1 us, the launch and its loads.
 template <typename T, int V, bool IL, int W, int NI>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(QkNormArgs p) {
     const int turn = (p.half + V - 1) / V, per = turn + (p.hd - 2 * p.half + 2 * V - 1) / (2 * V);
