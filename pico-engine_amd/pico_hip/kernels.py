@@ -1930,31 +1930,32 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     positions[t] as in rope_positions. Weights float32, (hd,) or one row a head, None: not normed; k None: q alone. ``out``:
     the two outputs, which may be q and k, and share no memory with them otherwise. Returns (q, k)."""
     dev = _one_gpu(q, k, q_weight, k_weight, positions, freqs, *(out or ()))
-    code = _CACHE_TYPE.get(q.dtype)
-    if code is None or q.dim() != 3 or (k is not None and (k.dim() != 3 or k.dtype is not q.dtype or
-                                                           (k.shape[0], k.shape[2]) != (q.shape[0], q.shape[2]))):
+    dtype, shape = q.dtype, q.shape
+    code = _CACHE_TYPE.get(dtype)
+    if code is None or len(shape) != 3 or (k is not None and k.dim() != 3):
         raise ValueError("q and k must be float32 or float16 (T, n_head, hd) and (T, n_kv, hd) tensors of one type")
-    T, n, hd = q.shape
+    T, n, hd = shape
     rot = _check_freqs(freqs, hd)
     pos = _ints(positions, T, "positions")
     m = 0 if k is None else k.shape[1]
+    a = QkNormArgs()
     if out is None:
         out = q.new_empty(T, n, hd), None if k is None else q.new_empty(T, m, hd)
-    elif (out[1] is None) != (k is None):
-        raise ValueError("out must hold an output for q and one for k, or None where k is")
-    yq, yk = out
-    a = QkNormArgs()
+        a.q_out_token, a.q_out_head, a.k_out_token, a.k_out_head = n * hd, hd, m * hd, hd
+    else:
+        if (out[1] is None) != (k is None):
+            raise ValueError("out must hold an output for q and one for k, or None where k is")
+        _, a.q_out_token, a.q_out_head = _heads(out[0], T, n, hd, dtype, "out's q")
+        if k is not None:
+            _, a.k_out_token, a.k_out_head = _heads(out[1], T, m, hd, dtype, "out's k")
     a.type, a.positions, a.pos_dtype, a.freqs, a.rot_dim = code, positions.data_ptr(), pos, freqs.data_ptr(), rot
     a.amp, a.interleaved, a.eps, a.tokens, a.n_head, a.head_dim = float(amp), int(interleaved), float(eps), T, n, hd
-    dtype = q.dtype
     q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
-    _, a.q_out_token, a.q_out_head = _heads(yq, T, n, hd, dtype, "out's q")
-    a.q, a.q_out = q.data_ptr(), yq.data_ptr()
+    a.q, a.q_out = q.data_ptr(), out[0].data_ptr()
     a.q_weight, a.q_weight_head = _weight(q_weight, hd, "q_weight", n)
     if k is not None:
         k, a.k_token, a.k_head = _heads(k, T, m, hd, dtype, "k", copy=True)
-        _, a.k_out_token, a.k_out_head = _heads(yk, T, m, hd, dtype, "out's k")
-        a.n_kv, a.k, a.k_out = m, k.data_ptr(), yk.data_ptr()
+        a.n_kv, a.k, a.k_out = m, k.data_ptr(), out[1].data_ptr()
         a.k_weight, a.k_weight_head = _weight(k_weight, hd, "k_weight", m)
     if T and (n or m):
         _launch(dev, "pe_qk_norm_rope", ctypes.byref(a))
@@ -2027,10 +2028,12 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: tor
         if q.dim() != 3 or q.shape[1] == 0:
             raise ValueError(f"q must be a {dtype} ({T}, n_head, {hd}) tensor")
         n = q.shape[1]
+        q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
         if out is None:
             out = q.new_empty(T, n, hd)
-        q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
-        _, a.q_out_token, a.q_out_head = _heads(out, T, n, hd, dtype, "out")
+            a.q_out_token, a.q_out_head = n * hd, hd
+        else:
+            _, a.q_out_token, a.q_out_head = _heads(out, T, n, hd, dtype, "out")
         a.n_head, a.q, a.q_out = n, q.data_ptr(), out.data_ptr()
         a.q_weight, _ = _weight(q_norm, hd, "q_norm")
     elif out is not None or q_norm is not None:
@@ -2083,11 +2086,11 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
     B = lengths.shape[0] if lengths.dim() == 1 else -1
     dev = _one_gpu(q, pages, table, lengths, starts, workspace, out)
     pool, n_kv, hd = _kv4_pool(pages, table, B)
-    code = _CACHE_TYPE.get(q.dtype)
-    if code is None or q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % n_kv or q.shape[2] != hd:
+    dtype, shape = q.dtype, q.shape
+    code = _CACHE_TYPE.get(dtype)
+    if code is None or len(shape) != 3 or shape[1] == 0 or shape[1] % n_kv:
         raise ValueError(f"q must be a float32 or float16 (T, n_head, {hd}) tensor, n_head a multiple of {n_kv}")
-    T, n, _ = q.shape
-    dtype = q.dtype
+    T, n, _ = shape
     a = Kv4AttnArgs()
     a.type, a.pool, a.tokens, a.batch, a.n_head, a.n_kv, a.head_dim, a.first = code, pool, T, B, n, n_kv, hd, int(first)
     q, a.q_token, a.q_head = _heads(q, T, n, hd, dtype, "q", copy=True)
@@ -2099,7 +2102,9 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
         raise ValueError(f"scale {scale}")
     if out is None:
         out = q.new_empty(T, n, hd)
-    _, a.out_token, a.out_head = _heads(out, T, n, hd, dtype, "out")
+        a.out_token, a.out_head = n * hd, hd
+    else:
+        _, a.out_token, a.out_head = _heads(out, T, n, hd, dtype, "out")
     a.out = out.data_ptr()
     if T == 0 or B == 0:
         return out
