@@ -134,6 +134,12 @@ PE_DEV int64_t uniform(int64_t v) {
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+// The value that lane `at` holds.
+PE_DEV int64_t lane_of(int64_t v, int at) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, at), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), at);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // A lane's run of E elements from channel `at` on (own), and of what each is turned with (other).
 template <typename T, int E, bool VEC>
 PE_DEV void load_pairs(const T* x, int at, int rot, int half, float* own, float* other) {
@@ -201,8 +207,8 @@ PE_DEV void turn_run(const Kv4AppendArgs& p, const float* own, const float* othe
 // A workgroup takes 16 heads of a token, of q or of k and v, 16 lanes each, a lane a run of HD / 16 elements. The
 // elements that a rotated one is made with are loaded beside it (they are in the same cache lines), so that a
 // lane holds a whole run of codes whatever the pairs are. The token's sines are made once, in LDS. VEC: the lanes'
-// runs are aligned in q, k, v and q_out, and so are their partners'. 4101 rows of 32 + 2 x 8 heads of 128, fp16, take 26.4 us,
-// 17 at the copy rate: 12300 workgroups of about 4 us each, their loads one behind the other (sequence, length, page), eight a CU.
+// runs are aligned in q, k, v and q_out, and so are their partners'. 4101 rows of 32 + 2 x 8 heads of 128, fp16, take 24.4 us,
+// 17 at the copy rate: 12300 workgroups of about 4 us each, loads one behind the other (sequence, page), eight a CU.
 template <typename T, int HD, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     constexpr int E = HD / 16;
@@ -217,18 +223,35 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4AppendArgs p) {
     const int h = (isq ? blockIdx.y : blockIdx.y - p.q_parts) * 16 + group;
     const bool isv = !isq && h >= p.n_kv, active = h < (isq ? p.n_head : 2 * p.n_kv);
     const int hh = isv ? h - p.n_kv : h, rot = p.freqs && !p.interleaved && !isv ? 2 * p.half : 0;
+    // first what the rest waits for: where every sequence begins and what it holds, one a lane, if there are few (26.4 ->
+    // 24.4 us against looking for the sequence, then for its length, behind the rows' loads)
+    const int wl = threadIdx.x & 63;
+    const bool few = p.starts && p.batch < kWave;
+    int64_t start = 0, held = 0;
+    if (few && wl <= p.batch) {
+        start = int_at(p.starts, p.starts_wide, wl);
+        held = int_at(p.lengths, p.len_wide, wl < p.batch ? wl : 0);
+    }
+    const double freq = p.freqs && (int)threadIdx.x < p.half ? p.freqs[threadIdx.x] * 0.63661977236758134 : 0;
     float own[E] = {}, other[E] = {};
     if (active) {
         const T* x = static_cast<const T*>(isq ? p.q : isv ? p.v : p.k) + t * (isq ? p.q_token : isv ? p.v_token : p.k_token) +
                      hh * (isq ? p.q_head : isv ? p.v_head : p.k_head);
         load_pairs<T, E, VEC>(x, at, rot, p.half, own, other);
     }
-    const double freq = p.freqs && (int)threadIdx.x < p.half ? p.freqs[threadIdx.x] * 0.63661977236758134 : 0;
-    const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
-    if (b < 0) return;
-    int64_t len = uniform(int_at(p.lengths, p.len_wide, b));
+    int64_t b, len, lo;
+    if (few) {
+        b = __popcll(__ballot(wl <= p.batch && start <= t)) - 1;
+        if (b < 0 || b >= p.batch) return;
+        len = lane_of(held, (int)b);
+        lo = lane_of(start, (int)b);
+    } else {
+        b = sequence_of(p.starts, p.starts_wide, p.batch, t);
+        if (b < 0) return;
+        len = uniform(int_at(p.lengths, p.len_wide, b));
+        lo = p.starts ? uniform(int_at(p.starts, p.starts_wide, b)) : t;
+    }
     len = len > (1LL << 40) ? 1LL << 40 : len;
-    int64_t lo = p.starts ? uniform(int_at(p.starts, p.starts_wide, b)) : t;
     lo = lo < 0 ? 0 : lo;
     if (t < lo) return;  // starts that are out of order
     const int64_t slot = len + (t - lo);
