@@ -25,6 +25,18 @@ PE_DEV int64_t int_at(const void* p, int wide, int64_t i) {
     return wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int*>(p)[i];
 }
 
+// A value that all lanes hold, in scalar registers: what follows from it is then computed once a wave.
+PE_DEV int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The value that lane `at` holds.
+PE_DEV int64_t lane_of(int64_t v, int at) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, at), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), at);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Rows [lo, hi) of sequence b: one each where starts is NULL; clamped to the rows there are.
 PE_DEV void rows_of(const void* starts, int wide, int64_t b, int64_t tokens, int64_t& lo, int64_t& hi) {
     if (!starts) {

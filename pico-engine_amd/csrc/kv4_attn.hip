@@ -92,6 +92,7 @@ PE_DEV int wave_scan(int v) {
 
 struct Kv4Item {
     int b, block, chunk, chunks, blocks, base, span;  // span: keys of a chunk
+    Kv4Seq seq;
 };
 
 // Which work the item is: a (sequence, row block, chunk of keys). Every wave finds it for itself, from all lengths.
@@ -103,22 +104,23 @@ struct Kv4Item {
 template <int RB>
 PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
     const int lane = threadIdx.x & 63;
-    const auto look = [&](int b, int& nb, int& keys) {  // row blocks, keys of the last row
+    const auto look = [&](int b, Kv4Seq& s, int& nb, int& keys) {  // the sequence, its row blocks, keys of the last row
         nb = keys = 0;
         if (b >= p.batch) return;
-        const Kv4Seq s = kv4_seq(p, b);
+        s = kv4_seq(p, b);
         nb = (s.rows + RB - 1) / RB;
         if (nb) keys = kv4_keys(p, s.keys, s.rows / p.group - 1);
     };
     const auto chunks_of = [](int keys, int span) { return keys > span ? (int)((uint32_t)(keys + span - 1) / (uint32_t)span) : 1; };
+    Kv4Seq seq0{}, seq;
     int nb0, keys0;
-    look(lane, nb0, keys0);
+    look(lane, seq0, nb0, keys0);
     int span = 1 << 30;
     if (p.items > p.blocks) {
         int64_t cost = (int64_t)nb0 * keys0;
         for (int b = lane + 64; b < p.batch; b += 64) {
             int nb, keys;
-            look(b, nb, keys);
+            look(b, seq, nb, keys);
             cost += (int64_t)nb * keys;
         }
         const float all = wave_sum<64>((float)cost);
@@ -126,7 +128,7 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
         float count = (float)nb0 * (float)chunks_of(keys0, span);
         for (int b = lane + 64; b < p.batch; b += 64) {
             int nb, keys;
-            look(b, nb, keys);
+            look(b, seq, nb, keys);
             count += (float)nb * (float)chunks_of(keys, span);
         }
         // Up to 1.6 rounds of what is resident at once are made one, of longer chunks (5 rows on 80000 keys, 32 heads of
@@ -146,13 +148,15 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
     int base = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
         int nb = nb0, keys = keys0;
-        if (b0) look(b0 + lane, nb, keys);
+        seq = seq0;
+        if (b0) look(b0 + lane, seq, nb, keys);
         const int chunks = chunks_of(keys, span);
         const int upto = wave_scan(nb * chunks);
         const uint64_t beyond = __ballot(base + upto > item);
         if (beyond) {
             const int at = __builtin_ctzll(beyond);
             w.b = b0 + at;
+            w.seq = {lane_of(seq.lo, at), __builtin_amdgcn_readlane(seq.rows, at), lane_of(seq.keys, at)};
             w.blocks = __builtin_amdgcn_readlane(nb, at);
             w.chunks = __builtin_amdgcn_readlane(chunks, at);
             w.base = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     const int kvh = blockIdx.y;
     Kv4Item w;
     if (!kv4_find<R>(p, blockIdx.x, w)) return;
-    const Kv4Seq seq = kv4_seq(p, w.b);
+    const Kv4Seq& seq = w.seq;
     kv4_tell(p, w, kvh);
     const int r0 = w.block * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
     const int least = kv4_keys(p, seq.keys, r0 / p.group), most = kv4_keys(p, seq.keys, last / p.group);
@@ -656,7 +660,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
     const int kvh = blockIdx.y;
     Kv4Item w;
     if (!kv4_find<RB>(p, blockIdx.x, w)) return;
-    const Kv4Seq seq = kv4_seq(p, w.b);
+    const Kv4Seq& seq = w.seq;
     kv4_tell(p, w, kvh);
     // the workgroup's rows, and the wave's (it has none: it converts alone)
     const int b0 = w.block * RB, b1 = (b0 + RB < seq.rows ? b0 + RB : seq.rows) - 1;
@@ -838,11 +842,24 @@ __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
     int chunks = 0, r = 0;
     int64_t first = 0;
     if (t < p.tokens) {
-        const int64_t b = sequence_of(p.starts, p.starts_wide, p.batch, t);
+        int64_t b, lo = t;
+        int4 plan;
+        if (p.starts && p.batch < kWave) {  // few sequences: all of them at once (2 x 1021 rows: 32.3 -> 29.9 us, 5 rows 5.4 -> 5.2)
+            const int64_t start = lane <= p.batch ? int_at(p.starts, p.starts_wide, lane) : 0;
+            const int4 all = p.plan[lane < p.batch ? lane : 0];
+            b = __popcll(__ballot(lane <= p.batch && start <= t)) - 1;
+            b = b < p.batch ? b : -1;
+            const int at = b < 0 ? 0 : (int)b;
+            lo = lane_of(start, at);
+            plan = make_int4(__builtin_amdgcn_readlane(all.x, at), __builtin_amdgcn_readlane(all.y, at),
+                             __builtin_amdgcn_readlane(all.z, at), 0);
+        } else {
+            b = sequence_of(p.starts, p.starts_wide, p.batch, t);
+            plan = p.plan[b < 0 ? 0 : b];
+            if (p.starts) lo = uniform(int_at(p.starts, p.starts_wide, b < 0 ? 0 : b));
+        }
+        lo = lo < 0 ? 0 : lo;
         if (b >= 0) {
-            const int4 plan = p.plan[b];
-            int64_t lo, hi;
-            rows_of(p.starts, p.starts_wide, b, p.tokens, lo, hi);
             const int kvh = h / p.group;
             r = (int)(t - lo) * p.group + h - kvh * p.group;
             // (a plan that no workgroup wrote, of starts that are out of order, holds anything)
@@ -901,7 +918,7 @@ struct Kv4Plan {
     float weight;  // of all keys in the square of a chunk's length
 };
 
-static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, int n_kv, int hd, int64_t capacity) {
+static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, int n_kv, int hd, int64_t capacity, bool half) {
     Kv4Plan s;
     const int group = n_head / n_kv;
     const int64_t rows = ragged ? (tokens + batch - 1) / batch * group : group;  // of a sequence, on average
@@ -913,7 +930,9 @@ static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, 
     s.blocks = ragged ? tokens * group / s.rb + batch : batch * ((group + s.rb - 1) / s.rb);
     s.min_chunk = 64 * (s.split ? kKv4Waves : 4);
     s.rec_rows = ragged || group > s.rb ? s.rb : group;
-    s.weight = 0.75f * (float)n_kv;
+    // fp32 queries of 128 channels take longer over a key (33 x 4001 keys: 23.7 us with 0.75, 22.4 so; 64 x 4096 48.9 and 48.8;
+    // 8 x 8000 18.1 and 17.5); the other kinds lose by shorter chunks (64 x 16384 fp16 137 -> 138, 4 rows on 8 x 4000 18.4 -> 20.8)
+    s.weight = (s.split && !half && hd == 128 ? 0.5f : 0.75f) * (float)n_kv;
     // the most workgroups that a chunk's length makes of any lengths, within reason
     const int64_t chunks = (capacity + s.min_chunk - 1) / s.min_chunk;
     int64_t extra = (int64_t)sqrt((double)s.blocks * (double)capacity / s.weight) + 1;
@@ -967,7 +986,7 @@ using namespace pe;
 extern "C" int64_t pe_kv4_attn_workspace_bytes(int64_t tokens, int64_t batch, int ragged, int n_head, int n_kv, int head_dim,
                                                int64_t capacity) {
     if (!kv4_shape_ok(tokens, batch, ragged, n_head, n_kv, head_dim, capacity)) return -PE_ERR_SHAPE;
-    return kv4_bytes(kv4_plan(tokens, batch, ragged, n_head, n_kv, head_dim, capacity), batch, n_kv, head_dim);
+    return kv4_bytes(kv4_plan(tokens, batch, ragged, n_head, n_kv, head_dim, capacity, false), batch, n_kv, head_dim);
 }
 
 extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
@@ -978,14 +997,14 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
     if (a->tokens == 0 || a->batch == 0) return PE_OK;
     if (const int st = kv4_pool_ok(&a->pool, a->n_kv, a->head_dim)) return st;
     const int64_t T = a->tokens, capacity = a->pool.table_cols * a->pool.page_tokens;
-    const bool ragged = a->starts != nullptr;
+    const bool ragged = a->starts != nullptr, half = a->type == PE_TYPE_F16;
     if (!kv4_shape_ok(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity) || !std::isfinite(a->scale * kKv4Log2e) ||
         a->first < -(1LL << 40) || a->first > (1LL << 40) || a->q_token < 0 || a->q_head < 0 || a->out_token < 0 || a->out_head < 0 ||
         (a->n_head > 1 && a->out_head < a->head_dim) || (T > 1 && a->out_token < a->head_dim) ||
         (T > 1 && a->n_head > 1 && a->out_token < a->out_head * (a->n_head - 1) + a->head_dim &&
          a->out_head < a->out_token * (T - 1) + a->head_dim))
         return PE_ERR_SHAPE;
-    const Kv4Plan s = kv4_plan(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity);
+    const Kv4Plan s = kv4_plan(T, a->batch, ragged, a->n_head, a->n_kv, a->head_dim, capacity, half);
     const int64_t need = kv4_bytes(s, a->batch, a->n_kv, a->head_dim);
     if (!a->q || !a->out || !a->lengths || (need && !a->workspace)) return PE_ERR_NULL;
     const size_t e = a->type == PE_TYPE_F16 ? 2 : 4;
@@ -998,10 +1017,9 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
     const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
     // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores;
     // fp16 ones only turned by its sign, so that their parts stay exact
-    const bool half = a->type == PE_TYPE_F16;
     const float scale = half && a->scale != 0 ? std::fabs(a->scale) * kKv4Log2e : 1.f;
     const double q_scale = half ? (a->scale > 0) - (a->scale < 0) : (double)a->scale * 1.4426950408889634;
-    const float round = (s.split ? half || a->head_dim == 64 ? 4 : 3 : 2) * 256.f / (float)a->n_kv;
+    const float round = (s.split ? 4 : 2) * 256.f / (float)a->n_kv;
     int4* plan = need ? static_cast<int4*>(a->workspace) : nullptr;
     float* record = need ? reinterpret_cast<float*>(plan + a->batch) : nullptr;
     Kv4AttnArgs p{a->q, a->q_token, a->q_head, a->out, a->out_token, a->out_head, static_cast<const uint8_t*>(a->pool.pages),

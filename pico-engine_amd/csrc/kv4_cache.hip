@@ -128,18 +128,6 @@ PE_DEV uint32_t encode(const uint32_t* y, uint32_t& scale) {
     return codes;
 }
 
-// A value that all lanes hold, in scalar registers: what follows from it is then computed once a wave.
-PE_DEV int64_t uniform(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-// The value that lane `at` holds.
-PE_DEV int64_t lane_of(int64_t v, int at) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, at), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), at);
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
 // A lane's run of E elements from channel `at` on (own), and of what each is turned with (other).
 template <typename T, int E, bool VEC>
 PE_DEV void load_pairs(const T* x, int at, int rot, int half, float* own, float* other) {

@@ -373,6 +373,33 @@ def test_attn_far_pages(K):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("B", [1, 62, 63, 64, 65, 129])
+def test_ragged_around_a_wave(K, B):
+    """As many sequences as a wave finds at once, one fewer and more: rows before the first and behind the last stay as they
+    were, sequences without rows, two chunks and more to join."""
+    nh, n_kv, hd, page = 8, 1, 64, 16
+    sizes = [(b * 7 + 3) % 4 if b else 2 for b in range(B)]
+    pages, table = tables(K, B, n_kv, hd, page, 1600, 7, spare=0)
+    lengths = torch.randint(0, 1590, (B,), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    starts = torch.tensor([2 + sum(sizes[:b]) for b in range(B + 1)], device=DEV)
+    T = int(starts[-1]) + 3
+    q, k, v = rand(2, T, nh, hd) * 0.5, rand(3, T, n_kv, hd), rand(4, T, n_kv, hd)
+    out = torch.full_like(q, 7.0)
+    K.kv4_attn(q, pages, table, lengths, starts=starts, out=out)
+    before = pages.clone()
+    turned = torch.full_like(q, 7.0)
+    K.kv4_append(k, v, pages, table, lengths, starts=starts, q=q, out=turned)
+    for y in (out, turned):
+        assert bool((y[:2] == 7).all() and (y[-3:] == 7).all())
+    assert torch.equal(turned[2:-3], q[2:-3])
+    some = sorted({b for b in (0, 1, B // 2, B - 3, B - 2, B - 1) if 0 <= b < B})
+    for b in some:
+        lo, hi = starts[b:b + 2].tolist()
+        if hi > lo:
+            close(out[lo:hi], before, table[b:b + 1], lengths[b:b + 1], q[lo:hi], starts=torch.tensor([0, hi - lo], device=DEV))
+    assert torch.equal(pages.cpu(), appended(before, table, lengths, starts, k, v, None, 1.0, False, None, 0))
+
+
 def test_starts_out_of_order(K):
     """They name rows twice or before their sequence begins: only pages of the table and rows of the output are written."""
     nh, n_kv, hd, page, T = 4, 1, 64, 16, 64
