@@ -540,7 +540,7 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
 // keys in turn, each with a state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x
 // 16384 keys of 8 heads of 128, fp16: 136 to 143 us with the join, 4.1 to 4.3 TB/s), else the start's chain of loads (lengths,
 // queries, table, keys), about 4 us of a workgroup's time (28 heads of 128 on 33 x 4001 keys, fp32: 22 us with the join, 7.4 at
-// the copy rate). Three and four waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of
+// the copy rate). Four waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of
 // 64 keys, two waves, 145 us where this is 135; with a second step in registers 150.
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
@@ -648,7 +648,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
 // Many rows (pieces of prompts): 32 rows a wave, 128 a workgroup, all on the same keys. The waves convert a step's codes
 // for one another, into LDS in the order of the products' operands, two steps deep; the queries are in registers. Bound by
 // the matrix cores and the vector instructions, which add up with two waves a SIMD (2 x 1021 rows of 28 heads of 128
-// on 8000 keys, fp16: 45 % and 54 % of the cycles, 330 us, the join of the chunks 34; the two parts of each factor alone are 273
+// on 8000 keys, fp16: 45 % and 54 % of the cycles, 330 us, the join of the chunks 30; the two parts of each factor alone are 273
 // at the rate of a large product). With every wave converting for itself 367 and, fp32, 588 us; so 360 and 490.
 template <typename T, int HD>
 constexpr int kKv4RowTiles = sizeof(T) == 4 && HD == 128 ? 2 : 4;  // 16 keys a step; fp32's queries take half the registers
