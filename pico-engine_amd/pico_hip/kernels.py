@@ -2081,7 +2081,8 @@ def kv4_attn(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lengths:
     float16, any row and head strides. Sequence b's rows are starts[b] .. starts[b + 1] - 1 (None: one each, T == B); its row
     i sees the first lengths[b] + first + i slots: with the lengths from before kv4_append's rows, all keys up to its own.
     A row that sees none, or of a sequence of negative length (one that takes no part), gets zeros; rows of no sequence are left as they
-    were. Keys and values are taken exactly as stored, float32 queries in 24 bits. Returns (T, n_head, hd) of q's type;
+    were. Keys and values are taken exactly as stored, float32 queries in 24 bits; sums are float32 (64 times that of the values'
+    magnitudes must stay in its range). Returns (T, n_head, hd) of q's type;
     ``out`` shares no memory with q."""
     B = lengths.shape[0] if lengths.dim() == 1 else -1
     dev = _one_gpu(q, pages, table, lengths, starts, workspace, out)
