@@ -1973,14 +1973,19 @@ def kv4_pages(n_pages: int, n_kv: int, hd: int, page_tokens: int, device) -> tor
 
 def _kv4_pool(pages: torch.Tensor, table: torch.Tensor, batch: int) -> tuple[Kv4Pool, int, int]:
     """The C view of a pool and its table, with n_kv and hd."""
-    shape, s, ts = pages.shape, pages.stride(), table.stride()
-    if pages.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in (17 * 64, 17 * 128) or shape[0] == 0 or \
-            s[1:] != (shape[2] * shape[3], shape[3], 1):
-        raise ValueError("pages must be a uint8 (n_pages, n_kv, page_tokens / 16, 17 hd) pool (kv4_pages), each page contiguous")
+    shape, there = pages.shape, table.shape
+    if pages.dtype is not torch.uint8 or len(shape) != 4:
+        raise ValueError("pages must be a uint8 (n_pages, n_kv, page_tokens / 16, 17 hd) pool (kv4_pages)")
     n, n_kv, tiles, tile = shape
-    cols = table.shape[-1] if len(ts) else 0
-    if table.dtype is not torch.int32 or table.shape != (batch, cols) or (cols > 1 and ts[1] != 1):
-        raise ValueError(f"table must hold int32 page numbers, ({batch}, pages of a sequence), its rows contiguous")
+    s = pages.stride()
+    if (tile != 17 * 64 and tile != 17 * 128) or n == 0 or s[3] != 1 or (tiles > 1 and s[2] != tile) or \
+            (n_kv > 1 and s[1] != tiles * tile):
+        raise ValueError("pages must hold pages of hd 64 or 128 (kv4_pages), each contiguous")
+    if table.dtype is not torch.int32 or len(there) != 2 or there[0] != batch:
+        raise ValueError(f"table must hold int32 page numbers, ({batch}, pages of a sequence)")
+    cols, ts = there[1], table.stride()
+    if cols > 1 and ts[1] != 1:
+        raise ValueError("the table's rows must be contiguous")
     return Kv4Pool(pages.data_ptr(), n, s[0] if n > 1 else n_kv * tiles * tile, 16 * tiles, table.data_ptr(),
                    ts[0] if batch > 1 else cols, cols), n_kv, tile // 17
 
@@ -2053,7 +2058,8 @@ def kv4_read(pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, ro
     if dtype not in _CACHE_TYPE or rows < 0:
         raise ValueError(f"{rows} rows of {dtype}: dtype must be float32 or float16")
     code = _ints(lengths, B, "lengths")
-    k, v = pages.new_empty((B, n_kv, rows, hd), dtype=dtype), pages.new_empty((B, n_kv, rows, hd), dtype=dtype)
+    k = pages.new_empty((B, n_kv, rows, hd), dtype=dtype)
+    v = torch.empty_like(k)
     if B and rows:
         _launch(dev, "pe_kv4_read", _CACHE_TYPE[dtype], ctypes.byref(pool), lengths.data_ptr(), code, B, n_kv, hd, int(rows),
                 k.data_ptr(), v.data_ptr())

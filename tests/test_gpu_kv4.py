@@ -350,6 +350,22 @@ def test_attn_strides(K, dtype):
                        want[:1].expand(B, nh, hd))
 
 
+def test_pages_of_one_head(K):
+    """Pools whose one kv head, or one tile, has a stride of any kind."""
+    q, lengths = rand(1, 2, 4, 64), torch.tensor([40, 20], device=DEV)
+    for heads, tiles in ((1, 2), (1, 1), (2, 1)):
+        pages, table = tables(K, 2, heads, 64, 16 * tiles, 64, 3, spare=0)
+        want = K.kv4_attn(q, pages, table, lengths)
+        odd = torch.empty_strided(pages.shape, (heads * tiles * 1088, 7 if heads == 1 else 1088, 5 if tiles == 1 else 1088, 1),
+                                  dtype=torch.uint8, device=DEV)
+        odd.copy_(pages)
+        assert torch.equal(K.kv4_attn(q, odd, table, lengths), want)
+    pages, table = tables(K, 2, 2, 64, 32, 64, 3, spare=0)
+    for bad in (pages.transpose(1, 2), pages.flatten(1)):
+        with pytest.raises(ValueError):
+            K.kv4_attn(q, bad, table, lengths)
+
+
 def test_attn_far_pages(K):
     """A pool of more than 4 GB, the pages at its end."""
     page, n_kv, hd = 256, 8, 128
