@@ -971,8 +971,9 @@ int pe_kv4_read(int type, const pe_kv4_pool* pool, const void* lengths, int leng
  * Head h takes kv head h / (n_head / n_kv); q and out of `type` (PE_TYPE_F32 or PE_TYPE_F16), head h of row t at t * token stride + h * head
  * stride; out's rows must not overlap and share no memory with q. Numbers of keys are clamped to the table's; a row that sees none, or whose
  * sequence has a negative length, gets zeros. What lies in slots that a row does not see may be anything. scale: under 2^127, of any sign.
- * The cache's values are taken exactly, fp32 queries and their probabilities in 24 bits, fp16 queries exactly and their
- * probabilities in 16 bits; sums and softmax statistics are fp32. Queries of 2^127 and more, infinite ones and NaN make their row NaN.
+ * The cache's values are taken exactly, fp32 queries (elements from 2^-94 of their row's largest on) and their probabilities in
+ * 24 bits, fp16 queries exactly and their probabilities in 16 bits; sums and softmax statistics are fp32. Infinite queries and NaN
+ * make their row NaN; fp32 ones times the scale must stay under 2^252.
  * Scores times log2 e, and 64 times the sum of the values' magnitudes that a row sees, must stay under 2^127 (else infinite or NaN).
  * workspace: pe_kv4_attn_workspace_bytes(...) bytes (0: NULL will do), any contents; capacity = table_cols * page_tokens, ragged: starts
  * is given. Calls in order on one stream, and graphs replayed in order, may share it, calls that overlap must not. One

@@ -45,8 +45,8 @@ struct Kv4AttnArgs {
     int starts_wide;
     int64_t tokens;
     int batch, n_head, n_kv, group;
-    float scale;        // of scores, above 0
-    double q_scale;     // of queries: their product is the scale times log2 e
+    float scale;        // of fp16 queries' scores, above 0
+    double q_scale;     // of queries: with the scores' factor the scale times log2 e
     int64_t capacity;   // slots of a sequence
     int vec;            // q's rows are whole pieces of 16 bytes
     int items, blocks;  // workgroups a kv head, row blocks at most
@@ -297,6 +297,7 @@ template <int HD, int RT>
 struct Kv4State {
     f4v o[RT][HD / 16];  // O^T: channel (4 g + i) HD/16 + j of row lane % 16 in o[j][i]
     float m[RT], l[RT];  // what exponents are taken from (of the row), sum (of the lane's keys), base 2
+    float scale[RT];     // of the row's scores
     int lim[RT];         // keys that the lane's row sees
 };
 
@@ -400,7 +401,7 @@ PE_DEV void kv4_no_numbers(const int* keys, int g, const uint32_t* bad, Kv4State
 constexpr float kKv4Slack = 6.f;
 
 template <int HD, int RT, int NP, int TS>
-PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT>& st, const f4v (&s)[RT][TS], uint32_t (&pr)[RT][TS / 2][NP][4]) {
+PE_DEV void kv4_softmax(Kv4State<HD, RT>& st, const f4v (&s)[RT][TS], uint32_t (&pr)[RT][TS / 2][NP][4]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = -INFINITY;
@@ -408,7 +409,7 @@ PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT>& st, const f4v (&s)[RT][TS
         for (int i = 0; i < TS; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) top = fmaxf(top, s[t][i][c]);
-        top *= scale;
+        top *= st.scale[t];
         if (__ballot(top > st.m[t] + kKv4Slack)) {
             const float m = fmaxf(st.m[t], swap32_max(swap16_max(top)));
             const float shrink = __builtin_amdgcn_exp2f(st.m[t] - (m == -INFINITY ? 0.f : m));
@@ -423,7 +424,7 @@ PE_DEV void kv4_softmax(float scale, Kv4State<HD, RT>& st, const f4v (&s)[RT][TS
             float e[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                e[c] = __builtin_amdgcn_exp2f(fmaf(s[t][i][c], scale, base));
+                e[c] = __builtin_amdgcn_exp2f(fmaf(s[t][i][c], st.scale[t], base));
                 st.l[t] += e[c];
             }
 #pragma unroll
@@ -488,9 +489,13 @@ template <typename T>
 constexpr int kKv4Parts = sizeof(T) == 2 ? 2 : 3;
 
 // A lane's HD / 4 elements of query row `row` (of the sequence's rows times heads) as operands: to(j, z) gets the NP
-// parts z[four words][NP] of the j-th 32 channels; zeros where the row is not there.
+// parts z[four words][NP] of the j-th 32 channels; zeros where the row is not there. Returns the factor of the row's scores.
+//
+// An fp32 row times its scale is moved by a power of two, which its scores get back: its largest element then lies in
+// [2^-9, 2^-8), so that no sum of products with keys (under 2^127.6 each) leaves fp32 and the parts of elements down to
+// 2^-94 of the largest are normal numbers, wherever queries, scale and keys lie.
 template <typename T, int HD, int NP, typename F>
-PE_DEV void kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row, int last, int g, const F& to) {
+PE_DEV float kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row, int last, int g, const F& to) {
     const bool there = row < seq.rows;
     row = there ? row : last;
     const int i = row / p.group;
@@ -509,16 +514,29 @@ PE_DEV void kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row,
 #pragma unroll
         for (int j = 0; j < HD / 4; ++j) q[j] = (float)x[j];
     }
+    double q_scale = p.q_scale;
+    float scale = p.scale;
+    if constexpr (sizeof(T) == 4) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < HD / 4; ++j) top = fmaxf(top, fabsf(q[j]));
+        top = swap32_max(swap16_max(top));
+        int e = __builtin_amdgcn_frexp_exp(top * q_scale) + 8;  // (0, infinite, no number: 8)
+        e = e < -126 ? -126 : e > 126 ? 126 : e;
+        q_scale = __builtin_amdgcn_ldexp(q_scale, -e);
+        scale = __uint_as_float((uint32_t)(e + 127) << 23);
+    }
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) {
         uint32_t z[4][NP];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float a = (float)(q[8 * j + 2 * c] * p.q_scale), b = (float)(q[8 * j + 2 * c + 1] * p.q_scale);
+            const float a = (float)(q[8 * j + 2 * c] * q_scale), b = (float)(q[8 * j + 2 * c + 1] * q_scale);
             split_pair<NP>(there ? a : 0.f, there ? b : 0.f, z[c]);
         }
         to(j, z);
     }
+    return scale;
 }
 
 template <int TS>
@@ -554,14 +572,18 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     const int r0 = w.block * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
     const int least = kv4_keys(p, seq.keys, r0 / p.group), most = kv4_keys(p, seq.keys, last / p.group);
     const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
+    // (behind the queries the factor of an fp32 row's scores, where a lane reads it with the same address register)
     constexpr int QUERIES = NP * (HD / 32) * 64, PART = kKv4Waves * R * (HD + 4 + 2) * 4;
-    __shared__ __attribute__((aligned(16))) char lds[PART > QUERIES * 16 ? PART : QUERIES * 16];
+    static_assert(PART >= (QUERIES + 64) * 16, "queries lie in the merge's room");
+    __shared__ __attribute__((aligned(16))) char lds[PART];
     u4v* queries = reinterpret_cast<u4v*>(lds) + lane;
-    if (wave == 0)
-        kv4_query<T, HD, NP>(p, seq, kvh, r0 + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
+    if (wave == 0) {
+        const float scale = kv4_query<T, HD, NP>(p, seq, kvh, r0 + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) queries[(k * (HD / 32) + j) * 64] = u4v{z[0][k], z[1][k], z[2][k], z[3][k]};
         });
+        if (sizeof(T) == 4) queries[QUERIES][0] = __float_as_uint(scale);
+    }
     Kv4State<HD, 1> st;
     st.lim[0] = r0 + n < seq.rows ? kv4_keys(p, seq.keys, (r0 + n) / p.group) : 0;
     st.m[0] = -INFINITY;
@@ -592,13 +614,14 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
             const bool more = walk.next < walk.end;
             f4v s[1][TS];
             kv4_scores<HD, NP, TS>(keys, queries, s[0]);
+            st.scale[0] = sizeof(T) == 4 ? __uint_as_float(queries[QUERIES][0]) : p.scale;
             if (more) {
                 kv4_advance<HD, TS>(p, table, head, walk);
                 kv4_load_keys<HD, TS>(walk, lane, keys);
             }
             uint32_t bad[TS / 2] = {}, pr[1][TS / 2][NP][4];
             if (masked) kv4_mask_scores<HD, 1, TS>(at, g, st, s, most, &values, bad);
-            kv4_softmax<HD, 1, NP, TS>(p.scale, st, s, pr);
+            kv4_softmax<HD, 1, NP, TS>(st, s, pr);
             kv4_values<HD, NP, TS>(values, st, pr);
             if (masked) kv4_no_numbers<HD, 1, TS>(at, g, bad, st);
             if (!more) break;
@@ -683,8 +706,9 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
     uint32_t q[RT][NP][N][4] = {};
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+        st.scale[t] = p.scale;
         if (rows)
-            kv4_query<T, HD, NP>(p, seq, kvh, r0 + 16 * t + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
+            st.scale[t] = kv4_query<T, HD, NP>(p, seq, kvh, r0 + 16 * t + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k)
 #pragma unroll
@@ -777,7 +801,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
             if (masked) kv4_mask_scores<HD, RT, TS>(keys_at, g, st, s);
             mask(at ^ 1);
             uint32_t pr[RT][TS / 2][NP][4];
-            kv4_softmax<HD, RT, NP, TS>(p.scale, st, s, pr);
+            kv4_softmax<HD, RT, NP, TS>(st, s, pr);
             // the next step's conversions beside this one's second product
             convert(at ^ 1);
 #pragma unroll
@@ -1015,8 +1039,8 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
     if ((s.items + 7) * a->n_kv >= (1 << 24) || T * a->n_head > (1LL << 26) - 4) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
     const int piece = (int)(16 / e);
     const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
-    // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores;
-    // fp16 ones only turned by its sign, so that their parts stay exact
+    // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores (what
+    // power of two the scores get back is the row's own); fp16 ones only turned by its sign, so that their parts stay exact
     const float scale = half && a->scale != 0 ? std::fabs(a->scale) * kKv4Log2e : 1.f;
     const double q_scale = half ? (a->scale > 0) - (a->scale < 0) : (double)a->scale * 1.4426950408889634;
     const float round = (s.split ? 4 : 2) * 256.f / (float)a->n_kv;
