@@ -491,9 +491,10 @@ constexpr int kKv4Parts = sizeof(T) == 2 ? 2 : 3;
 // A lane's HD / 4 elements of query row `row` (of the sequence's rows times heads) as operands: to(j, z) gets the NP
 // parts z[four words][NP] of the j-th 32 channels; zeros where the row is not there. Returns the factor of the row's scores.
 //
-// An fp32 row times its scale is moved by a power of two, which its scores get back: its largest element then lies in
+// An fp32 row times its scale is moved by a power of two 2^e, which its scores get back: its largest element then lies in
 // [2^-9, 2^-8), so that no sum of products with keys (under 2^127.6 each) leaves fp32 and the parts of elements down to
-// 2^-94 of the largest are normal numbers, wherever queries, scale and keys lie.
+// 2^-94 of the largest are normal numbers, wherever queries, scale and keys lie. Up to e = 64: what falls under fp32's
+// normal numbers is then less than 2^-55 of a score, and beyond it the scores themselves leave 2^64 of room.
 template <typename T, int HD, int NP, typename F>
 PE_DEV float kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row, int last, int g, const F& to) {
     const bool there = row < seq.rows;
@@ -522,7 +523,7 @@ PE_DEV float kv4_query(const Kv4AttnArgs& p, const Kv4Seq& seq, int kvh, int row
         for (int j = 0; j < HD / 4; ++j) top = fmaxf(top, fabsf(q[j]));
         top = swap32_max(swap16_max(top));
         int e = __builtin_amdgcn_frexp_exp(top * q_scale) + 8;  // (0, infinite, no number: 8)
-        e = e < -126 ? -126 : e > 126 ? 126 : e;
+        e = e < -126 ? -126 : e <= 64 ? e : e <= 64 + 8 + 126 ? 64 : e <= 126 + 8 + 126 ? e - 8 - 126 : 126;
         q_scale = __builtin_amdgcn_ldexp(q_scale, -e);
         scale = __uint_as_float((uint32_t)(e + 127) << 23);
     }

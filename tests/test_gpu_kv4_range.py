@@ -27,7 +27,7 @@ def case(K, nh, n_kv, hd, sizes, seed):
 
 
 @pytest.mark.parametrize("nh,n_kv,hd,sizes", SIZES)
-@pytest.mark.parametrize("query,scale,key", [(-121, None, 122), (-112, None, 112), (-30, 2.0 ** -93, 122), (60, 2.0 ** 36, -97)])
+@pytest.mark.parametrize("query,scale,key", [(-121, None, 122), (-112, None, 112), (-30, 2.0 ** -93, 122), (60, 2.0 ** 36, -97), (60, 2.0 ** 38, -99)])
 def test_small_and_large_queries(K, nh, n_kv, hd, sizes, query, scale, key):  # noqa: F811
     pages, table, lengths, starts, q = case(K, nh, n_kv, hd, sizes, 3)
     moved(pages, key)
