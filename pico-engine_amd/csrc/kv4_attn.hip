@@ -1042,8 +1042,13 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
     const int vec = (a->q_token | a->q_head) % piece == 0 && aligned(a->q, 16);
     // fp32 queries are scaled in 64 bits before they are split, so that no rounding of the scale is left in the scores (what
     // power of two the scores get back is the row's own); fp16 ones only turned by its sign, so that their parts stay exact
-    const float scale = half && a->scale != 0 ? std::fabs(a->scale) * kKv4Log2e : 1.f;
-    const double q_scale = half ? (a->scale > 0) - (a->scale < 0) : (double)a->scale * 1.4426950408889634;
+    //
+    // fp16 queries (2^-24 to 2^16, in parts down to 2^-24) go 2^24 down, where no sum of products with keys leaves fp32, and
+    // their scores back up. Not with scales from 2^64 on: what falls under 2^-126 would show there (below, less than 2^-31 of
+    // a score does), and sums that are too large are scores that are.
+    const float up = half && std::fabs(a->scale) < 0x1p64f ? 0x1p24f : 1.f;
+    const float scale = half && a->scale != 0 ? std::fabs(a->scale) * up * kKv4Log2e : 1.f;
+    const double q_scale = half ? ((a->scale > 0) - (a->scale < 0)) / up : (double)a->scale * 1.4426950408889634;
     const float round = (s.split ? 4 : 2) * 256.f / (float)a->n_kv;
     int4* plan = need ? static_cast<int4*>(a->workspace) : nullptr;
     float* record = need ? reinterpret_cast<float*>(plan + a->batch) : nullptr;

@@ -58,6 +58,16 @@ def test_products_beyond_the_range(K, nh, n_kv, hd, sizes, query, scale):  # noq
 
 
 @pytest.mark.parametrize("nh,n_kv,hd,sizes", SIZES)
+def test_half_queries_and_large_keys(K, nh, n_kv, hd, sizes):  # noqa: F811
+    """Products of fp16 queries and keys beyond fp32 before a small scale."""
+    pages, table, lengths, starts, q = case(K, nh, n_kv, hd, sizes, 7)
+    moved(pages, 122)
+    q = (q * 2000).half()
+    for scale in (2.0 ** -134, -2.0 ** -133):
+        close(K.kv4_attn(q, pages, table, lengths, starts=starts, scale=scale), pages, table, lengths, q, starts=starts, scale=scale)
+
+
+@pytest.mark.parametrize("nh,n_kv,hd,sizes", SIZES)
 def test_half_queries_and_scales(K, nh, n_kv, hd, sizes):  # noqa: F811
     """Scales of every kind for fp16 queries, the smallest among them."""
     pages, table, lengths, starts, q = case(K, nh, n_kv, hd, sizes, 9)
