@@ -137,9 +137,9 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
         count = wave_sum<64>(count);
         if (count > p.round && count < 1.6f * p.round)
             span = ((int)((float)span * count / p.round) + kKv4Span - 1) / kKv4Span * kKv4Span;
-        // more than the launch has: keys times blocks shared out evenly, in 32-bit floats, and a 4096th more, which is beyond
-        // what their rounding takes off
-        if (count > (float)p.items * (1.f - 1.f / 4096)) {
+        // more than the launch has (both are whole numbers, exact below 2^24, and there are fewer items): keys times blocks
+        // shared out evenly, in 32-bit floats, and a 4096th more, which is beyond what their rounding takes off
+        if (count > (float)p.items) {
             const float safe = all / (float)(p.items - p.blocks) * (1.f + 1.f / 4096) + kKv4Span;
             span = safe < (float)(1 << 30) ? (int)safe / kKv4Span * kKv4Span : 1 << 30;
             span = span < p.min_chunk ? p.min_chunk : span;

@@ -167,3 +167,12 @@ def test_pieces_in_a_graph(K, nh, n_kv, hd, rows, dtype):  # noqa: F811
             close(want, mine, table, lengths, q, starts=starts)
             _, plan = attn(K, q, mine, table, lengths, starts)
             hold(plan, sizes, nh // n_kv, rows, (2,))
+
+
+def test_chunks_that_fit(K):  # noqa: F811
+    """As many chunks as the launch has room for are taken: 5005 keys in 20 of 256, for three blocks of rows."""
+    pages, table = tables(K, 1, 2, 64, 64, 5120, 7)
+    lengths, starts, q = torch.tensor([5000], device=DEV), torch.tensor([0, 5], device=DEV), rand(8, 5, 14, 64) * 0.5
+    got, plan = attn(K, q, pages, table, lengths, starts)
+    assert plan == [[20, 3]]
+    close(got, pages, table, lengths, q, starts=starts)
