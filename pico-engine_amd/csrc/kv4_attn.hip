@@ -50,13 +50,14 @@ struct Kv4AttnArgs {
     int64_t capacity;   // slots of a sequence
     int vec;            // q's rows are whole pieces of 16 bytes
     int items, blocks;  // workgroups a kv head, row blocks at most
+    int records;        // chunks that there is room for, a kv head
     int min_chunk;      // least keys of a chunk
     float weight;       // of all keys in the square of a chunk's length
     int rec_rows;       // rows of a record
     float round;        // workgroups of a kv head that are resident at once
-    int4* plan;         // of every sequence: first item, chunks, row blocks
-    float* record;      // [kv head][items][row][HD], a row block's chunks one after the other
-    float* stat;        // [kv head][items][row] (maximum, sum)
+    int4* plan;         // of every sequence: first record (if it is cut), chunks, row blocks
+    float* record;      // [kv head][records][row][HD], a row block's chunks one after the other
+    float* stat;        // [kv head][records][row] (maximum, sum)
 };
 
 // Work of a sequence.
@@ -91,7 +92,7 @@ PE_DEV int wave_scan(int v) {
 }
 
 struct Kv4Item {
-    int b, block, chunk, chunks, blocks, base, span;  // span: keys of a chunk
+    int b, block, chunk, chunks, blocks, record, span;  // record: the sequence's first, if it is cut; span: keys of a chunk
     Kv4Seq seq;
 };
 
@@ -101,6 +102,9 @@ struct Kv4Item {
 // at once, is least at S = sqrt(all keys F / (256 c a)). Keys of all kv heads times row blocks, and 0.75 for the rest: with 0.25,
 // 0.75 and 2.5 one new row on 33 x 4001 keys (28 heads of 128, fp32) takes 24.9, 21.2 and 22.9 us, on 64 x 16384 (32
 // heads, fp16) 152, 143 and 142, 2 x 1021 rows on 8000 keys 421, 385 and 396.
+//
+// Records are numbered as items are, in blocks of 128 rows cut sequences' alone: a second scan of all sequences, which costs a call of
+// few rows more than the room is worth (one row on 700 keys 9.6 -> 10.0 us).
 template <int RB>
 PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
     const int lane = threadIdx.x & 63;
@@ -111,6 +115,7 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
         nb = (s.rows + RB - 1) / RB;
         if (nb) keys = kv4_keys(p, s.keys, s.rows / p.group - 1);
     };
+    constexpr bool CUT_ALONE = RB > 16;
     const auto chunks_of = [](int keys, int span) { return keys > span ? (int)((uint32_t)(keys + span - 1) / (uint32_t)span) : 1; };
     Kv4Seq seq0{}, seq;
     int nb0, keys0;
@@ -125,11 +130,13 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
         }
         const float all = wave_sum<64>((float)cost);
         span = ((int)fmaxf(sqrtf(all * p.weight), (float)p.min_chunk) + kKv4Span - 1) / kKv4Span * kKv4Span;
-        float count = (float)nb0 * (float)chunks_of(keys0, span);
+        float count = (float)nb0 * (float)chunks_of(keys0, span), cut = CUT_ALONE && keys0 > span ? count : 0.f;
         for (int b = lane + 64; b < p.batch; b += 64) {
             int nb, keys;
             look(b, seq, nb, keys);
-            count += (float)nb * (float)chunks_of(keys, span);
+            const float c = (float)nb * (float)chunks_of(keys, span);
+            count += c;
+            if (CUT_ALONE && keys > span) cut += c;
         }
         // Up to 1.6 rounds of what is resident at once are made one, of longer chunks (5 rows on 80000 keys, 32 heads of
         // 128, fp16: 47.9 -> 43.7 us, on 120000 63.5 -> 59.3; 128 x 8000, 14 heads of 64: 36.4 -> 34.4; 2 x 700 rows on
@@ -139,19 +146,19 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             span = ((int)((float)span * count / p.round) + kKv4Span - 1) / kKv4Span * kKv4Span;
         // more than the launch has (both are whole numbers, exact below 2^24, and there are fewer items): keys times blocks
         // shared out evenly, in 32-bit floats, and a 4096th more, which is beyond what their rounding takes off
-        if (count > (float)p.items) {
+        if (count > (float)p.items || (CUT_ALONE && wave_sum<64>(cut) > (float)p.records)) {
             const float safe = all / (float)(p.items - p.blocks) * (1.f + 1.f / 4096) + kKv4Span;
             span = safe < (float)(1 << 30) ? (int)safe / kKv4Span * kKv4Span : 1 << 30;
             span = span < p.min_chunk ? p.min_chunk : span;
         }
     }
-    int base = 0;
+    int base = 0, records = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
         int nb = nb0, keys = keys0;
         seq = seq0;
         if (b0) look(b0 + lane, seq, nb, keys);
         const int chunks = chunks_of(keys, span);
-        const int upto = wave_scan(nb * chunks);
+        const int upto = wave_scan(nb * chunks), recorded = CUT_ALONE ? wave_scan(chunks > 1 ? nb * chunks : 0) : upto;
         const uint64_t beyond = __ballot(base + upto > item);
         if (beyond) {
             const int at = __builtin_ctzll(beyond);
@@ -159,11 +166,13 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             w.seq = {lane_of(seq.lo, at), __builtin_amdgcn_readlane(seq.rows, at), lane_of(seq.keys, at)};
             w.blocks = __builtin_amdgcn_readlane(nb, at);
             w.chunks = __builtin_amdgcn_readlane(chunks, at);
-            w.base = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
+            const int first = base + __builtin_amdgcn_readlane(upto, at) - w.blocks * w.chunks;
+            w.record = CUT_ALONE ? records + __builtin_amdgcn_readlane(recorded, at) - w.blocks * w.chunks : first;
             w.span = span;
-            // starts that are out of order can ask for more items than there are room for
-            if (w.base < 0 || w.base + (int64_t)w.blocks * w.chunks > p.items) return false;
-            const int local = item - w.base;
+            // starts that are out of order can ask for more than there is room for
+            if (first < 0 || first + (int64_t)w.blocks * w.chunks > p.items) return false;
+            if (CUT_ALONE && w.chunks > 1 && (w.record < 0 || w.record + (int64_t)w.blocks * w.chunks > p.records)) return false;
+            const int local = item - first;
             if (w.blocks == 1) {
                 w.chunk = local, w.block = 0;
             } else if (RB == 16) {
@@ -180,6 +189,7 @@ PE_DEV bool kv4_find(const Kv4AttnArgs& p, int item, Kv4Item& w) {
             return true;
         }
         base += __builtin_amdgcn_readlane(upto, 63);
+        if (CUT_ALONE) records += __builtin_amdgcn_readlane(recorded, 63);
     }
     return false;
 }
@@ -550,9 +560,15 @@ PE_DEV void kv4_begin(const Kv4AttnArgs& p, Kv4Walk<TS>& w, int first, int end, 
     w.tile = first / kKv4Tile - w.col * p.tiles;
 }
 
+// Records of a kv head (as in kv4_find).
+template <int RB>
+PE_DEV int64_t kv4_room(const Kv4AttnArgs& p) {
+    return RB > 16 ? p.records : p.items;
+}
+
 PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
     if (w.chunk == 0 && w.block == 0 && kvh == 0 && threadIdx.x == 0 && p.plan)
-        p.plan[w.b] = make_int4(w.base, w.chunks, w.blocks, 0);
+        p.plan[w.b] = make_int4(w.record, w.chunks, w.blocks, 0);
 }
 
 // Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32
@@ -631,7 +647,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     }
     st.l[0] = swap32_sum(swap16_sum(st.l[0]));
 
-    const int64_t rec = ((int64_t)kvh * p.items + w.base + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;
+    const int64_t rec = (kvh * kv4_room<R>(p) + w.record + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;  // (if cut)
     float(*part)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(lds);
     float(*pm)[R] = reinterpret_cast<float(*)[R]>(lds + kKv4Waves * R * (HD + 4) * 4), (*pl)[R] = pm + kKv4Waves;
     __syncthreads();  // the queries have been read
@@ -830,7 +846,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) st.l[t] = swap32_sum(swap16_sum(st.l[t]));
-    const int64_t rec = ((int64_t)kvh * p.items + w.base + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;
+    const int64_t rec = (kvh * kv4_room<RB>(p) + w.record + (int64_t)w.block * w.chunks + w.chunk) * p.rec_rows;  // (if cut)
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = wave * R + 16 * t + n, r = r0 + 16 * t + n;
@@ -888,9 +904,9 @@ __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
             const int kvh = h / p.group;
             r = (int)(t - lo) * p.group + h - kvh * p.group;
             // (a plan that no workgroup wrote, of starts that are out of order, holds anything)
-            if (plan.y > 1 && plan.z > 0 && plan.x >= 0 && r >= 0 && r / RB < plan.z && (int64_t)plan.x + (int64_t)plan.y * plan.z <= p.items) {
+            if (plan.y > 1 && plan.z > 0 && plan.x >= 0 && r >= 0 && r / RB < plan.z && (int64_t)plan.x + (int64_t)plan.y * plan.z <= kv4_room<RB>(p)) {
                 chunks = plan.y;
-                first = ((int64_t)kvh * p.items + plan.x + (int64_t)(r / RB) * plan.y) * p.rec_rows + r % RB;
+                first = (kvh * kv4_room<RB>(p) + plan.x + (int64_t)(r / RB) * plan.y) * p.rec_rows + r % RB;
             }
         }
     }
@@ -938,7 +954,7 @@ __global__ __launch_bounds__(256) void k_kv4_merge(Kv4AttnArgs p) {
 struct Kv4Plan {
     int rt, split;   // 16-row tiles of a wave; the waves share the rows and split the keys
     int rb;          // rows of a workgroup
-    int64_t blocks, items;
+    int64_t blocks, items, records;  // (of a kv head)
     int min_chunk, rec_rows;
     float weight;  // of all keys in the square of a chunk's length
 };
@@ -969,6 +985,12 @@ static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, 
     else if (extra > s.blocks * (chunks - 1))
         extra = s.blocks * (chunks - 1);
     s.items = s.blocks + extra;
+    // A record for every workgroup, in blocks of 128 rows for those of cut sequences alone: their chunks are two a row block at
+    // least, so no more than twice those beyond the first of each row block; of these there are `extra`, and one a sequence where
+    // the count of blocks above is over (65536 rows of 32 heads on 8 of 128 behind as many keys: 1.1 GB instead of 1.6; 2^20 rows
+    // of 16 sequences 1.1 instead of 18). Rows of no sequence make that count larger still; the device then takes longer chunks.
+    s.records = extra == 0 ? 0 : s.items;
+    if (!s.split && extra + (ragged ? batch : 0) < s.records / 2) s.records = 2 * (extra + (ragged ? batch : 0));
     return s;
 }
 
@@ -979,7 +1001,7 @@ static bool kv4_shape_ok(int64_t tokens, int64_t batch, bool ragged, int n_head,
 }
 
 static int64_t kv4_bytes(const Kv4Plan& s, int64_t batch, int n_kv, int hd) {
-    return s.items > s.blocks ? (batch * 16 + s.items * n_kv * s.rec_rows * (int64_t)(hd + 2) * 4 + 15) / 16 * 16 : 0;
+    return s.records ? (batch * 16 + s.records * n_kv * s.rec_rows * (int64_t)(hd + 2) * 4 + 15) / 16 * 16 : 0;
 }
 
 template <typename T, int HD, int RB>
@@ -1056,8 +1078,8 @@ extern "C" int pe_kv4_attn(const pe_kv4_attn_args* a, pe_stream_t stream) {
                   a->pool.page_stride, (int)a->pool.n_pages, (int)(a->pool.page_tokens / kKv4Tile), a->pool.table,
                   a->pool.table_stride, (int)a->pool.table_cols, a->lengths, a->lengths_dtype == 2, a->first, a->starts,
                   a->starts_dtype == 2, T, (int)a->batch, a->n_head, a->n_kv, a->n_head / a->n_kv, scale, q_scale, capacity, vec,
-                  (int)s.items, (int)s.blocks, s.min_chunk, s.weight, s.rec_rows, round, plan, record,
-                  need ? record + s.items * a->n_kv * s.rec_rows * a->head_dim : nullptr};
+                  (int)s.items, (int)s.blocks, (int)s.records, s.min_chunk, s.weight, s.rec_rows, round, plan, record,
+                  need ? record + s.records * a->n_kv * s.rec_rows * a->head_dim : nullptr};
     hipStream_t st = (hipStream_t)stream;
     if (a->type == PE_TYPE_F16)
         a->head_dim == 64 ? launch_kv4<_Float16, 64>(p, s, st) : launch_kv4<_Float16, 128>(p, s, st);

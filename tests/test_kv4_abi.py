@@ -154,3 +154,14 @@ def test_quantize():
     assert value(code, scale)[0, :10].tolist() == [6, 0, 1, 1, 2, 2, 4, 4, -6, -0.5] and scale[:, 0].tolist() == [127, 128, 255, 27]
     assert value(code, scale)[1, 0] == 8 and bool(value(code, scale)[2].isnan().all()) and bool((value(code, scale)[3] == 0).all())
     assert len(MAGS) == 8
+
+
+@pytest.mark.parametrize("tokens,batch,n_head,n_kv,hd,capacity", [
+    (65536, 1, 32, 8, 128, 65536), (1 << 20, 16, 32, 8, 128, 65536), (200000, 3, 14, 2, 64, 100000), (64, 64, 32, 8, 128, 16384),
+    (5, 1, 14, 2, 64, 5120), (1 << 20, 1 << 20, 8, 1, 64, 4096)])
+def test_attn_workspace_bound(lib, tokens, batch, n_head, n_kv, hd, capacity):
+    """Room for the chunks of keys that are cut alone, 2^14 a launch and two a sequence, however many rows there are."""
+    ragged = tokens != batch
+    got = lib.pe_kv4_attn_workspace_bytes(tokens, batch, int(ragged), n_head, n_kv, hd, capacity)
+    rows = 128 if -(-tokens // batch) * (n_head // n_kv) > 512 else 16
+    assert 0 < got <= batch * 16 + (2 ** 14 + n_kv * 2 * (1 + batch)) * rows * (hd + 2) * 4 + 16
