@@ -578,7 +578,7 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
 // the copy rate). Four waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of
 // 64 keys, two waves, 145 us where this is 135; with a second step in registers 150.
 template <typename T, int HD>
-__global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
+__global__ __launch_bounds__(64 * kKv4Waves, 4) void k_kv4_attn(Kv4AttnArgs p) {
     constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16, TS = 2;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.y;
@@ -589,17 +589,17 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
     const int r0 = w.block * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
     const int least = kv4_keys(p, seq.keys, r0 / p.group), most = kv4_keys(p, seq.keys, last / p.group);
     const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
-    // (behind the queries the factor of an fp32 row's scores, where a lane reads it with the same address register)
     constexpr int QUERIES = NP * (HD / 32) * 64, PART = kKv4Waves * R * (HD + 4 + 2) * 4;
-    static_assert(PART >= (QUERIES + 64) * 16, "queries lie in the merge's room");
+    static_assert(PART >= QUERIES * 16, "queries lie in the merge's room");
     __shared__ __attribute__((aligned(16))) char lds[PART];
+    __shared__ float scales[R];  // of fp32 rows' scores
     u4v* queries = reinterpret_cast<u4v*>(lds) + lane;
     if (wave == 0) {
         const float scale = kv4_query<T, HD, NP>(p, seq, kvh, r0 + n, last, g, [&](int j, const uint32_t (&z)[4][NP]) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) queries[(k * (HD / 32) + j) * 64] = u4v{z[0][k], z[1][k], z[2][k], z[3][k]};
         });
-        if (sizeof(T) == 4) queries[QUERIES][0] = __float_as_uint(scale);
+        if (sizeof(T) == 4 && g == 0) scales[n] = scale;
     }
     Kv4State<HD, 1> st;
     st.lim[0] = r0 + n < seq.rows ? kv4_keys(p, seq.keys, (r0 + n) / p.group) : 0;
@@ -608,6 +608,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
 #pragma unroll
     for (int j = 0; j < E; ++j) st.o[0][j] = f4v{};
     __syncthreads();
+    st.scale[0] = sizeof(T) == 4 ? scales[n] : p.scale;
     Kv4Walk<TS> walk;
     kv4_begin(p, walk, (int)begin + wave * TS * kKv4Tile, (int)(stop < most ? stop : most), TS * kKv4Waves);
     if (walk.next < walk.end) {
@@ -631,7 +632,6 @@ __global__ __launch_bounds__(64 * kKv4Waves, 3) void k_kv4_attn(Kv4AttnArgs p) {
             const bool more = walk.next < walk.end;
             f4v s[1][TS];
             kv4_scores<HD, NP, TS>(keys, queries, s[0]);
-            st.scale[0] = sizeof(T) == 4 ? __uint_as_float(queries[QUERIES][0]) : p.scale;
             if (more) {
                 kv4_advance<HD, TS>(p, table, head, walk);
                 kv4_load_keys<HD, TS>(walk, lane, keys);
