@@ -879,7 +879,9 @@ int pe_adjust_logits(const pe_logit_args* args, pe_stream_t stream);
  * pe_rope_positions. type PE_TYPE_F32 or PE_TYPE_F16 (computed in fp32, rounded once). Head h of token t at t * token
  * stride + h * head stride (elements; rows of an output must not overlap). Weights fp32, head h's at h * weight
  * head stride (0: one for all), NULL: no norm. An output may be its input, with the same strides; otherwise outputs share no
- * memory with inputs or each other. n_head or n_kv may be 0 (that side's pointers are not looked at), each up to 4096; head_dim up to 512. */
+ * memory with inputs or each other. n_head or n_kv may be 0 (that side's pointers are not looked at), each up to 4096; head_dim up to 512.
+ * tokens up to 2^26 - 4, and more where rows are whole pieces of 16 bytes. The squares of a normed head are summed in fp32: the sum must stay
+ * under 2^128, what is under 2^-126 in it is lost. */
 typedef struct pe_qk_norm_args {
     int type;
     const void* q;

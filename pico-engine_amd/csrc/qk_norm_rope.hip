@@ -145,7 +145,7 @@ static int launch_qk_norm(QkNormArgs p, hipStream_t s) {
     const int64_t lanes = p.tokens * W, want = (524288 + lanes - 1) / lanes;
     p.groups = (int)(want < p.heads ? want : p.heads);
     const int64_t blocks = (p.tokens * p.groups + 256 / W - 1) / (256 / W);
-    if (blocks >= (1 << 23)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
+    if (blocks >= (1 << 24)) return PE_ERR_SHAPE;  // a grid holds 2^32 threads
     hipLaunchKernelGGL((k_qk_norm_rope<T, V, IL, W, NI>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     return launch_status();
 }

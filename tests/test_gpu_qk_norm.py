@@ -139,3 +139,15 @@ def test_another_stream_and_graph(K):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, want[0]) and torch.equal(b, want[1]), step
+
+
+def test_many_rows(K):
+    """Rows beyond 2^25, single elements a lane: a wave takes a row of one short head."""
+    T, w = (1 << 25) + 37, torch.tensor([1.0, 1.25], device=DEV)
+    q = (rand(1, T, 1, 2) * 2).half()
+    pos = torch.arange(T, device=DEV, dtype=torch.int32) % 5000
+    freqs, _ = K.rope_freqs(2, 10000.0)
+    a, _ = K.qk_norm_rope(q, None, w, None, pos, freqs, eps=1e-5)
+    for at in (slice(0, 3000), slice((1 << 25) - 2000, T)):
+        close(a[at], q[at], w, pos[at], freqs, 1.0, False, 1e-5)
+    assert bool(a.isfinite().all())

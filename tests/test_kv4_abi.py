@@ -165,3 +165,11 @@ def test_attn_workspace_bound(lib, tokens, batch, n_head, n_kv, hd, capacity):
     got = lib.pe_kv4_attn_workspace_bytes(tokens, batch, int(ragged), n_head, n_kv, hd, capacity)
     rows = 128 if -(-tokens // batch) * (n_head // n_kv) > 512 else 16
     assert 0 < got <= batch * 16 + (2 ** 14 + n_kv * 2 * (1 + batch)) * rows * (hd + 2) * 4 + 16
+
+
+def test_qk_norm_most_rows(lib):
+    """2^26 rows of single elements, four a workgroup: a grid of 2^32 threads."""
+    from pico_hip._lib import QkNormArgs
+    d = dict(type=0, q=F, q_token=2, q_head=2, q_out=F, q_out_token=2, q_out_head=2, positions=F, pos_dtype=2, freqs=F, rot_dim=2,
+             amp=1.0, eps=1e-6, tokens=1 << 26, n_head=1, n_kv=0, head_dim=2)
+    assert call_of(lib.pe_qk_norm_rope, QkNormArgs, d)() == 3
