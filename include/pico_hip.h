@@ -931,11 +931,12 @@ typedef struct pe_kv4_pool {
 /* Appends `tokens` new rows to the sequences of a batch: sequence b's are the rows starts[b] .. starts[b + 1] - 1
  * (starts NULL: row b alone, tokens == batch), and row i of them goes to slot lengths[b] + i. k (and q, unless it is NULL) is
  * normed by k_weight / q_weight (fp32, head_dim elements, NULL: not) and rotated by the slot's number (freqs NULL: not) as in
- * pe_qk_norm_rope; v is taken as it is. q_out gets the q rows of q's type. Keys are computed in 64 bits, so that what is
- * stored depends on no rounding before its own. A slot behind the table, or of a sequence of negative length (one that takes
- * no part), is not written; its q row is. Rows before starts[0] or from starts[batch] on are left out, their q_out rows
- * as they were. starts must not fall; where they do, some of the rows may be left out or be wrong, and nothing else is touched. Two rows of a call must not go to one slot. tokens below 2^23, and below 2^24 over (n_head + 15) / 16 + (2 n_kv + 15) / 16;
- * strides as in pe_qk_norm_rope (q_out may be q). */
+ * pe_qk_norm_rope (lengths beyond 2^40 count as 2^40); v is taken as it is. q_out gets the q rows of q's type. Keys are computed
+ * in 64 bits, so that what is stored depends on no rounding before its own. A slot behind the table, or of a sequence of
+ * negative length (one that takes no part), is not written; its q row is. Rows before starts[0] or from starts[batch] on are
+ * left out, their q_out rows as they were. starts must not fall; where they do, some of the rows may be left out or be wrong,
+ * and nothing else is touched. Two rows of a call must not go to one slot. tokens below 2^23, and below 2^24 over
+ * (n_head + 15) / 16 + (2 n_kv + 15) / 16; strides as in pe_qk_norm_rope (q_out may be q). */
 typedef struct pe_kv4_append_args {
     int type; /* of q, k, v: PE_TYPE_F32 or PE_TYPE_F16 */
     const void* q;
@@ -978,8 +979,10 @@ int pe_kv4_read(int type, const pe_kv4_pool* pool, const void* lengths, int leng
  * make their row NaN; fp32 ones times the scale must stay under 2^252.
  * Scores times log2 e, and 64 times the sum of the values' magnitudes that a row sees, must stay under 2^127 (else infinite or NaN).
  * workspace: pe_kv4_attn_workspace_bytes(...) bytes (0: NULL will do), any contents; capacity = table_cols * page_tokens, ragged: starts
- * is given. Calls in order on one stream, and graphs replayed in order, may share it, calls that overlap must not. One
- * launch, or two where keys are cut. tokens up to 2^22, tokens times n_head up to 2^26 - 4. */
+ * is given. Where sequences have more than 512 rows a kv head on average it holds 2^14 + 2 n_kv (batch + 1) records of 128 rows
+ * at most (1.1 GB for few sequences and heads of 128), however many rows there are. Calls in order on one stream, and graphs
+ * replayed in order, may share it, calls that overlap must not. One launch, or two where keys are cut. tokens up to 2^22,
+ * tokens times n_head up to 2^26 - 4. */
 typedef struct pe_kv4_attn_args {
     int type;
     const void* q;

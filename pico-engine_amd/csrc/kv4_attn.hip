@@ -99,9 +99,11 @@ struct Kv4Item {
 // Which work the item is: a (sequence, row block, chunk of keys). Every wave finds it for itself, from all lengths.
 // A chunk's length S weighs what workgroups cost beside their keys against the time that the last one takes
 // alone: all keys' time + S a + (all keys / S) F / (256 c), with a of a key, F of a workgroup, c of them on a CU
-// at once, is least at S = sqrt(all keys F / (256 c a)). Keys of all kv heads times row blocks, and 0.75 for the rest: with 0.25,
-// 0.75 and 2.5 one new row on 33 x 4001 keys (28 heads of 128, fp32) takes 24.9, 21.2 and 22.9 us, on 64 x 16384 (32
-// heads, fp16) 152, 143 and 142, 2 x 1021 rows on 8000 keys 421, 385 and 396.
+// at once, is least at S = sqrt(all keys F / (256 c a)). Keys of all kv heads times row blocks, and a weight for the rest,
+// 0.75, for a few fp32 queries of 128 channels, which take longer over a key, 0.5. In us with 0.25, 0.5, 0.75 and 2.5 (28 heads
+// of 128, fp32) one new row on 33 x 4001 keys 23.4, 22.9, 24.4 and 24.6, on 8 x 8000 18.3, 16.7, 18.6 and 19.6, on 64 x 4096
+// 53, 49.6, 49 and 55, 2 x 1021 rows on 8000 keys 537, 516, 508 and 522; fp16: 64 x 16384 (32 heads) 146, 145, 142 and 150, 2 x
+// 1021 rows 404, 378, 368 and 369.
 //
 // Records are numbered as items are, in blocks of 128 rows cut sequences' alone: a second scan of all sequences, which costs a call of
 // few rows more than the room is worth (one row on 700 keys 9.6 -> 10.0 us).
@@ -573,10 +575,11 @@ PE_DEV void kv4_tell(const Kv4AttnArgs& p, const Kv4Item& w, int kvh) {
 
 // Few rows (one new token, drafted ones, up to short pieces of prompts): 16 rows a workgroup, its waves take steps of 32
 // keys in turn, each with a state of its own, and are merged in LDS. What bounds it: memory once the caches are long (64 x
-// 16384 keys of 8 heads of 128, fp16: 136 to 143 us with the join, 4.1 to 4.3 TB/s), else the start's chain of loads (lengths,
-// queries, table, keys), about 4 us of a workgroup's time (28 heads of 128 on 33 x 4001 keys, fp32: 22 us with the join, 7.4 at
-// the copy rate). Four waves a SIMD are what keeps enough keys under way: with the queries in registers and steps of
-// 64 keys, two waves, 145 us where this is 135; with a second step in registers 150.
+// 16384 keys of 8 heads of 128, fp16: 127 us a call, 4.6 TB/s, and 136 to 145 replayed back to back, when the clock is lower;
+// with the join), else the start's chain of loads (lengths, queries, table, keys), about 4 us of a workgroup's time (28 heads of
+// 128 on 33 x 4001 keys, fp32: 21 to 22 us with the join, 8.0 at the copy rate). Four waves a SIMD, 128 registers each, are what
+// keeps enough keys under way: with the queries in registers and steps of 64 keys, two waves, 145 us where this was 135; with a
+// second step in registers 150.
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kKv4Waves, 4) void k_kv4_attn(Kv4AttnArgs p) {
     constexpr int NP = kKv4Parts<T>, E = HD / 16, R = 16, TS = 2;
@@ -688,8 +691,8 @@ __global__ __launch_bounds__(64 * kKv4Waves, 4) void k_kv4_attn(Kv4AttnArgs p) {
 // Many rows (pieces of prompts): 32 rows a wave, 128 a workgroup, all on the same keys. The waves convert a step's codes
 // for one another, into LDS in the order of the products' operands, two steps deep; the queries are in registers. Bound by
 // the matrix cores and the vector instructions, which add up with two waves a SIMD (2 x 1021 rows of 28 heads of 128
-// on 8000 keys, fp16: 45 % and 54 % of the cycles, 330 us, the join of the chunks 30; the two parts of each factor alone are 273
-// at the rate of a large product). With every wave converting for itself 367 and, fp32, 588 us; so 360 and 490.
+// on 8000 keys, fp16: 45 % and 54 % of the cycles, 290 to 365 us by the card's clock, the join of the chunks 30; the two parts of
+// each factor alone are 265 at the rate of a large product). With every wave converting for itself 367 and, fp32, 588 us; so 360 and 493.
 template <typename T, int HD>
 constexpr int kKv4RowTiles = sizeof(T) == 4 && HD == 128 ? 2 : 4;  // 16 keys a step; fp32's queries take half the registers
 
@@ -707,7 +710,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, 2) void k_kv4_attn_rows(Kv4AttnArgs
     const int least_all = kv4_keys(p, seq.keys, b0 / p.group), most_all = kv4_keys(p, seq.keys, b1 / p.group);
     const int r0 = b0 + wave * R, last = (r0 + R < seq.rows ? r0 + R : seq.rows) - 1;
     const bool rows = r0 < seq.rows;
-    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0, most = rows ? kv4_keys(p, seq.keys, last / p.group) : 0;
+    const int least = rows ? kv4_keys(p, seq.keys, r0 / p.group) : 0;
     const int64_t begin = (int64_t)w.chunk * w.span, stop = begin + w.span;
     const int end = (int)(stop < most_all ? stop : most_all);
 
@@ -971,8 +974,6 @@ static Kv4Plan kv4_plan(int64_t tokens, int64_t batch, bool ragged, int n_head, 
     s.blocks = ragged ? tokens * group / s.rb + batch : batch * ((group + s.rb - 1) / s.rb);
     s.min_chunk = 64 * (s.split ? kKv4Waves : 4);
     s.rec_rows = ragged || group > s.rb ? s.rb : group;
-    // fp32 queries of 128 channels take longer over a key (33 x 4001 keys: 23.7 us with 0.75, 22.4 so; 64 x 4096 48.9 and 48.8;
-    // 8 x 8000 18.1 and 17.5); the other kinds lose by shorter chunks (64 x 16384 fp16 137 -> 138, 4 rows on 8 x 4000 18.4 -> 20.8)
     s.weight = (s.split && !half && hd == 128 ? 0.5f : 0.75f) * (float)n_kv;
     // the most workgroups that a chunk's length makes of any lengths, within reason
     const int64_t chunks = (capacity + s.min_chunk - 1) / s.min_chunk;
