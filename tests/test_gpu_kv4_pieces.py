@@ -176,3 +176,27 @@ def test_chunks_that_fit(K):  # noqa: F811
     got, plan = attn(K, q, pages, table, lengths, starts)
     assert plan == [[20, 3]]
     close(got, pages, table, lengths, q, starts=starts)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_cut_among_many_rows(K, hd, dtype):  # noqa: F811
+    """Cut sequences around one of many rows that is not: the workspace has fewer records than the launch has workgroups, and
+    theirs follow one another."""
+    heads, sizes, lengths = 16, [600, 19000, 590], [400, -1, 430]
+    pages, table = tables(K, 3, heads, hd, 64, 1024, 7)
+    starts, ln, T = ragged(sizes, 0), torch.tensor(lengths, device=DEV), sum(sizes)
+    q = (rand(8, T, heads, hd) * 0.5).to(dtype)
+    need = K.kv4_attn_workspace(T, 3, heads, heads, hd, 1024, DEV, ragged=True).numel()
+    assert need < heads * (-(-T // 128) + 100) * 128 * (hd + 2) * 4
+    room = torch.full((need + 4096,), 77, device=DEV, dtype=torch.uint8)
+    got = K.kv4_attn(q, pages, table, ln, starts=starts, workspace=room[:need])
+    plan = room[:48].view(torch.int32).view(3, 4).tolist()
+    assert plan[0][1] > 1 and plan[1][1] == 1 and plan[2][1] > 1
+    assert plan[0][0] == 0 and plan[2][0] == plan[0][1] * plan[0][2] and bool((room[need:] == 77).all())
+    assert bool((got[600:-590] == 0).all())
+    for b, rows in ((0, slice(0, 600)), (2, slice(T - 590, T))):
+        some = slice(rows.start, rows.stop, 37)                  # (the oracle goes row by row)
+        for t in range(some.start, some.stop, some.step):
+            seen = ln[b:b + 1] + (t - rows.start)
+            close(got[t:t + 1], pages, table[b:b + 1], seen, q[t:t + 1])
